@@ -50,7 +50,7 @@ extern "C" {
 #define QS_ERR_ALLOC (-3)       /* device or host allocation failed */
 #define QS_ERR_UNSUPPORTED (-4) /* valid request outside this build's limits */
 
-typedef enum { QS_F32 = 0, QS_BF16 = 1 } qs_dtype;
+typedef enum { QS_F32 = 0, QS_BF16 = 1, QS_F16 = 2 /* scales of 4-bit weights only */ } qs_dtype;
 
 /* Bit flags for the sampling calls. */
 #define QS_FLAG_WRITE_PENALIZED 1u /* fp32 only: write penalised logits back */
@@ -321,6 +321,144 @@ QS_API int qs_lm_head_status(qs_sampler* s, void* stream);
  * the kernel give up cleanly (error flag set, TMEM freed, the context still
  * usable) without any fault.  Not for production use. */
 QS_API int qs_lm_head_set_wait_limit(unsigned long long ns);
+
+/* The lm_head with its weight held in 4 bits, for few tokens (batches of up to
+ * a few dozen rows, where the projection is the stream of its weight: 80 MB
+ * instead of 311 MB for Qwen3-0.6B).  Weight column k of vocabulary row v is
+ *   w[v][k] = scale[v][k / group] * (code[v][k] - zero[v][k / group])
+ * with codes and zero points in 0..15.  No counterpart in the reference
+ * (its weights are bf16).
+ *
+ * A weight's plain form: codes uint8 [vocab, hidden_dim / 2], the even column
+ * in the low half of a byte; scales bf16 or fp16 [vocab, hidden_dim / group];
+ * zero points uint8 [vocab, hidden_dim / group], or none (all 8).
+ * qs_w4_quantize makes one from a bf16 weight [vocab, hidden_dim]: per group
+ * scale = bf16(range / 15) over the range that holds the group and zero,
+ * codes rounded to nearest.  qs_w4_pack lays a plain weight out in the order
+ * the kernel reads, into buffers of qs_w4_codes_bytes, qs_w4_scales_bytes and
+ * qs_w4_zeros_bytes bytes (16-byte aligned); the plain buffers are not needed
+ * after it.  vocab <= qs_max_vocab(); hidden_dim a multiple of 64 up to 8192;
+ * group 32, 64 or 128, dividing hidden_dim. */
+typedef struct {
+    const void* d_codes;  /* laid out by qs_w4_pack */
+    const void* d_scales;
+    const void* d_zeros;  /* NULL: every zero point is 8 */
+    int vocab;
+    int hidden_dim;
+    int group;
+    int scale_dtype; /* QS_BF16 or QS_F16 */
+} qs_w4_weight;
+
+QS_API size_t qs_w4_codes_bytes(int vocab, int hidden_dim);
+QS_API size_t qs_w4_scales_bytes(int vocab, int hidden_dim, int group);
+QS_API size_t qs_w4_zeros_bytes(int vocab, int hidden_dim, int group);
+QS_API int qs_w4_quantize(const void* d_weight, int vocab, int hidden_dim, int group,
+                          void* d_plain_codes, void* d_plain_scales, void* d_plain_zeros, void* stream);
+QS_API int qs_w4_pack(const void* d_plain_codes, const void* d_plain_scales, const void* d_plain_zeros,
+                      int vocab, int hidden_dim, int group, int scale_dtype, void* d_codes,
+                      void* d_scales, void* d_zeros, void* stream);
+
+/* qs_lm_head with such a weight:
+ *   normed[b] as qs_lm_head's, logits[b] = bf16(normed[b] . w^T)
+ * Products of codes and normed rows are exact; sums are fp32 per group, then
+ * scaled and added in fp32.  d_hidden and d_normed bf16 [batch, hidden_dim],
+ * d_logits bf16 [batch, vocab], all 16-byte aligned.  The weight is streamed
+ * once per block of 8 to 32 rows (the most whose normed rows fit in shared
+ * memory).  Allocates nothing. */
+QS_API int qs_lm_head_w4(const void* d_hidden, const void* d_norm_weight, const qs_w4_weight* weight,
+                         int batch, void* d_normed, void* d_logits, void* stream);
+
+/* qs_lm_head_sample with such a weight (weight->vocab must be the handle's):
+ * qs_lm_head_w4 into the handle's workspace, then qs_sample on its logits. */
+QS_API int qs_lm_head_w4_sample(qs_sampler* s, const void* d_hidden, const void* d_norm_weight,
+                                const qs_w4_weight* weight, int batch, int* d_tokens, void* stream,
+                                unsigned flags);
+
+/* Scoring and training on sampled tokens.  No counterpart in the reference
+ * (it only samples).
+ *
+ * Conventions of the four calls below.  d_logits is [rows, vocab] fp32 or
+ * bf16; rows lie row_stride elements apart (>= vocab) and need only their
+ * element's alignment.  d_tokens[i] is the token row i scores; a row whose
+ * token lies outside [0, vocab) scores nothing: its log-probability is 0, its
+ * gradient zero, and its logits are not read.  With x = row i and t its token,
+ *   logprob = (x[t] - max x) / T - log sum_j exp((x[j] - max x) / T)
+ * for temperature T >= 1e-6.  Entries of -inf (masked tokens) have probability 0; a row
+ * with a NaN, with +inf or with nothing above -inf has a NaN log-probability
+ * and gradient.  Gradients are d loss / d logits, [rows, vocab] in the logits'
+ * type, rows grad_row_stride elements apart; d_grad may be d_logits itself
+ * with the same stride (the gradient then replaces the logits), and may not
+ * overlap it otherwise.  Exponentials are fp32 (relative error below 2^-20),
+ * sums over rows and sequences 64-bit, in a fixed order: the same inputs give
+ * the same bits.  vocab <= qs_max_vocab(), rows <= 2^27.  Nothing is
+ * allocated and no state is kept; calls that overlap on the GPU need
+ * workspaces of their own. */
+
+/* d_logprobs fp32 [rows]; d_stats fp32 [rows, 2] (for the backward call): the
+ * row's maximum, and sum_j exp((x[j] - max x) / T) - 1 (the maximum's own term
+ * left out, so that a peaked row keeps its precision); both 0 for a row that
+ * scores nothing. */
+QS_API int qs_token_logprobs(const void* d_logits, int dtype, int rows, int vocab, long long row_stride,
+                             const int* d_tokens, double temperature, float* d_logprobs, float* d_stats,
+                             void* stream);
+
+/* grad[i][j] = g[i] * ([j = t] - exp((x[j] - max x) / T) / sum) / T from the
+ * forward call's d_stats and the incoming d_grad_logprobs g, fp32 [rows].  A
+ * row with g[i] = 0 gets zeros and is not read. */
+QS_API int qs_token_logprobs_backward(const void* d_logits, int dtype, int rows, int vocab,
+                                      long long row_stride, const int* d_tokens, const float* d_stats,
+                                      const float* d_grad_logprobs, double temperature, void* d_grad,
+                                      long long grad_row_stride, void* stream);
+
+/* Clipped policy loss with a KL term, and its gradient in the same pass:
+ *   r = exp(logprob - old[i])
+ *   l = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+ *       + kl_coef (exp(d) - d - 1),  d = ref[i] - logprob
+ *   loss = sum_i w[i] l
+ * A = d_advantages[i]; w = d_weights[i] (NULL: 1 / rows).  A row with w[i] = 0
+ * scores nothing.  d_ref may be NULL when kl_coef is 0 (and is not read then).
+ * Where r leaves the clip range on the side that A favours (A > 0 and
+ * r > 1 + clip_high, or A < 0 and r < 1 - clip_low) the first term's gradient
+ * is 0, elsewhere -A r.  d_loss fp32 [1], d_logprobs fp32 [rows] or NULL,
+ * d_grad NULL for the loss alone.  0 <= clip_low <= 1, clip_high >= 0,
+ * kl_coef >= 0. */
+typedef struct {
+    double clip_low;
+    double clip_high;
+    double kl_coef;
+    double temperature;
+} qs_policy_params;
+
+QS_API size_t qs_policy_loss_workspace(int rows);
+QS_API int qs_policy_loss(const void* d_logits, int dtype, int rows, int vocab, long long row_stride,
+                          const int* d_tokens, const float* d_old_logprobs, const float* d_ref_logprobs,
+                          const float* d_advantages, const float* d_weights, const qs_policy_params* params,
+                          float* d_loss, float* d_logprobs, void* d_grad, long long grad_row_stride,
+                          void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* Preference loss over pairs of sequences, and its gradient.  Sequence q holds
+ * rows [offsets[q], offsets[q + 1]) (d_seq_offsets int [2 pairs + 1]); sequence
+ * p is chosen over sequence pairs + p.  With S[q] the sum of its rows'
+ * log-probabilities (T = 1) and ref[q] the reference model's (d_ref_logprobs
+ * fp32 [2 pairs]),
+ *   z = beta ((S[p] - ref[p]) - (S[pairs + p] - ref[pairs + p]))
+ *   loss = sum_p w[p] (-(1 - label_smoothing) log sigmoid(z) - label_smoothing log sigmoid(-z))
+ * w = d_weights[p] (NULL: 1 / pairs); a pair with w[p] = 0 adds nothing.  Rows
+ * in no sequence have a zero gradient.  A pair whose offsets fall, or leave
+ * [0, rows], has a NaN loss and touches no row.  d_loss fp32 [1], d_seq_logprobs fp32 [2 pairs] (S) or NULL, d_grad
+ * NULL for the loss alone.  beta > 0, 0 <= label_smoothing < 0.5. */
+typedef struct {
+    double beta;
+    double label_smoothing;
+} qs_preference_params;
+
+QS_API size_t qs_preference_loss_workspace(int rows, int pairs);
+QS_API int qs_preference_loss(const void* d_logits, int dtype, int rows, int vocab, long long row_stride,
+                              const int* d_tokens, const int* d_seq_offsets, int pairs,
+                              const float* d_ref_logprobs, const float* d_weights,
+                              const qs_preference_params* params, float* d_loss, float* d_seq_logprobs,
+                              void* d_grad, long long grad_row_stride, void* d_workspace,
+                              size_t workspace_bytes, void* stream);
 
 /* Message for the last error on the calling thread ("" if none). */
 QS_API const char* qs_last_error(void);

@@ -20,6 +20,7 @@ QS_ERR_UNSUPPORTED = -4
 
 QS_F32 = 0
 QS_BF16 = 1
+QS_F16 = 2  # scales of 4-bit weights only
 
 QS_FLAG_WRITE_PENALIZED = 1
 QS_FLAG_INDEX_TIES = 2
@@ -34,7 +35,12 @@ EXPORTS = (
     "qs_argmax_rows_static", "qs_lm_head", "qs_lm_head_sample", "qs_lm_head_logits",
     "qs_lm_head_status", "qs_lm_head_set_wait_limit", "qs_lm_head_shard", "qs_ipc_handle_bytes", "qs_ipc_alloc", "qs_ipc_open",
     "qs_ipc_close", "qs_ipc_free", "qs_shard_handshake", "qs_copy_async",
+    "qs_w4_codes_bytes", "qs_w4_scales_bytes", "qs_w4_zeros_bytes", "qs_w4_quantize", "qs_w4_pack",
+    "qs_lm_head_w4", "qs_lm_head_w4_sample", "qs_token_logprobs", "qs_token_logprobs_backward",
+    "qs_policy_loss_workspace", "qs_policy_loss", "qs_preference_loss_workspace", "qs_preference_loss",
 )
+_SIZES = ("qs_w4_codes_bytes", "qs_w4_scales_bytes", "qs_w4_zeros_bytes", "qs_policy_loss_workspace",
+          "qs_preference_loss_workspace")
 
 
 class Params(C.Structure):
@@ -55,6 +61,21 @@ class Profile(C.Structure):
                 ("emit_ms", C.c_double), ("calls", C.c_longlong), ("launches", C.c_longlong),
                 ("row_launches", C.c_longlong), ("timed_calls", C.c_longlong),
                 ("tie_clusters", C.c_longlong)]
+
+
+class W4Desc(C.Structure):
+    _fields_ = [("d_codes", C.c_void_p), ("d_scales", C.c_void_p), ("d_zeros", C.c_void_p),
+                ("vocab", C.c_int), ("hidden_dim", C.c_int), ("group", C.c_int),
+                ("scale_dtype", C.c_int)]
+
+
+class PolicyParams(C.Structure):
+    _fields_ = [("clip_low", C.c_double), ("clip_high", C.c_double), ("kl_coef", C.c_double),
+                ("temperature", C.c_double)]
+
+
+class PreferenceParams(C.Structure):
+    _fields_ = [("beta", C.c_double), ("label_smoothing", C.c_double)]
 
 
 ROW_DEBUG_FIELDS = [f for f, _ in RowDebug._fields_]
@@ -107,12 +128,28 @@ def _load() -> C.CDLL:
     lib.qs_ipc_free.argtypes = [vp]
     lib.qs_shard_handshake.argtypes = [P(vp), i32, i32, C.c_size_t, u32, C.c_ulonglong, vp, vp]
     lib.qs_copy_async.argtypes = [vp, vp, C.c_size_t, vp]
+    i64, f64, sz = C.c_longlong, C.c_double, C.c_size_t
+    lib.qs_w4_codes_bytes.argtypes = [i32, i32]
+    lib.qs_w4_scales_bytes.argtypes = [i32, i32, i32]
+    lib.qs_w4_zeros_bytes.argtypes = [i32, i32, i32]
+    lib.qs_w4_quantize.argtypes = [vp, i32, i32, i32, vp, vp, vp, vp]
+    lib.qs_w4_pack.argtypes = [vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp]
+    lib.qs_lm_head_w4.argtypes = [vp, vp, P(W4Desc), i32, vp, vp, vp]
+    lib.qs_lm_head_w4_sample.argtypes = [vp, vp, vp, P(W4Desc), i32, vp, vp, u32]
+    lib.qs_token_logprobs.argtypes = [vp, i32, i32, i32, i64, vp, f64, vp, vp, vp]
+    lib.qs_token_logprobs_backward.argtypes = [vp, i32, i32, i32, i64, vp, vp, vp, f64, vp, i64, vp]
+    lib.qs_policy_loss_workspace.argtypes = [i32]
+    lib.qs_policy_loss.argtypes = [vp, i32, i32, i32, i64, vp, vp, vp, vp, vp, P(PolicyParams), vp, vp,
+                                   vp, i64, vp, sz, vp]
+    lib.qs_preference_loss_workspace.argtypes = [i32, i32]
+    lib.qs_preference_loss.argtypes = [vp, i32, i32, i32, i64, vp, vp, i32, vp, vp, P(PreferenceParams),
+                                       vp, vp, vp, i64, vp, sz, vp]
     lib.qs_last_error.restype = C.c_char_p
     lib.qs_last_error.argtypes = []
     lib.qs_max_vocab.argtypes = []
     for name in EXPORTS:
         if name not in ("qs_last_error",):
-            getattr(lib, name).restype = C.c_int
+            getattr(lib, name).restype = sz if name in _SIZES else C.c_int
     return lib
 
 

@@ -19,6 +19,7 @@
 #include <vector>
 
 #include "qs_common.cuh"
+#include "qs_w4.h"
 #include "qwen600_sampler.h"
 
 namespace qs {
@@ -85,6 +86,14 @@ static int fail(int code, const char* fmt, ...) {
     g_err = buf;
     return code;
 }
+
+namespace qs {
+// Lets the other files' entry points report through qs_last_error.
+int set_error(int code, const char* msg) {
+    g_err = msg;
+    return code;
+}
+}  // namespace qs
 
 #define CK(call)                                                                        \
     do {                                                                                \
@@ -967,15 +976,9 @@ int qs_shard_handshake(void* const* d_bufs, int nranks, int rank, size_t flag_of
     return QS_OK;
 }
 
-int qs_lm_head_sample(qs_sampler* s, const void* d_hidden, const void* d_norm_weight,
-                      const void* d_weight, int batch, int hidden_dim, int* d_tokens, void* stream,
-                      unsigned flags) {
-    g_err.clear();
-    if (!s) return fail(QS_ERR_INVALID, "sampler is NULL");
-    int rc = lm_head_args(d_hidden, d_weight, batch, hidden_dim, s->vocab);
-    if (rc) return rc;
-    if (batch > s->max_batch) return fail(QS_ERR_INVALID, "batch %d > max_batch %d", batch, s->max_batch);
-    DeviceGuard dg(s->device);
+// The decode tail's workspace in the handle, allocated on first use (and for a
+// new hidden size).
+static int tail_workspace(qs_sampler* s, int hidden_dim) {
     if (s->lh_dim != hidden_dim) {
         // first use (or a new hidden size): the tail's workspace
         if (s->lh_normed) cudaFree(s->lh_normed);
@@ -994,6 +997,20 @@ int qs_lm_head_sample(qs_sampler* s, const void* d_hidden, const void* d_norm_we
         CK(cudaMalloc(&s->lh_segk, sizeof(uint32_t) * n));
         CK(cudaMemset(s->lh_segk, 0, sizeof(uint32_t) * n));
     }
+    return QS_OK;
+}
+
+int qs_lm_head_sample(qs_sampler* s, const void* d_hidden, const void* d_norm_weight,
+                      const void* d_weight, int batch, int hidden_dim, int* d_tokens, void* stream,
+                      unsigned flags) {
+    g_err.clear();
+    if (!s) return fail(QS_ERR_INVALID, "sampler is NULL");
+    int rc = lm_head_args(d_hidden, d_weight, batch, hidden_dim, s->vocab);
+    if (rc) return rc;
+    if (batch > s->max_batch) return fail(QS_ERR_INVALID, "batch %d > max_batch %d", batch, s->max_batch);
+    DeviceGuard dg(s->device);
+    rc = tail_workspace(s, hidden_dim);
+    if (rc) return rc;
     // batches below kWideMinRows: the epilogue forms the segment maxima and
     // the sampler's scan reads only the window's segments from the logits
     uint32_t* segk = batch < kWideMinRows ? s->lh_segk : nullptr;
@@ -1004,6 +1021,117 @@ int qs_lm_head_sample(qs_sampler* s, const void* d_hidden, const void* d_norm_we
     if (rc && segk)  // the scan did not consume (and zero) the maxima
         cudaMemsetAsync(segk, 0, sizeof(uint32_t) * (size_t)batch * s->lh_segs, (cudaStream_t)stream);
     return rc;
+}
+
+// ---- the decode tail with 4-bit weights (no counterpart in the reference)
+static int w4_shape(int vocab, int hidden_dim, int group, int scale_dtype) {
+    if (vocab < 1 || vocab > kMaxVocab)
+        return fail(QS_ERR_UNSUPPORTED, "vocab %d outside [1, %d]", vocab, kMaxVocab);
+    if (hidden_dim < 64 || hidden_dim % 64 != 0 || hidden_dim > kW4MaxHidden)
+        return fail(QS_ERR_UNSUPPORTED, "hidden_dim %d is not a multiple of 64 up to %d", hidden_dim, kW4MaxHidden);
+    if (group != 32 && group != 64 && group != 128)
+        return fail(QS_ERR_UNSUPPORTED, "group %d is not 32, 64 or 128", group);
+    if (hidden_dim % group != 0)
+        return fail(QS_ERR_UNSUPPORTED, "hidden_dim %d is not a multiple of group %d", hidden_dim, group);
+    if (scale_dtype != QS_BF16 && scale_dtype != QS_F16)
+        return fail(QS_ERR_INVALID, "scale dtype %d is not QS_BF16 or QS_F16", scale_dtype);
+    return QS_OK;
+}
+
+static int w4_weight(const qs_w4_weight* w) {
+    if (!w) return fail(QS_ERR_INVALID, "weight is NULL");
+    const int rc = w4_shape(w->vocab, w->hidden_dim, w->group, w->scale_dtype);
+    if (rc) return rc;
+    if (!w->d_codes || !w->d_scales) return fail(QS_ERR_INVALID, "NULL device pointer");
+    if ((((uintptr_t)w->d_codes) | ((uintptr_t)w->d_scales) | ((uintptr_t)w->d_zeros)) & 15)
+        return fail(QS_ERR_INVALID, "codes, scales and zero points must be 16-byte aligned");
+    return QS_OK;
+}
+
+static int w4_launch(const void* d_hidden, const void* d_norm_weight, const qs_w4_weight* w, int batch,
+                     __nv_bfloat16* normed, __nv_bfloat16* logits, int num_sms, cudaStream_t st,
+                     uint32_t* segk = nullptr, int segk_stride = 0) {
+    if (batch == 0) return QS_OK;
+    CK(launch_rmsnorm((const __nv_bfloat16*)d_hidden, (const __nv_bfloat16*)d_norm_weight, normed, batch,
+                      w->hidden_dim, st));
+    const W4View v{(const unsigned char*)w->d_codes, w->d_scales, (const unsigned char*)w->d_zeros,
+                   w->vocab, w->hidden_dim, w->group, w->scale_dtype};
+    CK(launch_lm_head_w4(normed, v, logits, batch, num_sms, segk, segk_stride, st));
+    return QS_OK;
+}
+
+size_t qs_w4_codes_bytes(int vocab, int hidden_dim) { return w4_codes_bytes(vocab, hidden_dim); }
+size_t qs_w4_scales_bytes(int vocab, int hidden_dim, int group) { return w4_scales_bytes(vocab, hidden_dim, group); }
+size_t qs_w4_zeros_bytes(int vocab, int hidden_dim, int group) { return w4_zeros_bytes(vocab, hidden_dim, group); }
+
+int qs_w4_quantize(const void* d_weight, int vocab, int hidden_dim, int group, void* d_plain_codes,
+                   void* d_plain_scales, void* d_plain_zeros, void* stream) {
+    g_err.clear();
+    const int rc = w4_shape(vocab, hidden_dim, group, QS_BF16);
+    if (rc) return rc;
+    if (!d_weight || !d_plain_codes || !d_plain_scales || !d_plain_zeros)
+        return fail(QS_ERR_INVALID, "NULL device pointer");
+    if ((((uintptr_t)d_weight) | ((uintptr_t)d_plain_scales)) & 1)
+        return fail(QS_ERR_INVALID, "weight and scales must be aligned to their element");
+    CK(launch_w4_quantize((const __nv_bfloat16*)d_weight, vocab, hidden_dim, group, (unsigned char*)d_plain_codes,
+                          (__nv_bfloat16*)d_plain_scales, (unsigned char*)d_plain_zeros, (cudaStream_t)stream));
+    return QS_OK;
+}
+
+int qs_w4_pack(const void* d_plain_codes, const void* d_plain_scales, const void* d_plain_zeros, int vocab,
+               int hidden_dim, int group, int scale_dtype, void* d_codes, void* d_scales, void* d_zeros,
+               void* stream) {
+    g_err.clear();
+    const int rc = w4_shape(vocab, hidden_dim, group, scale_dtype);
+    if (rc) return rc;
+    if (!d_plain_codes || !d_plain_scales || !d_codes || !d_scales || (d_plain_zeros && !d_zeros))
+        return fail(QS_ERR_INVALID, "NULL device pointer");
+    if (((uintptr_t)d_plain_scales) & 1) return fail(QS_ERR_INVALID, "scales must be aligned to their element");
+    if ((((uintptr_t)d_codes) | ((uintptr_t)d_scales) | ((uintptr_t)d_zeros)) & 15)
+        return fail(QS_ERR_INVALID, "the packed buffers must be 16-byte aligned");
+    CK(launch_w4_pack((const unsigned char*)d_plain_codes, d_plain_scales, (const unsigned char*)d_plain_zeros, vocab,
+                      hidden_dim, group, (unsigned char*)d_codes, d_scales, (unsigned char*)d_zeros,
+                      (cudaStream_t)stream));
+    return QS_OK;
+}
+
+int qs_lm_head_w4(const void* d_hidden, const void* d_norm_weight, const qs_w4_weight* weight, int batch,
+                  void* d_normed, void* d_logits, void* stream) {
+    g_err.clear();
+    int rc = w4_weight(weight);
+    if (rc) return rc;
+    rc = lm_head_args(d_hidden, weight->d_codes, batch, weight->hidden_dim, weight->vocab);
+    if (rc) return rc;
+    if (!d_normed || !d_logits) return fail(QS_ERR_INVALID, "NULL output buffer");
+    if ((((uintptr_t)d_normed) | ((uintptr_t)d_logits)) & 15)
+        return fail(QS_ERR_INVALID, "normed and logits must be 16-byte aligned");
+    if (((uintptr_t)d_norm_weight) & 3) return fail(QS_ERR_INVALID, "norm_weight must be 4-byte aligned");
+    int dev = 0, sms = 148;
+    CK(cudaGetDevice(&dev));
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1) sms = 148;
+    return w4_launch(d_hidden, d_norm_weight, weight, batch, (__nv_bfloat16*)d_normed, (__nv_bfloat16*)d_logits, sms,
+                     (cudaStream_t)stream);
+}
+
+int qs_lm_head_w4_sample(qs_sampler* s, const void* d_hidden, const void* d_norm_weight,
+                         const qs_w4_weight* weight, int batch, int* d_tokens, void* stream, unsigned flags) {
+    g_err.clear();
+    if (!s) return fail(QS_ERR_INVALID, "sampler is NULL");
+    int rc = w4_weight(weight);
+    if (rc) return rc;
+    if (weight->vocab != s->vocab)
+        return fail(QS_ERR_INVALID, "weight has %d vocabulary rows, the sampler %d", weight->vocab, s->vocab);
+    rc = lm_head_args(d_hidden, weight->d_codes, batch, weight->hidden_dim, s->vocab);
+    if (rc) return rc;
+    if (((uintptr_t)d_norm_weight) & 3) return fail(QS_ERR_INVALID, "norm_weight must be 4-byte aligned");
+    if (batch > s->max_batch) return fail(QS_ERR_INVALID, "batch %d > max_batch %d", batch, s->max_batch);
+    DeviceGuard dg(s->device);
+    rc = tail_workspace(s, weight->hidden_dim);
+    if (rc) return rc;
+    rc = w4_launch(d_hidden, d_norm_weight, weight, batch, s->lh_normed, s->lh_logits, s->num_sms,
+                   (cudaStream_t)stream);
+    if (rc) return rc;
+    return sample_stateful(s, s->lh_logits, QS_BF16, batch, d_tokens, stream, flags, nullptr, 0);
 }
 
 int qs_lm_head_logits(qs_sampler* s, const void** d_logits) {

@@ -234,8 +234,11 @@ class Sampler:
                        stream=None):
         """Final RMSNorm + lm_head + stateful sample() for the rows of
         ``hidden`` (bf16 [B, hidden_dim] device tensor; ``weight`` bf16
-        [vocab, hidden_dim]); returns int32 tokens [B] on the device."""
+        [vocab, hidden_dim], or a ``w4.W4Weight``); returns int32 tokens [B] on
+        the device."""
         torch = _torch()
+        if hasattr(weight, "_w4_desc"):
+            return self._lm_head_w4_sample(hidden, weight, norm_weight, out, flags, stream)
         h = hidden if hidden.dim() == 2 else hidden.view(1, -1)
         for t in (h, weight) + ((norm_weight,) if norm_weight is not None else ()):
             if not t.is_cuda or not t.is_contiguous() or t.dtype != torch.bfloat16:
@@ -247,6 +250,24 @@ class Sampler:
         check(_lib.lib.qs_lm_head_sample(self._h, _ptr(h), _ptr(norm_weight), _ptr(weight), B,
                                          int(h.shape[1]), _ptr(out), _stream_handle(stream),
                                          int(flags)))
+        return out
+
+    def _lm_head_w4_sample(self, hidden, weight, norm_weight, out, flags: int, stream):
+        torch = _torch()
+        from .losses import _Launch
+        from .w4 import _check_rows
+        h = _check_rows(hidden, weight, norm_weight)
+        B = int(h.shape[0])
+        if out is not None and (out.dtype != torch.int32 or not out.is_contiguous() or out.numel() < B
+                                or out.device != weight.device):
+            raise SamplerError(_lib.QS_ERR_INVALID, f"out must be a contiguous int32 tensor [{B}] on {weight.device}")
+        if weight.device.index != self.device:
+            raise SamplerError(_lib.QS_ERR_INVALID, f"weight on {weight.device}, the sampler on cuda:{self.device}")
+        with _Launch(weight.device, stream, h, norm_weight, weight.codes, weight.scales, weight.zeros, out) as st:
+            if out is None:
+                out = torch.empty(B, dtype=torch.int32, device=h.device)
+            check(_lib.lib.qs_lm_head_w4_sample(self._h, _ptr(h), _ptr(norm_weight), C.byref(weight._w4_desc), B,
+                                                _ptr(out), st, int(flags)))
         return out
 
     def lm_head_logits(self, batch: int):

@@ -1,0 +1,277 @@
+"""The lm_head with 4-bit weights against its formula in 64 bits.
+
+Tolerance of a logit: a product of a code minus its zero point (an integer
+below 16) and a bf16 value is exact in fp32; each of the K additions and each
+group's scaling may lose a whole step of fp32 (tensor-core sums may truncate),
+2^-23 of the sum of magnitudes; the output is rounded to bf16, 2^-8 of its
+value at most."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+
+
+def plain_weight(V, K, group, zeros, scale, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    q = torch.randint(0, 16, (V, K), generator=g, device="cuda", dtype=torch.uint8)
+    codes = q[:, 0::2] | (q[:, 1::2] << 4)
+    scales = (0.001 + 0.02 * torch.rand((V, K // group), generator=g, device="cuda")).to(scale)
+    scales *= (torch.rand((V, K // group), generator=g, device="cuda") < 0.9).to(scale) * 2 - 1  # some negative
+    z = torch.randint(0, 16, (V, K // group), generator=g, device="cuda", dtype=torch.uint8) if zeros else None
+    return codes.contiguous(), scales, z, g
+
+
+def dense(codes, scales, zeros):
+    """The weight in 64 bits."""
+    V, K = codes.shape[0], 2 * codes.shape[1]
+    q = torch.stack([codes & 15, codes >> 4], dim=2).view(V, scales.shape[1], -1).double()
+    z = 8.0 if zeros is None else zeros.double()[:, :, None]
+    return ((q - z) * scales.double()[:, :, None]).view(V, K)
+
+
+def check_logits(normed, w, logits):
+    K = w.shape[1]
+    for a in range(0, w.shape[0], 1 << 15):
+        b = w[a:a + (1 << 15)]
+        ref = normed.double() @ b.t()
+        tol = 2.0 ** -8 * ref.abs() + (K + 8) * 2.0 ** -23 * (normed.double().abs() @ b.abs().t()) * 1.01 + 1e-38
+        off = (logits[:, a:a + (1 << 15)].double() - ref).abs()
+        assert (off <= tol).all(), f"off by {float((off / tol).max()):.3g} tolerances"
+
+
+def inputs(g, B, K):
+    h = torch.randn((B, K), generator=g, device="cuda").to(torch.bfloat16)
+    nw = (1.0 + 0.1 * torch.randn((K,), generator=g, device="cuda")).to(torch.bfloat16)
+    return h, nw
+
+
+@pytest.mark.parametrize("B,V,K,group", [
+    (1, 1, 64, 32), (1, 151936, 1024, 128), (1, 1003, 1024, 64), (2, 16, 128, 128), (3, 17, 192, 64), (5, 4099, 320, 32),
+    (7, 33, 8192, 128), (8, 1000, 1024, 32), (9, 1000, 1024, 128), (16, 32003, 4096, 64), (17, 257, 2048, 128),
+    (31, 75968, 1024, 128), (32, 5000, 1024, 32), (33, 2500, 4096, 128), (70, 1003, 1024, 64), (130, 300, 256, 128)])
+@pytest.mark.parametrize("zeros,scale", [(False, torch.bfloat16), (True, torch.float16)])
+def test_lm_head_w4(B, V, K, group, zeros, scale):
+    from qwen600_engine_b200.sampler import lm_head
+    from qwen600_engine_b200.w4 import W4Weight, lm_head_w4
+    codes, scales, z, g = plain_weight(V, K, group, zeros, scale, seed=V + K)
+    w = W4Weight.pack(codes, scales, z)
+    assert (w.vocab, w.hidden_dim, w.group) == (V, K, group)
+    h, nw = inputs(g, B, K)
+    normed, logits = lm_head_w4(h, w, nw)
+    assert normed.shape == (B, K) and logits.shape == (B, V) and logits.dtype == torch.bfloat16
+    assert torch.equal(normed, lm_head(h, torch.zeros((8, K), dtype=torch.bfloat16, device="cuda"), nw)[0])
+    check_logits(normed, dense(codes, scales, z), logits)
+    plain = lm_head_w4(h, w)[0]  # no norm weight: ones
+    assert torch.equal(plain, lm_head(h, torch.zeros((8, K), dtype=torch.bfloat16, device="cuda"))[0])
+
+
+def test_every_code_at_every_place():
+    """One weight column at a time: each code and zero point reaches its own product, at full precision."""
+    from qwen600_engine_b200.w4 import W4Weight, lm_head_w4
+    for group in (32, 64, 128):
+        K, V = 256, 256
+        g = torch.Generator(device="cuda")
+        g.manual_seed(group)
+        q = torch.randint(0, 16, (V, K), generator=g, device="cuda", dtype=torch.uint8)
+        codes = (q[:, 0::2] | (q[:, 1::2] << 4)).contiguous()
+        scales = torch.full((V, K // group), 0.5, dtype=torch.bfloat16, device="cuda")
+        scales *= 2.0 ** torch.randint(-3, 4, scales.shape, generator=g, device="cuda").to(torch.bfloat16)
+        z = torch.randint(0, 16, (V, K // group), generator=g, device="cuda", dtype=torch.uint8)
+        w = W4Weight.pack(codes, scales, z)
+        h = torch.eye(K, device="cuda").to(torch.bfloat16)  # row k picks column k, scaled by the norm to 16
+        normed, logits = lm_head_w4(h, w)
+        ref = normed.double() @ dense(codes, scales, z).t()
+        assert torch.equal(logits.double(), ref.to(torch.bfloat16).double())
+
+
+def test_one_row_does_not_depend_on_the_batch():
+    """The rows of a batch are independent: values that are not numbers in one leave the others as they are."""
+    from qwen600_engine_b200.w4 import W4Weight, lm_head_w4
+    codes, scales, z, g = plain_weight(3001, 1024, 64, True, torch.bfloat16, seed=5)
+    w = W4Weight.pack(codes, scales, z)
+    h, nw = inputs(g, 13, 1024)
+    a = lm_head_w4(h, w, nw)[1]
+    h[4] = float("nan")
+    h[7, 3] = float("inf")
+    b = lm_head_w4(h, w, nw)[1]
+    keep = [r for r in range(13) if r not in (4, 7)]
+    assert torch.equal(a[keep], b[keep])
+    assert torch.isnan(b[[4, 7]]).all()
+
+
+def test_quantize():
+    from qwen600_engine_b200.w4 import W4Weight, lm_head_w4, quantize_w4
+    g = torch.Generator(device="cuda")
+    g.manual_seed(9)
+    V, K = 1003, 512
+    wt = (0.02 * torch.randn((V, K), generator=g, device="cuda")).to(torch.bfloat16)
+    wt[5] = 0.0
+    wt[6, :128] = 0.25      # one sign only: the range holds zero too
+    wt[7, :128] = -0.25
+    for group in (32, 64, 128):
+        codes, scales, z = quantize_w4(wt, group)
+        d = dense(codes, scales, z)
+        x = wt.double().view(V, -1, group)
+        lo, hi = x.amin(2).clamp(max=0), x.amax(2).clamp(min=0)
+        assert torch.equal(scales, ((hi - lo).float() / 15).to(torch.bfloat16))
+        # half a step, and what rounding the scale (2^-8 of 15 steps) and the zero point to whole numbers takes from the ends
+        step = scales.double()[:, :, None]
+        off = (d.view(V, -1, group) - x).abs()
+        assert (off <= step * (0.5 + 0.5 + 15 * 2.0 ** -8 + 1e-6)).all()
+        inner = (x > lo[:, :, None] + 1.1 * step) & (x < hi[:, :, None] - 1.1 * step)
+        assert (off[inner] <= (0.5 + 1e-4) * step.expand_as(off)[inner]).all()
+        assert (d[5] == 0).all()
+    h, nw = inputs(g, 4, K)
+    codes, scales, z = quantize_w4(wt, 128)
+    normed, logits = lm_head_w4(h, W4Weight.quantize(wt, 128), nw)
+    check_logits(normed, dense(codes, scales, z), logits)
+
+
+@pytest.mark.parametrize("B,V,params", [
+    (1, 151936, (0.6, 0.95, 0.05, 20, 1.1, 0.5, 0.3)), (8, 50021, (0.8, 0.9, 0.0, 0, 1.2, 0.0, 0.0)),
+    (40, 4096, (0.0, 1.0, 0.0, 0, 1.3, 0.0, 0.2)), (5, 1003, (0.7, 0.95, 0.1, 50, 1.15, 0.0, 0.0)),
+    (300, 1000, (0.7, 0.95, 0.1, 50, 1.15, 0.0, 0.0))])
+def test_sample_from_4_bit_weights(B, V, params):
+    """lm_head_sample with such a weight draws what sample() draws from lm_head_w4's logits, step after step."""
+    from qwen600_engine_b200.sampler import Sampler
+    from qwen600_engine_b200.w4 import W4Weight, lm_head_w4
+    codes, scales, z, g = plain_weight(V, 1024, 64, True, torch.bfloat16, seed=V)
+    w = W4Weight.pack(codes, scales, z)
+    T, topp, minp, k, rp, fp, pp = params
+    fused, apart = (Sampler(T, topp, minp, k, rp, fp, pp, 64, 7, max_batch=B, vocab=V) for _ in range(2))
+    for step in range(4):
+        h, nw = inputs(g, B, 1024)
+        tok = fused.lm_head_sample(h, w, nw)
+        logits = lm_head_w4(h, w, nw)[1]
+        assert torch.equal(fused.lm_head_logits(B), logits)
+        want = apart.sample(logits)
+        torch.cuda.synchronize()
+        np.testing.assert_array_equal(tok.cpu().numpy(), want.cpu().numpy(), err_msg=f"step {step}")
+    np.testing.assert_array_equal(fused.rng_state, apart.rng_state)
+    # the same handle goes on with a bf16 weight
+    wt = (0.02 * torch.randn((V, 1024), generator=g, device="cuda")).to(torch.bfloat16)
+    tok = fused.lm_head_sample(h, wt, nw)
+    want = apart.sample(fused.lm_head_logits(B).clone())
+    assert torch.equal(tok, want)
+    fused.free()
+    apart.free()
+
+
+def test_streams_and_graphs():
+    from qwen600_engine_b200.w4 import W4Weight, lm_head_w4
+    codes, scales, z, g = plain_weight(50021, 1024, 128, False, torch.bfloat16, seed=3)
+    w = W4Weight.pack(codes, scales, z)
+    rows = [inputs(g, b, 1024) for b in (1, 6)]
+    want = [lm_head_w4(h, w, nw) for h, nw in rows]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        got = [lm_head_w4(h, w, nw, stream=s) for (h, nw), s in zip(rows, streams)]
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    graphs, outs = [], []
+    for h, nw in rows:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(lm_head_w4(h, w, nw))
+        graphs.append(gr)
+    for h, nw in rows:
+        h.copy_(h.flip(1))
+    want = [lm_head_w4(h, w, nw) for h, nw in rows]
+    torch.cuda.synchronize()
+    for gr, s in zip(graphs, streams):
+        with torch.cuda.stream(s):
+            gr.replay()
+            gr.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(outs, want):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    for gr in graphs:
+        gr.reset()
+
+
+def test_refused_on_the_gpu():
+    from qwen600_engine_b200._lib import SamplerError
+    from qwen600_engine_b200.sampler import Sampler
+    from qwen600_engine_b200.w4 import W4Weight, lm_head_w4
+    codes, scales, z, g = plain_weight(1000, 1024, 64, True, torch.bfloat16, seed=1)
+    w = W4Weight.pack(codes, scales, z)
+    h, nw = inputs(g, 2, 1024)
+    with pytest.raises(SamplerError, match="columns"):
+        lm_head_w4(h[:, :512].contiguous(), w)
+    with pytest.raises(SamplerError, match="bf16"):
+        lm_head_w4(h.float(), w)
+    with pytest.raises(SamplerError, match="norm_weight has"):
+        lm_head_w4(h, w, nw[:64].contiguous())
+    with pytest.raises(SamplerError, match="group"):
+        W4Weight.pack(codes, scales[:, :1].contiguous())
+    assert lm_head_w4(h[:0], w)[1].shape == (0, 1000)
+    s = Sampler(max_batch=1, vocab=1000)
+    with pytest.raises(SamplerError, match="max_batch"):
+        s.lm_head_sample(h, w, nw)
+    s.free()
+    s = Sampler(max_batch=2, vocab=999)
+    with pytest.raises(SamplerError, match="vocabulary rows"):
+        s.lm_head_sample(h, w, nw)
+    s.free()
+
+
+def test_rollout_and_learning_step():
+    """The operators together: the 4-bit tail answers, its tokens are scored, and the losses over them take a step on
+    the bf16 logits of the same rows; gradients against the formula."""
+    from qwen600_engine_b200 import losses
+    from qwen600_engine_b200.sampler import Sampler, lm_head
+    from qwen600_engine_b200.w4 import W4Weight
+    g = torch.Generator(device="cuda")
+    g.manual_seed(77)
+    B, V, K, steps = 6, 5003, 256, 4
+    wt = (0.05 * torch.randn((V, K), generator=g, device="cuda")).to(torch.bfloat16)
+    w = W4Weight.quantize(wt, 64)
+    nw = torch.ones(K, dtype=torch.bfloat16, device="cuda")
+    s = Sampler(1.0, 1.0, 0.0, 0, 1.0, 0.0, 0.0, 0, 5, max_batch=B, vocab=V)
+    hs, toks, old = [], [], []
+    for _ in range(steps):
+        h = torch.randn((B, K), generator=g, device="cuda").to(torch.bfloat16)
+        t = s.lm_head_sample(h, w, nw)
+        old.append(losses.token_logprobs(s.lm_head_logits(B), t).logprobs)
+        hs.append(h)
+        toks.append(t)
+    s.free()
+    h = torch.stack(hs, 1).view(B * steps, K)           # sequence by sequence
+    tok = torch.stack(toks, 1).reshape(-1).contiguous()
+    old = torch.stack(old, 1).reshape(-1).contiguous()
+    assert (old < 0).all() and torch.isfinite(old).all()
+    logits = lm_head(h, wt, nw)[1]                      # the learner's weights are not rounded
+    ref = losses.token_logprobs(logits, tok).logprobs
+    adv = torch.randn((B * steps,), generator=g, device="cuda")
+    r = losses.policy_loss(logits, tok, old, adv, ref_logprobs=ref, kl_coef=0.1)
+    assert torch.equal(r.logprobs, ref)                 # the same rows score the same bits
+    x = logits.double().requires_grad_(True)
+    lp = torch.log_softmax(x, 1).gather(1, tok.long()[:, None])[:, 0]
+    ratio = (lp - old.double()).exp()
+    d = ref.double() - lp
+    border = (((ratio - 0.8).abs() < 1e-4) | ((ratio - 1.2).abs() < 1e-4)).any()
+    assert not border
+    l = -torch.minimum(ratio * adv, ratio.clamp(0.8, 1.2) * adv) + 0.1 * (d.exp() - d - 1)
+    l.mean().backward()
+    assert abs(float(r.loss) - float(l.mean())) < 1e-5
+    # bf16 half a step, and log-probabilities good to 1e-5 in the coefficients
+    off = (r.grad.double() - x.grad).abs()
+    assert (off <= 2.0 ** -8 * x.grad.abs() + 2e-5 * adv.abs().max() / (B * steps)).all()
+    offsets = torch.arange(0, B * steps + 1, steps, dtype=torch.int32, device="cuda")
+    seq_ref = ref.view(B, steps).sum(1)
+    p = losses.preference_loss(logits, tok, offsets, seq_ref, beta=0.2)
+    assert abs(float(p.loss) - float(np.log(2.0))) < 1e-5  # the model is its own reference
+    y = logits.double().requires_grad_(True)
+    sl = torch.log_softmax(y, 1).gather(1, tok.long()[:, None])[:, 0].view(B, steps).sum(1) - seq_ref.double()
+    (-torch.nn.functional.logsigmoid(0.2 * (sl[:3] - sl[3:]))).mean().backward()
+    assert ((p.grad.double() - y.grad).abs() <= 2.0 ** -8 * y.grad.abs() + 1e-6).all()
