@@ -14,14 +14,14 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <type_traits>
+
 #include "qs_common.cuh"
 #include "qwen600_sampler.h"
 
 namespace qs {
 
 int set_error(int code, const char* msg);  // qs_api.cu
-
-constexpr int kLossThreads = 256;
 
 // What a scored row leaves for the losses and the gradient.
 struct RowScore {
@@ -55,92 +55,123 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
     return s;
 }
 
+// Vectors of 16 bytes of a row, at any alignment of its first element: up to
+// kN - 1 elements before the first aligned vector (head), whole vectors, up to
+// kN - 1 elements behind the last (tail).
 template <typename T>
-__global__ void __launch_bounds__(kLossThreads)
-score_rows_kernel(const T* __restrict__ logits, int V, long long ld, const int* __restrict__ tokens,
-                  const float* __restrict__ weights, double inv_t, RowScore* __restrict__ out,
-                  float* __restrict__ logprobs, float* __restrict__ stats) {
-    __shared__ float redf[32];
-    __shared__ double redd[32];
-    const int row = blockIdx.x, t = threadIdx.x;
-    const int tok = tokens[row];
-    const bool scored = tok >= 0 && tok < V && !(weights && weights[row] == 0.0f);
-    RowScore r{0.0, 0.0f, 0.0f, 0, 0};
-    if (scored) {
-        const T* x = logits + (size_t)row * ld;
-        float m = -INFINITY;
-        for (int j = t; j < V; j += kLossThreads) m = fmaxf(m, elem(x, j));
-        m = warp_max(m);
-        if ((t & 31) == 0) redf[t >> 5] = m;
-        __syncthreads();
-        m = redf[0];
-        for (int w = 1; w < kLossThreads / 32; w++) m = fmaxf(m, redf[w]);
-        const float scale = (float)(inv_t * 1.4426950408889634);
-        float s = 0.0f;
-        int n = 0;
-        for (int j = t; j < V; j += kLossThreads) {
-            const float d = elem(x, j) - m;
-            if (d == 0.0f) n++;
-            else s += exp2_fast(d * scale);
-        }
-        const double others = block_sum((double)s, redd);
-        const double at_max = block_sum((double)n, redd);
-        r.scored = 1;
-        r.max = m;
-        const double excess = isinf(m) ? (double)NAN : others + (at_max - 1.0);
-        r.excess = (float)excess;
-        r.logprob = ((double)elem(x, tok) - (double)m) * inv_t - log1p(excess);
+struct RowShape {
+    static constexpr int kN = 16 / (int)sizeof(T);
+    int head, vecs, tail;
+    __device__ __forceinline__ RowShape(const T* row, int V) {
+        head = min(V, (int)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T)));
+        vecs = (V - head) / kN;
+        tail = V - head - vecs * kN;
     }
-    if (t == 0) {
-        if (out) out[row] = r;
-        if (logprobs) logprobs[row] = (float)r.logprob;
-        if (stats) {
-            stats[2 * (size_t)row] = r.max;
-            stats[2 * (size_t)row + 1] = r.excess;
-        }
+    // The element outside the vectors that thread t of a row's first CTA takes, or -1.
+    __device__ __forceinline__ int edge(int t, int V) const {
+        return t < head ? t : t >= 8 && t < 8 + tail ? V - tail + t - 8 : -1;
     }
+};
+
+// Plain (coherent) loads that do not stay in L1: the same kernel may write the
+// gradient over the logits, so the read-only path is not used.
+__device__ __forceinline__ uint4 load16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ void store16(void* p, const uint4& v) {
+    asm volatile("st.global.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                 : "memory");
 }
 
-// grad = coef * ([j = t] - p_j) / T for one row per CTA.
+// 16 bytes of logits as floats and back.
 template <typename T>
-__global__ void __launch_bounds__(kLossThreads)
-grad_rows_kernel(const T* logits, int V, long long ld, const int* __restrict__ tokens,
-                 const float* __restrict__ stats, int stat_words, const float* __restrict__ coefs,
-                 double inv_t, T* grad, long long gld) {
-    const int row = blockIdx.x, t = threadIdx.x;
-    const int tok = tokens[row];
-    const float coef = coefs[row];
-    const T* x = logits + (size_t)row * ld;
-    T* g = grad + (size_t)row * gld;
-    if (tok < 0 || tok >= V || coef == 0.0f) {
-        for (int j = t; j < V; j += kLossThreads) put(g, j, 0.0f);
-        return;
+struct Pack;
+template <>
+struct Pack<float> {
+    static constexpr int kN = 4;
+    __device__ __forceinline__ static uint4 lowest() {
+        return make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u);
     }
-    const float* st = reinterpret_cast<const float*>(reinterpret_cast<const char*>(stats) + (size_t)row * stat_words * 4);
-    const float m = st[0];
-    const double excess = st[1];
-    const float scale = (float)(inv_t * 1.4426950408889634);
-    const double c = (double)coef * inv_t;
-    const float f = (float)(-c / (1.0 + excess));
-    for (int j = t; j < V; j += kLossThreads) {
-        const float v = elem(x, j);
-        if (j == tok) {
-            // 1 - p without cancellation where the token is the maximum
-            const double q = v == m ? excess / (1.0 + excess) : 1.0 - exp(((double)v - (double)m) * inv_t) / (1.0 + excess);
-            put(g, j, (float)(c * q));
-        } else {
-            put(g, j, f * exp2_fast((v - m) * scale));
+    __device__ __forceinline__ static void widen(const uint4& v, float* o) {
+        o[0] = __uint_as_float(v.x); o[1] = __uint_as_float(v.y);
+        o[2] = __uint_as_float(v.z); o[3] = __uint_as_float(v.w);
+    }
+    __device__ __forceinline__ static uint4 narrow(const float* o) {
+        return make_uint4(__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3]));
+    }
+    __device__ __forceinline__ static uint32_t max2(uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }
+};
+template <>
+struct Pack<__nv_bfloat16> {
+    static constexpr int kN = 8;
+    __device__ __forceinline__ static uint4 lowest() {
+        return make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u);
+    }
+    __device__ __forceinline__ static void widen(const uint4& v, float* o) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            o[2 * i] = __uint_as_float(w[i] << 16);
+            o[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
         }
     }
+    __device__ __forceinline__ static uint4 narrow(const float* o) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __device__ __forceinline__ static uint32_t max2(uint32_t a, uint32_t b) {
+        const __nv_bfloat162 h = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                         *reinterpret_cast<const __nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+};
+
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// One CTA's part of a row: its maximum, how many elements equal it, and the
+// sum of the others' exponentials against it.
+struct __align__(16) Part {
+    float max;
+    int at_max;
+    double others;
+};
+
+// Writes p to *slot of the cluster's CTA `rank`.
+__device__ __forceinline__ void push_part(Part* slot, int rank, const Part& p) {
+    uint32_t addr;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                 : "=r"(addr)
+                 : "r"((uint32_t)__cvta_generic_to_shared(slot)), "r"(rank));
+    const unsigned long long o = (unsigned long long)__double_as_longlong(p.others);
+    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(__float_as_uint(p.max)),
+                 "r"((uint32_t)p.at_max), "r"((uint32_t)o), "r"((uint32_t)(o >> 32))
+                 : "memory");
 }
 
 // Per-row term of the policy loss: returns l, and its slope dl / dlogprob.
 __device__ __forceinline__ double policy_term(double lp, double old_lp, double ref_lp, double adv, double lo,
                                               double hi, double kl, double* slope) {
     const double r = exp(lp - old_lp);
-    const double clipped = r < lo ? lo : r > hi ? hi : r;
     const bool cut = (adv > 0.0 && r > hi) || (adv < 0.0 && r < lo);
-    double l = -(cut ? clipped : r) * adv;
+    double l = -(cut ? (r > hi ? hi : lo) : r) * adv;
     double sl = cut ? 0.0 : -adv * r;
     if (kl > 0.0) {
         const double d = ref_lp - lp;
@@ -152,24 +183,311 @@ __device__ __forceinline__ double policy_term(double lp, double old_lp, double r
     return l;
 }
 
-__global__ void __launch_bounds__(1024)
-policy_rows_kernel(const RowScore* __restrict__ score, int rows, const float* __restrict__ old_lp,
-                   const float* __restrict__ ref_lp, const float* __restrict__ adv,
-                   const float* __restrict__ weights, qs_policy_params p, float* __restrict__ coefs,
-                   float* __restrict__ loss) {
-    __shared__ double red[32];
-    double sum = 0.0;
-    for (int i = threadIdx.x; i < rows; i += blockDim.x) {
-        double c = 0.0;
-        if (score[i].scored) {
-            const double w = weights ? (double)weights[i] : 1.0 / rows;
-            double slope;
-            sum += w * policy_term(score[i].logprob, old_lp[i], p.kl_coef > 0.0 ? (double)ref_lp[i] : 0.0, adv[i],
-                                   1.0 - p.clip_low, 1.0 + p.clip_high, p.kl_coef, &slope);
-            c = w * slope;
+// 1 - p of the target xt, without cancellation where it is the maximum.
+__device__ __forceinline__ double beyond(float xt, float max, double excess, double inv_t) {
+    return xt == max ? excess / (1.0 + excess) : 1.0 - exp(((double)xt - (double)max) * inv_t) / (1.0 + excess);
+}
+
+template <typename T>
+struct ScoreArgs {
+    const T* logits;
+    int rows, V;
+    long long ld;
+    const int* tokens;
+    float scale;  // log2(e) / T
+    double inv_t;
+    int log_c;    // 1 << log_c CTAs per row, one cluster
+    RowScore* out;
+    float* logprobs;
+    float* stats;
+    // the policy loss
+    const float* weights;
+    const float* old_lp;
+    const float* ref_lp;
+    const float* adv;
+    qs_policy_params p;
+    double* row_loss;
+    T* grad;
+    long long gld;
+};
+
+// Scores one row per cluster of 1 to 8 CTAs; with kPolicy it also forms the
+// row's policy loss and writes its gradient.  Each CTA takes a contiguous
+// share of the row's 16-byte vectors into registers, all its loads in flight
+// at once.  So the row is read once, its maximum is known before the first
+// exponential (no sum is rescaled), and the gradient is formed from the same
+// registers.  The CTAs exchange their parts, 16 bytes each, through
+// distributed shared memory.
+template <typename T, int kThr, int kVpt, bool kPolicy>
+__global__ void __launch_bounds__(kThr)
+score_kernel(const __grid_constant__ ScoreArgs<T> a) {
+    constexpr int kN = Pack<T>::kN;
+    constexpr int kW = kThr / 32;
+    __shared__ Part parts[8];
+    __shared__ float red_max[kW], red_sum[kW];
+    __shared__ int red_n[kW];
+    __shared__ float factor_s, max_s, target_s;
+    const int t = threadIdx.x, C = 1 << a.log_c;
+    const int row = blockIdx.x >> a.log_c, rank = blockIdx.x & (C - 1);
+    const int tok = a.tokens[row];
+    const bool scored = tok >= 0 && tok < a.V && !(kPolicy && a.weights && a.weights[row] == 0.0f);
+    const T* x = a.logits + (size_t)row * a.ld;
+    T* g = kPolicy && a.grad ? a.grad + (size_t)row * a.gld : nullptr;
+    dependents_may_start();
+    if (!scored) {  // alike for the whole cluster
+        if (rank == 0 && t == 0) {
+            if (a.out) a.out[row] = RowScore{0.0, 0.0f, 0.0f, 0, 0};
+            if (a.logprobs) a.logprobs[row] = 0.0f;
+            if (a.stats) a.stats[2 * (size_t)row] = a.stats[2 * (size_t)row + 1] = 0.0f;
+            if (kPolicy) a.row_loss[row] = 0.0;
         }
-        coefs[i] = (float)c;
+        if (kPolicy && g) {
+            const RowShape<T> gs(g, a.V);
+            for (int i = rank * kThr + t; i < gs.vecs; i += C * kThr)
+                store16(g + gs.head + (size_t)i * kN, make_uint4(0u, 0u, 0u, 0u));
+            const int e = rank == 0 ? gs.edge(t, a.V) : -1;
+            if (e >= 0) put(g, e, 0.0f);
+        }
+        return;
     }
+    if (C > 1) cluster_arrive_relaxed();  // waited for before the first store into another CTA
+
+    const RowShape<T> sh(x, a.V);
+    const int per = (sh.vecs + C - 1) >> a.log_c;
+    const int base = min(rank * per, sh.vecs), end = min(base + per, sh.vecs);
+    const T* body = x + sh.head;
+    uint4 v[kVpt];
+#pragma unroll
+    for (int i = 0; i < kVpt; i++) {
+        const int k = base + i * kThr + t;
+        v[i] = k < end ? load16(body + (size_t)k * kN) : Pack<T>::lowest();
+    }
+    const int edge = rank == 0 ? sh.edge(t, a.V) : -1;
+    const float xe = edge >= 0 ? elem(x, edge) : -INFINITY;
+    const float xt = elem(x, tok);
+
+    // the maximum of this CTA's part
+    float own_max = xe;
+    {
+        uint4 u = Pack<T>::lowest();
+#pragma unroll
+        for (int i = 0; i < kVpt; i++) {
+            u.x = Pack<T>::max2(u.x, v[i].x);
+            u.y = Pack<T>::max2(u.y, v[i].y);
+            u.z = Pack<T>::max2(u.z, v[i].z);
+            u.w = Pack<T>::max2(u.w, v[i].w);
+        }
+        float o[kN];
+        Pack<T>::widen(u, o);
+#pragma unroll
+        for (int j = 0; j < kN; j++) own_max = fmaxf(own_max, o[j]);
+    }
+    float m = warp_max(own_max);
+    if ((t & 31) == 0) red_max[t >> 5] = m;
+    __syncthreads();
+    m = red_max[0];
+#pragma unroll
+    for (int w = 1; w < kW; w++) m = fmaxf(m, red_max[w]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+
+    // the sum of exponentials against it; the maximum's own terms (exactly 1
+    // each) are counted apart, by the warps that hold one
+    float s = 0.0f;
+    int n = 0;
+    if (__any_sync(0xffffffffu, own_max == ref)) {
+#pragma unroll
+        for (int i = 0; i < kVpt; i++) {
+            float o[kN];
+            Pack<T>::widen(v[i], o);
+#pragma unroll
+            for (int j = 0; j < kN; j++) {
+                const float d = o[j] - ref;
+                const float e = exp2_fast(d * a.scale);
+                n += d == 0.0f;
+                s += d == 0.0f ? 0.0f : e;
+            }
+        }
+        const float d = xe - ref;
+        n += d == 0.0f;
+        s += d == 0.0f ? 0.0f : exp2_fast(d * a.scale);
+        n = warp_sum_int(n);
+    } else {
+        float s2[2] = {exp2_fast((xe - ref) * a.scale), 0.0f};
+#pragma unroll
+        for (int i = 0; i < kVpt; i++) {
+            float o[kN];
+            Pack<T>::widen(v[i], o);
+#pragma unroll
+            for (int j = 0; j < kN; j++) s2[j & 1] += exp2_fast((o[j] - ref) * a.scale);
+        }
+        s = s2[0] + s2[1];
+    }
+    s = warp_sum(s);
+    if ((t & 31) == 0) {
+        red_sum[t >> 5] = s;
+        red_n[t >> 5] = n;
+    }
+    __syncthreads();
+    if (C > 1) cluster_wait();  // every CTA of the cluster runs
+    if (t < C) {
+        Part p{m, 0, 0.0};
+        for (int w = 0; w < kW; w++) {
+            p.others += (double)red_sum[w];
+            p.at_max += red_n[w];
+        }
+        if (C > 1) push_part(&parts[rank], t, p);
+        else parts[0] = p;
+    }
+    if (C > 1) {
+        cluster_arrive();
+        cluster_wait();
+    }
+    if (!kPolicy && rank != 0) return;
+    if (t < 32) {
+        __syncwarp();
+        const Part p = t < C ? parts[t] : Part{-INFINITY, 0, 0.0};
+        const float M = warp_max(p.max);
+        const bool top = p.max == M;
+        int at_max = top ? p.at_max : 0;
+        double others = top ? p.others : t < C ? (double)exp2_fast((p.max - M) * a.scale) * (p.others + p.at_max) : 0.0;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+            others += __shfl_xor_sync(0xffffffffu, others, o);
+            at_max += __shfl_xor_sync(0xffffffffu, at_max, o);
+        }
+        if (t == 0) {
+            const double excess = isinf(M) ? (double)NAN : others + (double)(at_max - 1);
+            const double lp = ((double)xt - (double)M) * a.inv_t - log1p(excess);
+            if (rank == 0) {
+                if (a.out) a.out[row] = RowScore{lp, M, (float)excess, 1, 0};
+                if (a.logprobs) a.logprobs[row] = (float)lp;
+                if (a.stats) {
+                    a.stats[2 * (size_t)row] = M;
+                    a.stats[2 * (size_t)row + 1] = (float)excess;
+                }
+            }
+            if (kPolicy) {
+                const double w = a.weights ? (double)a.weights[row] : 1.0 / a.rows;
+                double slope;
+                const double l = policy_term(lp, a.old_lp[row], a.p.kl_coef > 0.0 ? (double)a.ref_lp[row] : 0.0,
+                                             a.adv[row], 1.0 - a.p.clip_low, 1.0 + a.p.clip_high, a.p.kl_coef, &slope);
+                if (rank == 0) a.row_loss[row] = w * l;
+                const double c = w * slope * a.inv_t;
+                factor_s = (float)(-c / (1.0 + excess));
+                target_s = c == 0.0 ? 0.0f : (float)(c * beyond(xt, M, excess, a.inv_t));
+                max_s = M;
+            }
+        }
+    }
+    if (!kPolicy || !g) return;
+    __syncthreads();
+    const float f = factor_s, M = max_s;
+    const bool aligned = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
+    T* gbody = g + sh.head;
+#pragma unroll
+    for (int i = 0; i < kVpt; i++) {
+        const int k = base + i * kThr + t;
+        float o[kN];
+        Pack<T>::widen(v[i], o);
+#pragma unroll
+        for (int j = 0; j < kN; j++) o[j] = f == 0.0f ? 0.0f : f * exp2_fast((o[j] - M) * a.scale);
+        if (k < end) {
+            if (aligned) {
+                store16(gbody + (size_t)k * kN, Pack<T>::narrow(o));
+            } else {
+#pragma unroll
+                for (int j = 0; j < kN; j++) put(gbody, (long long)k * kN + j, o[j]);
+            }
+        }
+    }
+    if (edge >= 0 && edge != tok) put(g, edge, f == 0.0f ? 0.0f : f * exp2_fast((xe - M) * a.scale));
+    // the target, by the thread that wrote its vector
+    const int at = tok - sh.head;
+    if (at < 0 || at >= sh.vecs * kN) {
+        if (edge == tok) put(g, tok, target_s);
+    } else {
+        const int k = at / kN - base;
+        if (k >= 0 && k < end - base && k % kThr == t) put(g, tok, target_s);
+    }
+}
+
+// grad = coef * ([j = t] - p_j) / T.  Rows are cut into pieces of kGradThreads
+// x kGradVpt vectors, one CTA each.  Rows are taken from the last to the
+// first: the scoring before read them in the other order, so the ones it read
+// last come from L2.
+constexpr int kGradThreads = 256;
+constexpr int kGradVpt = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(kGradThreads)
+grad_kernel(const T* logits, int rows, int V, long long ld, const int* __restrict__ tokens, const float* stats,
+            int stat_words, const float* coefs, float scale, double inv_t, T* grad, long long gld, int pieces) {
+    constexpr int kN = Pack<T>::kN;
+    const int t = threadIdx.x;
+    const int row = rows - 1 - (int)(blockIdx.x / (unsigned)pieces), piece = blockIdx.x % (unsigned)pieces;
+    const int tok = tokens[row];
+    const T* x = logits + (size_t)row * ld;
+    T* g = grad + (size_t)row * gld;
+    const RowShape<T> sh(x, V);
+    const int base = piece * kGradThreads * kGradVpt, end = min(base + kGradThreads * kGradVpt, sh.vecs);
+    const T* body = x + sh.head;
+    const bool scored = tok >= 0 && tok < V;
+    wait_for_previous();
+    const float coef = scored ? coefs[row] : 0.0f;
+    if (coef == 0.0f) {
+        const RowShape<T> gs(g, V);
+        for (int k = piece * kGradThreads + t; k < gs.vecs; k += pieces * kGradThreads)
+            store16(g + gs.head + (size_t)k * kN, make_uint4(0u, 0u, 0u, 0u));
+        const int e = piece == 0 ? gs.edge(t, V) : -1;
+        if (e >= 0) put(g, e, 0.0f);
+        return;
+    }
+    uint4 v[kGradVpt];
+#pragma unroll
+    for (int i = 0; i < kGradVpt; i++) {
+        const int k = base + i * kGradThreads + t;
+        v[i] = k < end ? load16(body + (size_t)k * kN) : Pack<T>::lowest();
+    }
+    const float* st = stats + (size_t)row * stat_words;
+    const float M = st[0];
+    const double excess = st[1], c = (double)coef * inv_t;
+    const float f = (float)-c / (float)(1.0 + excess);
+    const bool aligned = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
+    T* gbody = g + sh.head;
+    const int edge = piece == 0 ? sh.edge(t, V) : -1;
+    const float xe = edge >= 0 ? elem(x, edge) : 0.0f;
+    // the target's thread: it reads the target before anything of it is overwritten
+    const int at = tok - sh.head, kt = at / kN - base;
+    const bool mine = at < 0 || at >= sh.vecs * kN ? edge == tok
+                                                   : kt >= 0 && kt < end - base && kt % kGradThreads == t;
+    const float target = mine ? (float)(c * beyond(elem(x, tok), M, excess, inv_t)) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kGradVpt; i++) {
+        const int k = base + i * kGradThreads + t;
+        float o[kN];
+        Pack<T>::widen(v[i], o);
+#pragma unroll
+        for (int j = 0; j < kN; j++) o[j] = f * exp2_fast((o[j] - M) * scale);
+        if (k < end) {
+            if (aligned) {
+                store16(gbody + (size_t)k * kN, Pack<T>::narrow(o));
+            } else {
+#pragma unroll
+                for (int j = 0; j < kN; j++) put(gbody, (long long)k * kN + j, o[j]);
+            }
+        }
+    }
+    if (edge >= 0) put(g, edge, f * exp2_fast((xe - M) * scale));
+    if (mine) put(g, tok, target);
+}
+
+// The policy loss: the rows' terms, added in a fixed order.
+__global__ void __launch_bounds__(1024)
+sum_rows_kernel(const double* row_loss, int rows, float* __restrict__ loss) {
+    __shared__ double red[32];
+    wait_for_previous();
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < rows; i += blockDim.x) sum += row_loss[i];
     sum = block_sum(sum, red);
     if (threadIdx.x == 0) *loss = (float)sum;
 }
@@ -177,12 +495,14 @@ policy_rows_kernel(const RowScore* __restrict__ score, int rows, const float* __
 // One warp per pair in turn: the two sequences' sums, the pair's loss and the
 // coefficient of every row's gradient.
 __global__ void __launch_bounds__(1024)
-preference_pairs_kernel(const RowScore* __restrict__ score, int rows, const int* __restrict__ offsets, int pairs,
+preference_pairs_kernel(const RowScore* score, int rows, const int* __restrict__ offsets, int pairs,
                         const float* __restrict__ ref, const float* __restrict__ weights,
                         qs_preference_params p, float* __restrict__ coefs, float* __restrict__ seq_lp,
                         float* __restrict__ loss) {
     __shared__ double red[32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    dependents_may_start();
+    wait_for_previous();
     for (int i = threadIdx.x; i < rows; i += blockDim.x) coefs[i] = 0.0f;
     __syncthreads();
     double sum = 0.0;
@@ -231,11 +551,6 @@ static int fail(int code, const char* fmt, ...) {
     return set_error(code, buf);
 }
 
-static int check_launch(const char* what) {
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? QS_OK : fail(QS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
-}
-
 struct Rows {
     const void* logits;
     int dtype, rows, vocab;
@@ -272,27 +587,92 @@ static int check_rows(const Rows& r, double temperature) {
     return QS_OK;
 }
 
-static int score(const Rows& r, const float* weights, RowScore* out, float* logprobs, float* stats,
-                 cudaStream_t st) {
-    if (r.dtype == QS_F32)
-        score_rows_kernel<float><<<r.rows, kLossThreads, 0, st>>>((const float*)r.logits, r.vocab, r.ld, r.tokens,
-                                                                 weights, r.inv_t, out, logprobs, stats);
-    else
-        score_rows_kernel<__nv_bfloat16><<<r.rows, kLossThreads, 0, st>>>(
-            (const __nv_bfloat16*)r.logits, r.vocab, r.ld, r.tokens, weights, r.inv_t, out, logprobs, stats);
-    return check_launch("score_rows_kernel");
+// Launches `kernel` in clusters of `cluster` CTAs; `after`: it may start while
+// the kernel before it ends (it waits for it before it reads its results).
+template <typename... P, typename... A>
+static int launch(const char* name, void (*kernel)(P...), long long grid, int threads, int cluster, bool after,
+                  cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2] = {};
+    if (cluster > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = cluster;
+        attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        cfg.numAttrs++;
+    }
+    if (after) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs++;
+    }
+    cfg.attrs = attr;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    return e == cudaSuccess ? QS_OK : fail(QS_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
 }
 
-static int grad(const Rows& r, const float* stats, int stat_words, const float* coefs, cudaStream_t st) {
-    if (r.dtype == QS_F32)
-        grad_rows_kernel<float><<<r.rows, kLossThreads, 0, st>>>((const float*)r.logits, r.vocab, r.ld, r.tokens,
-                                                                stats, stat_words, coefs, r.inv_t, (float*)r.grad,
-                                                                r.gld);
-    else
-        grad_rows_kernel<__nv_bfloat16><<<r.rows, kLossThreads, 0, st>>>(
-            (const __nv_bfloat16*)r.logits, r.vocab, r.ld, r.tokens, stats, stat_words, coefs, r.inv_t,
-            (__nv_bfloat16*)r.grad, r.gld);
-    return check_launch("grad_rows_kernel");
+// How a row is spread: CTAs per row (a power of two up to 8) such that a CTA
+// holds at most 2560 vectors (40 KB, 10 vectors a thread), and more of them
+// while the rows alone would leave SMs idle and a CTA keeps 256 vectors.  Then
+// the smallest kernel that holds a share.
+template <typename T, bool kPolicy>
+static int score_launch(ScoreArgs<T>& a, cudaStream_t st) {
+    const int vecs = a.V / Pack<T>::kN;
+    int log_c = 0;
+    const auto share = [&] { return (vecs + (1 << log_c) - 1) >> log_c; };
+    while (log_c < 3 && (share() > 2560 || ((long long)a.rows << log_c) < 148 && share() > 256)) log_c++;
+    a.log_c = log_c;
+    const int need = share(), c = 1 << log_c;
+    const long long grid = (long long)a.rows << log_c;
+#define QS_SCORE(thr, vpt)             \
+    if (need <= (thr) * (vpt))         \
+    return launch("score_kernel", score_kernel<T, thr, vpt, kPolicy>, grid, thr, c, false, st, a)
+    QS_SCORE(256, 1);
+    QS_SCORE(256, 2);
+    QS_SCORE(256, 4);
+    QS_SCORE(256, 6);
+    QS_SCORE(256, 8);
+    QS_SCORE(256, 10);
+    QS_SCORE(512, 8);
+    QS_SCORE(512, 10);
+    QS_SCORE(512, 16);
+#undef QS_SCORE
+    return fail(QS_ERR_UNSUPPORTED, "vocab %d", a.V);
+}
+
+template <typename T>
+static ScoreArgs<T> score_args(const Rows& r) {
+    ScoreArgs<T> a = {};
+    a.logits = (const T*)r.logits;
+    a.rows = r.rows;
+    a.V = r.vocab;
+    a.ld = r.ld;
+    a.tokens = r.tokens;
+    a.scale = (float)(r.inv_t * 1.4426950408889634);
+    a.inv_t = r.inv_t;
+    a.grad = (T*)r.grad;
+    a.gld = r.gld;
+    return a;
+}
+
+template <typename T>
+static int score(const Rows& r, RowScore* out, float* logprobs, float* stats, cudaStream_t st) {
+    ScoreArgs<T> a = score_args<T>(r);
+    a.out = out;
+    a.logprobs = logprobs;
+    a.stats = stats;
+    return score_launch<T, false>(a, st);
+}
+
+template <typename T>
+static int grad(const Rows& r, const float* stats, int stat_words, const float* coefs, bool after, cudaStream_t st) {
+    const int vecs = r.vocab / Pack<T>::kN;
+    const int pieces = max(1, (vecs + kGradThreads * kGradVpt - 1) / (kGradThreads * kGradVpt));
+    return launch("grad_kernel", grad_kernel<T>, (long long)r.rows * pieces, kGradThreads, 1, after, st,
+                  (const T*)r.logits, r.rows, r.vocab, r.ld, r.tokens, stats, stat_words, coefs,
+                  (float)(r.inv_t * 1.4426950408889634), r.inv_t, (T*)r.grad, r.gld, pieces);
 }
 
 static size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -311,7 +691,9 @@ int qs_token_logprobs(const void* d_logits, int dtype, int rows, int vocab, long
     const int rc = check_rows(r, temperature);
     if (rc || rows == 0) return rc;
     if (!d_logprobs || !d_stats) return fail(QS_ERR_INVALID, "NULL output buffer");
-    return score(r, nullptr, nullptr, d_logprobs, d_stats, (cudaStream_t)stream);
+    const cudaStream_t st = (cudaStream_t)stream;
+    return dtype == QS_F32 ? score<float>(r, nullptr, d_logprobs, d_stats, st)
+                           : score<__nv_bfloat16>(r, nullptr, d_logprobs, d_stats, st);
 }
 
 int qs_token_logprobs_backward(const void* d_logits, int dtype, int rows, int vocab, long long row_stride,
@@ -323,13 +705,12 @@ int qs_token_logprobs_backward(const void* d_logits, int dtype, int rows, int vo
     if (rc || rows == 0) return rc;
     if (!d_stats || !d_grad_logprobs) return fail(QS_ERR_INVALID, "NULL device pointer");
     if (!d_grad) return fail(QS_ERR_INVALID, "NULL output buffer");
-    return grad(r, d_stats, 2, d_grad_logprobs, (cudaStream_t)stream);
+    const cudaStream_t st = (cudaStream_t)stream;
+    return dtype == QS_F32 ? grad<float>(r, d_stats, 2, d_grad_logprobs, false, st)
+                           : grad<__nv_bfloat16>(r, d_stats, 2, d_grad_logprobs, false, st);
 }
 
-size_t qs_policy_loss_workspace(int rows) {
-    const size_t n = rows > 0 ? (size_t)rows : 1;
-    return round256(n * sizeof(RowScore)) + round256(n * sizeof(float));
-}
+size_t qs_policy_loss_workspace(int rows) { return round256((rows > 0 ? (size_t)rows : 1) * sizeof(double)); }
 
 int qs_policy_loss(const void* d_logits, int dtype, int rows, int vocab, long long row_stride,
                    const int* d_tokens, const float* d_old_logprobs, const float* d_ref_logprobs,
@@ -353,17 +734,22 @@ int qs_policy_loss(const void* d_logits, int dtype, int rows, int vocab, long lo
         if (!d_workspace || workspace_bytes < qs_policy_loss_workspace(rows) || ((uintptr_t)d_workspace & 15))
             return fail(QS_ERR_INVALID, "workspace is NULL, unaligned or below %zu bytes", qs_policy_loss_workspace(rows));
     }
-    RowScore* sc = (RowScore*)d_workspace;
-    float* coefs = (float*)((char*)d_workspace + round256((size_t)rows * sizeof(RowScore)));
+    double* row_loss = (double*)d_workspace;
     if (rows > 0) {
-        const int e = score(r, d_weights, sc, d_logprobs, nullptr, st);
+        const auto go = [&](auto a) {
+            a.logprobs = d_logprobs;
+            a.weights = d_weights;
+            a.old_lp = d_old_logprobs;
+            a.ref_lp = d_ref_logprobs;
+            a.adv = d_advantages;
+            a.p = p;
+            a.row_loss = row_loss;
+            return score_launch<std::remove_pointer_t<decltype(a.grad)>, true>(a, st);
+        };
+        const int e = dtype == QS_F32 ? go(score_args<float>(r)) : go(score_args<__nv_bfloat16>(r));
         if (e) return e;
     }
-    policy_rows_kernel<<<1, 1024, 0, st>>>(sc, rows, d_old_logprobs, d_ref_logprobs, d_advantages, d_weights, p,
-                                          coefs, d_loss);
-    const int e = check_launch("policy_rows_kernel");
-    if (e || rows == 0 || !d_grad) return e;
-    return grad(r, &sc->max, sizeof(RowScore) / 4, coefs, st);
+    return launch("sum_rows_kernel", sum_rows_kernel, 1, 1024, 1, rows > 0, st, row_loss, rows, d_loss);
 }
 
 size_t qs_preference_loss_workspace(int rows, int pairs) {
@@ -395,14 +781,15 @@ int qs_preference_loss(const void* d_logits, int dtype, int rows, int vocab, lon
     RowScore* sc = (RowScore*)d_workspace;
     float* coefs = (float*)((char*)d_workspace + round256((size_t)rows * sizeof(RowScore)));
     if (rows > 0) {
-        const int e = score(r, nullptr, sc, nullptr, nullptr, st);
+        const int e = dtype == QS_F32 ? score<float>(r, sc, nullptr, nullptr, st)
+                                      : score<__nv_bfloat16>(r, sc, nullptr, nullptr, st);
         if (e) return e;
     }
-    preference_pairs_kernel<<<1, 1024, 0, st>>>(sc, rows, d_seq_offsets, pairs, d_ref_logprobs, d_weights, p, coefs,
-                                               d_seq_logprobs, d_loss);
-    const int e = check_launch("preference_pairs_kernel");
+    const int e = launch("preference_pairs_kernel", preference_pairs_kernel, 1, 1024, 1, rows > 0, st, sc, rows,
+                         d_seq_offsets, pairs, d_ref_logprobs, d_weights, p, coefs, d_seq_logprobs, d_loss);
     if (e || rows == 0 || !d_grad) return e;
-    return grad(r, &sc->max, sizeof(RowScore) / 4, coefs, st);
+    return dtype == QS_F32 ? grad<float>(r, &sc->max, sizeof(RowScore) / 4, coefs, true, st)
+                           : grad<__nv_bfloat16>(r, &sc->max, sizeof(RowScore) / 4, coefs, true, st);
 }
 
 }  // extern "C"
