@@ -1128,10 +1128,15 @@ int qs_lm_head_w4_sample(qs_sampler* s, const void* d_hidden, const void* d_norm
     DeviceGuard dg(s->device);
     rc = tail_workspace(s, weight->hidden_dim);
     if (rc) return rc;
+    // the epilogue hands the sampler the segment maxima, as in qs_lm_head_sample
+    uint32_t* segk = batch < kWideMinRows ? s->lh_segk : nullptr;
     rc = w4_launch(d_hidden, d_norm_weight, weight, batch, s->lh_normed, s->lh_logits, s->num_sms,
-                   (cudaStream_t)stream);
+                   (cudaStream_t)stream, segk, s->lh_segs);
     if (rc) return rc;
-    return sample_stateful(s, s->lh_logits, QS_BF16, batch, d_tokens, stream, flags, nullptr, 0);
+    rc = sample_stateful(s, s->lh_logits, QS_BF16, batch, d_tokens, stream, flags, segk, s->lh_segs);
+    if (rc && segk)  // the scan did not consume (and zero) the maxima
+        cudaMemsetAsync(segk, 0, sizeof(uint32_t) * (size_t)batch * s->lh_segs, (cudaStream_t)stream);
+    return rc;
 }
 
 int qs_lm_head_logits(qs_sampler* s, const void** d_logits) {

@@ -1,17 +1,22 @@
 // The lm_head with 4-bit weights for few tokens: quantisation, the packed
 // layout and the projection (include/qwen600_sampler.h gives the formulas).
+//
+// Bound: the stream of the codes.  For 151,936 x 1024 that is 78 MB, 12.3 us at
+// the measured 6549 GB/s, so all else has to fit beside 23 bytes a clock and
+// SM: the codes go from memory to registers (no staging), become bf16 pairs
+// with 11 instructions per 8 codes, and meet the tokens on mma.sync
+// m16n8k16: 16 vocabulary rows x 8 tokens, tokens on the narrow side.  (tcgen05
+// takes its wider operand from shared or tensor memory; 4-bit weights would
+// have to be written there as bf16, four times the bytes of their stream.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include "qs_common.cuh"
 #include "qs_w4.h"
+#include "qs_pipe.cuh"
 
 namespace qs {
-
-__device__ __forceinline__ float scale_at(const void* s, size_t i, int dtype) {
-    return dtype == QS_F16 ? __half2float(((const __half*)s)[i]) : __bfloat162float(((const __nv_bfloat16*)s)[i]);
-}
 
 // One thread per group of a row: the range that holds the group and zero, a
 // bf16 scale of a fifteenth of it, codes rounded to nearest.
@@ -48,50 +53,357 @@ cudaError_t launch_w4_quantize(const __nv_bfloat16* w, int V, int K, int group, 
     return cudaGetLastError();
 }
 
-size_t w4_codes_bytes(int V, int K) { return (size_t)V * K / 2; }
-size_t w4_scales_bytes(int V, int K, int group) { return (size_t)V * (K / group) * 2; }
-size_t w4_zeros_bytes(int V, int K, int group) { return (size_t)V * (K / group); }
+// ---------------------------------------------------------------- layout
+// Vocabulary rows in tiles of 16, columns in chunks of 128 (the last padded
+// with zeros).  A unit is one tile's chunk: 1 KB of codes, and units lie one
+// after another, tile by tile.  In a unit lane l = 4 g + q of a warp finds
+// 16 bytes for row g (first 512 bytes) and 16 for row g + 8: four words, word
+// w for columns 32 w + 8 q + 0..7 of the chunk.  Nibble i < 4 of a word is
+// column 2 i, nibble i + 4 column 2 i + 1, so (word >> 4 i) & 0x000F000F is a
+// pair of neighbouring columns, one in each half.  A group of 32 columns is
+// then one word of every lane, and any group is whole mma instructions.
+// Scales (16-bit) and zero points (bytes) of a unit: [g][group of the chunk]
+// [row g, row g + 8].
+constexpr int kUnitCodes = 1024;
+
+static int w4_chunks(int K) { return (K + 127) / 128; }
+static int w4_tiles(int V) { return (V + 15) / 16; }
+
+size_t w4_codes_bytes(int V, int K) { return (size_t)w4_tiles(V) * w4_chunks(K) * kUnitCodes; }
+size_t w4_scales_bytes(int V, int K, int group) { return (size_t)w4_tiles(V) * w4_chunks(K) * (128 / group) * 32; }
+size_t w4_zeros_bytes(int V, int K, int group) { return w4_scales_bytes(V, K, group) / 2; }
+
+__global__ void w4_pack_codes_kernel(const unsigned char* __restrict__ codes, int V, int K, int chunks, size_t n,
+                                     uint32_t* __restrict__ out) {
+    const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;  // one word
+    if (i >= n) return;
+    const int w = i & 3, lane = (i >> 2) & 31, half = (i >> 7) & 1;
+    const size_t unit = i >> 8;
+    const int row = (int)(unit / chunks) * 16 + half * 8 + (lane >> 2);
+    const int k = (int)(unit % chunks) * 128 + 32 * w + 8 * (lane & 3);
+    uint32_t word = 0;
+    if (row < V && k < K) {
+        const unsigned char* p = codes + ((size_t)row * K + k) / 2;
+        for (int b = 0; b < 4; b++) word |= (uint32_t)(p[b] & 15) << (4 * b) | (uint32_t)(p[b] >> 4) << (16 + 4 * b);
+    }
+    out[i] = word;
+}
+
+__global__ void w4_pack_scales_kernel(const uint16_t* __restrict__ scales, const unsigned char* __restrict__ zeros,
+                                      int V, int per_row, int chunks, int per_chunk, size_t n,
+                                      uint16_t* __restrict__ out_s, unsigned char* __restrict__ out_z) {
+    const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= n) return;
+    const int half = i & 1, j = (int)(i >> 1) % per_chunk, g = (int)((i >> 1) / per_chunk) & 7;
+    const size_t unit = i / (16 * per_chunk);
+    const int row = (int)(unit / chunks) * 16 + half * 8 + g, grp = (int)(unit % chunks) * per_chunk + j;
+    const bool in = row < V && grp < per_row;
+    out_s[i] = in ? scales[(size_t)row * per_row + grp] : 0;
+    if (zeros) out_z[i] = in ? zeros[(size_t)row * per_row + grp] & 15 : 0;
+}
 
 cudaError_t launch_w4_pack(const unsigned char* codes, const void* scales, const unsigned char* zeros, int V, int K,
                            int group, unsigned char* pc, void* ps, unsigned char* pz, cudaStream_t st) {
-    cudaError_t e = cudaMemcpyAsync(pc, codes, w4_codes_bytes(V, K), cudaMemcpyDeviceToDevice, st);
-    if (e == cudaSuccess) e = cudaMemcpyAsync(ps, scales, w4_scales_bytes(V, K, group), cudaMemcpyDeviceToDevice, st);
-    if (e == cudaSuccess && zeros)
-        e = cudaMemcpyAsync(pz, zeros, w4_zeros_bytes(V, K, group), cudaMemcpyDeviceToDevice, st);
-    return e;
+    const int chunks = w4_chunks(K);
+    size_t n = w4_codes_bytes(V, K) / 4;
+    w4_pack_codes_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(codes, V, K, chunks, n, (uint32_t*)pc);
+    n = w4_scales_bytes(V, K, group) / 2;
+    w4_pack_scales_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>((const uint16_t*)scales, zeros, V, K / group,
+                                                                      chunks, 128 / group, n, (uint16_t*)ps, pz);
+    return cudaGetLastError();
 }
 
-// One warp per vocabulary row and token.
-__global__ void __launch_bounds__(256)
-lm_head_w4_kernel(const __nv_bfloat16* __restrict__ x, W4View w, __nv_bfloat16* __restrict__ out) {
-    const int v = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, b = blockIdx.y;
-    if (v >= w.vocab) return;
-    const int per = w.hidden / w.group;
-    float acc = 0.0f;
-    for (int g = 0; g < per; g++) {
-        float part = 0.0f;
-        const float z = w.zeros ? (float)w.zeros[(size_t)v * per + g] : 8.0f;
-        for (int i = lane; i < w.group; i += 32) {
-            const int k = g * w.group + i;
-            const int c = w.codes[((size_t)v * w.hidden + k) / 2];
-            const float q = (float)((k & 1) ? c >> 4 : c & 15) - z;
-            part = __fmaf_rn(q, __bfloat162float(x[(size_t)b * w.hidden + k]), part);
-        }
-        acc = __fmaf_rn(scale_at(w.scales, (size_t)v * per + g, w.scale_dtype), part, acc);
+// -------------------------------------------------------------- projection
+constexpr int kW4Warps = 16;
+constexpr int kW4Depth = 4;  // units a warp has in flight
+
+__device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Codes 2 i and 2 i + 1 of a word minus the zero point, as bf16: 0x4300 | q is
+// 128 + q, and the difference of 128 + q and 128 + z is exact.
+__device__ __forceinline__ uint32_t code_pair(uint32_t word, int i, uint32_t zero) {
+    const uint32_t q = ((word >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&q),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&zero));
+    return *reinterpret_cast<const uint32_t*>(&d);
+}
+
+__device__ __forceinline__ float scale_of(uint32_t bits, bool f16) {
+    return f16 ? __half2float(__ushort_as_half((unsigned short)bits)) : __uint_as_float(bits << 16);
+}
+
+__device__ __forceinline__ uint4 load_codes(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+
+// One unit as a lane holds it.
+template <int kGroups>
+struct W4Unit {
+    uint4 lo, hi;               // codes of row g and of row g + 8
+    uint32_t scales[kGroups];   // row g in the low half, row g + 8 in the high one
+    uint32_t zeros[(kGroups + 1) / 2];
+};
+
+template <int kGroups>
+__device__ __forceinline__ void w4_load(W4Unit<kGroups>& u, const W4View& w, int unit, int lane) {
+    const uint4* c = reinterpret_cast<const uint4*>(w.codes + (size_t)unit * kUnitCodes) + lane;
+    u.lo = load_codes(c);
+    u.hi = load_codes(c + 32);
+    const size_t at = ((size_t)unit * 8 + (lane >> 2)) * kGroups;
+    const uint32_t* s = reinterpret_cast<const uint32_t*>(w.scales) + at;
+    if (kGroups == 1) {
+        u.scales[0] = __ldg(s);
+    } else if (kGroups == 2) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(s));
+        u.scales[0] = v.x; u.scales[1 % kGroups] = v.y;
+    } else {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(s));
+        u.scales[0] = v.x; u.scales[1 % kGroups] = v.y; u.scales[2 % kGroups] = v.z; u.scales[3 % kGroups] = v.w;
     }
-    acc = warp_sum(acc);
-    if (lane == 0) out[(size_t)b * w.vocab + v] = __float2bfloat16_rn(acc);
+    if (w.zeros) {
+        const unsigned char* z = w.zeros + at * 2;
+        if (kGroups == 1) {
+            u.zeros[0] = __ldg(reinterpret_cast<const unsigned short*>(z));
+        } else if (kGroups == 2) {
+            u.zeros[0] = __ldg(reinterpret_cast<const uint32_t*>(z));
+        } else {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(z));
+            u.zeros[0] = v.x; u.zeros[1 % ((kGroups + 1) / 2)] = v.y;
+        }
+    }
+}
+
+struct W4Out {
+    __nv_bfloat16* logits;
+    int tokens;  // rows of this launch
+    uint32_t* segk;
+    int segk_stride;
+};
+
+// Stores a finished tile: 16 vocabulary rows of up to 8 kNt tokens, through the
+// warp's staging rows so that a lane stores 16 bytes of one token.
+template <int kNt>
+__device__ __forceinline__ void w4_store(const float (&acc)[kNt][4], __nv_bfloat16* stage, const W4Out& o, int V, int tile,
+                                         int lane) {
+    const int g = lane >> 2, q = lane & 3;
+    __syncwarp();
+#pragma unroll
+    for (int n = 0; n < kNt; n++) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)  // j: row g or g + 8, token 2 q or 2 q + 1
+            stage[(n * 8 + 2 * q + (j & 1)) * 16 + g + (j >> 1) * 8] = __float2bfloat16_rn(acc[n][j]);
+    }
+    __syncwarp();
+    for (int p = lane; p < kNt * 16; p += 32) {
+        const int token = p >> 1, col = tile * 16 + (p & 1) * 8;
+        const uint4 v = *reinterpret_cast<const uint4*>(stage + p * 8);
+        const bool in = token < o.tokens;
+        if (in && col < V) {
+            __nv_bfloat16* d = o.logits + (size_t)token * V + col;
+            if (col + 8 <= V && (V & 7) == 0) {
+                *reinterpret_cast<uint4*>(d) = v;
+            } else {
+                const __nv_bfloat16* e = stage + p * 8;
+                for (int j = 0; j < 8 && col + j < V; j++) d[j] = e[j];
+            }
+        }
+        // whole tiles only: they never straddle a 256-column segment, and the
+        // sampler takes the maxima of whole segments
+        if (o.segk && in && tile * 16 + 16 <= V)
+            atomicMax(o.segk + (size_t)token * o.segk_stride + (tile >> 4), fkey(vec_max<__nv_bfloat16>(v)));
+    }
+}
+
+// A CTA takes a contiguous range of tiles and its warps equal shares of their
+// units, so warps end together whatever the number of tiles; a tile that
+// several warps share is added from their partial sums at the end, in order.
+// kNt blocks of 8 tokens, kGroups groups in a chunk.
+template <int kNt, int kGroups>
+__global__ void __launch_bounds__(kW4Warps * 32, 1)
+lm_head_w4_kernel(const __nv_bfloat16* x, const __grid_constant__ W4View w, const __grid_constant__ W4Out o, int chunks,
+                  int tiles) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int pitch = chunks * 256 + 64;  // bytes of a token's row: neighbours 64 bytes apart in the banks
+    unsigned char* xs = smem;
+    float4* slots = reinterpret_cast<float4*>(smem + kNt * 8 * pitch);  // [warp][continued, begun][kNt][lane]
+    __nv_bfloat16* stage = reinterpret_cast<__nv_bfloat16*>(slots + kW4Warps * 2 * kNt * 32);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    stage += warp * kNt * 128;
+    const int t0 = (int)((long long)blockIdx.x * tiles / gridDim.x), t1 = (int)((long long)(blockIdx.x + 1) * tiles / gridDim.x);
+    const int u0 = t0 * chunks, un = (t1 - t0) * chunks;
+    const auto share = [&](int wi) { return u0 + (int)((long long)un * wi / kW4Warps); };
+    const int a = share(warp), b = share(warp + 1);
+
+    W4Unit<kGroups> buf[kW4Depth];
+#pragma unroll
+    for (int d = 0; d < kW4Depth; d++)
+        if (a + d < b) w4_load(buf[d], w, a + d, lane);
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the RMSNorm's rows
+    for (int i = threadIdx.x; i < kNt * 8 * chunks * 16; i += kW4Warps * 32) {
+        const int row = i / (chunks * 16), c = i % (chunks * 16);
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (row < o.tokens && c * 8 < w.hidden)
+            v = *reinterpret_cast<const uint4*>(x + (size_t)row * w.hidden + c * 8);
+        *reinterpret_cast<uint4*>(xs + row * pitch + c * 16) = v;
+    }
+    __syncthreads();
+
+    const bool f16 = w.scale_dtype == QS_F16;
+    float acc[kNt][4];
+#pragma unroll
+    for (int n = 0; n < kNt; n++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[n][j] = 0.0f;
+    int tile = a / chunks, c = a - tile * chunks;
+    bool begun = c == 0;
+    for (int u = a; u < b; u += kW4Depth) {
+#pragma unroll
+        for (int d = 0; d < kW4Depth; d++) {
+            if (u + d >= b) break;
+            const unsigned char* xc = xs + g * pitch + c * 256 + q * 16;
+            const uint32_t* lo = reinterpret_cast<const uint32_t*>(&buf[d].lo);
+            const uint32_t* hi = reinterpret_cast<const uint32_t*>(&buf[d].hi);
+#pragma unroll
+            for (int j = 0; j < kGroups; j++) {
+                uint32_t zl = 0x43084308u, zh = 0x43084308u;
+                if (w.zeros) {
+                    const uint32_t z = buf[d].zeros[j / 2] >> (16 * (j & 1));
+                    zl = 0x43004300u | ((z & 0xFFu) * 0x00010001u);
+                    zh = 0x43004300u | (((z >> 8) & 0xFFu) * 0x00010001u);
+                }
+                float part[kNt][4];
+#pragma unroll
+                for (int n = 0; n < kNt; n++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) part[n][k] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4 / kGroups; k++) {
+                    const int word = j * (4 / kGroups) + k;
+                    uint32_t al[4], ah[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        al[i] = code_pair(lo[word], i, zl);
+                        ah[i] = code_pair(hi[word], i, zh);
+                    }
+#pragma unroll
+                    for (int n = 0; n < kNt; n++) {
+                        const uint4 xv = *reinterpret_cast<const uint4*>(xc + n * 8 * pitch + word * 64);
+                        mma_bf16(part[n], al[0], ah[0], al[1], ah[1], xv.x, xv.y);
+                        mma_bf16(part[n], al[2], ah[2], al[3], ah[3], xv.z, xv.w);
+                    }
+                }
+                const float sl = scale_of(buf[d].scales[j] & 0xFFFFu, f16), sh = scale_of(buf[d].scales[j] >> 16, f16);
+#pragma unroll
+                for (int n = 0; n < kNt; n++) {
+                    acc[n][0] = __fmaf_rn(sl, part[n][0], acc[n][0]);
+                    acc[n][1] = __fmaf_rn(sl, part[n][1], acc[n][1]);
+                    acc[n][2] = __fmaf_rn(sh, part[n][2], acc[n][2]);
+                    acc[n][3] = __fmaf_rn(sh, part[n][3], acc[n][3]);
+                }
+            }
+            if (u + d + kW4Depth < b) w4_load(buf[d], w, u + d + kW4Depth, lane);
+            const bool ends = ++c == chunks;
+            if (ends || u + d + 1 == b) {
+                if (ends && begun) {
+                    w4_store<kNt>(acc, stage, o, w.vocab, tile, lane);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < kNt; n++)
+                        slots[((warp * 2 + begun) * kNt + n) * 32 + lane] =
+                            make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+                }
+#pragma unroll
+                for (int n = 0; n < kNt; n++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) acc[n][j] = 0.0f;
+                if (ends) {
+                    c = 0;
+                    tile++;
+                    begun = true;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    // the warp that began a tile which later warps continued adds their sums
+    if (a < b && b % chunks != 0 && (b - 1) / chunks * chunks >= a) {
+        const int last = (b - 1) / chunks, stop = (last + 1) * chunks;
+        int first = warp * 2 + 1;  // its own part, then the following warps' continued ones
+        for (int wi = warp; wi < kW4Warps && share(wi) < stop; wi++) {
+            if (share(wi) < share(wi + 1)) {
+#pragma unroll
+                for (int n = 0; n < kNt; n++) {
+                    const float4 p = slots[(first * kNt + n) * 32 + lane];
+                    acc[n][0] += p.x; acc[n][1] += p.y; acc[n][2] += p.z; acc[n][3] += p.w;
+                }
+            }
+            first = (wi + 1) * 2;
+        }
+        w4_store<kNt>(acc, stage, o, w.vocab, last, lane);
+    }
+}
+
+static size_t w4_smem(int nt, int K) {
+    return (size_t)nt * 8 * (w4_chunks(K) * 256 + 64) + (size_t)kW4Warps * nt * (2 * 512 + 256);
+}
+
+template <int kNt, int kGroups>
+static cudaError_t w4_go(const __nv_bfloat16* x, const W4View& w, const W4Out& o, int grid, cudaStream_t st) {
+    const size_t smem = w4_smem(kNt, w.hidden);
+    cudaError_t e = cudaFuncSetAttribute(lm_head_w4_kernel<kNt, kGroups>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)smem);
+    if (e != cudaSuccess) return e;
+    // programmatic dependent launch: the first units are requested while the
+    // RMSNorm runs
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kW4Warps * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, lm_head_w4_kernel<kNt, kGroups>, x, w, o, w4_chunks(w.hidden), w4_tiles(w.vocab));
+}
+
+template <int kNt>
+static cudaError_t w4_group(const __nv_bfloat16* x, const W4View& w, const W4Out& o, int grid, cudaStream_t st) {
+    return w.group == 128 ? w4_go<kNt, 1>(x, w, o, grid, st)
+         : w.group == 64  ? w4_go<kNt, 2>(x, w, o, grid, st)
+                          : w4_go<kNt, 4>(x, w, o, grid, st);
 }
 
 cudaError_t launch_lm_head_w4(const __nv_bfloat16* normed, const W4View& w, __nv_bfloat16* logits, int batch,
                               int num_sms, uint32_t* segk, int segk_stride, cudaStream_t st) {
-    (void)num_sms; (void)segk; (void)segk_stride;
-    for (int b = 0; b < batch; b += 65535) {
-        const int n = batch - b < 65535 ? batch - b : 65535;
-        lm_head_w4_kernel<<<dim3((w.vocab + 7) / 8, n), 256, 0, st>>>(normed + (size_t)b * w.hidden, w,
-                                                                     logits + (size_t)b * w.vocab);
+    const int tiles = w4_tiles(w.vocab), grid = tiles < num_sms ? tiles : num_sms;
+    int most = 4;  // blocks of 8 tokens whose rows fit in shared memory
+    while (w4_smem(most, w.hidden) > 227 * 1024) most--;
+    for (int b = 0; b < batch;) {
+        const int left = (batch - b + 7) / 8, nt = left < most ? left : most;
+        const int n = batch - b < nt * 8 ? batch - b : nt * 8;
+        const W4Out o{logits + (size_t)b * w.vocab, n, segk ? segk + (size_t)b * segk_stride : nullptr, segk_stride};
+        const __nv_bfloat16* x = normed + (size_t)b * w.hidden;
+        const cudaError_t e = nt == 1 ? w4_group<1>(x, w, o, grid, st)
+                            : nt == 2 ? w4_group<2>(x, w, o, grid, st)
+                            : nt == 3 ? w4_group<3>(x, w, o, grid, st)
+                                      : w4_group<4>(x, w, o, grid, st);
+        if (e != cudaSuccess) return e;
+        b += n;
     }
-    return cudaGetLastError();
+    return cudaSuccess;
 }
 
 }  // namespace qs
