@@ -117,19 +117,29 @@ cudaError_t launch_w4_pack(const unsigned char* codes, const void* scales, const
 constexpr int kW4Warps = 16;
 constexpr int kW4Depth = 4;  // units a warp has in flight
 
-__device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+// d = a * b + c on 16 x 8 x 16; c in registers, or 0.
+__device__ __forceinline__ void mma_bf16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16_first(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                               uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // Codes 2 i and 2 i + 1 of a word minus the zero point, as bf16: 0x4300 | q is
 // 128 + q, and the difference of 128 + q and 128 + z is exact.
 __device__ __forceinline__ uint32_t code_pair(uint32_t word, int i, uint32_t zero) {
-    const uint32_t q = ((word >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+    uint32_t q;  // (word >> 4 i) & 0x000F000F | 0x43004300, the two in one instruction
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(q) : "r"(word >> (4 * i)), "r"(0x000F000Fu), "r"(0x43004300u));
     const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&q),
                                      *reinterpret_cast<const __nv_bfloat162*>(&zero));
     return *reinterpret_cast<const uint32_t*>(&d);
@@ -155,15 +165,22 @@ struct W4Unit {
     uint32_t zeros[(kGroups + 1) / 2];
 };
 
-template <int kGroups>
-__device__ __forceinline__ void w4_load(W4Unit<kGroups>& u, const W4View& w, int unit, int lane) {
-    const uint4* c = reinterpret_cast<const uint4*>(w.codes + (size_t)unit * kUnitCodes) + lane;
+// Where a lane's part of its warp's next unit lies.
+struct W4At {
+    const unsigned char* codes;
+    const unsigned char* scales;
+    const unsigned char* zeros;
+};
+
+// Loads the unit `ahead` units behind the next one.
+template <int kGroups, bool kZeros>
+__device__ __forceinline__ void w4_load(W4Unit<kGroups>& u, const W4At& at, int ahead) {
+    const uint4* c = reinterpret_cast<const uint4*>(at.codes + ahead * kUnitCodes);
     u.lo = load_codes(c);
     u.hi = load_codes(c + 32);
-    const size_t at = ((size_t)unit * 8 + (lane >> 2)) * kGroups;
-    const uint32_t* s = reinterpret_cast<const uint32_t*>(w.scales) + at;
+    const unsigned char* s = at.scales + ahead * (32 * kGroups);
     if (kGroups == 1) {
-        u.scales[0] = __ldg(s);
+        u.scales[0] = __ldg(reinterpret_cast<const uint32_t*>(s));
     } else if (kGroups == 2) {
         const uint2 v = __ldg(reinterpret_cast<const uint2*>(s));
         u.scales[0] = v.x; u.scales[1 % kGroups] = v.y;
@@ -171,8 +188,8 @@ __device__ __forceinline__ void w4_load(W4Unit<kGroups>& u, const W4View& w, int
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(s));
         u.scales[0] = v.x; u.scales[1 % kGroups] = v.y; u.scales[2 % kGroups] = v.z; u.scales[3 % kGroups] = v.w;
     }
-    if (w.zeros) {
-        const unsigned char* z = w.zeros + at * 2;
+    if (kZeros) {
+        const unsigned char* z = at.zeros + ahead * (16 * kGroups);
         if (kGroups == 1) {
             u.zeros[0] = __ldg(reinterpret_cast<const unsigned short*>(z));
         } else if (kGroups == 2) {
@@ -229,7 +246,7 @@ __device__ __forceinline__ void w4_store(const float (&acc)[kNt][4], __nv_bfloat
 // units, so warps end together whatever the number of tiles; a tile that
 // several warps share is added from their partial sums at the end, in order.
 // kNt blocks of 8 tokens, kGroups groups in a chunk.
-template <int kNt, int kGroups>
+template <int kNt, int kGroups, bool kZeros>
 __global__ void __launch_bounds__(kW4Warps * 32, 1)
 lm_head_w4_kernel(const __nv_bfloat16* x, const __grid_constant__ W4View w, const __grid_constant__ W4Out o, int chunks,
                   int tiles) {
@@ -245,10 +262,14 @@ lm_head_w4_kernel(const __nv_bfloat16* x, const __grid_constant__ W4View w, cons
     const auto share = [&](int wi) { return u0 + (int)((long long)un * wi / kW4Warps); };
     const int a = share(warp), b = share(warp + 1);
 
+    W4At at;
+    at.codes = w.codes + (size_t)a * kUnitCodes + lane * 16;
+    at.scales = reinterpret_cast<const unsigned char*>(w.scales) + ((size_t)a * 8 + g) * (4 * kGroups);
+    at.zeros = w.zeros + (kZeros ? ((size_t)a * 8 + g) * (2 * kGroups) : 0);
     W4Unit<kGroups> buf[kW4Depth];
 #pragma unroll
     for (int d = 0; d < kW4Depth; d++)
-        if (a + d < b) w4_load(buf[d], w, a + d, lane);
+        if (a + d < b) w4_load<kGroups, kZeros>(buf[d], at, d);
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the RMSNorm's rows
     for (int i = threadIdx.x; i < kNt * 8 * chunks * 16; i += kW4Warps * 32) {
         const int row = i / (chunks * 16), c = i % (chunks * 16);
@@ -267,26 +288,27 @@ lm_head_w4_kernel(const __nv_bfloat16* x, const __grid_constant__ W4View w, cons
         for (int j = 0; j < 4; j++) acc[n][j] = 0.0f;
     int tile = a / chunks, c = a - tile * chunks;
     bool begun = c == 0;
-    for (int u = a; u < b; u += kW4Depth) {
+    const unsigned char* xl = xs + g * pitch + q * 16;
+    const unsigned char* xc = xl + c * 256;
+    for (int left = b - a; left > 0; left -= kW4Depth) {
+        at.codes += kW4Depth * kUnitCodes;
+        at.scales += kW4Depth * 32 * kGroups;
+        if (kZeros) at.zeros += kW4Depth * 16 * kGroups;
 #pragma unroll
         for (int d = 0; d < kW4Depth; d++) {
-            if (u + d >= b) break;
-            const unsigned char* xc = xs + g * pitch + c * 256 + q * 16;
+            if (d >= left) break;
             const uint32_t* lo = reinterpret_cast<const uint32_t*>(&buf[d].lo);
             const uint32_t* hi = reinterpret_cast<const uint32_t*>(&buf[d].hi);
 #pragma unroll
             for (int j = 0; j < kGroups; j++) {
                 uint32_t zl = 0x43084308u, zh = 0x43084308u;
-                if (w.zeros) {
+                if (kZeros) {
                     const uint32_t z = buf[d].zeros[j / 2] >> (16 * (j & 1));
                     zl = 0x43004300u | ((z & 0xFFu) * 0x00010001u);
                     zh = 0x43004300u | (((z >> 8) & 0xFFu) * 0x00010001u);
                 }
-                float part[kNt][4];
-#pragma unroll
-                for (int n = 0; n < kNt; n++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) part[n][k] = 0.0f;
+                // two chains of sums a group, so that an mma does not wait for the one before it
+                float part[2][kNt][4];
 #pragma unroll
                 for (int k = 0; k < 4 / kGroups; k++) {
                     const int word = j * (4 / kGroups) + k;
@@ -299,22 +321,26 @@ lm_head_w4_kernel(const __nv_bfloat16* x, const __grid_constant__ W4View w, cons
 #pragma unroll
                     for (int n = 0; n < kNt; n++) {
                         const uint4 xv = *reinterpret_cast<const uint4*>(xc + n * 8 * pitch + word * 64);
-                        mma_bf16(part[n], al[0], ah[0], al[1], ah[1], xv.x, xv.y);
-                        mma_bf16(part[n], al[2], ah[2], al[3], ah[3], xv.z, xv.w);
+                        if (k == 0) {
+                            mma_bf16_first(part[0][n], al[0], ah[0], al[1], ah[1], xv.x, xv.y);
+                            mma_bf16_first(part[1][n], al[2], ah[2], al[3], ah[3], xv.z, xv.w);
+                        } else {
+                            mma_bf16(part[0][n], al[0], ah[0], al[1], ah[1], xv.x, xv.y);
+                            mma_bf16(part[1][n], al[2], ah[2], al[3], ah[3], xv.z, xv.w);
+                        }
                     }
                 }
                 const float sl = scale_of(buf[d].scales[j] & 0xFFFFu, f16), sh = scale_of(buf[d].scales[j] >> 16, f16);
 #pragma unroll
-                for (int n = 0; n < kNt; n++) {
-                    acc[n][0] = __fmaf_rn(sl, part[n][0], acc[n][0]);
-                    acc[n][1] = __fmaf_rn(sl, part[n][1], acc[n][1]);
-                    acc[n][2] = __fmaf_rn(sh, part[n][2], acc[n][2]);
-                    acc[n][3] = __fmaf_rn(sh, part[n][3], acc[n][3]);
-                }
+                for (int n = 0; n < kNt; n++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        acc[n][k] = __fmaf_rn(k < 2 ? sl : sh, part[0][n][k] + part[1][n][k], acc[n][k]);
             }
-            if (u + d + kW4Depth < b) w4_load(buf[d], w, u + d + kW4Depth, lane);
+            if (d + kW4Depth < left) w4_load<kGroups, kZeros>(buf[d], at, d);
             const bool ends = ++c == chunks;
-            if (ends || u + d + 1 == b) {
+            xc += 256;
+            if (ends || d + 1 == left) {
                 if (ends && begun) {
                     w4_store<kNt>(acc, stage, o, w.vocab, tile, lane);
                 } else {
@@ -329,6 +355,7 @@ lm_head_w4_kernel(const __nv_bfloat16* x, const __grid_constant__ W4View w, cons
                     for (int j = 0; j < 4; j++) acc[n][j] = 0.0f;
                 if (ends) {
                     c = 0;
+                    xc = xl;
                     tile++;
                     begun = true;
                 }
@@ -358,10 +385,10 @@ static size_t w4_smem(int nt, int K) {
     return (size_t)nt * 8 * (w4_chunks(K) * 256 + 64) + (size_t)kW4Warps * nt * (2 * 512 + 256);
 }
 
-template <int kNt, int kGroups>
+template <int kNt, int kGroups, bool kZeros>
 static cudaError_t w4_go(const __nv_bfloat16* x, const W4View& w, const W4Out& o, int grid, cudaStream_t st) {
     const size_t smem = w4_smem(kNt, w.hidden);
-    cudaError_t e = cudaFuncSetAttribute(lm_head_w4_kernel<kNt, kGroups>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(lm_head_w4_kernel<kNt, kGroups, kZeros>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)smem);
     if (e != cudaSuccess) return e;
     // programmatic dependent launch: the first units are requested while the
@@ -376,14 +403,19 @@ static cudaError_t w4_go(const __nv_bfloat16* x, const W4View& w, const W4Out& o
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, lm_head_w4_kernel<kNt, kGroups>, x, w, o, w4_chunks(w.hidden), w4_tiles(w.vocab));
+    return cudaLaunchKernelEx(&cfg, lm_head_w4_kernel<kNt, kGroups, kZeros>, x, w, o, w4_chunks(w.hidden), w4_tiles(w.vocab));
+}
+
+template <int kNt, int kGroups>
+static cudaError_t w4_zeros(const __nv_bfloat16* x, const W4View& w, const W4Out& o, int grid, cudaStream_t st) {
+    return w.zeros ? w4_go<kNt, kGroups, true>(x, w, o, grid, st) : w4_go<kNt, kGroups, false>(x, w, o, grid, st);
 }
 
 template <int kNt>
 static cudaError_t w4_group(const __nv_bfloat16* x, const W4View& w, const W4Out& o, int grid, cudaStream_t st) {
-    return w.group == 128 ? w4_go<kNt, 1>(x, w, o, grid, st)
-         : w.group == 64  ? w4_go<kNt, 2>(x, w, o, grid, st)
-                          : w4_go<kNt, 4>(x, w, o, grid, st);
+    return w.group == 128 ? w4_zeros<kNt, 1>(x, w, o, grid, st)
+         : w.group == 64  ? w4_zeros<kNt, 2>(x, w, o, grid, st)
+                          : w4_zeros<kNt, 4>(x, w, o, grid, st);
 }
 
 cudaError_t launch_lm_head_w4(const __nv_bfloat16* normed, const W4View& w, __nv_bfloat16* logits, int batch,
