@@ -360,16 +360,22 @@ QS_API int qs_w4_pack(const void* d_plain_codes, const void* d_plain_scales, con
 
 /* qs_lm_head with such a weight:
  *   normed[b] as qs_lm_head's, logits[b] = bf16(normed[b] . w^T)
- * Products of codes and normed rows are exact; sums are fp32 per group, then
- * scaled and added in fp32.  d_hidden and d_normed bf16 [batch, hidden_dim],
- * d_logits bf16 [batch, vocab], all 16-byte aligned.  The weight is streamed
- * once per block of 8 to 32 rows (the most whose normed rows fit in shared
- * memory).  Allocates nothing. */
+ * A normed row is taken at the fp16 precision of its values scaled to its
+ * largest one, which is exact for those within 2^-28 of it; products with codes
+ * are then exact.  Sums are fp32 per group, less the zero point times the
+ * group's sum, then scaled and added in fp32.  d_hidden and d_normed bf16
+ * [batch, hidden_dim], d_logits bf16 [batch, vocab], all 16-byte aligned, as
+ * d_workspace is (qs_lm_head_w4_workspace bytes; calls that overlap on the GPU
+ * need workspaces of their own).  The weight is streamed once per block of 8 to
+ * 32 rows (the most that fit in shared memory).  Allocates nothing. */
+QS_API size_t qs_lm_head_w4_workspace(int batch, int hidden_dim, int group);
 QS_API int qs_lm_head_w4(const void* d_hidden, const void* d_norm_weight, const qs_w4_weight* weight,
-                         int batch, void* d_normed, void* d_logits, void* stream);
+                         int batch, void* d_normed, void* d_logits, void* d_workspace,
+                         size_t workspace_bytes, void* stream);
 
 /* qs_lm_head_sample with such a weight (weight->vocab must be the handle's):
- * qs_lm_head_w4 into the handle's workspace, then qs_sample on its logits. */
+ * qs_lm_head_w4 into the handle's workspace (a first call, and one with a new
+ * hidden_dim or group, may allocate it), then qs_sample on its logits. */
 QS_API int qs_lm_head_w4_sample(qs_sampler* s, const void* d_hidden, const void* d_norm_weight,
                                 const qs_w4_weight* weight, int batch, int* d_tokens, void* stream,
                                 unsigned flags);

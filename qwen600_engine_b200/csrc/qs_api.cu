@@ -154,6 +154,8 @@ struct qs_sampler {
     int* lh_err = nullptr;
     uint32_t* lh_segk = nullptr;  // [max_batch, lh_segs]: the epilogue's segment maxima (order keys)
     int lh_segs = 0;
+    void* lh_w4 = nullptr;  // the rows of a 4-bit projection (allocated by the first qs_lm_head_w4_sample call)
+    size_t lh_w4_bytes = 0;
     ExpFix fix() const { return ExpFix{exp_off, exp_ent, exp_bloom, (uint32_t)QS_EXP_NB}; }
     // the row kernel's hand-over from a row's chunk scans to its finishing CTA
     float* rs_segm = nullptr;
@@ -237,7 +239,7 @@ static void release(qs_sampler* s) {
     void* ptrs[] = {s->ov_n, s->ov_idx, s->ov_val, s->res, s->slow_list, s->slow_count,
                     s->tie_scratch, s->tie_pos, s->ring, s->hcount, s->hpos, s->token_counts, s->slot_counts,
                     s->rng, s->d_in, s->d_tok, s->exp_off, s->exp_ent, s->exp_bloom,
-                    s->lh_normed, s->lh_logits, s->lh_err, s->lh_segk, s->rs_segm, s->rs_done,
+                    s->lh_normed, s->lh_logits, s->lh_err, s->lh_segk, s->lh_w4, s->rs_segm, s->rs_done,
                     s->rs_gmax, s->rs_stash, s->rs_used, s->rs_chunk, s->rs_chunk_lb, s->rs_fb, s->st_hist, s->st_counts, s->st_count, s->st_rng, s->ph_row, s->ph_sel};
     for (void* p : ptrs)
         if (p) cudaFree(p);
@@ -1049,14 +1051,13 @@ static int w4_weight(const qs_w4_weight* w) {
 }
 
 static int w4_launch(const void* d_hidden, const void* d_norm_weight, const qs_w4_weight* w, int batch,
-                     __nv_bfloat16* normed, __nv_bfloat16* logits, int num_sms, cudaStream_t st,
+                     __nv_bfloat16* normed, __nv_bfloat16* logits, void* ws, int num_sms, cudaStream_t st,
                      uint32_t* segk = nullptr, int segk_stride = 0) {
     if (batch == 0) return QS_OK;
-    CK(launch_rmsnorm((const __nv_bfloat16*)d_hidden, (const __nv_bfloat16*)d_norm_weight, normed, batch,
-                      w->hidden_dim, st));
     const W4View v{(const unsigned char*)w->d_codes, w->d_scales, (const unsigned char*)w->d_zeros,
                    w->vocab, w->hidden_dim, w->group, w->scale_dtype};
-    CK(launch_lm_head_w4(normed, v, logits, batch, num_sms, segk, segk_stride, st));
+    CK(launch_lm_head_w4((const __nv_bfloat16*)d_hidden, (const __nv_bfloat16*)d_norm_weight, v, batch, normed, logits,
+                         (unsigned char*)ws, num_sms, segk, segk_stride, st));
     return QS_OK;
 }
 
@@ -1095,8 +1096,13 @@ int qs_w4_pack(const void* d_plain_codes, const void* d_plain_scales, const void
     return QS_OK;
 }
 
+size_t qs_lm_head_w4_workspace(int batch, int hidden_dim, int group) {
+    if (batch < 1 || hidden_dim < 1 || (group != 32 && group != 64 && group != 128)) return 16;
+    return w4_workspace(batch, hidden_dim, group);
+}
+
 int qs_lm_head_w4(const void* d_hidden, const void* d_norm_weight, const qs_w4_weight* weight, int batch,
-                  void* d_normed, void* d_logits, void* stream) {
+                  void* d_normed, void* d_logits, void* d_workspace, size_t workspace_bytes, void* stream) {
     g_err.clear();
     int rc = w4_weight(weight);
     if (rc) return rc;
@@ -1106,11 +1112,14 @@ int qs_lm_head_w4(const void* d_hidden, const void* d_norm_weight, const qs_w4_w
     if ((((uintptr_t)d_normed) | ((uintptr_t)d_logits)) & 15)
         return fail(QS_ERR_INVALID, "normed and logits must be 16-byte aligned");
     if (((uintptr_t)d_norm_weight) & 3) return fail(QS_ERR_INVALID, "norm_weight must be 4-byte aligned");
+    const size_t need = qs_lm_head_w4_workspace(batch, weight->hidden_dim, weight->group);
+    if (!d_workspace || workspace_bytes < need || (((uintptr_t)d_workspace) & 15))
+        return fail(QS_ERR_INVALID, "workspace is NULL, unaligned or below %zu bytes", need);
     int dev = 0, sms = 148;
     CK(cudaGetDevice(&dev));
     if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1) sms = 148;
-    return w4_launch(d_hidden, d_norm_weight, weight, batch, (__nv_bfloat16*)d_normed, (__nv_bfloat16*)d_logits, sms,
-                     (cudaStream_t)stream);
+    return w4_launch(d_hidden, d_norm_weight, weight, batch, (__nv_bfloat16*)d_normed, (__nv_bfloat16*)d_logits,
+                     d_workspace, sms, (cudaStream_t)stream);
 }
 
 int qs_lm_head_w4_sample(qs_sampler* s, const void* d_hidden, const void* d_norm_weight,
@@ -1128,9 +1137,16 @@ int qs_lm_head_w4_sample(qs_sampler* s, const void* d_hidden, const void* d_norm
     DeviceGuard dg(s->device);
     rc = tail_workspace(s, weight->hidden_dim);
     if (rc) return rc;
+    const size_t need = qs_lm_head_w4_workspace(s->max_batch, weight->hidden_dim, weight->group);
+    if (s->lh_w4_bytes < need) {
+        if (s->lh_w4) cudaFree(s->lh_w4);
+        s->lh_w4 = nullptr; s->lh_w4_bytes = 0;
+        CK(cudaMalloc(&s->lh_w4, need));
+        s->lh_w4_bytes = need;
+    }
     // the epilogue hands the sampler the segment maxima, as in qs_lm_head_sample
     uint32_t* segk = batch < kWideMinRows ? s->lh_segk : nullptr;
-    rc = w4_launch(d_hidden, d_norm_weight, weight, batch, s->lh_normed, s->lh_logits, s->num_sms,
+    rc = w4_launch(d_hidden, d_norm_weight, weight, batch, s->lh_normed, s->lh_logits, s->lh_w4, s->num_sms,
                    (cudaStream_t)stream, segk, s->lh_segs);
     if (rc) return rc;
     rc = sample_stateful(s, s->lh_logits, QS_BF16, batch, d_tokens, stream, flags, segk, s->lh_segs);

@@ -29,10 +29,9 @@
 #include <string.h>
 #include <cudaTypedefs.h>
 
-#include <cub/block/block_reduce.cuh>
-
 #include "qs_common.cuh"
 #include "qs_pipe.cuh"
+#include "qs_rmsnorm.cuh"
 
 namespace qs {
 
@@ -392,37 +391,16 @@ cudaError_t launch_shard_handshake(void* const* bufs, size_t flag_off, int nrank
 }
 
 // Restates rms_norm_kernel (qwen_model.cuh:125-177) for one row per CTA.
-constexpr int kNormThreads = 256;
-
 __global__ void __launch_bounds__(kNormThreads)
 rmsnorm_rows_kernel(const __nv_bfloat16* __restrict__ X, const __nv_bfloat16* __restrict__ w,
                     __nv_bfloat16* __restrict__ Y, int D, float inv_d, float eps) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the lm_head may start its set-up
-    const int t = threadIdx.x;
     const int half = D / 2;
     const __nv_bfloat162* in = reinterpret_cast<const __nv_bfloat162*>(X + (size_t)blockIdx.x * D);
     const __nv_bfloat162* wt = reinterpret_cast<const __nv_bfloat162*>(w);
     __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(Y + (size_t)blockIdx.x * D);
-    float lsum = 0.0f;
-    for (int i = t; i < half; i += kNormThreads) {
-        const float2 v = __bfloat1622float2(in[i]);
-        lsum = __fmaf_rn(v.x, v.x, lsum);
-        lsum = __fmaf_rn(v.y, v.y, lsum);
-    }
-    using BlockReduce = cub::BlockReduce<float, kNormThreads>;
-    __shared__ typename BlockReduce::TempStorage tmp;
-    const float total = BlockReduce(tmp).Sum(lsum);
-    __shared__ float mul;
-    if (t == 0) mul = rsqrtf(__fmaf_rn(total, inv_d, eps));
-    __syncthreads();
-    const float m = mul;
-    for (int i = t; i < half; i += kNormThreads) {
-        float2 v = __bfloat1622float2(in[i]);
-        const float2 g = wt ? __bfloat1622float2(wt[i]) : make_float2(1.0f, 1.0f);
-        v.x = __fmul_rn(__fmul_rn(v.x, m), g.x);
-        v.y = __fmul_rn(__fmul_rn(v.y, m), g.y);
-        o[i] = __float22bfloat162_rn(v);
-    }
+    const float m = rms_factor(in, half, inv_d, eps);
+    for (int i = threadIdx.x; i < half; i += kNormThreads) o[i] = rms_scaled(in[i], m, wt, i);
 }
 
 // ------------------------------------------------------------- host side
@@ -548,7 +526,7 @@ cudaError_t launch_lm_head_shard(const __nv_bfloat16* normed, const __nv_bfloat1
 
 cudaError_t launch_rmsnorm(const __nv_bfloat16* x, const __nv_bfloat16* w, __nv_bfloat16* y, int B, int D,
                            cudaStream_t stream) {
-    rmsnorm_rows_kernel<<<B, kNormThreads, 0, stream>>>(x, w, y, D, 1.0f / (float)D, 1e-6f);
+    rmsnorm_rows_kernel<<<B, kNormThreads, 0, stream>>>(x, w, y, D, 1.0f / (float)D, kNormEps);
     return cudaGetLastError();
 }
 

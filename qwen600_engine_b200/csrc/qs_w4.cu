@@ -3,18 +3,26 @@
 //
 // Bound: the stream of the codes.  For 151,936 x 1024 that is 78 MB, 12.3 us at
 // the measured 6549 GB/s, so all else has to fit beside 23 bytes a clock and
-// SM: the codes go from memory to registers (no staging), become bf16 pairs
-// with 11 instructions per 8 codes, and meet the tokens on mma.sync
-// m16n8k16: 16 vocabulary rows x 8 tokens, tokens on the narrow side.  (tcgen05
-// takes its wider operand from shared or tensor memory; 4-bit weights would
-// have to be written there as bf16, four times the bytes of their stream.)
+// SM.  What counts is the instructions a code costs.  Codes go from memory to
+// registers and meet the tokens on mma.sync m16n8k16, 16 vocabulary rows x 8
+// tokens, tokens on the narrow side.  A code needs no conversion: as the low
+// bits of an fp16 number, q is the number q 2^-24 and 16 q is 16 q 2^-24, so a
+// word of 8 codes becomes four operand registers with one shift and four
+// ands.  (Made into bf16 pairs, shift, and / or, subtract, it took 11
+// instructions, and 21.4 us instead of REPLACE for one token.)  The tokens are
+// scaled by a power of two to fp16 (exact for values within 2^-28 of a row's
+// largest), the columns that meet 16 q by another 1 / 16, and the zero point is
+// taken out of a group's sum: sum (q - z) x = sum q x - z sum x, with the
+// group's sum x made once per launch.  (tcgen05 takes its wider operand
+// from shared or tensor memory; 4-bit weights would have to be written there
+// as 16-bit numbers, four times the bytes of their stream.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include "qs_common.cuh"
 #include "qs_w4.h"
-#include "qs_pipe.cuh"
+#include "qs_rmsnorm.cuh"
 
 namespace qs {
 
@@ -59,9 +67,9 @@ cudaError_t launch_w4_quantize(const __nv_bfloat16* w, int V, int K, int group, 
 // after another, tile by tile.  In a unit lane l = 4 g + q of a warp finds
 // 16 bytes for row g (first 512 bytes) and 16 for row g + 8: four words, word
 // w for columns 32 w + 8 q + 0..7 of the chunk.  Nibble i < 4 of a word is
-// column 2 i, nibble i + 4 column 2 i + 1, so (word >> 4 i) & 0x000F000F is a
-// pair of neighbouring columns, one in each half.  A group of 32 columns is
-// then one word of every lane, and any group is whole mma instructions.
+// column 2 i, nibble i + 4 column 2 i + 1, so masks take pairs of neighbouring
+// columns, one in each half.  A group of 32 columns is then one word of every
+// lane, and any group is whole mma instructions.
 // Scales (16-bit) and zero points (bytes) of a unit: [g][group of the chunk]
 // [row g, row g + 8].
 constexpr int kUnitCodes = 1024;
@@ -113,36 +121,109 @@ cudaError_t launch_w4_pack(const unsigned char* codes, const void* scales, const
     return cudaGetLastError();
 }
 
+// -------------------------------------------------------------------- rows
+// RMSNorm of one token's row per CTA, and the row as the products take it, in
+// the workspace: fp16 columns scaled by 2^s so that the largest finite value
+// lies in [2^14, 2^15) (columns 2, 3, 6 and 7 of each 8 meet 16 q and get
+// 2^(s - 4)), the sums of its groups' columns times 2^(s - 24) (the products'
+// scale), and 2^(24 - s) as two factors.
+__host__ __device__ static inline size_t w4_row_bytes(int chunks, int groups) {
+    return (size_t)chunks * 256 + 16 + (((size_t)chunks * groups * 4 + 15) & ~(size_t)15);
+}
+
+constexpr int kW4Pairs = kW4MaxHidden / 2 / kNormThreads;  // column pairs of a thread
+
+__global__ void __launch_bounds__(kNormThreads)
+w4_rows_kernel(const __nv_bfloat16* __restrict__ X, const __nv_bfloat16* __restrict__ w, __nv_bfloat16* __restrict__ Y,
+               int K, int chunks, int groups, unsigned char* __restrict__ ws, float inv_d, float eps) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the projection may request its first codes
+    __shared__ float red_max[kNormThreads / 32], red_sum[kW4Pairs][kNormThreads / 32];
+    const int t = threadIdx.x, warp = t >> 5, half = K / 2;
+    const __nv_bfloat162* in = reinterpret_cast<const __nv_bfloat162*>(X + (size_t)blockIdx.x * K);
+    __nv_bfloat162* out = reinterpret_cast<__nv_bfloat162*>(Y + (size_t)blockIdx.x * K);
+    ws += blockIdx.x * w4_row_bytes(chunks, groups);
+    uint32_t* xs = reinterpret_cast<uint32_t*>(ws);
+    float2* unscale = reinterpret_cast<float2*>(ws + (size_t)chunks * 256);
+    float* sums = reinterpret_cast<float*>(ws + (size_t)chunks * 256 + 16);
+    const float mul = rms_factor(in, half, inv_d, eps);
+    float2 y[kW4Pairs];
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kW4Pairs; j++) {
+        const int i = j * kNormThreads + t;
+        y[j] = make_float2(0.0f, 0.0f);
+        if (i < half) {
+            const __nv_bfloat162 b = rms_scaled(in[i], mul, reinterpret_cast<const __nv_bfloat162*>(w), i);
+            out[i] = b;
+            y[j] = __bfloat1622float2(b);
+            const float a0 = fabsf(y[j].x), a1 = fabsf(y[j].y);
+            if (a0 < INFINITY) m = fmaxf(m, a0);
+            if (a1 < INFINITY) m = fmaxf(m, a1);
+        }
+    }
+    m = warp_max(m);
+    if ((t & 31) == 0) red_max[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kNormThreads / 32; k++) m = fmaxf(m, red_max[k]);
+    const int e = (int)(__float_as_uint(m) >> 23) - 127;
+    const int s = m == 0.0f ? 0 : min(14 - e, 120);
+    const float up = __uint_as_float((uint32_t)(s + 127) << 23), f = t & 1 ? 0.0625f : 1.0f;
+    if (t == 0) {
+        const int h = (24 - s) >> 1, r = 24 - s - h;
+        *unscale = make_float2(__uint_as_float((uint32_t)(h + 127) << 23), __uint_as_float((uint32_t)(r + 127) << 23));
+    }
+    const int per = 64 / groups;  // pairs of a group: 16, 32 or 64
+#pragma unroll
+    for (int j = 0; j < kW4Pairs; j++) {
+        const int i = j * kNormThreads + t;
+        if (j * kNormThreads + warp * 32 >= chunks * 64) break;  // alike for the warp: 64 pairs a chunk
+        const float a = y[j].x * up, b = y[j].y * up;
+        const __half2 h = __floats2half2_rn(a * f, b * f);
+        xs[i] = *reinterpret_cast<const uint32_t*>(&h);
+        float sum = (a + b) * 0x1p-24f;
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (per == 16) {
+            if ((t & 15) == 0) sums[i / 16] = sum;
+        } else {
+            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+            if (per == 32) {
+                if ((t & 31) == 0) sums[i / 32] = sum;
+            } else if ((t & 31) == 0) {
+                red_sum[j][warp] = sum;
+            }
+        }
+    }
+    if (per == 64) {
+        __syncthreads();
+        for (int i = t; i < chunks; i += kNormThreads) {
+            const int j = i / 4, k = (i & 3) * 2;
+            sums[i] = red_sum[j][k] + red_sum[j][k + 1];
+        }
+    }
+}
+
 // -------------------------------------------------------------- projection
 constexpr int kW4Warps = 16;
 constexpr int kW4Depth = 4;  // units a warp has in flight
 
 // d = a * b + c on 16 x 8 x 16; c in registers, or 0.
-__device__ __forceinline__ void mma_bf16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+__device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16_first(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+__device__ __forceinline__ void mma_first(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                                uint32_t b1) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%10, %10, %10, %10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
-}
-
-// Codes 2 i and 2 i + 1 of a word minus the zero point, as bf16: 0x4300 | q is
-// 128 + q, and the difference of 128 + q and 128 + z is exact.
-__device__ __forceinline__ uint32_t code_pair(uint32_t word, int i, uint32_t zero) {
-    uint32_t q;  // (word >> 4 i) & 0x000F000F | 0x43004300, the two in one instruction
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(q) : "r"(word >> (4 * i)), "r"(0x000F000Fu), "r"(0x43004300u));
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&q),
-                                     *reinterpret_cast<const __nv_bfloat162*>(&zero));
-    return *reinterpret_cast<const uint32_t*>(&d);
 }
 
 __device__ __forceinline__ float scale_of(uint32_t bits, bool f16) {
@@ -211,15 +292,18 @@ struct W4Out {
 // Stores a finished tile: 16 vocabulary rows of up to 8 kNt tokens, through the
 // warp's staging rows so that a lane stores 16 bytes of one token.
 template <int kNt>
-__device__ __forceinline__ void w4_store(const float (&acc)[kNt][4], __nv_bfloat16* stage, const W4Out& o, int V, int tile,
-                                         int lane) {
+__device__ __forceinline__ void w4_store(const float (&acc)[kNt][4], const float2* unscale, __nv_bfloat16* stage,
+                                         const W4Out& o, int V, int tile, int lane) {
     const int g = lane >> 2, q = lane & 3;
     __syncwarp();
 #pragma unroll
     for (int n = 0; n < kNt; n++) {
 #pragma unroll
-        for (int j = 0; j < 4; j++)  // j: row g or g + 8, token 2 q or 2 q + 1
-            stage[(n * 8 + 2 * q + (j & 1)) * 16 + g + (j >> 1) * 8] = __float2bfloat16_rn(acc[n][j]);
+        for (int j = 0; j < 4; j++) {  // j: row g or g + 8, token 2 q or 2 q + 1
+            const int token = n * 8 + 2 * q + (j & 1);
+            const float2 f = unscale[token];
+            stage[token * 16 + g + (j >> 1) * 8] = __float2bfloat16_rn(acc[n][j] * f.x * f.y);
+        }
     }
     __syncwarp();
     for (int p = lane; p < kNt * 16; p += 32) {
@@ -248,13 +332,15 @@ __device__ __forceinline__ void w4_store(const float (&acc)[kNt][4], __nv_bfloat
 // kNt blocks of 8 tokens, kGroups groups in a chunk.
 template <int kNt, int kGroups, bool kZeros>
 __global__ void __launch_bounds__(kW4Warps * 32, 1)
-lm_head_w4_kernel(const __nv_bfloat16* x, const __grid_constant__ W4View w, const __grid_constant__ W4Out o, int chunks,
+lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, const __grid_constant__ W4Out o, int chunks,
                   int tiles) {
     extern __shared__ __align__(16) unsigned char smem[];
     const int pitch = chunks * 256 + 64;  // bytes of a token's row: neighbours 64 bytes apart in the banks
-    unsigned char* xs = smem;
+    unsigned char* xs = smem;                                           // fp16 rows
     float4* slots = reinterpret_cast<float4*>(smem + kNt * 8 * pitch);  // [warp][continued, begun][kNt][lane]
     __nv_bfloat16* stage = reinterpret_cast<__nv_bfloat16*>(slots + kW4Warps * 2 * kNt * 32);
+    float2* unscale = reinterpret_cast<float2*>(stage + kW4Warps * kNt * 128);  // [token] two factors
+    float* sums = reinterpret_cast<float*>(unscale + kNt * 8);                  // [group][token] sum of its columns
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     stage += warp * kNt * 128;
     const int t0 = (int)((long long)blockIdx.x * tiles / gridDim.x), t1 = (int)((long long)(blockIdx.x + 1) * tiles / gridDim.x);
@@ -271,12 +357,17 @@ lm_head_w4_kernel(const __nv_bfloat16* x, const __grid_constant__ W4View w, cons
     for (int d = 0; d < kW4Depth; d++)
         if (a + d < b) w4_load<kGroups, kZeros>(buf[d], at, d);
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the RMSNorm's rows
+    const size_t row_bytes = w4_row_bytes(chunks, kGroups);
     for (int i = threadIdx.x; i < kNt * 8 * chunks * 16; i += kW4Warps * 32) {
-        const int row = i / (chunks * 16), c = i % (chunks * 16);
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (row < o.tokens && c * 8 < w.hidden)
-            v = *reinterpret_cast<const uint4*>(x + (size_t)row * w.hidden + c * 8);
-        *reinterpret_cast<uint4*>(xs + row * pitch + c * 16) = v;
+        const int row = i / (chunks * 16), c = i - row * (chunks * 16);
+        *reinterpret_cast<uint4*>(xs + row * pitch + c * 16) =
+            row < o.tokens ? *reinterpret_cast<const uint4*>(rows + row * row_bytes + c * 16) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    for (int i = threadIdx.x; i < kNt * 8 * (chunks * kGroups + 1); i += kW4Warps * 32) {
+        const int row = i % (kNt * 8), j = i / (kNt * 8);
+        const unsigned char* p = rows + row * row_bytes + chunks * 256;
+        if (j == 0) unscale[row] = row < o.tokens ? *reinterpret_cast<const float2*>(p) : make_float2(0.0f, 0.0f);
+        else sums[i - kNt * 8] = row < o.tokens ? reinterpret_cast<const float*>(p + 16)[j - 1] : 0.0f;
     }
     __syncthreads();
 
@@ -290,6 +381,8 @@ lm_head_w4_kernel(const __nv_bfloat16* x, const __grid_constant__ W4View w, cons
     bool begun = c == 0;
     const unsigned char* xl = xs + g * pitch + q * 16;
     const unsigned char* xc = xl + c * 256;
+    const float* sl0 = sums + 2 * q;
+    const float* sc = sl0 + c * kGroups * kNt * 8;
     for (int left = b - a; left > 0; left -= kW4Depth) {
         at.codes += kW4Depth * kUnitCodes;
         at.scales += kW4Depth * 32 * kGroups;
@@ -301,48 +394,52 @@ lm_head_w4_kernel(const __nv_bfloat16* x, const __grid_constant__ W4View w, cons
             const uint32_t* hi = reinterpret_cast<const uint32_t*>(&buf[d].hi);
 #pragma unroll
             for (int j = 0; j < kGroups; j++) {
-                uint32_t zl = 0x43084308u, zh = 0x43084308u;
-                if (kZeros) {
-                    const uint32_t z = buf[d].zeros[j / 2] >> (16 * (j & 1));
-                    zl = 0x43004300u | ((z & 0xFFu) * 0x00010001u);
-                    zh = 0x43004300u | (((z >> 8) & 0xFFu) * 0x00010001u);
-                }
                 // two chains of sums a group, so that an mma does not wait for the one before it
                 float part[2][kNt][4];
 #pragma unroll
                 for (int k = 0; k < 4 / kGroups; k++) {
                     const int word = j * (4 / kGroups) + k;
-                    uint32_t al[4], ah[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        al[i] = code_pair(lo[word], i, zl);
-                        ah[i] = code_pair(hi[word], i, zh);
-                    }
+                    const uint32_t l8 = lo[word] >> 8, h8 = hi[word] >> 8;
+                    const uint32_t al[4] = {lo[word] & 0x000F000Fu, lo[word] & 0x00F000F0u, l8 & 0x000F000Fu,
+                                            l8 & 0x00F000F0u};
+                    const uint32_t ah[4] = {hi[word] & 0x000F000Fu, hi[word] & 0x00F000F0u, h8 & 0x000F000Fu,
+                                            h8 & 0x00F000F0u};
 #pragma unroll
                     for (int n = 0; n < kNt; n++) {
                         const uint4 xv = *reinterpret_cast<const uint4*>(xc + n * 8 * pitch + word * 64);
                         if (k == 0) {
-                            mma_bf16_first(part[0][n], al[0], ah[0], al[1], ah[1], xv.x, xv.y);
-                            mma_bf16_first(part[1][n], al[2], ah[2], al[3], ah[3], xv.z, xv.w);
+                            mma_first(part[0][n], al[0], ah[0], al[1], ah[1], xv.x, xv.y);
+                            mma_first(part[1][n], al[2], ah[2], al[3], ah[3], xv.z, xv.w);
                         } else {
-                            mma_bf16(part[0][n], al[0], ah[0], al[1], ah[1], xv.x, xv.y);
-                            mma_bf16(part[1][n], al[2], ah[2], al[3], ah[3], xv.z, xv.w);
+                            mma(part[0][n], al[0], ah[0], al[1], ah[1], xv.x, xv.y);
+                            mma(part[1][n], al[2], ah[2], al[3], ah[3], xv.z, xv.w);
                         }
                     }
                 }
                 const float sl = scale_of(buf[d].scales[j] & 0xFFFFu, f16), sh = scale_of(buf[d].scales[j] >> 16, f16);
+                float zl = -8.0f, zh = -8.0f;
+                if (kZeros) {
+                    const uint32_t z = buf[d].zeros[j / 2] >> (16 * (j & 1));
+                    zl = -(float)(z & 0xFFu);
+                    zh = -(float)((z >> 8) & 0xFFu);
+                }
 #pragma unroll
-                for (int n = 0; n < kNt; n++)
+                for (int n = 0; n < kNt; n++) {
+                    const float2 sx = *reinterpret_cast<const float2*>(sc + j * kNt * 8 + n * 8);
 #pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        acc[n][k] = __fmaf_rn(k < 2 ? sl : sh, part[0][n][k] + part[1][n][k], acc[n][k]);
+                    for (int k = 0; k < 4; k++) {
+                        const float sum = __fmaf_rn(k < 2 ? zl : zh, k & 1 ? sx.y : sx.x, part[0][n][k] + part[1][n][k]);
+                        acc[n][k] = __fmaf_rn(k < 2 ? sl : sh, sum, acc[n][k]);
+                    }
+                }
             }
             if (d + kW4Depth < left) w4_load<kGroups, kZeros>(buf[d], at, d);
             const bool ends = ++c == chunks;
             xc += 256;
+            sc += kGroups * kNt * 8;
             if (ends || d + 1 == left) {
                 if (ends && begun) {
-                    w4_store<kNt>(acc, stage, o, w.vocab, tile, lane);
+                    w4_store<kNt>(acc, unscale, stage, o, w.vocab, tile, lane);
                 } else {
 #pragma unroll
                     for (int n = 0; n < kNt; n++)
@@ -356,6 +453,7 @@ lm_head_w4_kernel(const __nv_bfloat16* x, const __grid_constant__ W4View w, cons
                 if (ends) {
                     c = 0;
                     xc = xl;
+                    sc = sl0;
                     tile++;
                     begun = true;
                 }
@@ -377,17 +475,18 @@ lm_head_w4_kernel(const __nv_bfloat16* x, const __grid_constant__ W4View w, cons
             }
             first = (wi + 1) * 2;
         }
-        w4_store<kNt>(acc, stage, o, w.vocab, last, lane);
+        w4_store<kNt>(acc, unscale, stage, o, w.vocab, last, lane);
     }
 }
 
-static size_t w4_smem(int nt, int K) {
-    return (size_t)nt * 8 * (w4_chunks(K) * 256 + 64) + (size_t)kW4Warps * nt * (2 * 512 + 256);
+static size_t w4_smem(int nt, int K, int group) {
+    return (size_t)nt * 8 * (w4_chunks(K) * 256 + 64) + (size_t)kW4Warps * nt * (2 * 512 + 256) +
+           (size_t)nt * 8 * (sizeof(float2) + w4_chunks(K) * (128 / group) * sizeof(float));
 }
 
 template <int kNt, int kGroups, bool kZeros>
-static cudaError_t w4_go(const __nv_bfloat16* x, const W4View& w, const W4Out& o, int grid, cudaStream_t st) {
-    const size_t smem = w4_smem(kNt, w.hidden);
+static cudaError_t w4_go(const unsigned char* rows, const W4View& w, const W4Out& o, int grid, cudaStream_t st) {
+    const size_t smem = w4_smem(kNt, w.hidden, w.group);
     cudaError_t e = cudaFuncSetAttribute(lm_head_w4_kernel<kNt, kGroups, kZeros>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)smem);
     if (e != cudaSuccess) return e;
@@ -403,35 +502,43 @@ static cudaError_t w4_go(const __nv_bfloat16* x, const W4View& w, const W4Out& o
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, lm_head_w4_kernel<kNt, kGroups, kZeros>, x, w, o, w4_chunks(w.hidden), w4_tiles(w.vocab));
+    return cudaLaunchKernelEx(&cfg, lm_head_w4_kernel<kNt, kGroups, kZeros>, rows, w, o, w4_chunks(w.hidden), w4_tiles(w.vocab));
 }
 
 template <int kNt, int kGroups>
-static cudaError_t w4_zeros(const __nv_bfloat16* x, const W4View& w, const W4Out& o, int grid, cudaStream_t st) {
-    return w.zeros ? w4_go<kNt, kGroups, true>(x, w, o, grid, st) : w4_go<kNt, kGroups, false>(x, w, o, grid, st);
+static cudaError_t w4_zeros(const unsigned char* rows, const W4View& w, const W4Out& o, int grid, cudaStream_t st) {
+    return w.zeros ? w4_go<kNt, kGroups, true>(rows, w, o, grid, st) : w4_go<kNt, kGroups, false>(rows, w, o, grid, st);
 }
 
 template <int kNt>
-static cudaError_t w4_group(const __nv_bfloat16* x, const W4View& w, const W4Out& o, int grid, cudaStream_t st) {
-    return w.group == 128 ? w4_zeros<kNt, 1>(x, w, o, grid, st)
-         : w.group == 64  ? w4_zeros<kNt, 2>(x, w, o, grid, st)
-                          : w4_zeros<kNt, 4>(x, w, o, grid, st);
+static cudaError_t w4_group(const unsigned char* rows, const W4View& w, const W4Out& o, int grid, cudaStream_t st) {
+    return w.group == 128 ? w4_zeros<kNt, 1>(rows, w, o, grid, st)
+         : w.group == 64  ? w4_zeros<kNt, 2>(rows, w, o, grid, st)
+                          : w4_zeros<kNt, 4>(rows, w, o, grid, st);
 }
 
-cudaError_t launch_lm_head_w4(const __nv_bfloat16* normed, const W4View& w, __nv_bfloat16* logits, int batch,
-                              int num_sms, uint32_t* segk, int segk_stride, cudaStream_t st) {
+size_t w4_workspace(int batch, int K, int group) { return (size_t)batch * w4_row_bytes(w4_chunks(K), 128 / group); }
+
+cudaError_t launch_lm_head_w4(const __nv_bfloat16* hidden, const __nv_bfloat16* norm_weight, const W4View& w, int batch,
+                              __nv_bfloat16* normed, __nv_bfloat16* logits, unsigned char* ws, int num_sms,
+                              uint32_t* segk, int segk_stride, cudaStream_t st) {
+    const int chunks = w4_chunks(w.hidden), groups = 128 / w.group;
+    w4_rows_kernel<<<batch, kNormThreads, 0, st>>>(hidden, norm_weight, normed, w.hidden, chunks, groups, ws,
+                                                  1.0f / (float)w.hidden, kNormEps);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
     const int tiles = w4_tiles(w.vocab), grid = tiles < num_sms ? tiles : num_sms;
     int most = 4;  // blocks of 8 tokens whose rows fit in shared memory
-    while (w4_smem(most, w.hidden) > 227 * 1024) most--;
+    while (w4_smem(most, w.hidden, w.group) > 227 * 1024) most--;
     for (int b = 0; b < batch;) {
         const int left = (batch - b + 7) / 8, nt = left < most ? left : most;
         const int n = batch - b < nt * 8 ? batch - b : nt * 8;
         const W4Out o{logits + (size_t)b * w.vocab, n, segk ? segk + (size_t)b * segk_stride : nullptr, segk_stride};
-        const __nv_bfloat16* x = normed + (size_t)b * w.hidden;
-        const cudaError_t e = nt == 1 ? w4_group<1>(x, w, o, grid, st)
-                            : nt == 2 ? w4_group<2>(x, w, o, grid, st)
-                            : nt == 3 ? w4_group<3>(x, w, o, grid, st)
-                                      : w4_group<4>(x, w, o, grid, st);
+        const unsigned char* rows = ws + b * w4_row_bytes(chunks, groups);
+        e = nt == 1 ? w4_group<1>(rows, w, o, grid, st)
+          : nt == 2 ? w4_group<2>(rows, w, o, grid, st)
+          : nt == 3 ? w4_group<3>(rows, w, o, grid, st)
+                    : w4_group<4>(rows, w, o, grid, st);
         if (e != cudaSuccess) return e;
         b += n;
     }

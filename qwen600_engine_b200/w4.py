@@ -113,8 +113,11 @@ def lm_head_w4(hidden, weight: W4Weight, norm_weight=None, *, stream=None):
         normed = torch.empty((B, weight.hidden_dim), dtype=torch.bfloat16, device=dev)
         logits = torch.empty((B, weight.vocab), dtype=torch.bfloat16, device=dev)
         if B:
+            size = _lib.lib.qs_lm_head_w4_workspace(B, weight.hidden_dim, weight.group)
+            work = torch.empty(size, dtype=torch.uint8, device=dev)
             check(_lib.lib.qs_lm_head_w4(h.data_ptr(), None if norm_weight is None else norm_weight.data_ptr(),
-                                         C.byref(weight._w4_desc), B, normed.data_ptr(), logits.data_ptr(), st))
+                                         C.byref(weight._w4_desc), B, normed.data_ptr(), logits.data_ptr(),
+                                         work.data_ptr(), size, st))
     return normed, logits
 
 

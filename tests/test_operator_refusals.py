@@ -88,20 +88,23 @@ BAD_WEIGHTS = [(dict(vocab=0), QS_ERR_UNSUPPORTED), (dict(vocab=1 << 20), QS_ERR
 @pytest.mark.parametrize("bad,code", BAD_WEIGHTS)
 def test_w4_weight_refused(bad, code):
     w = weight(**bad)
-    assert L.qs_lm_head_w4(P, None, C.byref(w), 1, P, P, None) == code
+    assert L.qs_lm_head_w4(P, None, C.byref(w), 1, P, P, P, 1 << 20, None) == code
     assert L.qs_last_error()
 
 
 def test_w4_calls_refused():
     w = weight()
     r = C.byref(w)
-    assert L.qs_lm_head_w4(P, None, None, 1, P, P, None) == QS_ERR_INVALID
-    assert L.qs_lm_head_w4(None, None, r, 1, P, P, None) == QS_ERR_INVALID
-    assert L.qs_lm_head_w4(P + 4, None, r, 1, P, P, None) == QS_ERR_INVALID
-    assert L.qs_lm_head_w4(P, None, r, -1, P, P, None) == QS_ERR_INVALID
-    assert L.qs_lm_head_w4(P, None, r, 1, None, P, None) == QS_ERR_INVALID
-    assert L.qs_lm_head_w4(P, None, r, 1, P, P + 2, None) == QS_ERR_INVALID
-    assert L.qs_lm_head_w4(P, P + 2, r, 1, P, P, None) == QS_ERR_INVALID
+    assert L.qs_lm_head_w4(P, None, None, 1, P, P, P, 1 << 20, None) == QS_ERR_INVALID
+    assert L.qs_lm_head_w4(None, None, r, 1, P, P, P, 1 << 20, None) == QS_ERR_INVALID
+    assert L.qs_lm_head_w4(P + 4, None, r, 1, P, P, P, 1 << 20, None) == QS_ERR_INVALID
+    assert L.qs_lm_head_w4(P, None, r, -1, P, P, P, 1 << 20, None) == QS_ERR_INVALID
+    assert L.qs_lm_head_w4(P, None, r, 1, None, P, P, 1 << 20, None) == QS_ERR_INVALID
+    assert L.qs_lm_head_w4(P, None, r, 1, P, P + 2, P, 1 << 20, None) == QS_ERR_INVALID
+    assert L.qs_lm_head_w4(P, P + 2, r, 1, P, P, P, 1 << 20, None) == QS_ERR_INVALID
+    assert L.qs_lm_head_w4(P, None, r, 1, P, P, None, 1 << 20, None) == QS_ERR_INVALID
+    assert L.qs_lm_head_w4(P, None, r, 1, P, P, P + 8, 1 << 20, None) == QS_ERR_INVALID
+    assert L.qs_lm_head_w4(P, None, r, 1, P, P, P, 64, None) == QS_ERR_INVALID
     assert L.qs_lm_head_w4_sample(None, P, None, r, 1, P, None, 0) == QS_ERR_INVALID
     assert L.qs_w4_pack(P, P, None, 1000, 1024, 128, QS_F32, P, P, None, None) == QS_ERR_INVALID
     assert L.qs_w4_pack(P, P, P, 1000, 1024, 128, QS_BF16, P, P, None, None) == QS_ERR_INVALID
