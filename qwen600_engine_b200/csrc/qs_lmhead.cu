@@ -399,8 +399,11 @@ rmsnorm_rows_kernel(const __nv_bfloat16* __restrict__ X, const __nv_bfloat16* __
     const __nv_bfloat162* in = reinterpret_cast<const __nv_bfloat162*>(X + (size_t)blockIdx.x * D);
     const __nv_bfloat162* wt = reinterpret_cast<const __nv_bfloat162*>(w);
     __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(Y + (size_t)blockIdx.x * D);
-    const float m = rms_factor(in, half, inv_d, eps);
-    for (int i = threadIdx.x; i < half; i += kNormThreads) o[i] = rms_scaled(in[i], m, wt, i);
+    float lsum = 0.0f;
+    for (int i = threadIdx.x; i < half; i += kNormThreads) lsum = rms_add(lsum, in[i]);
+    const float m = rms_factor(lsum, inv_d, eps);
+    for (int i = threadIdx.x; i < half; i += kNormThreads)
+        o[i] = rms_scaled(in[i], m, wt ? __bfloat1622float2(wt[i]) : make_float2(1.0f, 1.0f));
 }
 
 // ------------------------------------------------------------- host side

@@ -11,14 +11,14 @@ namespace qs {
 constexpr int kNormThreads = 256;
 constexpr float kNormEps = 1e-6f;
 
-// The factor of a row of 2 * half values; the same for every thread.
-__device__ __forceinline__ float rms_factor(const __nv_bfloat162* in, int half, float inv_d, float eps) {
-    float lsum = 0.0f;
-    for (int i = threadIdx.x; i < half; i += kNormThreads) {
-        const float2 v = __bfloat1622float2(in[i]);
-        lsum = __fmaf_rn(v.x, v.x, lsum);
-        lsum = __fmaf_rn(v.y, v.y, lsum);
-    }
+// A thread's chain over its pairs threadIdx.x, + kNormThreads, ...
+__device__ __forceinline__ float rms_add(float lsum, __nv_bfloat162 x) {
+    const float2 v = __bfloat1622float2(x);
+    return __fmaf_rn(v.y, v.y, __fmaf_rn(v.x, v.x, lsum));
+}
+
+// The row's factor from the threads' chains; the same for every thread.
+__device__ __forceinline__ float rms_factor(float lsum, float inv_d, float eps) {
     using BlockReduce = cub::BlockReduce<float, kNormThreads>;
     __shared__ typename BlockReduce::TempStorage tmp;
     const float total = BlockReduce(tmp).Sum(lsum);
@@ -28,9 +28,8 @@ __device__ __forceinline__ float rms_factor(const __nv_bfloat162* in, int half, 
     return mul;
 }
 
-__device__ __forceinline__ __nv_bfloat162 rms_scaled(__nv_bfloat162 x, float m, const __nv_bfloat162* w, int i) {
+__device__ __forceinline__ __nv_bfloat162 rms_scaled(__nv_bfloat162 x, float m, float2 g) {
     float2 v = __bfloat1622float2(x);
-    const float2 g = w ? __bfloat1622float2(w[i]) : make_float2(1.0f, 1.0f);
     v.x = __fmul_rn(__fmul_rn(v.x, m), g.x);
     v.y = __fmul_rn(__fmul_rn(v.y, m), g.y);
     return __float22bfloat162_rn(v);

@@ -131,29 +131,42 @@ __host__ __device__ static inline size_t w4_row_bytes(int chunks, int groups) {
     return (size_t)chunks * 256 + 16 + (((size_t)chunks * groups * 4 + 15) & ~(size_t)15);
 }
 
-constexpr int kW4Pairs = kW4MaxHidden / 2 / kNormThreads;  // column pairs of a thread
-
+// kPairs: column pairs of a thread, the row's whole share, requested with its
+// norm weights before anything waits.
+template <int kPairs>
 __global__ void __launch_bounds__(kNormThreads)
 w4_rows_kernel(const __nv_bfloat16* __restrict__ X, const __nv_bfloat16* __restrict__ w, __nv_bfloat16* __restrict__ Y,
                int K, int chunks, int groups, unsigned char* __restrict__ ws, float inv_d, float eps) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the projection may request its first codes
-    __shared__ float red_max[kNormThreads / 32], red_sum[kW4Pairs][kNormThreads / 32];
+    __shared__ float red_max[kNormThreads / 32], red_sum[kPairs][kNormThreads / 32];
     const int t = threadIdx.x, warp = t >> 5, half = K / 2;
     const __nv_bfloat162* in = reinterpret_cast<const __nv_bfloat162*>(X + (size_t)blockIdx.x * K);
+    const __nv_bfloat162* wt = reinterpret_cast<const __nv_bfloat162*>(w);
     __nv_bfloat162* out = reinterpret_cast<__nv_bfloat162*>(Y + (size_t)blockIdx.x * K);
     ws += blockIdx.x * w4_row_bytes(chunks, groups);
     uint32_t* xs = reinterpret_cast<uint32_t*>(ws);
     float2* unscale = reinterpret_cast<float2*>(ws + (size_t)chunks * 256);
     float* sums = reinterpret_cast<float*>(ws + (size_t)chunks * 256 + 16);
-    const float mul = rms_factor(in, half, inv_d, eps);
-    float2 y[kW4Pairs];
+    __nv_bfloat162 xv[kPairs], wv[kPairs];
+#pragma unroll
+    for (int j = 0; j < kPairs; j++) {
+        const int i = j * kNormThreads + t;
+        if (i < half) xv[j] = in[i];
+        if (wt && i < half) wv[j] = wt[i];
+    }
+    float lsum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kPairs; j++)
+        if (j * kNormThreads + t < half) lsum = rms_add(lsum, xv[j]);
+    const float mul = rms_factor(lsum, inv_d, eps);
+    float2 y[kPairs];
     float m = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kW4Pairs; j++) {
+    for (int j = 0; j < kPairs; j++) {
         const int i = j * kNormThreads + t;
         y[j] = make_float2(0.0f, 0.0f);
         if (i < half) {
-            const __nv_bfloat162 b = rms_scaled(in[i], mul, reinterpret_cast<const __nv_bfloat162*>(w), i);
+            const __nv_bfloat162 b = rms_scaled(xv[j], mul, wt ? __bfloat1622float2(wv[j]) : make_float2(1.0f, 1.0f));
             out[i] = b;
             y[j] = __bfloat1622float2(b);
             const float a0 = fabsf(y[j].x), a1 = fabsf(y[j].y);
@@ -175,7 +188,7 @@ w4_rows_kernel(const __nv_bfloat16* __restrict__ X, const __nv_bfloat16* __restr
     }
     const int per = 64 / groups;  // pairs of a group: 16, 32 or 64
 #pragma unroll
-    for (int j = 0; j < kW4Pairs; j++) {
+    for (int j = 0; j < kPairs; j++) {
         const int i = j * kNormThreads + t;
         if (j * kNormThreads + warp * 32 >= chunks * 64) break;  // alike for the warp: 64 pairs a chunk
         const float a = y[j].x * up, b = y[j].y * up;
@@ -523,8 +536,9 @@ cudaError_t launch_lm_head_w4(const __nv_bfloat16* hidden, const __nv_bfloat16* 
                               __nv_bfloat16* normed, __nv_bfloat16* logits, unsigned char* ws, int num_sms,
                               uint32_t* segk, int segk_stride, cudaStream_t st) {
     const int chunks = w4_chunks(w.hidden), groups = 128 / w.group;
-    w4_rows_kernel<<<batch, kNormThreads, 0, st>>>(hidden, norm_weight, normed, w.hidden, chunks, groups, ws,
-                                                  1.0f / (float)w.hidden, kNormEps);
+    const auto rows_kernel = w.hidden <= 1024 ? w4_rows_kernel<2> : w.hidden <= 4096 ? w4_rows_kernel<8> : w4_rows_kernel<16>;
+    rows_kernel<<<batch, kNormThreads, 0, st>>>(hidden, norm_weight, normed, w.hidden, chunks, groups, ws,
+                                               1.0f / (float)w.hidden, kNormEps);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     const int tiles = w4_tiles(w.vocab), grid = tiles < num_sms ? tiles : num_sms;
