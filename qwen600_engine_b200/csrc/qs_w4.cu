@@ -125,8 +125,9 @@ cudaError_t launch_w4_pack(const unsigned char* codes, const void* scales, const
 // RMSNorm of one token's row per CTA, and the row as the products take it, in
 // the workspace: fp16 columns scaled by 2^s so that the largest finite value
 // lies in [2^14, 2^15) (columns 2, 3, 6 and 7 of each 8 meet 16 q and get
-// 2^(s - 4)), the sums of its groups' columns times 2^(s - 24) (the products'
-// scale), and 2^(24 - s) as two factors.
+// 2^(s - 4)), the sums of its groups' columns times -2^(s - 24) (the products'
+// scale) and, where every zero point is 8, times that; and 2^(24 - s) as two
+// factors.
 __host__ __device__ static inline size_t w4_row_bytes(int chunks, int groups) {
     return (size_t)chunks * 256 + 16 + (((size_t)chunks * groups * 4 + 15) & ~(size_t)15);
 }
@@ -136,7 +137,7 @@ __host__ __device__ static inline size_t w4_row_bytes(int chunks, int groups) {
 template <int kPairs>
 __global__ void __launch_bounds__(kNormThreads)
 w4_rows_kernel(const __nv_bfloat16* __restrict__ X, const __nv_bfloat16* __restrict__ w, __nv_bfloat16* __restrict__ Y,
-               int K, int chunks, int groups, unsigned char* __restrict__ ws, float inv_d, float eps) {
+               int K, int chunks, int groups, bool zeros, unsigned char* __restrict__ ws, float inv_d, float eps) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the projection may request its first codes
     __shared__ float red_max[kNormThreads / 32], red_sum[kPairs][kNormThreads / 32];
     const int t = threadIdx.x, warp = t >> 5, half = K / 2;
@@ -187,6 +188,7 @@ w4_rows_kernel(const __nv_bfloat16* __restrict__ X, const __nv_bfloat16* __restr
         *unscale = make_float2(__uint_as_float((uint32_t)(h + 127) << 23), __uint_as_float((uint32_t)(r + 127) << 23));
     }
     const int per = 64 / groups;  // pairs of a group: 16, 32 or 64
+    const float by = zeros ? -0x1p-24f : -0x1p-21f;
 #pragma unroll
     for (int j = 0; j < kPairs; j++) {
         const int i = j * kNormThreads + t;
@@ -194,7 +196,7 @@ w4_rows_kernel(const __nv_bfloat16* __restrict__ X, const __nv_bfloat16* __restr
         const float a = y[j].x * up, b = y[j].y * up;
         const __half2 h = __floats2half2_rn(a * f, b * f);
         xs[i] = *reinterpret_cast<const uint32_t*>(&h);
-        float sum = (a + b) * 0x1p-24f;
+        float sum = (a + b) * by;
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (per == 16) {
@@ -221,7 +223,7 @@ w4_rows_kernel(const __nv_bfloat16* __restrict__ X, const __nv_bfloat16* __restr
 constexpr int kW4Warps = 16;
 constexpr int kW4Depth = 4;  // units a warp has in flight
 
-// d = a * b + c on 16 x 8 x 16; c in registers, or 0.
+// d = a * b + d, or + c, on 16 x 8 x 16.
 __device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
     asm volatile(
@@ -230,17 +232,20 @@ __device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_first(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                               uint32_t b1) {
+__device__ __forceinline__ void mma_first(float* d, float c0, float c1, float c2, float c3, uint32_t a0, uint32_t a1,
+                                          uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%10, %10, %10, %10};"
+        "{%10, %11, %12, %13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
-__device__ __forceinline__ float scale_of(uint32_t bits, bool f16) {
-    return f16 ? __half2float(__ushort_as_half((unsigned short)bits)) : __uint_as_float(bits << 16);
+// The scales of rows g (low half) and g + 8.
+template <bool kF16>
+__device__ __forceinline__ float2 scales_of(uint32_t bits) {
+    if (kF16) return __half22float2(*reinterpret_cast<const __half2*>(&bits));
+    return make_float2(__uint_as_float(bits << 16), __uint_as_float(bits & 0xFFFF0000u));
 }
 
 __device__ __forceinline__ uint4 load_codes(const uint4* p) {
@@ -343,7 +348,7 @@ __device__ __forceinline__ void w4_store(const float (&acc)[kNt][4], const float
 // units, so warps end together whatever the number of tiles; a tile that
 // several warps share is added from their partial sums at the end, in order.
 // kNt blocks of 8 tokens, kGroups groups in a chunk.
-template <int kNt, int kGroups, bool kZeros>
+template <int kNt, int kGroups, bool kZeros, bool kF16>
 __global__ void __launch_bounds__(kW4Warps * 32, 1)
 lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, const __grid_constant__ W4Out o, int chunks,
                   int tiles) {
@@ -384,7 +389,6 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
     }
     __syncthreads();
 
-    const bool f16 = w.scale_dtype == QS_F16;
     float acc[kNt][4];
 #pragma unroll
     for (int n = 0; n < kNt; n++)
@@ -407,8 +411,16 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
             const uint32_t* hi = reinterpret_cast<const uint32_t*>(&buf[d].hi);
 #pragma unroll
             for (int j = 0; j < kGroups; j++) {
-                // two chains of sums a group, so that an mma does not wait for the one before it
-                float part[2][kNt][4];
+                // a group's sum begins at minus its zero point times the group's sum of x
+                float zl = 0.0f, zh = 0.0f;
+                if (kZeros) {
+                    const uint32_t z = buf[d].zeros[j / 2] >> (16 * (j & 1));
+                    zl = (float)(z & 0xFFu);
+                    zh = (float)((z >> 8) & 0xFFu);
+                }
+                // with one long group a chunk, in two chains, so that an mma does not wait for the one before it
+                constexpr int kChains = kGroups == 1 ? 2 : 1;
+                float part[kChains][kNt][4];
 #pragma unroll
                 for (int k = 0; k < 4 / kGroups; k++) {
                     const int word = j * (4 / kGroups) + k;
@@ -420,31 +432,32 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
 #pragma unroll
                     for (int n = 0; n < kNt; n++) {
                         const uint4 xv = *reinterpret_cast<const uint4*>(xc + n * 8 * pitch + word * 64);
+                        float* p0 = part[0][n];
+                        float* p1 = part[kChains - 1][n];
                         if (k == 0) {
-                            mma_first(part[0][n], al[0], ah[0], al[1], ah[1], xv.x, xv.y);
-                            mma_first(part[1][n], al[2], ah[2], al[3], ah[3], xv.z, xv.w);
+                            const float2 sx = *reinterpret_cast<const float2*>(sc + j * kNt * 8 + n * 8);
+                            if (kZeros)
+                                mma_first(p0, zl * sx.x, zl * sx.y, zh * sx.x, zh * sx.y, al[0], ah[0], al[1], ah[1],
+                                          xv.x, xv.y);
+                            else
+                                mma_first(p0, sx.x, sx.y, sx.x, sx.y, al[0], ah[0], al[1], ah[1], xv.x, xv.y);
                         } else {
-                            mma(part[0][n], al[0], ah[0], al[1], ah[1], xv.x, xv.y);
-                            mma(part[1][n], al[2], ah[2], al[3], ah[3], xv.z, xv.w);
+                            mma(p0, al[0], ah[0], al[1], ah[1], xv.x, xv.y);
                         }
+                        if (k == 0 && kChains == 2)
+                            mma_first(p1, 0.0f, 0.0f, 0.0f, 0.0f, al[2], ah[2], al[3], ah[3], xv.z, xv.w);
+                        else
+                            mma(p1, al[2], ah[2], al[3], ah[3], xv.z, xv.w);
                     }
                 }
-                const float sl = scale_of(buf[d].scales[j] & 0xFFFFu, f16), sh = scale_of(buf[d].scales[j] >> 16, f16);
-                float zl = -8.0f, zh = -8.0f;
-                if (kZeros) {
-                    const uint32_t z = buf[d].zeros[j / 2] >> (16 * (j & 1));
-                    zl = -(float)(z & 0xFFu);
-                    zh = -(float)((z >> 8) & 0xFFu);
-                }
+                const float2 sg = scales_of<kF16>(buf[d].scales[j]);
 #pragma unroll
-                for (int n = 0; n < kNt; n++) {
-                    const float2 sx = *reinterpret_cast<const float2*>(sc + j * kNt * 8 + n * 8);
+                for (int n = 0; n < kNt; n++)
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        const float sum = __fmaf_rn(k < 2 ? zl : zh, k & 1 ? sx.y : sx.x, part[0][n][k] + part[1][n][k]);
-                        acc[n][k] = __fmaf_rn(k < 2 ? sl : sh, sum, acc[n][k]);
+                        const float sum = kChains == 2 ? part[0][n][k] + part[kChains - 1][n][k] : part[0][n][k];
+                        acc[n][k] = __fmaf_rn(k < 2 ? sg.x : sg.y, sum, acc[n][k]);
                     }
-                }
             }
             if (d + kW4Depth < left) w4_load<kGroups, kZeros>(buf[d], at, d);
             const bool ends = ++c == chunks;
@@ -497,10 +510,10 @@ static size_t w4_smem(int nt, int K, int group) {
            (size_t)nt * 8 * (sizeof(float2) + w4_chunks(K) * (128 / group) * sizeof(float));
 }
 
-template <int kNt, int kGroups, bool kZeros>
+template <int kNt, int kGroups, bool kZeros, bool kF16>
 static cudaError_t w4_go(const unsigned char* rows, const W4View& w, const W4Out& o, int grid, cudaStream_t st) {
     const size_t smem = w4_smem(kNt, w.hidden, w.group);
-    cudaError_t e = cudaFuncSetAttribute(lm_head_w4_kernel<kNt, kGroups, kZeros>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(lm_head_w4_kernel<kNt, kGroups, kZeros, kF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)smem);
     if (e != cudaSuccess) return e;
     // programmatic dependent launch: the first units are requested while the
@@ -515,19 +528,22 @@ static cudaError_t w4_go(const unsigned char* rows, const W4View& w, const W4Out
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, lm_head_w4_kernel<kNt, kGroups, kZeros>, rows, w, o, w4_chunks(w.hidden), w4_tiles(w.vocab));
+    return cudaLaunchKernelEx(&cfg, lm_head_w4_kernel<kNt, kGroups, kZeros, kF16>, rows, w, o, w4_chunks(w.hidden), w4_tiles(w.vocab));
 }
 
 template <int kNt, int kGroups>
-static cudaError_t w4_zeros(const unsigned char* rows, const W4View& w, const W4Out& o, int grid, cudaStream_t st) {
-    return w.zeros ? w4_go<kNt, kGroups, true>(rows, w, o, grid, st) : w4_go<kNt, kGroups, false>(rows, w, o, grid, st);
+static cudaError_t w4_types(const unsigned char* rows, const W4View& w, const W4Out& o, int grid, cudaStream_t st) {
+    const bool f16 = w.scale_dtype == QS_F16;
+    if (w.zeros)
+        return f16 ? w4_go<kNt, kGroups, true, true>(rows, w, o, grid, st) : w4_go<kNt, kGroups, true, false>(rows, w, o, grid, st);
+    return f16 ? w4_go<kNt, kGroups, false, true>(rows, w, o, grid, st) : w4_go<kNt, kGroups, false, false>(rows, w, o, grid, st);
 }
 
 template <int kNt>
 static cudaError_t w4_group(const unsigned char* rows, const W4View& w, const W4Out& o, int grid, cudaStream_t st) {
-    return w.group == 128 ? w4_zeros<kNt, 1>(rows, w, o, grid, st)
-         : w.group == 64  ? w4_zeros<kNt, 2>(rows, w, o, grid, st)
-                          : w4_zeros<kNt, 4>(rows, w, o, grid, st);
+    return w.group == 128 ? w4_types<kNt, 1>(rows, w, o, grid, st)
+         : w.group == 64  ? w4_types<kNt, 2>(rows, w, o, grid, st)
+                          : w4_types<kNt, 4>(rows, w, o, grid, st);
 }
 
 size_t w4_workspace(int batch, int K, int group) { return (size_t)batch * w4_row_bytes(w4_chunks(K), 128 / group); }
@@ -537,7 +553,8 @@ cudaError_t launch_lm_head_w4(const __nv_bfloat16* hidden, const __nv_bfloat16* 
                               uint32_t* segk, int segk_stride, cudaStream_t st) {
     const int chunks = w4_chunks(w.hidden), groups = 128 / w.group;
     const auto rows_kernel = w.hidden <= 1024 ? w4_rows_kernel<2> : w.hidden <= 4096 ? w4_rows_kernel<8> : w4_rows_kernel<16>;
-    rows_kernel<<<batch, kNormThreads, 0, st>>>(hidden, norm_weight, normed, w.hidden, chunks, groups, ws,
+    rows_kernel<<<batch, kNormThreads, 0, st>>>(hidden, norm_weight, normed, w.hidden, chunks, groups,
+                                               w.zeros != nullptr, ws,
                                                1.0f / (float)w.hidden, kNormEps);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
