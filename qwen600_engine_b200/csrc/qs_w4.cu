@@ -223,6 +223,33 @@ w4_rows_kernel(const __nv_bfloat16* __restrict__ X, const __nv_bfloat16* __restr
 constexpr int kW4Warps = 16;
 constexpr int kW4Depth = 4;  // units a warp has in flight
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ unsigned long long pair2(float x, float y) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpair2(unsigned long long v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // d = a * b + d, or + c, on 16 x 8 x 16.
 __device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -436,11 +463,13 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
                         float* p1 = part[kChains - 1][n];
                         if (k == 0) {
                             const float2 sx = *reinterpret_cast<const float2*>(sc + j * kNt * 8 + n * 8);
-                            if (kZeros)
-                                mma_first(p0, zl * sx.x, zl * sx.y, zh * sx.x, zh * sx.y, al[0], ah[0], al[1], ah[1],
-                                          xv.x, xv.y);
-                            else
+                            if (kZeros) {
+                                const unsigned long long sx2 = pair2(sx.x, sx.y);
+                                const float2 cl = unpair2(mul2(pair2(zl, zl), sx2)), ch = unpair2(mul2(pair2(zh, zh), sx2));
+                                mma_first(p0, cl.x, cl.y, ch.x, ch.y, al[0], ah[0], al[1], ah[1], xv.x, xv.y);
+                            } else {
                                 mma_first(p0, sx.x, sx.y, sx.x, sx.y, al[0], ah[0], al[1], ah[1], xv.x, xv.y);
+                            }
                         } else {
                             mma(p0, al[0], ah[0], al[1], ah[1], xv.x, xv.y);
                         }
@@ -454,9 +483,15 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
 #pragma unroll
                 for (int n = 0; n < kNt; n++)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const float sum = kChains == 2 ? part[0][n][k] + part[kChains - 1][n][k] : part[0][n][k];
-                        acc[n][k] = __fmaf_rn(k < 2 ? sg.x : sg.y, sum, acc[n][k]);
+                    for (int h = 0; h < 2; h++) {  // row g, row g + 8; both tokens at once
+                        unsigned long long sum = pair2(part[0][n][2 * h], part[0][n][2 * h + 1]);
+                        if (kChains == 2)
+                            sum = add2(sum, pair2(part[kChains - 1][n][2 * h], part[kChains - 1][n][2 * h + 1]));
+                        const float f = h ? sg.y : sg.x;
+                        const float2 v =
+                            unpair2(fma2(pair2(f, f), sum, pair2(acc[n][2 * h], acc[n][2 * h + 1])));
+                        acc[n][2 * h] = v.x;
+                        acc[n][2 * h + 1] = v.y;
                     }
             }
             if (d + kW4Depth < left) w4_load<kGroups, kZeros>(buf[d], at, d);
