@@ -62,32 +62,32 @@ cudaError_t launch_w4_quantize(const __nv_bfloat16* w, int V, int K, int group, 
 }
 
 // ---------------------------------------------------------------- layout
-// Vocabulary rows in tiles of 16, columns in chunks of 128 (the last padded
-// with zeros).  A unit is one tile's chunk: 1 KB of codes, and units lie one
+// Vocabulary rows in tiles of 32, columns in chunks of 128 (the last padded
+// with zeros).  A unit is one tile's chunk: 2 KB of codes, and units lie one
 // after another, tile by tile.  In a unit lane l = 4 g + q of a warp finds
-// 16 bytes for row g (first 512 bytes) and 16 for row g + 8: four words, word
-// w for columns 32 w + 8 q + 0..7 of the chunk.  Nibble i < 4 of a word is
-// column 2 i, nibble i + 4 column 2 i + 1, so masks take pairs of neighbouring
-// columns, one in each half.  A group of 32 columns is then one word of every
-// lane, and any group is whole mma instructions.
+// 16 bytes for each of rows g, g + 8, g + 16 and g + 24 (512 bytes apart): four
+// words, word w for columns 32 w + 8 q + 0..7 of the chunk.  Nibble i < 4 of a
+// word is column 2 i, nibble i + 4 column 2 i + 1, so masks take pairs of
+// neighbouring columns, one in each half.  A group of 32 columns is then one
+// word of every lane, and any group is whole mma instructions.
 // Scales (16-bit) and zero points (bytes) of a unit: [g][group of the chunk]
-// [row g, row g + 8].
-constexpr int kUnitCodes = 1024;
+// [rows g, g + 8, g + 16, g + 24].
+constexpr int kUnitCodes = 2048;
 
 static int w4_chunks(int K) { return (K + 127) / 128; }
-static int w4_tiles(int V) { return (V + 15) / 16; }
+static int w4_tiles(int V) { return (V + 31) / 32; }
 
 size_t w4_codes_bytes(int V, int K) { return (size_t)w4_tiles(V) * w4_chunks(K) * kUnitCodes; }
-size_t w4_scales_bytes(int V, int K, int group) { return (size_t)w4_tiles(V) * w4_chunks(K) * (128 / group) * 32; }
+size_t w4_scales_bytes(int V, int K, int group) { return (size_t)w4_tiles(V) * w4_chunks(K) * (128 / group) * 64; }
 size_t w4_zeros_bytes(int V, int K, int group) { return w4_scales_bytes(V, K, group) / 2; }
 
 __global__ void w4_pack_codes_kernel(const unsigned char* __restrict__ codes, int V, int K, int chunks, size_t n,
                                      uint32_t* __restrict__ out) {
     const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;  // one word
     if (i >= n) return;
-    const int w = i & 3, lane = (i >> 2) & 31, half = (i >> 7) & 1;
-    const size_t unit = i >> 8;
-    const int row = (int)(unit / chunks) * 16 + half * 8 + (lane >> 2);
+    const int w = i & 3, lane = (i >> 2) & 31, block = (i >> 7) & 3;
+    const size_t unit = i >> 9;
+    const int row = (int)(unit / chunks) * 32 + block * 8 + (lane >> 2);
     const int k = (int)(unit % chunks) * 128 + 32 * w + 8 * (lane & 3);
     uint32_t word = 0;
     if (row < V && k < K) {
@@ -102,9 +102,9 @@ __global__ void w4_pack_scales_kernel(const uint16_t* __restrict__ scales, const
                                       uint16_t* __restrict__ out_s, unsigned char* __restrict__ out_z) {
     const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= n) return;
-    const int half = i & 1, j = (int)(i >> 1) % per_chunk, g = (int)((i >> 1) / per_chunk) & 7;
-    const size_t unit = i / (16 * per_chunk);
-    const int row = (int)(unit / chunks) * 16 + half * 8 + g, grp = (int)(unit % chunks) * per_chunk + j;
+    const int block = i & 3, j = (int)(i >> 2) % per_chunk, g = (int)((i >> 2) / per_chunk) & 7;
+    const size_t unit = i / (32 * per_chunk);
+    const int row = (int)(unit / chunks) * 32 + block * 8 + g, grp = (int)(unit % chunks) * per_chunk + j;
     const bool in = row < V && grp < per_row;
     out_s[i] = in ? scales[(size_t)row * per_row + grp] : 0;
     if (zeros) out_z[i] = in ? zeros[(size_t)row * per_row + grp] & 15 : 0;
@@ -220,8 +220,7 @@ w4_rows_kernel(const __nv_bfloat16* __restrict__ X, const __nv_bfloat16* __restr
 }
 
 // -------------------------------------------------------------- projection
-constexpr int kW4Warps = 16;
-constexpr int kW4Depth = 4;  // units a warp has in flight
+constexpr int kW4Depth = 2;  // units a warp has in flight
 
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ unsigned long long pair2(float x, float y) {
@@ -286,9 +285,9 @@ __device__ __forceinline__ uint4 load_codes(const uint4* p) {
 // One unit as a lane holds it.
 template <int kGroups>
 struct W4Unit {
-    uint4 lo, hi;               // codes of row g and of row g + 8
-    uint32_t scales[kGroups];   // row g in the low half, row g + 8 in the high one
-    uint32_t zeros[(kGroups + 1) / 2];
+    uint4 codes[4];                // rows g, g + 8, g + 16, g + 24
+    uint32_t scales[2 * kGroups];  // of a group: rows g and g + 8, rows g + 16 and g + 24
+    uint32_t zeros[kGroups];
 };
 
 // Where a lane's part of its warp's next unit lies.
@@ -298,33 +297,30 @@ struct W4At {
     const unsigned char* zeros;
 };
 
+template <int kWords>
+__device__ __forceinline__ void load_words(uint32_t* out, const void* p) {
+    if (kWords == 1) {
+        out[0] = __ldg(static_cast<const uint32_t*>(p));
+    } else if (kWords == 2) {
+        const uint2 v = __ldg(static_cast<const uint2*>(p));
+        out[0] = v.x; out[1 % kWords] = v.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < kWords / 4; i++) {
+            const uint4 v = __ldg(static_cast<const uint4*>(p) + i);
+            out[4 * i] = v.x; out[(4 * i + 1) % kWords] = v.y; out[(4 * i + 2) % kWords] = v.z; out[(4 * i + 3) % kWords] = v.w;
+        }
+    }
+}
+
 // Loads the unit `ahead` units behind the next one.
 template <int kGroups, bool kZeros>
 __device__ __forceinline__ void w4_load(W4Unit<kGroups>& u, const W4At& at, int ahead) {
     const uint4* c = reinterpret_cast<const uint4*>(at.codes + ahead * kUnitCodes);
-    u.lo = load_codes(c);
-    u.hi = load_codes(c + 32);
-    const unsigned char* s = at.scales + ahead * (32 * kGroups);
-    if (kGroups == 1) {
-        u.scales[0] = __ldg(reinterpret_cast<const uint32_t*>(s));
-    } else if (kGroups == 2) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(s));
-        u.scales[0] = v.x; u.scales[1 % kGroups] = v.y;
-    } else {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(s));
-        u.scales[0] = v.x; u.scales[1 % kGroups] = v.y; u.scales[2 % kGroups] = v.z; u.scales[3 % kGroups] = v.w;
-    }
-    if (kZeros) {
-        const unsigned char* z = at.zeros + ahead * (16 * kGroups);
-        if (kGroups == 1) {
-            u.zeros[0] = __ldg(reinterpret_cast<const unsigned short*>(z));
-        } else if (kGroups == 2) {
-            u.zeros[0] = __ldg(reinterpret_cast<const uint32_t*>(z));
-        } else {
-            const uint2 v = __ldg(reinterpret_cast<const uint2*>(z));
-            u.zeros[0] = v.x; u.zeros[1 % ((kGroups + 1) / 2)] = v.y;
-        }
-    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) u.codes[i] = load_codes(c + 32 * i);
+    load_words<2 * kGroups>(u.scales, at.scales + ahead * (64 * kGroups));
+    if (kZeros) load_words<kGroups>(u.zeros, at.zeros + ahead * (32 * kGroups));
 }
 
 struct W4Out {
@@ -334,81 +330,86 @@ struct W4Out {
     int segk_stride;
 };
 
-// Stores a finished tile: 16 vocabulary rows of up to 8 kNt tokens, through the
+// Stores a finished tile: 32 vocabulary rows of up to 8 kNt tokens, through the
 // warp's staging rows so that a lane stores 16 bytes of one token.
 template <int kNt>
-__device__ __forceinline__ void w4_store(const float (&acc)[kNt][4], const float2* unscale, __nv_bfloat16* stage,
+__device__ __forceinline__ void w4_store(const float (&acc)[2][kNt][4], const float2* unscale, __nv_bfloat16* stage,
                                          const W4Out& o, int V, int tile, int lane) {
     const int g = lane >> 2, q = lane & 3;
     __syncwarp();
 #pragma unroll
     for (int n = 0; n < kNt; n++) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) {  // j: row g or g + 8, token 2 q or 2 q + 1
-            const int token = n * 8 + 2 * q + (j & 1);
+        for (int j = 0; j < 2; j++) {  // token 2 q or 2 q + 1
+            const int token = n * 8 + 2 * q + j;
             const float2 f = unscale[token];
-            stage[token * 16 + g + (j >> 1) * 8] = __float2bfloat16_rn(acc[n][j] * f.x * f.y);
+#pragma unroll
+            for (int b = 0; b < 4; b++)  // row g + 8 b
+                stage[token * 32 + g + b * 8] = __float2bfloat16_rn(acc[b >> 1][n][(b & 1) * 2 + j] * f.x * f.y);
         }
     }
     __syncwarp();
-    for (int p = lane; p < kNt * 16; p += 32) {
-        const int token = p >> 1, col = tile * 16 + (p & 1) * 8;
+#pragma unroll
+    for (int i = 0; i < kNt; i++) {
+        const int p = i * 32 + lane, token = p >> 2, col = tile * 32 + (p & 3) * 8;
         const uint4 v = *reinterpret_cast<const uint4*>(stage + p * 8);
-        const bool in = token < o.tokens;
-        if (in && col < V) {
-            __nv_bfloat16* d = o.logits + (size_t)token * V + col;
-            if (col + 8 <= V && (V & 7) == 0) {
-                *reinterpret_cast<uint4*>(d) = v;
-            } else {
-                const __nv_bfloat16* e = stage + p * 8;
-                for (int j = 0; j < 8 && col + j < V; j++) d[j] = e[j];
-            }
+        if (token >= o.tokens || col >= V) continue;
+        __nv_bfloat16* d = o.logits + (size_t)token * V + col;
+        if (col + 8 <= V && (V & 7) == 0) {
+            *reinterpret_cast<uint4*>(d) = v;
+        } else {
+            const __nv_bfloat16* e = stage + p * 8;
+            for (int j = 0; j < 8 && col + j < V; j++) d[j] = e[j];
         }
-        // whole tiles only: they never straddle a 256-column segment, and the
+        // whole blocks of 16 columns, as the bf16 epilogue folds them: they never straddle a 256-column segment, and the
         // sampler takes the maxima of whole segments
-        if (o.segk && in && tile * 16 + 16 <= V)
-            atomicMax(o.segk + (size_t)token * o.segk_stride + (tile >> 4), fkey(vec_max<__nv_bfloat16>(v)));
+        if (o.segk && (col & ~15) + 16 <= V)
+            atomicMax(o.segk + (size_t)token * o.segk_stride + (col >> 8), fkey(vec_max<__nv_bfloat16>(v)));
     }
 }
 
 // A CTA takes a contiguous range of tiles and its warps equal shares of their
 // units, so warps end together whatever the number of tiles; a tile that
 // several warps share is added from their partial sums at the end, in order.
-// kNt blocks of 8 tokens, kGroups groups in a chunk.
+// kNt blocks of 8 tokens, kGroups groups in a chunk.  A tile is two mma rows of
+// 16, so that a token's columns, read from shared memory, serve both (with one,
+// these reads were 54% of the L1 pipe at 16 tokens: 29.5 us).  Up to 16 tokens
+// 16 warps of 128 registers, above 8 of 255.
 template <int kNt, int kGroups, bool kZeros, bool kF16>
-__global__ void __launch_bounds__(kW4Warps * 32, 1)
+__global__ void __launch_bounds__(kNt <= 2 ? 512 : 256, 1)
 lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, const __grid_constant__ W4Out o, int chunks,
                   int tiles) {
+    constexpr int kWarps = kNt <= 2 ? 16 : 8;
     extern __shared__ __align__(16) unsigned char smem[];
     const int pitch = chunks * 256 + 64;  // bytes of a token's row: neighbours 64 bytes apart in the banks
     unsigned char* xs = smem;                                           // fp16 rows
-    float4* slots = reinterpret_cast<float4*>(smem + kNt * 8 * pitch);  // [warp][continued, begun][kNt][lane]
-    __nv_bfloat16* stage = reinterpret_cast<__nv_bfloat16*>(slots + kW4Warps * 2 * kNt * 32);
-    float2* unscale = reinterpret_cast<float2*>(stage + kW4Warps * kNt * 128);  // [token] two factors
-    float* sums = reinterpret_cast<float*>(unscale + kNt * 8);                  // [group][token] sum of its columns
+    float4* slots = reinterpret_cast<float4*>(smem + kNt * 8 * pitch);  // [warp][continued, begun][2][kNt][lane]
+    __nv_bfloat16* stage = reinterpret_cast<__nv_bfloat16*>(slots + kWarps * 2 * 2 * kNt * 32);
+    float2* unscale = reinterpret_cast<float2*>(stage + kWarps * kNt * 256);  // [token] two factors
+    float* sums = reinterpret_cast<float*>(unscale + kNt * 8);                // [group][token] sum of its columns
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-    stage += warp * kNt * 128;
+    stage += warp * kNt * 256;
     const int t0 = (int)((long long)blockIdx.x * tiles / gridDim.x), t1 = (int)((long long)(blockIdx.x + 1) * tiles / gridDim.x);
     const int u0 = t0 * chunks, un = (t1 - t0) * chunks;
-    const auto share = [&](int wi) { return u0 + (int)((long long)un * wi / kW4Warps); };
+    const auto share = [&](int wi) { return u0 + (int)((long long)un * wi / kWarps); };
     const int a = share(warp), b = share(warp + 1);
 
     W4At at;
     at.codes = w.codes + (size_t)a * kUnitCodes + lane * 16;
-    at.scales = reinterpret_cast<const unsigned char*>(w.scales) + ((size_t)a * 8 + g) * (4 * kGroups);
-    at.zeros = w.zeros + (kZeros ? ((size_t)a * 8 + g) * (2 * kGroups) : 0);
+    at.scales = reinterpret_cast<const unsigned char*>(w.scales) + ((size_t)a * 8 + g) * (8 * kGroups);
+    at.zeros = w.zeros + (kZeros ? ((size_t)a * 8 + g) * (4 * kGroups) : 0);
     W4Unit<kGroups> buf[kW4Depth];
 #pragma unroll
     for (int d = 0; d < kW4Depth; d++)
         if (a + d < b) w4_load<kGroups, kZeros>(buf[d], at, d);
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the RMSNorm's rows
     const size_t row_bytes = w4_row_bytes(chunks, kGroups);
-    for (int i = threadIdx.x; i < kNt * 8 * chunks * 16; i += kW4Warps * 32) {
+    for (int i = threadIdx.x; i < kNt * 8 * chunks * 16; i += kWarps * 32) {
         const int row = i / (chunks * 16), c = i - row * (chunks * 16);
         *reinterpret_cast<uint4*>(xs + row * pitch + c * 16) =
             row < o.tokens ? *reinterpret_cast<const uint4*>(rows + row * row_bytes + c * 16) : make_uint4(0u, 0u, 0u, 0u);
     }
-    for (int i = threadIdx.x; i < kNt * 8 * (chunks * kGroups + 1); i += kW4Warps * 32) {
+    for (int i = threadIdx.x; i < kNt * 8 * (chunks * kGroups + 1); i += kWarps * 32) {
         const int row = i % (kNt * 8), j = i / (kNt * 8);
         const unsigned char* p = rows + row * row_bytes + chunks * 256;
         if (j == 0) unscale[row] = row < o.tokens ? *reinterpret_cast<const float2*>(p) : make_float2(0.0f, 0.0f);
@@ -416,11 +417,16 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
     }
     __syncthreads();
 
-    float acc[kNt][4];
+    float acc[2][kNt][4];
+    const auto clear = [&] {
 #pragma unroll
-    for (int n = 0; n < kNt; n++)
+        for (int m = 0; m < 2; m++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) acc[n][j] = 0.0f;
+            for (int n = 0; n < kNt; n++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[m][n][j] = 0.0f;
+    };
+    clear();
     int tile = a / chunks, c = a - tile * chunks;
     bool begun = c == 0;
     const unsigned char* xl = xs + g * pitch + q * 16;
@@ -429,70 +435,64 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
     const float* sc = sl0 + c * kGroups * kNt * 8;
     for (int left = b - a; left > 0; left -= kW4Depth) {
         at.codes += kW4Depth * kUnitCodes;
-        at.scales += kW4Depth * 32 * kGroups;
-        if (kZeros) at.zeros += kW4Depth * 16 * kGroups;
+        at.scales += kW4Depth * 64 * kGroups;
+        if (kZeros) at.zeros += kW4Depth * 32 * kGroups;
 #pragma unroll
         for (int d = 0; d < kW4Depth; d++) {
             if (d >= left) break;
-            const uint32_t* lo = reinterpret_cast<const uint32_t*>(&buf[d].lo);
-            const uint32_t* hi = reinterpret_cast<const uint32_t*>(&buf[d].hi);
 #pragma unroll
             for (int j = 0; j < kGroups; j++) {
-                // a group's sum begins at minus its zero point times the group's sum of x
-                float zl = 0.0f, zh = 0.0f;
-                if (kZeros) {
-                    const uint32_t z = buf[d].zeros[j / 2] >> (16 * (j & 1));
-                    zl = (float)(z & 0xFFu);
-                    zh = (float)((z >> 8) & 0xFFu);
-                }
-                // with one long group a chunk, in two chains, so that an mma does not wait for the one before it
-                constexpr int kChains = kGroups == 1 ? 2 : 1;
-                float part[kChains][kNt][4];
+                float part[2][kNt][4];
 #pragma unroll
                 for (int k = 0; k < 4 / kGroups; k++) {
                     const int word = j * (4 / kGroups) + k;
-                    const uint32_t l8 = lo[word] >> 8, h8 = hi[word] >> 8;
-                    const uint32_t al[4] = {lo[word] & 0x000F000Fu, lo[word] & 0x00F000F0u, l8 & 0x000F000Fu,
-                                            l8 & 0x00F000F0u};
-                    const uint32_t ah[4] = {hi[word] & 0x000F000Fu, hi[word] & 0x00F000F0u, h8 & 0x000F000Fu,
-                                            h8 & 0x00F000F0u};
+                    uint32_t r[4][4];  // codes of rows g + 8 b: q, 16 q, q, 16 q
+#pragma unroll
+                    for (int b4 = 0; b4 < 4; b4++) {
+                        const uint32_t v = reinterpret_cast<const uint32_t*>(&buf[d].codes[b4])[word], v8 = v >> 8;
+                        r[b4][0] = v & 0x000F000Fu;
+                        r[b4][1] = v & 0x00F000F0u;
+                        r[b4][2] = v8 & 0x000F000Fu;
+                        r[b4][3] = v8 & 0x00F000F0u;
+                    }
 #pragma unroll
                     for (int n = 0; n < kNt; n++) {
                         const uint4 xv = *reinterpret_cast<const uint4*>(xc + n * 8 * pitch + word * 64);
-                        float* p0 = part[0][n];
-                        float* p1 = part[kChains - 1][n];
-                        if (k == 0) {
-                            const float2 sx = *reinterpret_cast<const float2*>(sc + j * kNt * 8 + n * 8);
-                            if (kZeros) {
+                        float2 sx;
+                        if (k == 0) sx = *reinterpret_cast<const float2*>(sc + j * kNt * 8 + n * 8);
+#pragma unroll
+                        for (int m = 0; m < 2; m++) {
+                            const uint32_t *lo = r[2 * m], *hi = r[2 * m + 1];
+                            // a group's sum begins at minus its zero point times the group's sum of x
+                            if (k == 0 && kZeros) {
+                                const uint32_t z = buf[d].zeros[j] >> (16 * m);
+                                const float zl = (float)(z & 0xFFu), zh = (float)((z >> 8) & 0xFFu);
                                 const unsigned long long sx2 = pair2(sx.x, sx.y);
                                 const float2 cl = unpair2(mul2(pair2(zl, zl), sx2)), ch = unpair2(mul2(pair2(zh, zh), sx2));
-                                mma_first(p0, cl.x, cl.y, ch.x, ch.y, al[0], ah[0], al[1], ah[1], xv.x, xv.y);
+                                mma_first(part[m][n], cl.x, cl.y, ch.x, ch.y, lo[0], hi[0], lo[1], hi[1], xv.x, xv.y);
+                            } else if (k == 0) {
+                                mma_first(part[m][n], sx.x, sx.y, sx.x, sx.y, lo[0], hi[0], lo[1], hi[1], xv.x, xv.y);
                             } else {
-                                mma_first(p0, sx.x, sx.y, sx.x, sx.y, al[0], ah[0], al[1], ah[1], xv.x, xv.y);
+                                mma(part[m][n], lo[0], hi[0], lo[1], hi[1], xv.x, xv.y);
                             }
-                        } else {
-                            mma(p0, al[0], ah[0], al[1], ah[1], xv.x, xv.y);
+                            mma(part[m][n], lo[2], hi[2], lo[3], hi[3], xv.z, xv.w);
                         }
-                        if (k == 0 && kChains == 2)
-                            mma_first(p1, 0.0f, 0.0f, 0.0f, 0.0f, al[2], ah[2], al[3], ah[3], xv.z, xv.w);
-                        else
-                            mma(p1, al[2], ah[2], al[3], ah[3], xv.z, xv.w);
                     }
                 }
-                const float2 sg = scales_of<kF16>(buf[d].scales[j]);
 #pragma unroll
-                for (int n = 0; n < kNt; n++)
+                for (int m = 0; m < 2; m++) {
+                    const float2 sg = scales_of<kF16>(buf[d].scales[2 * j + m]);
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {  // row g, row g + 8; both tokens at once
-                        unsigned long long sum = pair2(part[0][n][2 * h], part[0][n][2 * h + 1]);
-                        if (kChains == 2)
-                            sum = add2(sum, pair2(part[kChains - 1][n][2 * h], part[kChains - 1][n][2 * h + 1]));
-                        const float f = h ? sg.y : sg.x;
-                        const float2 v =
-                            unpair2(fma2(pair2(f, f), sum, pair2(acc[n][2 * h], acc[n][2 * h + 1])));
-                        acc[n][2 * h] = v.x;
-                        acc[n][2 * h + 1] = v.y;
-                    }
+                    for (int n = 0; n < kNt; n++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {  // row g, row g + 8; both tokens at once
+                            const float f = h ? sg.y : sg.x;
+                            const float2 v = unpair2(fma2(pair2(f, f), pair2(part[m][n][2 * h], part[m][n][2 * h + 1]),
+                                                          pair2(acc[m][n][2 * h], acc[m][n][2 * h + 1])));
+                            acc[m][n][2 * h] = v.x;
+                            acc[m][n][2 * h + 1] = v.y;
+                        }
+                }
             }
             if (d + kW4Depth < left) w4_load<kGroups, kZeros>(buf[d], at, d);
             const bool ends = ++c == chunks;
@@ -503,14 +503,13 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
                     w4_store<kNt>(acc, unscale, stage, o, w.vocab, tile, lane);
                 } else {
 #pragma unroll
-                    for (int n = 0; n < kNt; n++)
-                        slots[((warp * 2 + begun) * kNt + n) * 32 + lane] =
-                            make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+                    for (int m = 0; m < 2; m++)
+#pragma unroll
+                        for (int n = 0; n < kNt; n++)
+                            slots[(((warp * 2 + begun) * 2 + m) * kNt + n) * 32 + lane] =
+                                make_float4(acc[m][n][0], acc[m][n][1], acc[m][n][2], acc[m][n][3]);
                 }
-#pragma unroll
-                for (int n = 0; n < kNt; n++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) acc[n][j] = 0.0f;
+                clear();
                 if (ends) {
                     c = 0;
                     xc = xl;
@@ -525,23 +524,25 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
     // the warp that began a tile which later warps continued adds their sums
     if (a < b && b % chunks != 0 && (b - 1) / chunks * chunks >= a) {
         const int last = (b - 1) / chunks, stop = (last + 1) * chunks;
-        int first = warp * 2 + 1;  // its own part, then the following warps' continued ones
-        for (int wi = warp; wi < kW4Warps && share(wi) < stop; wi++) {
+        int slot = warp * 2 + 1;  // its own part, then the following warps' continued ones
+        for (int wi = warp; wi < kWarps && share(wi) < stop; wi++) {
             if (share(wi) < share(wi + 1)) {
 #pragma unroll
-                for (int n = 0; n < kNt; n++) {
-                    const float4 p = slots[(first * kNt + n) * 32 + lane];
-                    acc[n][0] += p.x; acc[n][1] += p.y; acc[n][2] += p.z; acc[n][3] += p.w;
-                }
+                for (int m = 0; m < 2; m++)
+#pragma unroll
+                    for (int n = 0; n < kNt; n++) {
+                        const float4 p = slots[((slot * 2 + m) * kNt + n) * 32 + lane];
+                        acc[m][n][0] += p.x; acc[m][n][1] += p.y; acc[m][n][2] += p.z; acc[m][n][3] += p.w;
+                    }
             }
-            first = (wi + 1) * 2;
+            slot = (wi + 1) * 2;
         }
         w4_store<kNt>(acc, unscale, stage, o, w.vocab, last, lane);
     }
 }
 
 static size_t w4_smem(int nt, int K, int group) {
-    return (size_t)nt * 8 * (w4_chunks(K) * 256 + 64) + (size_t)kW4Warps * nt * (2 * 512 + 256) +
+    return (size_t)nt * 8 * (w4_chunks(K) * 256 + 64) + (size_t)(nt <= 2 ? 16 : 8) * nt * (2 * 2 * 512 + 512) +
            (size_t)nt * 8 * (sizeof(float2) + w4_chunks(K) * (128 / group) * sizeof(float));
 }
 
@@ -555,7 +556,7 @@ static cudaError_t w4_go(const unsigned char* rows, const W4View& w, const W4Out
     // RMSNorm runs
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kW4Warps * 32);
+    cfg.blockDim = dim3(kNt <= 2 ? 512 : 256);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1] = {};
