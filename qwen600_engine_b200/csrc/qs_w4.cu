@@ -20,6 +20,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "qs_common.cuh"
 #include "qs_w4.h"
 #include "qs_rmsnorm.cuh"
@@ -549,8 +551,14 @@ static size_t w4_smem(int nt, int K, int group) {
 template <int kNt, int kGroups, bool kZeros, bool kF16>
 static cudaError_t w4_go(const unsigned char* rows, const W4View& w, const W4Out& o, int grid, cudaStream_t st) {
     const size_t smem = w4_smem(kNt, w.hidden, w.group);
-    cudaError_t e = cudaFuncSetAttribute(lm_head_w4_kernel<kNt, kGroups, kZeros, kF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)smem);
+    static std::atomic<unsigned long long> raised{0};  // devices on which the kernel may use all shared memory
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev >= 64 || !(raised.load() >> dev & 1))) {
+        e = cudaFuncSetAttribute(lm_head_w4_kernel<kNt, kGroups, kZeros, kF16>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+        if (e == cudaSuccess && dev < 64) raised.fetch_or(1ull << dev);
+    }
     if (e != cudaSuccess) return e;
     // programmatic dependent launch: the first units are requested while the
     // RMSNorm runs

@@ -50,38 +50,29 @@ def _invalid(msg: str) -> SamplerError:
     return SamplerError(QS_ERR_INVALID, msg)
 
 
-class _Launch:
-    """The device and stream of one call: buffers made inside belong to the
-    stream that uses them, and inputs used on another stream than the current
-    one are kept until it is done with them."""
+_current_device = torch.cuda.current_device
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
-    __slots__ = ("device", "stream", "inputs", "ctx")
 
-    def __init__(self, device, stream, *inputs):
-        if device.type != "cuda":
-            raise _invalid("the tensors must be on a GPU")
-        self.device, self.stream, self.inputs, self.ctx = device, stream, inputs, None
-
-    def __enter__(self) -> int:
-        s = self.stream
-        if s is None:
-            if torch.cuda.current_device() != self.device.index:
-                self.ctx = torch.cuda.device(self.device)
-                self.ctx.__enter__()
-            return torch.cuda.current_stream().cuda_stream
-        if s.device != self.device:
-            raise _invalid(f"stream of {s.device} for tensors on {self.device}")
-        if s != torch.cuda.current_stream(self.device):
-            for t in self.inputs:
-                if t is not None:
-                    t.record_stream(s)
-        self.ctx = torch.cuda.stream(s)
-        self.ctx.__enter__()
-        return s.cuda_stream
-
-    def __exit__(self, *exc) -> None:
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
+def _on_stream(device, stream, inputs, run):
+    """run(stream handle) on the device and stream of one call.  Buffers made
+    by run belong to the stream that uses them, and inputs used on another
+    stream than the current one are kept until it is done with them."""
+    if device.type != "cuda":
+        raise _invalid("the tensors must be on a GPU")
+    if stream is None:
+        if _current_device() == device.index:
+            return run(_raw_stream(device.index))
+        with torch.cuda.device(device):
+            return run(_raw_stream(device.index))
+    if stream.device != device:
+        raise _invalid(f"stream of {stream.device} for tensors on {device}")
+    if stream != torch.cuda.current_stream(device):
+        for t in inputs:
+            if t is not None:
+                t.record_stream(stream)
+    with torch.cuda.stream(stream):
+        return run(stream.cuda_stream)
 
 
 def _matrix(name: str, t):
@@ -105,10 +96,10 @@ def _vector(name: str, t, dtype, n: int, device) -> int:
     return t.data_ptr()
 
 
-def _grad_buffer(out, logits):
-    """The gradient's buffer and row stride: the caller's, or a new one."""
+def _grad_stride(out, logits) -> int:
+    """The row stride of the caller's buffer for the gradient, or of a new one."""
     if out is None:
-        return None
+        return logits.shape[1]
     if out.dtype != logits.dtype or out.shape != logits.shape or out.device != logits.device:
         raise _invalid(f"the gradient's buffer must be {logits.dtype} {tuple(logits.shape)} on {logits.device}")
     return _matrix("the gradient's buffer", out)[2]
@@ -120,12 +111,15 @@ def token_logprobs(logits, tokens, *, temperature: float = 1.0, stream=None) -> 
     rows, vocab, ld, code = _matrix("logits", logits)
     dev = logits.device
     tok = _vector("tokens", tokens, torch.int32, rows, dev)
-    with _Launch(dev, stream, logits, tokens) as st:
+
+    def run(st):
         lp = torch.empty(rows, dtype=torch.float32, device=dev)
         stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
         check(_lib.lib.qs_token_logprobs(logits.data_ptr(), code, rows, vocab, ld, tok, temperature, lp.data_ptr(),
                                          stats.data_ptr(), st))
-    return TokenLogprobs(lp, stats)
+        return TokenLogprobs(lp, stats)
+
+    return _on_stream(dev, stream, (logits, tokens), run)
 
 
 def token_logprobs_backward(logits, tokens, stats, grad_logprobs, *, temperature: float = 1.0, out=None, stream=None):
@@ -138,13 +132,15 @@ def token_logprobs_backward(logits, tokens, stats, grad_logprobs, *, temperature
     if stats.dtype != torch.float32 or stats.shape != (rows, 2) or not stats.is_contiguous() or stats.device != dev:
         raise _invalid(f"stats must be a contiguous float32 tensor [{rows}, 2] on {dev}")
     g = _vector("grad_logprobs", grad_logprobs, torch.float32, rows, dev)
-    gld = _grad_buffer(out, logits)
-    with _Launch(dev, stream, logits, tokens, stats, grad_logprobs, out) as st:
-        if out is None:
-            out, gld = torch.empty((rows, vocab), dtype=logits.dtype, device=dev), vocab
+    gld = _grad_stride(out, logits)
+
+    def run(st):
+        buf = logits.new_empty((rows, vocab)) if out is None else out
         check(_lib.lib.qs_token_logprobs_backward(logits.data_ptr(), code, rows, vocab, ld, tok, stats.data_ptr(), g,
-                                                  temperature, out.data_ptr(), gld, st))
-    return out
+                                                  temperature, buf.data_ptr(), gld, st))
+        return buf
+
+    return _on_stream(dev, stream, (logits, tokens, stats, grad_logprobs, out), run)
 
 
 def policy_loss(logits, tokens, old_logprobs, advantages, *, ref_logprobs=None, weights=None, clip_low: float = 0.2,
@@ -163,19 +159,21 @@ def policy_loss(logits, tokens, old_logprobs, advantages, *, ref_logprobs=None, 
     w = None if weights is None else _vector("weights", weights, torch.float32, rows, dev)
     if out is not None and not grad:
         raise _invalid("a buffer for the gradient without a gradient")
-    gld = _grad_buffer(out, logits)
+    gld = _grad_stride(out, logits)
     params = PolicyParams(clip_low, clip_high, kl_coef, temperature)
-    with _Launch(dev, stream, logits, tokens, old_logprobs, advantages, ref_logprobs, weights, out) as st:
-        if grad and out is None:
-            out, gld = torch.empty((rows, vocab), dtype=logits.dtype, device=dev), vocab
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        lp = torch.empty(rows, dtype=torch.float32, device=dev)
+
+    def run(st):
+        buf = logits.new_empty((rows, vocab)) if grad and out is None else out
+        loss = old_logprobs.new_empty(())
+        lp = old_logprobs.new_empty(rows)
         size = _lib.lib.qs_policy_loss_workspace(rows)
         work = torch.empty(size, dtype=torch.uint8, device=dev)
         check(_lib.lib.qs_policy_loss(logits.data_ptr(), code, rows, vocab, ld, tok, old, ref, adv, w, C.byref(params),
-                                      loss.data_ptr(), lp.data_ptr(), out.data_ptr() if grad else None, gld or 0,
+                                      loss.data_ptr(), lp.data_ptr(), buf.data_ptr() if grad else None, gld,
                                       work.data_ptr(), size, st))
-    return PolicyLoss(loss, lp, out)
+        return PolicyLoss(loss, lp, buf)
+
+    return _on_stream(dev, stream, (logits, tokens, old_logprobs, advantages, ref_logprobs, weights, out), run)
 
 
 def preference_loss(logits, tokens, seq_offsets, ref_logprobs, *, beta: float = 0.1, label_smoothing: float = 0.0,
@@ -198,19 +196,21 @@ def preference_loss(logits, tokens, seq_offsets, ref_logprobs, *, beta: float = 
     w = None if weights is None else _vector("weights", weights, torch.float32, pairs, dev)
     if out is not None and not grad:
         raise _invalid("a buffer for the gradient without a gradient")
-    gld = _grad_buffer(out, logits)
+    gld = _grad_stride(out, logits)
     params = PreferenceParams(beta, label_smoothing)
-    with _Launch(dev, stream, logits, tokens, seq_offsets, ref_logprobs, weights, out) as st:
-        if grad and out is None:
-            out, gld = torch.empty((rows, vocab), dtype=logits.dtype, device=dev), vocab
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        seq = torch.empty(2 * pairs, dtype=torch.float32, device=dev)
+
+    def run(st):
+        buf = logits.new_empty((rows, vocab)) if grad and out is None else out
+        loss = ref_logprobs.new_empty(())
+        seq = ref_logprobs.new_empty(2 * pairs)
         size = _lib.lib.qs_preference_loss_workspace(rows, pairs)
         work = torch.empty(size, dtype=torch.uint8, device=dev)
         check(_lib.lib.qs_preference_loss(logits.data_ptr(), code, rows, vocab, ld, tok, off, pairs, ref, w,
                                           C.byref(params), loss.data_ptr(), seq.data_ptr(),
-                                          out.data_ptr() if grad else None, gld or 0, work.data_ptr(), size, st))
-    return PreferenceLoss(loss, seq, out)
+                                          buf.data_ptr() if grad else None, gld, work.data_ptr(), size, st))
+        return PreferenceLoss(loss, seq, buf)
+
+    return _on_stream(dev, stream, (logits, tokens, seq_offsets, ref_logprobs, weights, out), run)
 
 
 __all__ = ["TokenLogprobs", "PolicyLoss", "PreferenceLoss", "token_logprobs", "token_logprobs_backward", "policy_loss",

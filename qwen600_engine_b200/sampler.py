@@ -254,7 +254,7 @@ class Sampler:
 
     def _lm_head_w4_sample(self, hidden, weight, norm_weight, out, flags: int, stream):
         torch = _torch()
-        from .losses import _Launch
+        from .losses import _on_stream
         from .w4 import _check_rows
         h = _check_rows(hidden, weight, norm_weight)
         B = int(h.shape[0])
@@ -263,12 +263,14 @@ class Sampler:
             raise SamplerError(_lib.QS_ERR_INVALID, f"out must be a contiguous int32 tensor [{B}] on {weight.device}")
         if weight.device.index != self.device:
             raise SamplerError(_lib.QS_ERR_INVALID, f"weight on {weight.device}, the sampler on cuda:{self.device}")
-        with _Launch(weight.device, stream, h, norm_weight, weight.codes, weight.scales, weight.zeros, out) as st:
-            if out is None:
-                out = torch.empty(B, dtype=torch.int32, device=h.device)
-            check(_lib.lib.qs_lm_head_w4_sample(self._h, _ptr(h), _ptr(norm_weight), C.byref(weight._w4_desc), B,
-                                                _ptr(out), st, int(flags)))
-        return out
+
+        def run(st):
+            tokens = torch.empty(B, dtype=torch.int32, device=h.device) if out is None else out
+            check(_lib.lib.qs_lm_head_w4_sample(self._h, _ptr(h), _ptr(norm_weight), weight._w4_ref, B, _ptr(tokens), st,
+                                                int(flags)))
+            return tokens
+
+        return _on_stream(weight.device, stream, (h, norm_weight, weight.codes, weight.scales, weight.zeros, out), run)
 
     def lm_head_logits(self, batch: int):
         """The bf16 logits [batch, vocab] the last lm_head_sample produced (a

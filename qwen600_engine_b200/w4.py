@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from ._lib import QS_BF16, QS_F16, check
-from .losses import _invalid, _Launch
+from .losses import _invalid, _on_stream
 
 _SCALES = {torch.bfloat16: QS_BF16, torch.float16: QS_F16}
 
@@ -31,6 +31,8 @@ class W4Weight:
         self.device = codes.device
         self._w4_desc = _lib.W4Desc(codes.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(),
                                     vocab, hidden_dim, group, scale_dtype)
+        self._w4_ref = C.byref(self._w4_desc)
+        self._row_bytes = _lib.lib.qs_lm_head_w4_workspace(1, hidden_dim, group)
 
     @classmethod
     def pack(cls, codes, scales, zeros=None, *, stream=None) -> "W4Weight":
@@ -53,7 +55,8 @@ class W4Weight:
                 raise _invalid("codes, scales and zeros must be contiguous and on one device")
         dev, code = codes.device, _SCALES[scales.dtype]
         L = _lib.lib
-        with _Launch(dev, stream, codes, scales, zeros) as st:
+
+        def run(st):
             if vocab < 1 or vocab > L.qs_max_vocab() or hidden < 64:
                 raise _invalid(f"vocab {vocab} or hidden_dim {hidden} outside the library's limits")
             pc = torch.empty(L.qs_w4_codes_bytes(vocab, hidden), dtype=torch.uint8, device=dev)
@@ -63,6 +66,11 @@ class W4Weight:
             check(L.qs_w4_pack(codes.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), vocab,
                                hidden, group, code, pc.data_ptr(), ps.data_ptr(), None if pz is None else pz.data_ptr(),
                                st))
+            return pc, ps, pz
+
+        if group not in (32, 64, 128):
+            raise _invalid(f"scales make a group of {group} columns (want 32, 64 or 128)")
+        pc, ps, pz = _on_stream(dev, stream, (codes, scales, zeros), run)
         return cls(pc, ps, pz, vocab, hidden, group, code)
 
     @classmethod
@@ -82,19 +90,22 @@ def quantize_w4(weight, group: int = 128, *, stream=None):
     if group not in (32, 64, 128) or hidden % group:
         raise _invalid(f"group {group} must be 32, 64 or 128 and divide hidden_dim {hidden}")
     dev = weight.device
-    with _Launch(dev, stream, weight) as st:
+
+    def run(st):
         codes = torch.empty((vocab, hidden // 2), dtype=torch.uint8, device=dev)
         scales = torch.empty((vocab, hidden // group), dtype=torch.bfloat16, device=dev)
         zeros = torch.empty((vocab, hidden // group), dtype=torch.uint8, device=dev)
         check(_lib.lib.qs_w4_quantize(weight.data_ptr(), vocab, hidden, group, codes.data_ptr(), scales.data_ptr(),
                                       zeros.data_ptr(), st))
-    return codes, scales, zeros
+        return codes, scales, zeros
+
+    return _on_stream(dev, stream, (weight,), run)
 
 
 def _check_rows(hidden, weight: W4Weight, norm_weight):
     h = hidden if hidden.dim() == 2 else hidden.view(1, -1)
-    for t in (h,) + ((norm_weight,) if norm_weight is not None else ()):
-        if t.dtype != torch.bfloat16 or not t.is_contiguous() or t.device != weight.device:
+    for t in (h, norm_weight):
+        if t is not None and (t.dtype != torch.bfloat16 or not t.is_contiguous() or t.device != weight.device):
             raise _invalid(f"hidden and norm_weight must be contiguous bf16 tensors on {weight.device}")
     if h.shape[1] != weight.hidden_dim:
         raise _invalid(f"hidden has {h.shape[1]} columns, the weight {weight.hidden_dim}")
@@ -108,17 +119,19 @@ def lm_head_w4(hidden, weight: W4Weight, norm_weight=None, *, stream=None):
     [B, hidden_dim]; returns (normed [B, hidden_dim], logits [B, vocab]) bf16,
     as ``sampler.lm_head`` does."""
     h = _check_rows(hidden, weight, norm_weight)
-    B, dev = int(h.shape[0]), weight.device
-    with _Launch(dev, stream, h, norm_weight, weight.codes, weight.scales, weight.zeros) as st:
-        normed = torch.empty((B, weight.hidden_dim), dtype=torch.bfloat16, device=dev)
-        logits = torch.empty((B, weight.vocab), dtype=torch.bfloat16, device=dev)
+    B, dev = h.shape[0], weight.device
+
+    def run(st):
+        normed = torch.empty_like(h)
+        logits = h.new_empty((B, weight.vocab))
         if B:
-            size = _lib.lib.qs_lm_head_w4_workspace(B, weight.hidden_dim, weight.group)
-            work = torch.empty(size, dtype=torch.uint8, device=dev)
+            work = torch.empty(B * weight._row_bytes, dtype=torch.uint8, device=dev)
             check(_lib.lib.qs_lm_head_w4(h.data_ptr(), None if norm_weight is None else norm_weight.data_ptr(),
-                                         C.byref(weight._w4_desc), B, normed.data_ptr(), logits.data_ptr(),
-                                         work.data_ptr(), size, st))
-    return normed, logits
+                                         weight._w4_ref, B, normed.data_ptr(), logits.data_ptr(), work.data_ptr(),
+                                         B * weight._row_bytes, st))
+        return normed, logits
+
+    return _on_stream(dev, stream, (h, norm_weight, weight.codes, weight.scales, weight.zeros), run)
 
 
 __all__ = ["W4Weight", "quantize_w4", "lm_head_w4"]
