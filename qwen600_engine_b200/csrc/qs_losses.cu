@@ -43,6 +43,38 @@ __device__ __forceinline__ float exp2_fast(float v) {
     return r;
 }
 
+// Two fp32 operations in one instruction.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair2(float x, float y) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpair2(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 exp2_pair(f32x2 v) {
+    const float2 t = unpair2(v);
+    return pair2(exp2_fast(t.x), exp2_fast(t.y));
+}
+
 // Block-wide sum of one double per thread, in a fixed order.
 __device__ __forceinline__ double block_sum(double v, double* red) {
 #pragma unroll
@@ -141,7 +173,7 @@ struct Pack<__nv_bfloat16> {
 __device__ __forceinline__ void cluster_arrive_relaxed() {
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_release() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -252,6 +284,14 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
     }
     if (C > 1) cluster_arrive_relaxed();  // waited for before the first store into another CTA
 
+    // what the row's term takes, requested before anything waits
+    float w_row = 0.0f, old_lp = 0.0f, ref_lp = 0.0f, adv = 0.0f;
+    if (kPolicy && t == 0) {
+        if (a.weights) w_row = a.weights[row];
+        old_lp = a.old_lp[row];
+        adv = a.adv[row];
+        if (a.p.kl_coef > 0.0) ref_lp = a.ref_lp[row];
+    }
     const RowShape<T> sh(x, a.V);
     const int per = (sh.vecs + C - 1) >> a.log_c;
     const int base = min(rank * per, sh.vecs), end = min(base + per, sh.vecs);
@@ -290,11 +330,17 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
     for (int w = 1; w < kW; w++) m = fmaxf(m, red_max[w]);
     const float ref = m == -INFINITY ? 0.0f : m;
 
-    // the sum of exponentials against it; the maximum's own terms (exactly 1
-    // each) are counted apart, by the warps that hold one
+    // The sum of exponentials against it.  The maximum's own terms (exactly 1
+    // each) are counted apart, by the warps that hold one; they also subtract
+    // before they scale.  The others scale and subtract in one instruction,
+    // 2^(x scale - bias), where bias = ref scale rounded makes every term
+    // 2^-slip too large; their sum is set right below.  A maximum whose
+    // multiple is not finite leaves all warps to the first way.
+    const float bias = ref * a.scale;
+    const bool apart = __any_sync(0xffffffffu, own_max == ref) || !(fabsf(bias) < INFINITY);
     float s = 0.0f;
     int n = 0;
-    if (__any_sync(0xffffffffu, own_max == ref)) {
+    if (apart) {
 #pragma unroll
         for (int i = 0; i < kVpt; i++) {
             float o[kN];
@@ -312,15 +358,18 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
         s += d == 0.0f ? 0.0f : exp2_fast(d * a.scale);
         n = warp_sum_int(n);
     } else {
-        float s2[2] = {exp2_fast((xe - ref) * a.scale), 0.0f};
+        const f32x2 scale2 = pair2(a.scale, a.scale), bias2 = pair2(-bias, -bias);
+        f32x2 s2 = pair2(exp2_fast(__fmaf_rn(xe, a.scale, -bias)), 0.0f);
 #pragma unroll
         for (int i = 0; i < kVpt; i++) {
             float o[kN];
             Pack<T>::widen(v[i], o);
 #pragma unroll
-            for (int j = 0; j < kN; j++) s2[j & 1] += exp2_fast((o[j] - ref) * a.scale);
+            for (int j = 0; j < kN; j += 2) s2 = add2(s2, exp2_pair(fma2(pair2(o[j], o[j + 1]), scale2, bias2)));
         }
-        s = s2[0] + s2[1];
+        const float2 u = unpair2(s2);
+        const float slip = __fmaf_rn(ref, a.scale, -bias);
+        s = (u.x + u.y) * exp2_fast(-slip);
     }
     s = warp_sum(s);
     if ((t & 31) == 0) {
@@ -338,8 +387,9 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
         if (C > 1) push_part(&parts[rank], t, p);
         else parts[0] = p;
     }
-    if (C > 1) {
-        cluster_arrive();
+    if (C > 1) {  // only the warp that stored into the others has stores to release
+        if (t < 32) cluster_arrive_release();
+        else cluster_arrive_relaxed();
         cluster_wait();
     }
     if (!kPolicy && rank != 0) return;
@@ -367,10 +417,10 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
                 }
             }
             if (kPolicy) {
-                const double w = a.weights ? (double)a.weights[row] : 1.0 / a.rows;
+                const double w = a.weights ? (double)w_row : 1.0 / a.rows;
                 double slope;
-                const double l = policy_term(lp, a.old_lp[row], a.p.kl_coef > 0.0 ? (double)a.ref_lp[row] : 0.0,
-                                             a.adv[row], 1.0 - a.p.clip_low, 1.0 + a.p.clip_high, a.p.kl_coef, &slope);
+                const double l = policy_term(lp, old_lp, ref_lp, adv, 1.0 - a.p.clip_low, 1.0 + a.p.clip_high,
+                                             a.p.kl_coef, &slope);
                 if (rank == 0) a.row_loss[row] = w * l;
                 const double c = w * slope * a.inv_t;
                 factor_s = (float)(-c / (1.0 + excess));
@@ -381,7 +431,14 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
     }
     if (!kPolicy || !g) return;
     __syncthreads();
-    const float f = factor_s, M = max_s;
+    float f = factor_s;
+    const float M = max_s, top = M * a.scale;
+    const bool plain = fabsf(top) < INFINITY;
+    if (plain) f *= exp2_fast(-__fmaf_rn(M, a.scale, -top));
+    const auto grad_of = [&](float v) {
+        return f == 0.0f ? 0.0f : f * exp2_fast(plain ? __fmaf_rn(v, a.scale, -top) : (v - M) * a.scale);
+    };
+    const f32x2 f2 = pair2(f, f), scale2 = pair2(a.scale, a.scale), top2 = pair2(-top, -top);
     const bool aligned = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
     T* gbody = g + sh.head;
 #pragma unroll
@@ -389,8 +446,17 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
         const int k = base + i * kThr + t;
         float o[kN];
         Pack<T>::widen(v[i], o);
+        if (plain && f != 0.0f) {
 #pragma unroll
-        for (int j = 0; j < kN; j++) o[j] = f == 0.0f ? 0.0f : f * exp2_fast((o[j] - M) * a.scale);
+            for (int j = 0; j < kN; j += 2) {
+                const float2 r = unpair2(mul2(f2, exp2_pair(fma2(pair2(o[j], o[j + 1]), scale2, top2))));
+                o[j] = r.x;
+                o[j + 1] = r.y;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kN; j++) o[j] = grad_of(o[j]);
+        }
         if (k < end) {
             if (aligned) {
                 store16(gbody + (size_t)k * kN, Pack<T>::narrow(o));
@@ -400,7 +466,7 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
             }
         }
     }
-    if (edge >= 0 && edge != tok) put(g, edge, f == 0.0f ? 0.0f : f * exp2_fast((xe - M) * a.scale));
+    if (edge >= 0 && edge != tok) put(g, edge, grad_of(xe));
     // the target, by the thread that wrote its vector
     const int at = tok - sh.head;
     if (at < 0 || at >= sh.vecs * kN) {
