@@ -14,9 +14,11 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "qs_common.cuh"
+#include "qs_pipe.cuh"
 #include "qwen600_sampler.h"
 
 namespace qs {
@@ -220,6 +222,9 @@ __device__ __forceinline__ double beyond(float xt, float max, double excess, dou
     return xt == max ? excess / (1.0 + excess) : 1.0 - exp(((double)xt - (double)max) * inv_t) / (1.0 + excess);
 }
 
+constexpr int kScoreThreads = 256;                        // at most, in a CTA
+constexpr unsigned long long kLoadWaitNs = 2000000000ull;  // a copy that has not landed by then: NaN
+
 template <typename T>
 struct ScoreArgs {
     const T* logits;
@@ -244,22 +249,30 @@ struct ScoreArgs {
 };
 
 // Scores one row per cluster of 1 to 8 CTAs; with kPolicy it also forms the
-// row's policy loss and writes its gradient.  Each CTA takes a contiguous
-// share of the row's 16-byte vectors into registers, all its loads in flight
-// at once.  So the row is read once, its maximum is known before the first
+// row's policy loss and writes its gradient.  Each CTA brings a contiguous
+// share of the row's 16-byte vectors to shared memory with one bulk copy.  So
+// the row is read from memory once, its maximum is known before the first
 // exponential (no sum is rescaled), and the gradient is formed from the same
-// registers.  The CTAs exchange their parts, 16 bytes each, through
-// distributed shared memory.
-template <typename T, int kThr, int kVpt, bool kPolicy>
-__global__ void __launch_bounds__(kThr)
+// copy.  The CTAs exchange their parts, 16 bytes each, through distributed
+// shared memory.
+//
+// Bound: memory, as long as enough rows are under way: from its copy to its
+// last store a CTA of 38 KB (a bf16 row of 151,936 over 8) takes about 8 us, so
+// an SM needs some 200 KB in flight.  Shared memory holds five such CTAs; in
+// registers (80 a thread of 256) it were three, 293 us for REPLACE.
+template <typename T, bool kPolicy>
+__global__ void __launch_bounds__(kScoreThreads)
 score_kernel(const __grid_constant__ ScoreArgs<T> a) {
     constexpr int kN = Pack<T>::kN;
-    constexpr int kW = kThr / 32;
+    constexpr int kW = kScoreThreads / 32;
+    extern __shared__ __align__(16) uint4 vecs[];
     __shared__ Part parts[8];
     __shared__ float red_max[kW], red_sum[kW];
     __shared__ int red_n[kW];
     __shared__ float factor_s, max_s, target_s;
-    const int t = threadIdx.x, C = 1 << a.log_c;
+    __shared__ unsigned long long loaded;
+    __shared__ int gave_up;
+    const int t = threadIdx.x, thr = blockDim.x, C = 1 << a.log_c;
     const int row = blockIdx.x >> a.log_c, rank = blockIdx.x & (C - 1);
     const int tok = a.tokens[row];
     const bool scored = tok >= 0 && tok < a.V && !(kPolicy && a.weights && a.weights[row] == 0.0f);
@@ -275,15 +288,31 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
         }
         if (kPolicy && g) {
             const RowShape<T> gs(g, a.V);
-            for (int i = rank * kThr + t; i < gs.vecs; i += C * kThr)
+            for (int i = rank * thr + t; i < gs.vecs; i += C * thr)
                 store16(g + gs.head + (size_t)i * kN, make_uint4(0u, 0u, 0u, 0u));
             const int e = rank == 0 ? gs.edge(t, a.V) : -1;
             if (e >= 0) put(g, e, 0.0f);
         }
         return;
     }
-    if (C > 1) cluster_arrive_relaxed();  // waited for before the first store into another CTA
 
+    const RowShape<T> sh(x, a.V);
+    const int per = (sh.vecs + C - 1) >> a.log_c;
+    const int first = min(rank * per, sh.vecs), cnt = min(per, sh.vecs - first);
+    if (t == 0) {
+        gave_up = 0;
+        mbar_init(&loaded, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_expect_tx(&loaded, (uint32_t)cnt * 16u);
+        if (cnt > 0)
+            asm volatile(
+                "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                    smem_u32(vecs)),
+                "l"(x + sh.head + (size_t)first * kN), "r"((uint32_t)cnt * 16u), "r"(smem_u32(&loaded))
+                : "memory");
+    }
+    if (C > 1) cluster_arrive_relaxed();  // waited for before the first store into another CTA
     // what the row's term takes, requested before anything waits
     float w_row = 0.0f, old_lp = 0.0f, ref_lp = 0.0f, adv = 0.0f;
     if (kPolicy && t == 0) {
@@ -292,30 +321,24 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
         adv = a.adv[row];
         if (a.p.kl_coef > 0.0) ref_lp = a.ref_lp[row];
     }
-    const RowShape<T> sh(x, a.V);
-    const int per = (sh.vecs + C - 1) >> a.log_c;
-    const int base = min(rank * per, sh.vecs), end = min(base + per, sh.vecs);
-    const T* body = x + sh.head;
-    uint4 v[kVpt];
-#pragma unroll
-    for (int i = 0; i < kVpt; i++) {
-        const int k = base + i * kThr + t;
-        v[i] = k < end ? load16(body + (size_t)k * kN) : Pack<T>::lowest();
-    }
     const int edge = rank == 0 ? sh.edge(t, a.V) : -1;
     const float xe = edge >= 0 ? elem(x, edge) : -INFINITY;
     const float xt = elem(x, tok);
+    __syncthreads();
+    const bool whole = mbar_wait(&loaded, 0, &gave_up, kLoadWaitNs);
+    if (!whole) mbar_wait(&loaded, 0, &gave_up, kLoadWaitNs, false);  // the copy lands before the CTA leaves
 
     // the maximum of this CTA's part
     float own_max = xe;
     {
         uint4 u = Pack<T>::lowest();
-#pragma unroll
-        for (int i = 0; i < kVpt; i++) {
-            u.x = Pack<T>::max2(u.x, v[i].x);
-            u.y = Pack<T>::max2(u.y, v[i].y);
-            u.z = Pack<T>::max2(u.z, v[i].z);
-            u.w = Pack<T>::max2(u.w, v[i].w);
+#pragma unroll 4
+        for (int k = t; k < cnt; k += thr) {
+            const uint4 v = vecs[k];
+            u.x = Pack<T>::max2(u.x, v.x);
+            u.y = Pack<T>::max2(u.y, v.y);
+            u.z = Pack<T>::max2(u.z, v.z);
+            u.w = Pack<T>::max2(u.w, v.w);
         }
         float o[kN];
         Pack<T>::widen(u, o);
@@ -326,8 +349,7 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
     if ((t & 31) == 0) red_max[t >> 5] = m;
     __syncthreads();
     m = red_max[0];
-#pragma unroll
-    for (int w = 1; w < kW; w++) m = fmaxf(m, red_max[w]);
+    for (int w = 1; w < thr / 32; w++) m = fmaxf(m, red_max[w]);
     const float ref = m == -INFINITY ? 0.0f : m;
 
     // The sum of exponentials against it.  The maximum's own terms (exactly 1
@@ -341,10 +363,10 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
     float s = 0.0f;
     int n = 0;
     if (apart) {
-#pragma unroll
-        for (int i = 0; i < kVpt; i++) {
+#pragma unroll 2
+        for (int k = t; k < cnt; k += thr) {
             float o[kN];
-            Pack<T>::widen(v[i], o);
+            Pack<T>::widen(vecs[k], o);
 #pragma unroll
             for (int j = 0; j < kN; j++) {
                 const float d = o[j] - ref;
@@ -360,10 +382,10 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
     } else {
         const f32x2 scale2 = pair2(a.scale, a.scale), bias2 = pair2(-bias, -bias);
         f32x2 s2 = pair2(exp2_fast(__fmaf_rn(xe, a.scale, -bias)), 0.0f);
-#pragma unroll
-        for (int i = 0; i < kVpt; i++) {
+#pragma unroll 2
+        for (int k = t; k < cnt; k += thr) {
             float o[kN];
-            Pack<T>::widen(v[i], o);
+            Pack<T>::widen(vecs[k], o);
 #pragma unroll
             for (int j = 0; j < kN; j += 2) s2 = add2(s2, exp2_pair(fma2(pair2(o[j], o[j + 1]), scale2, bias2)));
         }
@@ -379,8 +401,8 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
     __syncthreads();
     if (C > 1) cluster_wait();  // every CTA of the cluster runs
     if (t < C) {
-        Part p{m, 0, 0.0};
-        for (int w = 0; w < kW; w++) {
+        Part p{m, 0, whole ? 0.0 : (double)NAN};
+        for (int w = 0; w < thr / 32; w++) {
             p.others += (double)red_sum[w];
             p.at_max += red_n[w];
         }
@@ -440,12 +462,11 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
     };
     const f32x2 f2 = pair2(f, f), scale2 = pair2(a.scale, a.scale), top2 = pair2(-top, -top);
     const bool aligned = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
-    T* gbody = g + sh.head;
-#pragma unroll
-    for (int i = 0; i < kVpt; i++) {
-        const int k = base + i * kThr + t;
+    T* gbody = g + sh.head + (size_t)first * kN;
+#pragma unroll 2
+    for (int k = t; k < cnt; k += thr) {
         float o[kN];
-        Pack<T>::widen(v[i], o);
+        Pack<T>::widen(vecs[k], o);
         if (plain && f != 0.0f) {
 #pragma unroll
             for (int j = 0; j < kN; j += 2) {
@@ -457,13 +478,11 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
 #pragma unroll
             for (int j = 0; j < kN; j++) o[j] = grad_of(o[j]);
         }
-        if (k < end) {
-            if (aligned) {
-                store16(gbody + (size_t)k * kN, Pack<T>::narrow(o));
-            } else {
+        if (aligned) {
+            store16(gbody + (size_t)k * kN, Pack<T>::narrow(o));
+        } else {
 #pragma unroll
-                for (int j = 0; j < kN; j++) put(gbody, (long long)k * kN + j, o[j]);
-            }
+            for (int j = 0; j < kN; j++) put(gbody, (long long)k * kN + j, o[j]);
         }
     }
     if (edge >= 0 && edge != tok) put(g, edge, grad_of(xe));
@@ -472,8 +491,8 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
     if (at < 0 || at >= sh.vecs * kN) {
         if (edge == tok) put(g, tok, target_s);
     } else {
-        const int k = at / kN - base;
-        if (k >= 0 && k < end - base && k % kThr == t) put(g, tok, target_s);
+        const int k = at / kN - first;
+        if (k >= 0 && k < cnt && k % thr == t) put(g, tok, target_s);
     }
 }
 
@@ -656,11 +675,12 @@ static int check_rows(const Rows& r, double temperature) {
 // Launches `kernel` in clusters of `cluster` CTAs; `after`: it may start while
 // the kernel before it ends (it waits for it before it reads its results).
 template <typename... P, typename... A>
-static int launch(const char* name, void (*kernel)(P...), long long grid, int threads, int cluster, bool after,
-                  cudaStream_t st, A... args) {
+static int launch(const char* name, void (*kernel)(P...), long long grid, int threads, int cluster, size_t smem,
+                  bool after, cudaStream_t st, A... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2] = {};
     if (cluster > 1) {
@@ -679,10 +699,9 @@ static int launch(const char* name, void (*kernel)(P...), long long grid, int th
     return e == cudaSuccess ? QS_OK : fail(QS_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
 }
 
-// How a row is spread: CTAs per row (a power of two up to 8) such that a CTA
-// holds at most 2560 vectors (40 KB, 10 vectors a thread), and more of them
-// while the rows alone would leave SMs idle and a CTA keeps 256 vectors.  Then
-// the smallest kernel that holds a share.
+// How a row is spread: CTAs per row (a power of two up to 8) such that a share
+// is at most 40 KB, and more of them while the rows alone would leave SMs idle
+// and a share keeps 4 KB.
 template <typename T, bool kPolicy>
 static int score_launch(ScoreArgs<T>& a, cudaStream_t st) {
     const int vecs = a.V / Pack<T>::kN;
@@ -690,22 +709,20 @@ static int score_launch(ScoreArgs<T>& a, cudaStream_t st) {
     const auto share = [&] { return (vecs + (1 << log_c) - 1) >> log_c; };
     while (log_c < 3 && (share() > 2560 || ((long long)a.rows << log_c) < 148 && share() > 256)) log_c++;
     a.log_c = log_c;
-    const int need = share(), c = 1 << log_c;
-    const long long grid = (long long)a.rows << log_c;
-#define QS_SCORE(thr, vpt)             \
-    if (need <= (thr) * (vpt))         \
-    return launch("score_kernel", score_kernel<T, thr, vpt, kPolicy>, grid, thr, c, false, st, a)
-    QS_SCORE(256, 1);
-    QS_SCORE(256, 2);
-    QS_SCORE(256, 4);
-    QS_SCORE(256, 6);
-    QS_SCORE(256, 8);
-    QS_SCORE(256, 10);
-    QS_SCORE(512, 8);
-    QS_SCORE(512, 10);
-    QS_SCORE(512, 16);
-#undef QS_SCORE
-    return fail(QS_ERR_UNSUPPORTED, "vocab %d", a.V);
+    const int threads = share() > 128 ? 256 : 128;
+    const size_t smem = (size_t)share() * 16;
+    if (smem > 40 * 1024) {
+        static std::atomic<unsigned long long> raised{0};  // devices on which the kernel may use all shared memory
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e == cudaSuccess && (dev >= 64 || !(raised.load() >> dev & 1))) {
+            e = cudaFuncSetAttribute(score_kernel<T, kPolicy>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+            if (e == cudaSuccess && dev < 64) raised.fetch_or(1ull << dev);
+        }
+        if (e != cudaSuccess) return fail(QS_ERR_CUDA, "score_kernel: %s", cudaGetErrorString(e));
+    }
+    return launch("score_kernel", score_kernel<T, kPolicy>, (long long)a.rows << log_c, threads, 1 << log_c, smem, false,
+                  st, a);
 }
 
 template <typename T>
@@ -736,7 +753,7 @@ template <typename T>
 static int grad(const Rows& r, const float* stats, int stat_words, const float* coefs, bool after, cudaStream_t st) {
     const int vecs = r.vocab / Pack<T>::kN;
     const int pieces = max(1, (vecs + kGradThreads * kGradVpt - 1) / (kGradThreads * kGradVpt));
-    return launch("grad_kernel", grad_kernel<T>, (long long)r.rows * pieces, kGradThreads, 1, after, st,
+    return launch("grad_kernel", grad_kernel<T>, (long long)r.rows * pieces, kGradThreads, 1, 0, after, st,
                   (const T*)r.logits, r.rows, r.vocab, r.ld, r.tokens, stats, stat_words, coefs,
                   (float)(r.inv_t * 1.4426950408889634), r.inv_t, (T*)r.grad, r.gld, pieces);
 }
@@ -815,7 +832,7 @@ int qs_policy_loss(const void* d_logits, int dtype, int rows, int vocab, long lo
         const int e = dtype == QS_F32 ? go(score_args<float>(r)) : go(score_args<__nv_bfloat16>(r));
         if (e) return e;
     }
-    return launch("sum_rows_kernel", sum_rows_kernel, 1, 1024, 1, rows > 0, st, row_loss, rows, d_loss);
+    return launch("sum_rows_kernel", sum_rows_kernel, 1, 1024, 1, 0, rows > 0, st, row_loss, rows, d_loss);
 }
 
 size_t qs_preference_loss_workspace(int rows, int pairs) {
@@ -851,7 +868,7 @@ int qs_preference_loss(const void* d_logits, int dtype, int rows, int vocab, lon
                                       : score<__nv_bfloat16>(r, sc, nullptr, nullptr, st);
         if (e) return e;
     }
-    const int e = launch("preference_pairs_kernel", preference_pairs_kernel, 1, 1024, 1, rows > 0, st, sc, rows,
+    const int e = launch("preference_pairs_kernel", preference_pairs_kernel, 1, 1024, 1, 0, rows > 0, st, sc, rows,
                          d_seq_offsets, pairs, d_ref_logprobs, d_weights, p, coefs, d_seq_logprobs, d_loss);
     if (e || rows == 0 || !d_grad) return e;
     return dtype == QS_F32 ? grad<float>(r, &sc->max, sizeof(RowScore) / 4, coefs, true, st)
