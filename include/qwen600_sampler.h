@@ -397,16 +397,19 @@ QS_API int qs_lm_head_w4_sample(qs_sampler* s, const void* d_hidden, const void*
  * overlap it otherwise.  Exponentials are fp32 (relative error below 2^-20),
  * sums over rows and sequences 64-bit, in a fixed order: the same inputs give
  * the same bits.  vocab <= qs_max_vocab(), rows <= 2^27.  Nothing is
- * allocated and no state is kept; calls that overlap on the GPU need
- * workspaces of their own. */
+ * allocated and no state is kept.  A workspace of the *_workspace call's bytes
+ * (where that is 0, it may be NULL) is 16-byte aligned, needs no
+ * initialisation, and belongs to the call until it is done: calls that overlap
+ * on the GPU need workspaces of their own. */
 
 /* d_logprobs fp32 [rows]; d_stats fp32 [rows, 2] (for the backward call): the
  * row's maximum, and sum_j exp((x[j] - max x) / T) - 1 (the maximum's own term
  * left out, so that a peaked row keeps its precision); both 0 for a row that
  * scores nothing. */
+QS_API size_t qs_token_logprobs_workspace(int dtype, int rows, int vocab);
 QS_API int qs_token_logprobs(const void* d_logits, int dtype, int rows, int vocab, long long row_stride,
                              const int* d_tokens, double temperature, float* d_logprobs, float* d_stats,
-                             void* stream);
+                             void* d_workspace, size_t workspace_bytes, void* stream);
 
 /* grad[i][j] = g[i] * ([j = t] - exp((x[j] - max x) / T) / sum) / T from the
  * forward call's d_stats and the incoming d_grad_logprobs g, fp32 [rows].  A
@@ -458,7 +461,7 @@ typedef struct {
     double label_smoothing;
 } qs_preference_params;
 
-QS_API size_t qs_preference_loss_workspace(int rows, int pairs);
+QS_API size_t qs_preference_loss_workspace(int dtype, int rows, int vocab);
 QS_API int qs_preference_loss(const void* d_logits, int dtype, int rows, int vocab, long long row_stride,
                               const int* d_tokens, const int* d_seq_offsets, int pairs,
                               const float* d_ref_logprobs, const float* d_weights,

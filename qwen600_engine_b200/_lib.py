@@ -36,10 +36,11 @@ EXPORTS = (
     "qs_lm_head_status", "qs_lm_head_set_wait_limit", "qs_lm_head_shard", "qs_ipc_handle_bytes", "qs_ipc_alloc", "qs_ipc_open",
     "qs_ipc_close", "qs_ipc_free", "qs_shard_handshake", "qs_copy_async",
     "qs_w4_codes_bytes", "qs_w4_scales_bytes", "qs_w4_zeros_bytes", "qs_w4_quantize", "qs_w4_pack",
-    "qs_lm_head_w4_workspace", "qs_lm_head_w4", "qs_lm_head_w4_sample", "qs_token_logprobs", "qs_token_logprobs_backward",
+    "qs_lm_head_w4_workspace", "qs_lm_head_w4", "qs_lm_head_w4_sample", "qs_token_logprobs_workspace", "qs_token_logprobs",
+    "qs_token_logprobs_backward",
     "qs_policy_loss_workspace", "qs_policy_loss", "qs_preference_loss_workspace", "qs_preference_loss",
 )
-_SIZES = ("qs_lm_head_w4_workspace", "qs_w4_codes_bytes", "qs_w4_scales_bytes", "qs_w4_zeros_bytes", "qs_policy_loss_workspace",
+_SIZES = ("qs_token_logprobs_workspace", "qs_lm_head_w4_workspace", "qs_w4_codes_bytes", "qs_w4_scales_bytes", "qs_w4_zeros_bytes", "qs_policy_loss_workspace",
           "qs_preference_loss_workspace")
 
 
@@ -137,12 +138,13 @@ def _load() -> C.CDLL:
     lib.qs_lm_head_w4_workspace.argtypes = [i32, i32, i32]
     lib.qs_lm_head_w4.argtypes = [vp, vp, P(W4Desc), i32, vp, vp, vp, sz, vp]
     lib.qs_lm_head_w4_sample.argtypes = [vp, vp, vp, P(W4Desc), i32, vp, vp, u32]
-    lib.qs_token_logprobs.argtypes = [vp, i32, i32, i32, i64, vp, f64, vp, vp, vp]
+    lib.qs_token_logprobs_workspace.argtypes = [i32, i32, i32]
+    lib.qs_token_logprobs.argtypes = [vp, i32, i32, i32, i64, vp, f64, vp, vp, vp, sz, vp]
     lib.qs_token_logprobs_backward.argtypes = [vp, i32, i32, i32, i64, vp, vp, vp, f64, vp, i64, vp]
     lib.qs_policy_loss_workspace.argtypes = [i32]
     lib.qs_policy_loss.argtypes = [vp, i32, i32, i32, i64, vp, vp, vp, vp, vp, P(PolicyParams), vp, vp,
                                    vp, i64, vp, sz, vp]
-    lib.qs_preference_loss_workspace.argtypes = [i32, i32]
+    lib.qs_preference_loss_workspace.argtypes = [i32, i32, i32]
     lib.qs_preference_loss.argtypes = [vp, i32, i32, i32, i64, vp, vp, i32, vp, vp, P(PreferenceParams),
                                        vp, vp, vp, i64, vp, sz, vp]
     lib.qs_last_error.restype = C.c_char_p

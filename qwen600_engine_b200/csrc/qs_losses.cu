@@ -496,6 +496,277 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
     }
 }
 
+// ------------------------------------------------- scoring many rows
+// Without a gradient a row need not stay on the chip, and a call of many rows
+// is a stream: rows are cut into units of 256 vectors (4 KB), every warp of a
+// persistent grid takes units in turn through its own ring of bulk copies and
+// leaves each unit's maximum and sum of exponentials, and a second kernel joins
+// a row's units.  Warps never wait for one another, so the copies keep running
+// while others compute (the cluster kernel spends a third of its time
+// waiting: 68.7 us against REPLACE for 1024 bf16 rows of 151,936).
+constexpr int kUnitVecs = 256;
+constexpr int kStreamWarps = 24;
+constexpr int kStreamStages = 2;
+
+template <typename T>
+struct StreamArgs {
+    const T* logits;
+    int rows, V;
+    long long ld;
+    const int* tokens;
+    float scale;
+    double inv_t;
+    int units;     // per row
+    float2* parts; // [rows][units]: maximum, sum of exponentials against it
+    RowScore* out;
+    float* logprobs;
+    float* stats;
+};
+
+// Where a warp is in its units: it takes every stride-th one.
+struct UnitAt {
+    int row, unit;
+    __device__ __forceinline__ void step(int rows, int units, int units_per_row) {
+        row += rows;
+        unit += units;
+        if (unit >= units_per_row) {
+            unit -= units_per_row;
+            row++;
+        }
+    }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kStreamWarps * 32, 1)
+stream_kernel(const __grid_constant__ StreamArgs<T> a) {
+    constexpr int kN = Pack<T>::kN;
+    extern __shared__ __align__(128) uint4 ring[];  // [warp][stage][kUnitVecs]
+    __shared__ unsigned long long full[kStreamWarps][kStreamStages];
+    __shared__ int gave_up;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint4* mine = ring + (size_t)warp * kStreamStages * kUnitVecs;
+    if (threadIdx.x == 0) gave_up = 0;
+    if (lane == 0) {
+        for (int i = 0; i < kStreamStages; i++) mbar_init(&full[warp][i], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+    dependents_may_start();
+
+    const long long stride = (long long)gridDim.x * kStreamWarps, begin = (long long)warp * gridDim.x + blockIdx.x;
+    const int dr = (int)(stride / a.units), du = (int)(stride % a.units);
+    UnitAt now{(int)(begin / a.units), (int)(begin % a.units)}, ahead = now;
+    const auto scored = [&](int row) {
+        if (row >= a.rows) return false;
+        const int tok = a.tokens[row];
+        return tok >= 0 && tok < a.V;
+    };
+    const auto request = [&](const UnitAt& u, int stage) {
+        if (lane == 0) {
+            const T* x = a.logits + (size_t)u.row * a.ld;
+            const RowShape<T> sh(x, a.V);
+            const int first = u.unit * kUnitVecs, cnt = max(0, min(kUnitVecs, sh.vecs - first));
+            mbar_expect_tx(&full[warp][stage], (uint32_t)cnt * 16u);
+            if (cnt > 0)
+                asm volatile(
+                    "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                        smem_u32(mine + stage * kUnitVecs)),
+                    "l"(x + sh.head + (size_t)first * kN), "r"((uint32_t)cnt * 16u), "r"(smem_u32(&full[warp][stage]))
+                    : "memory");
+        }
+    };
+    uint32_t live = 0;    // stages with a copy under way
+    uint32_t phases = 0;  // the parity each stage's next copy completes
+#pragma unroll
+    for (int i = 0; i < kStreamStages; i++) {
+        if (scored(ahead.row)) {
+            request(ahead, i);
+            live |= 1u << i;
+        }
+        ahead.step(dr, du, a.units);
+    }
+    bool next = scored(ahead.row);  // looked up one unit before it is asked for
+    bool dead = false;
+    for (int stage = 0; now.row < a.rows; stage = stage + 1 == kStreamStages ? 0 : stage + 1) {
+        if (live >> stage & 1) {
+            const bool landed = !dead && mbar_wait(&full[warp][stage], phases >> stage & 1, &gave_up, kLoadWaitNs);
+            if (!landed) {
+                mbar_wait(&full[warp][stage], phases >> stage & 1, &gave_up, kLoadWaitNs, false);
+                dead = true;
+            }
+            phases ^= 1u << stage;
+            const T* x = a.logits + (size_t)now.row * a.ld;
+            const RowShape<T> sh(x, a.V);
+            const int cnt = max(0, min(kUnitVecs, sh.vecs - now.unit * kUnitVecs));
+            const int edge = now.unit == 0 ? sh.edge(lane, a.V) : -1;
+            const float xe = edge >= 0 ? elem(x, edge) : -INFINITY;
+            uint4 v[kUnitVecs / 32];
+            uint4 u = Pack<T>::lowest();
+#pragma unroll
+            for (int i = 0; i < kUnitVecs / 32; i++) {
+                const int k = i * 32 + lane;
+                v[i] = k < cnt ? mine[stage * kUnitVecs + k] : Pack<T>::lowest();
+                u.x = Pack<T>::max2(u.x, v[i].x);
+                u.y = Pack<T>::max2(u.y, v[i].y);
+                u.z = Pack<T>::max2(u.z, v[i].z);
+                u.w = Pack<T>::max2(u.w, v[i].w);
+            }
+            __syncwarp();  // every lane has read the stage
+            live &= ~(1u << stage);
+            if (next && !dead) {
+                request(ahead, stage);
+                live |= 1u << stage;
+            }
+            float o[kN];
+            Pack<T>::widen(u, o);
+            float m = xe;
+#pragma unroll
+            for (int j = 0; j < kN; j++) m = fmaxf(m, o[j]);
+            m = warp_max(m);
+            const float ref = m == -INFINITY ? 0.0f : m;
+            // 2^(x scale - bias), each 2^-slip too large for the rounding of bias
+            const float bias = ref * a.scale;
+            float s;
+            if (fabsf(bias) < INFINITY) {
+                const f32x2 scale2 = pair2(a.scale, a.scale), bias2 = pair2(-bias, -bias);
+                f32x2 s2 = pair2(exp2_fast(__fmaf_rn(xe, a.scale, -bias)), 0.0f);
+#pragma unroll
+                for (int i = 0; i < kUnitVecs / 32; i++) {
+                    Pack<T>::widen(v[i], o);
+#pragma unroll
+                    for (int j = 0; j < kN; j += 2) s2 = add2(s2, exp2_pair(fma2(pair2(o[j], o[j + 1]), scale2, bias2)));
+                }
+                const float2 r = unpair2(s2);
+                s = (r.x + r.y) * exp2_fast(-__fmaf_rn(ref, a.scale, -bias));
+            } else {
+                s = exp2_fast((xe - ref) * a.scale);
+#pragma unroll 1
+                for (int i = 0; i < kUnitVecs / 32; i++) {
+                    uint4 w = v[0];
+#pragma unroll
+                    for (int k = 1; k < kUnitVecs / 32; k++)
+                        if (k == i) w = v[k];
+                    Pack<T>::widen(w, o);
+                    for (int j = 0; j < kN; j++) s += exp2_fast((o[j] - ref) * a.scale);
+                }
+            }
+            s = warp_sum(s);
+            if (lane == 0) a.parts[(size_t)now.row * a.units + now.unit] = make_float2(m, dead ? NAN : s);
+        } else {
+            if (lane == 0 && dead) a.parts[(size_t)now.row * a.units + now.unit] = make_float2(0.0f, NAN);
+            if (next && !dead) {
+                request(ahead, stage);
+                live |= 1u << stage;
+            }
+        }
+        now.step(dr, du, a.units);
+        ahead.step(dr, du, a.units);
+        next = scored(ahead.row);
+    }
+}
+
+// Joins a row's units, one warp a row.  The maximum's own term is exactly 1;
+// where the others together are less than that, the unit that holds it is read
+// again to sum the others apart from it (beyond, the 1 in a fp32 sum costs less
+// than the exponentials do).
+constexpr int kJoinRows = 4;                                    // a CTA: small enough to start beside the stream
+constexpr int kMaxUnits = kMaxVocab / 4 / kUnitVecs;            // of a row
+static_assert(kMaxUnits % 32 == 0, "units of a lane");
+
+template <typename T>
+__global__ void __launch_bounds__(kJoinRows * 32)
+join_kernel(const __grid_constant__ StreamArgs<T> a) {
+    constexpr int kN = Pack<T>::kN;
+    constexpr int kMine = kMaxUnits / 32;
+    const int row = blockIdx.x * kJoinRows + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    dependents_may_start();
+    const int tok = row < a.rows ? a.tokens[row] : -1;
+    const bool scored = tok >= 0 && tok < a.V;
+    const T* x = a.logits + (size_t)row * a.ld;
+    const float xt = scored ? elem(x, tok) : 0.0f;
+    wait_for_previous();
+    if (row >= a.rows) return;
+    RowScore r{0.0, 0.0f, 0.0f, 0, 0};
+    if (scored) {
+        const float2* all = a.parts + (size_t)row * a.units;
+        float2 p[kMine];
+        float M = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kMine; i++) {
+            p[i] = i * 32 + lane < a.units ? all[i * 32 + lane] : make_float2(-INFINITY, 0.0f);
+            M = fmaxf(M, p[i].x);
+        }
+        M = warp_max(M);
+        double rest = 0.0, held = 0.0;  // units below the maximum, units that hold it
+        uint32_t hold = 0;              // this lane's units that hold it
+#pragma unroll
+        for (int i = 0; i < kMine; i++) {
+            const bool in = i * 32 + lane < a.units, top = in && p[i].x == M;
+            if (top) held += (double)p[i].y;
+            else if (in) rest += (double)(exp2_fast((p[i].x - M) * a.scale) * p[i].y);
+            hold |= (uint32_t)top << i;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            rest += __shfl_xor_sync(0xffffffffu, rest, o);
+            held += __shfl_xor_sync(0xffffffffu, held, o);
+        }
+        double excess = rest + held - 1.0;
+        if (excess < 1.0) {
+            const RowShape<T> sh(x, a.V);
+            double sum = 0.0;
+            int n = 0;
+#pragma unroll 1
+            for (int i = 0; i < kMine; i++) {
+                uint32_t lanes = __ballot_sync(0xffffffffu, hold >> i & 1);
+                for (; lanes; lanes &= lanes - 1) {
+                    const int unit = i * 32 + __ffs(lanes) - 1, first = unit * kUnitVecs;
+                    const int cnt = max(0, min(kUnitVecs, sh.vecs - first));
+                    const int edge = unit == 0 ? sh.edge(lane, a.V) : -1;
+                    float s = 0.0f;
+                    const auto add = [&](float v) {
+                        const float d = v - M;
+                        n += d == 0.0f;
+                        s += d == 0.0f ? 0.0f : exp2_fast(d * a.scale);
+                    };
+                    if (edge >= 0) add(elem(x, edge));
+                    uint4 v[kUnitVecs / 32];
+#pragma unroll
+                    for (int k = 0; k < kUnitVecs / 32; k++)
+                        v[k] = k * 32 + lane < cnt ? load16(x + sh.head + (size_t)(first + k * 32 + lane) * kN)
+                                                   : Pack<T>::lowest();
+#pragma unroll
+                    for (int k = 0; k < kUnitVecs / 32; k++) {
+                        float o[kN];
+                        Pack<T>::widen(v[k], o);
+#pragma unroll
+                        for (int j = 0; j < kN; j++) add(o[j]);
+                    }
+                    sum += (double)s;
+                }
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            n = warp_sum_int(n);
+            excess = rest + sum + (double)(n - 1);
+        }
+        if (isinf(M)) excess = NAN;
+        r.scored = 1;
+        r.max = M;
+        r.excess = (float)excess;
+        if (lane == 0) r.logprob = ((double)xt - (double)M) * a.inv_t - log1p(excess);
+    }
+    if (lane == 0) {
+        if (a.out) a.out[row] = r;
+        if (a.logprobs) a.logprobs[row] = (float)r.logprob;
+        if (a.stats) {
+            a.stats[2 * (size_t)row] = r.max;
+            a.stats[2 * (size_t)row + 1] = r.excess;
+        }
+    }
+}
+
 // grad = coef * ([j = t] - p_j) / T.  Rows are cut into pieces of kGradThreads
 // x kGradVpt vectors, one CTA each.  Rows are taken from the last to the
 // first: the scoring before read them in the other order, so the ones it read
@@ -636,6 +907,8 @@ static int fail(int code, const char* fmt, ...) {
     return set_error(code, buf);
 }
 
+static size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
+
 struct Rows {
     const void* logits;
     int dtype, rows, vocab;
@@ -646,6 +919,11 @@ struct Rows {
     long long gld;
     size_t esz() const { return dtype == QS_F32 ? 4 : 2; }
 };
+
+static int check_workspace(const void* p, size_t bytes, size_t need) {
+    if (need == 0 || (p && bytes >= need && ((uintptr_t)p & 15) == 0)) return QS_OK;
+    return fail(QS_ERR_INVALID, "workspace is NULL, unaligned or below %zu bytes", need);
+}
 
 static int check_rows(const Rows& r, double temperature) {
     if (r.dtype != QS_F32 && r.dtype != QS_BF16) return fail(QS_ERR_INVALID, "unknown dtype %d", r.dtype);
@@ -671,6 +949,20 @@ static int check_rows(const Rows& r, double temperature) {
     }
     return QS_OK;
 }
+
+// Lets a kernel use `bytes` of dynamic shared memory, once on each device.
+struct DeviceOnce {
+    std::atomic<unsigned long long> done{0};
+    int raise(const void* kernel, int bytes) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e == cudaSuccess && (dev >= 64 || !(done.load() >> dev & 1))) {
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+            if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev);
+        }
+        return e == cudaSuccess ? QS_OK : fail(QS_ERR_CUDA, "shared memory: %s", cudaGetErrorString(e));
+    }
+};
 
 // Launches `kernel` in clusters of `cluster` CTAs; `after`: it may start while
 // the kernel before it ends (it waits for it before it reads its results).
@@ -711,16 +1003,9 @@ static int score_launch(ScoreArgs<T>& a, cudaStream_t st) {
     a.log_c = log_c;
     const int threads = share() > 128 ? 256 : 128;
     const size_t smem = (size_t)share() * 16;
-    if (smem > 40 * 1024) {
-        static std::atomic<unsigned long long> raised{0};  // devices on which the kernel may use all shared memory
-        int dev = 0;
-        cudaError_t e = cudaGetDevice(&dev);
-        if (e == cudaSuccess && (dev >= 64 || !(raised.load() >> dev & 1))) {
-            e = cudaFuncSetAttribute(score_kernel<T, kPolicy>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-            if (e == cudaSuccess && dev < 64) raised.fetch_or(1ull << dev);
-        }
-        if (e != cudaSuccess) return fail(QS_ERR_CUDA, "score_kernel: %s", cudaGetErrorString(e));
-    }
+    static DeviceOnce once;
+    const int rc = once.raise((const void*)score_kernel<T, kPolicy>, 200 * 1024);
+    if (rc) return rc;
     return launch("score_kernel", score_kernel<T, kPolicy>, (long long)a.rows << log_c, threads, 1 << log_c, smem, false,
                   st, a);
 }
@@ -740,13 +1025,55 @@ static ScoreArgs<T> score_args(const Rows& r) {
     return a;
 }
 
+// Calls of at least this many bytes of logits stream; below, a cluster per row
+// ends sooner, in one launch: 13.7 us against 16.6 for 39 MB, 78 against 62.5
+// for 311 MB, even near 74 MB.
+constexpr size_t kStreamBytes = (size_t)72 << 20;
+
+static int row_units(int dtype, int vocab) {
+    const int vecs = vocab / (dtype == QS_F32 ? 4 : 8);
+    return vecs > kUnitVecs ? (vecs + kUnitVecs - 1) / kUnitVecs : 1;
+}
+static bool streams(int dtype, int rows, int vocab) {
+    return (size_t)rows * vocab * (dtype == QS_F32 ? 4 : 2) >= kStreamBytes;
+}
+static size_t score_workspace(int dtype, int rows, int vocab) {
+    return streams(dtype, rows, vocab) ? round256((size_t)rows * row_units(dtype, vocab) * sizeof(float2)) : 0;
+}
+
 template <typename T>
-static int score(const Rows& r, RowScore* out, float* logprobs, float* stats, cudaStream_t st) {
-    ScoreArgs<T> a = score_args<T>(r);
+static int score(const Rows& r, RowScore* out, float* logprobs, float* stats, float2* parts, cudaStream_t st) {
+    if (!streams(r.dtype, r.rows, r.vocab)) {
+        ScoreArgs<T> a = score_args<T>(r);
+        a.out = out;
+        a.logprobs = logprobs;
+        a.stats = stats;
+        return score_launch<T, false>(a, st);
+    }
+    StreamArgs<T> a = {};
+    a.logits = (const T*)r.logits;
+    a.rows = r.rows;
+    a.V = r.vocab;
+    a.ld = r.ld;
+    a.tokens = r.tokens;
+    a.scale = (float)(r.inv_t * 1.4426950408889634);
+    a.inv_t = r.inv_t;
+    a.units = row_units(r.dtype, r.vocab);
+    a.parts = parts;
     a.out = out;
     a.logprobs = logprobs;
     a.stats = stats;
-    return score_launch<T, false>(a, st);
+    const size_t smem = (size_t)kStreamWarps * kStreamStages * kUnitVecs * 16;
+    static DeviceOnce once;
+    int rc = once.raise((const void*)stream_kernel<T>, (int)smem);
+    if (rc) return rc;
+    int dev = 0, sms = 148;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return fail(QS_ERR_CUDA, "device: %s", cudaGetErrorString(e));
+    rc = launch("stream_kernel", stream_kernel<T>, sms, kStreamWarps * 32, 1, smem, false, st, a);
+    if (rc) return rc;
+    return launch("join_kernel", join_kernel<T>, (r.rows + kJoinRows - 1) / kJoinRows, kJoinRows * 32, 1, 0, true, st, a);
 }
 
 template <typename T>
@@ -758,25 +1085,30 @@ static int grad(const Rows& r, const float* stats, int stat_words, const float* 
                   (float)(r.inv_t * 1.4426950408889634), r.inv_t, (T*)r.grad, r.gld, pieces);
 }
 
-static size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
-
 }  // namespace qs
 
 using namespace qs;
 
 extern "C" {
 
+size_t qs_token_logprobs_workspace(int dtype, int rows, int vocab) {
+    return dtype != QS_F32 && dtype != QS_BF16 || rows < 1 || vocab < 1 || vocab > kMaxVocab ? 0
+                                                                                             : score_workspace(dtype, rows, vocab);
+}
+
 int qs_token_logprobs(const void* d_logits, int dtype, int rows, int vocab, long long row_stride,
                       const int* d_tokens, double temperature, float* d_logprobs, float* d_stats,
-                      void* stream) {
+                      void* d_workspace, size_t workspace_bytes, void* stream) {
     set_error(QS_OK, "");
     const Rows r{d_logits, dtype, rows, vocab, row_stride, d_tokens, 1.0 / temperature, nullptr, 0};
-    const int rc = check_rows(r, temperature);
+    int rc = check_rows(r, temperature);
     if (rc || rows == 0) return rc;
     if (!d_logprobs || !d_stats) return fail(QS_ERR_INVALID, "NULL output buffer");
+    rc = check_workspace(d_workspace, workspace_bytes, score_workspace(dtype, rows, vocab));
+    if (rc) return rc;
     const cudaStream_t st = (cudaStream_t)stream;
-    return dtype == QS_F32 ? score<float>(r, nullptr, d_logprobs, d_stats, st)
-                           : score<__nv_bfloat16>(r, nullptr, d_logprobs, d_stats, st);
+    return dtype == QS_F32 ? score<float>(r, nullptr, d_logprobs, d_stats, (float2*)d_workspace, st)
+                           : score<__nv_bfloat16>(r, nullptr, d_logprobs, d_stats, (float2*)d_workspace, st);
 }
 
 int qs_token_logprobs_backward(const void* d_logits, int dtype, int rows, int vocab, long long row_stride,
@@ -814,8 +1146,8 @@ int qs_policy_loss(const void* d_logits, int dtype, int rows, int vocab, long lo
     if (rows > 0) {
         if (!d_old_logprobs || !d_advantages) return fail(QS_ERR_INVALID, "NULL device pointer");
         if (p.kl_coef > 0.0 && !d_ref_logprobs) return fail(QS_ERR_INVALID, "kl_coef %g needs ref_logprobs", p.kl_coef);
-        if (!d_workspace || workspace_bytes < qs_policy_loss_workspace(rows) || ((uintptr_t)d_workspace & 15))
-            return fail(QS_ERR_INVALID, "workspace is NULL, unaligned or below %zu bytes", qs_policy_loss_workspace(rows));
+        const int bad = check_workspace(d_workspace, workspace_bytes, qs_policy_loss_workspace(rows));
+        if (bad) return bad;
     }
     double* row_loss = (double*)d_workspace;
     if (rows > 0) {
@@ -835,10 +1167,10 @@ int qs_policy_loss(const void* d_logits, int dtype, int rows, int vocab, long lo
     return launch("sum_rows_kernel", sum_rows_kernel, 1, 1024, 1, 0, rows > 0, st, row_loss, rows, d_loss);
 }
 
-size_t qs_preference_loss_workspace(int rows, int pairs) {
-    (void)pairs;
-    const size_t n = rows > 0 ? (size_t)rows : 1;
-    return round256(n * sizeof(RowScore)) + round256(n * sizeof(float));
+size_t qs_preference_loss_workspace(int dtype, int rows, int vocab) {
+    if (rows < 1) return 0;
+    return round256((size_t)rows * sizeof(RowScore)) + round256((size_t)rows * sizeof(float)) +
+           qs_token_logprobs_workspace(dtype, rows, vocab);
 }
 
 int qs_preference_loss(const void* d_logits, int dtype, int rows, int vocab, long long row_stride,
@@ -858,14 +1190,15 @@ int qs_preference_loss(const void* d_logits, int dtype, int rows, int vocab, lon
         return fail(QS_ERR_INVALID, "label_smoothing %g outside [0, 0.5)", p.label_smoothing);
     if (!d_loss) return fail(QS_ERR_INVALID, "NULL output buffer");
     if (pairs > 0 && (!d_seq_offsets || !d_ref_logprobs)) return fail(QS_ERR_INVALID, "NULL device pointer");
-    if (rows > 0 && (!d_workspace || workspace_bytes < qs_preference_loss_workspace(rows, pairs) || ((uintptr_t)d_workspace & 15)))
-        return fail(QS_ERR_INVALID, "workspace is NULL, unaligned or below %zu bytes", qs_preference_loss_workspace(rows, pairs));
+    const int bad = check_workspace(d_workspace, workspace_bytes, qs_preference_loss_workspace(dtype, rows, vocab));
+    if (bad) return bad;
     const cudaStream_t st = (cudaStream_t)stream;
     RowScore* sc = (RowScore*)d_workspace;
     float* coefs = (float*)((char*)d_workspace + round256((size_t)rows * sizeof(RowScore)));
+    float2* parts = (float2*)((char*)coefs + round256((size_t)rows * sizeof(float)));
     if (rows > 0) {
-        const int e = dtype == QS_F32 ? score<float>(r, sc, nullptr, nullptr, st)
-                                      : score<__nv_bfloat16>(r, sc, nullptr, nullptr, st);
+        const int e = dtype == QS_F32 ? score<float>(r, sc, nullptr, nullptr, parts, st)
+                                      : score<__nv_bfloat16>(r, sc, nullptr, nullptr, parts, st);
         if (e) return e;
     }
     const int e = launch("preference_pairs_kernel", preference_pairs_kernel, 1, 1024, 1, 0, rows > 0, st, sc, rows,

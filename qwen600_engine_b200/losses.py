@@ -105,6 +105,10 @@ def _grad_stride(out, logits) -> int:
     return _matrix("the gradient's buffer", out)[2]
 
 
+def _new_grad(logits):
+    return torch.empty_like(logits) if logits.is_contiguous() else logits.new_empty(logits.shape)
+
+
 def token_logprobs(logits, tokens, *, temperature: float = 1.0, stream=None) -> TokenLogprobs:
     """log softmax(logits / temperature) of each row's token, and the row
     statistics that ``token_logprobs_backward`` takes."""
@@ -115,8 +119,10 @@ def token_logprobs(logits, tokens, *, temperature: float = 1.0, stream=None) -> 
     def run(st):
         lp = torch.empty(rows, dtype=torch.float32, device=dev)
         stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
+        size = _lib.lib.qs_token_logprobs_workspace(code, rows, vocab)
+        work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         check(_lib.lib.qs_token_logprobs(logits.data_ptr(), code, rows, vocab, ld, tok, temperature, lp.data_ptr(),
-                                         stats.data_ptr(), st))
+                                         stats.data_ptr(), work.data_ptr() if size else None, size, st))
         return TokenLogprobs(lp, stats)
 
     return _on_stream(dev, stream, (logits, tokens), run)
@@ -135,7 +141,7 @@ def token_logprobs_backward(logits, tokens, stats, grad_logprobs, *, temperature
     gld = _grad_stride(out, logits)
 
     def run(st):
-        buf = logits.new_empty((rows, vocab)) if out is None else out
+        buf = _new_grad(logits) if out is None else out
         check(_lib.lib.qs_token_logprobs_backward(logits.data_ptr(), code, rows, vocab, ld, tok, stats.data_ptr(), g,
                                                   temperature, buf.data_ptr(), gld, st))
         return buf
@@ -163,11 +169,10 @@ def policy_loss(logits, tokens, old_logprobs, advantages, *, ref_logprobs=None, 
     params = PolicyParams(clip_low, clip_high, kl_coef, temperature)
 
     def run(st):
-        buf = logits.new_empty((rows, vocab)) if grad and out is None else out
-        loss = old_logprobs.new_empty(())
-        lp = old_logprobs.new_empty(rows)
+        buf = _new_grad(logits) if grad and out is None else out
         size = _lib.lib.qs_policy_loss_workspace(rows)
-        work = torch.empty(size, dtype=torch.uint8, device=dev)
+        work = torch.empty(size // 4 + 1 + rows, dtype=torch.float32, device=dev)  # and the small outputs behind it
+        loss, lp = work[size // 4], work[size // 4 + 1:]
         check(_lib.lib.qs_policy_loss(logits.data_ptr(), code, rows, vocab, ld, tok, old, ref, adv, w, C.byref(params),
                                       loss.data_ptr(), lp.data_ptr(), buf.data_ptr() if grad else None, gld,
                                       work.data_ptr(), size, st))
@@ -200,10 +205,10 @@ def preference_loss(logits, tokens, seq_offsets, ref_logprobs, *, beta: float = 
     params = PreferenceParams(beta, label_smoothing)
 
     def run(st):
-        buf = logits.new_empty((rows, vocab)) if grad and out is None else out
-        loss = ref_logprobs.new_empty(())
-        seq = ref_logprobs.new_empty(2 * pairs)
-        size = _lib.lib.qs_preference_loss_workspace(rows, pairs)
+        buf = _new_grad(logits) if grad and out is None else out
+        small = torch.empty(1 + 2 * pairs, dtype=torch.float32, device=dev)
+        loss, seq = small[0], small[1:]
+        size = _lib.lib.qs_preference_loss_workspace(code, rows, vocab)
         work = torch.empty(size, dtype=torch.uint8, device=dev)
         check(_lib.lib.qs_preference_loss(logits.data_ptr(), code, rows, vocab, ld, tok, off, pairs, ref, w,
                                           C.byref(params), loss.data_ptr(), seq.data_ptr(),

@@ -202,6 +202,71 @@ def test_masked_and_special_logits(dtype):
     check(out, ref, (rel_sum(V) + 100 * U + half_step(dtype)) * ref.abs().nan_to_num(0) + 4 * U * rel_sum(V) + 1e-30, "gradient")
 
 
+# Calls of 72 MB of logits and more take the kernels that stream many rows.
+MANY = [(torch.bfloat16, 250, 151936, 0, 0), (torch.bfloat16, 800, 50021, 3, 1), (torch.float32, 128, 151936, 0, 0),
+        (torch.float32, 500, 37999, 1, 2), (torch.bfloat16, 38000, 1003, 0, 0), (torch.float32, 19000, 1024, 8, 0),
+        (torch.bfloat16, 150, 262144, 0, 0)]
+
+
+@pytest.mark.parametrize("dtype,N,V,pad,shift", MANY)
+@pytest.mark.parametrize("kind", ["mixed", "peaked"])
+def test_many_rows(dtype, N, V, pad, shift, kind):
+    x, tok, g = rows_of(N, V, dtype, seed=N + V, pad=pad, shift=shift, kind=kind)
+    tok[::2] = x[::2].argmax(1).to(torch.int32)
+    tok[3::11] = -1
+    x[3::22] = math.nan
+    T = 0.8
+    r = L().token_logprobs(x, tok, temperature=T)
+    again = L().token_logprobs(x, tok, temperature=T)
+    assert torch.equal(r.logprobs, again.logprobs) and torch.equal(r.stats, again.stats)
+    x[3::22] = 0
+    out = (tok == -1).nonzero()[:, 0]
+    assert (r.logprobs[out] == 0).all() and (r.stats[out] == 0).all()
+    for a in range(0, N, 512):
+        b = slice(a, min(a + 512, N))
+        lp, _, excess, m, tol = exact(x[b], tok[b], T)
+        # a log-probability near 0 keeps its relative precision
+        near = (rel_sum(V) + 4 * U) * lp.abs() + 1e-30
+        check(r.logprobs[b], lp, torch.where((lp.abs() < 0.5) & (tok[b] >= 0), near, tol), "logprobs")
+        on = tok[b] >= 0
+        assert torch.equal(r.stats[b][on, 0].double(), m[on])
+        check(r.stats[b][on, 1], excess[on], (rel_sum(V) + U) * excess[on] + 1e-30, "excess")
+
+
+def test_many_rows_with_special_logits():
+    N, V = 300, 131075
+    x, tok, _ = rows_of(N, V, torch.bfloat16, seed=15)
+    low = torch.finfo(torch.bfloat16).min
+    x[0, 1::2] = -math.inf
+    x[1, :] = -math.inf
+    x[1, 17] = 2.5
+    x[2, :] = -math.inf
+    x[3, :] = low
+    x[4, 500:] = low
+    x[5, 9] = math.nan
+    x[6, V - 1] = math.inf
+    x[7, : V - 13] = -math.inf
+    x[8, :] = torch.finfo(torch.bfloat16).max
+    x[9, 3] = torch.finfo(torch.bfloat16).max
+    x[10, :] = math.nan
+    x[11, :100000] = math.nan
+    x[11, 100000:] = -math.inf
+    x[12, :] = 0.0
+    tok[0], tok[1], tok[4], tok[7], tok[9] = 2, 17, 3, V - 2, 3
+    r = L().token_logprobs(x, tok)
+    lp = torch.log_softmax(x.double(), 1).gather(1, tok.long()[:, None])[:, 0]
+    lp[3] = lp[8] = lp[12] = -math.log(V)
+    check(r.logprobs, lp, rel_sum(V) + U * lp.abs().nan_to_num(0, 0, 0) + 1e-12, "logprobs")
+    assert torch.isnan(r.logprobs).nonzero()[:, 0].tolist() == [2, 5, 6, 10, 11]
+
+
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 151936), (torch.float32, 50021)])
+def test_preference_many_rows(dtype, V):
+    x, tok, off, ref, w = pairs_case(4, V, dtype, seed=V + 2, lengths=[60, 1, 82, 44, 34, 72, 0, 98], tail=2)
+    r = L().preference_loss(x, tok, off, ref, weights=w, beta=0.2, label_smoothing=0.1)
+    check_preference(r, x, tok, off, ref, w, 0.2, 0.1)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_that_score_nothing(dtype):
     """Tokens outside the vocabulary: log-probability 0, zero gradient, logits not used."""

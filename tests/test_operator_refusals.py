@@ -15,8 +15,8 @@ P = 0x10000  # a 16-byte aligned address that no refused call follows
 FAR = 0x7F0000000000
 
 
-def logprobs(logits=P, dtype=QS_BF16, rows=4, vocab=1000, ld=1000, tokens=P, T=1.0, lp=P, stats=P):
-    return L.qs_token_logprobs(logits, dtype, rows, vocab, ld, tokens, T, lp, stats, None)
+def logprobs(logits=P, dtype=QS_BF16, rows=4, vocab=1000, ld=1000, tokens=P, T=1.0, lp=P, stats=P, ws=P, size=1 << 30):
+    return L.qs_token_logprobs(logits, dtype, rows, vocab, ld, tokens, T, lp, stats, ws, size, None)
 
 
 def backward(logits=P, dtype=QS_BF16, rows=4, vocab=1000, ld=1000, tokens=P, stats=P, g=P, T=1.0, grad=FAR, gld=1000):
@@ -45,7 +45,9 @@ TEMPS = [dict(T=0.0), dict(T=1e-7), dict(T=-1.0), dict(T=NAN), dict(T=INF)]
 GRADS = [dict(grad=P + 2), dict(grad=P + 2000), dict(grad=P, gld=1008), dict(grad=P - 16), dict(gld=999), dict(grad=FAR + 1)]
 
 
-@pytest.mark.parametrize("call,bad", [(logprobs, b) for b in ROWS + TEMPS + [dict(lp=None), dict(stats=None)]]
+@pytest.mark.parametrize("call,bad", [(logprobs, b) for b in ROWS + TEMPS + [
+                             dict(lp=None), dict(stats=None), dict(rows=100000, ws=None), dict(rows=100000, ws=P + 4),
+                             dict(rows=100000, size=1000)]]
                          + [(backward, b) for b in ROWS + TEMPS + GRADS + [dict(stats=None), dict(g=None), dict(grad=None)]]
                          + [(policy, b) for b in ROWS + TEMPS + GRADS + [
                              dict(old=None), dict(adv=None), dict(loss=None), dict(params=False), dict(kl=0.1, ref=None),
@@ -68,7 +70,7 @@ def test_c_abi_limits(call, bad):
 
 
 def test_empty_batches_need_no_buffers():
-    assert L.qs_token_logprobs(None, QS_BF16, 0, 1000, 1000, None, 1.0, None, None, None) == _lib.QS_OK
+    assert L.qs_token_logprobs(None, QS_BF16, 0, 1000, 1000, None, 1.0, None, None, None, 0, None) == _lib.QS_OK
     assert L.qs_token_logprobs_backward(None, QS_F32, 0, 1000, 1000, None, None, None, 1.0, None, 0, None) == _lib.QS_OK
 
 
