@@ -389,14 +389,14 @@ QS_API int qs_lm_head_w4_sample(qs_sampler* s, const void* d_hidden, const void*
  * token lies outside [0, vocab) scores nothing: its log-probability is 0, its
  * gradient zero, and its logits are not read.  With x = row i and t its token,
  *   logprob = (x[t] - max x) / T - log sum_j exp((x[j] - max x) / T)
- * for temperature T >= 1e-6.  Entries of -inf (masked tokens) have probability 0; a row
+ * for a temperature T in [1e-6, 1e6].  Entries of -inf (masked tokens) have probability 0; a row
  * with a NaN, with +inf or with nothing above -inf has a NaN log-probability
  * and gradient.  Gradients are d loss / d logits, [rows, vocab] in the logits'
  * type, rows grad_row_stride elements apart; d_grad may be d_logits itself
  * with the same stride (the gradient then replaces the logits), and may not
- * overlap it otherwise.  Exponentials are fp32 (relative error below 2^-20),
- * sums over rows and sequences 64-bit, in a fixed order: the same inputs give
- * the same bits.  vocab <= qs_max_vocab(), rows <= 2^27.  Nothing is
+ * overlap it otherwise.  Exponentials and the first steps of a row's sum are
+ * fp32, what joins them, the losses and their slopes 64-bit, all in a fixed
+ * order: the same inputs give the same bits.  vocab <= qs_max_vocab(), rows <= 2^27.  Nothing is
  * allocated and no state is kept.  A workspace of the *_workspace call's bytes
  * (where that is 0, it may be NULL) is 16-byte aligned, needs no
  * initialisation, and belongs to the call until it is done: calls that overlap

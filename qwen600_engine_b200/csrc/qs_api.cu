@@ -1061,9 +1061,20 @@ static int w4_launch(const void* d_hidden, const void* d_norm_weight, const qs_w
     return QS_OK;
 }
 
-size_t qs_w4_codes_bytes(int vocab, int hidden_dim) { return w4_codes_bytes(vocab, hidden_dim); }
-size_t qs_w4_scales_bytes(int vocab, int hidden_dim, int group) { return w4_scales_bytes(vocab, hidden_dim, group); }
-size_t qs_w4_zeros_bytes(int vocab, int hidden_dim, int group) { return w4_zeros_bytes(vocab, hidden_dim, group); }
+// Sizes outside the limits have no layout: 0 bytes.
+static bool w4_sizes(int vocab, int hidden_dim, int group) {
+    return vocab >= 1 && vocab <= kMaxVocab && hidden_dim >= 1 && hidden_dim <= kW4MaxHidden &&
+           (group == 32 || group == 64 || group == 128);
+}
+size_t qs_w4_codes_bytes(int vocab, int hidden_dim) {
+    return w4_sizes(vocab, hidden_dim, 128) ? w4_codes_bytes(vocab, hidden_dim) : 0;
+}
+size_t qs_w4_scales_bytes(int vocab, int hidden_dim, int group) {
+    return w4_sizes(vocab, hidden_dim, group) ? w4_scales_bytes(vocab, hidden_dim, group) : 0;
+}
+size_t qs_w4_zeros_bytes(int vocab, int hidden_dim, int group) {
+    return w4_sizes(vocab, hidden_dim, group) ? w4_zeros_bytes(vocab, hidden_dim, group) : 0;
+}
 
 int qs_w4_quantize(const void* d_weight, int vocab, int hidden_dim, int group, void* d_plain_codes,
                    void* d_plain_scales, void* d_plain_zeros, void* stream) {
@@ -1097,8 +1108,7 @@ int qs_w4_pack(const void* d_plain_codes, const void* d_plain_scales, const void
 }
 
 size_t qs_lm_head_w4_workspace(int batch, int hidden_dim, int group) {
-    if (batch < 1 || hidden_dim < 1 || (group != 32 && group != 64 && group != 128)) return 16;
-    return w4_workspace(batch, hidden_dim, group);
+    return batch >= 1 && w4_sizes(1, hidden_dim, group) ? w4_workspace(batch, hidden_dim, group) : 0;
 }
 
 int qs_lm_head_w4(const void* d_hidden, const void* d_norm_weight, const qs_w4_weight* weight, int batch,
@@ -1113,7 +1123,7 @@ int qs_lm_head_w4(const void* d_hidden, const void* d_norm_weight, const qs_w4_w
         return fail(QS_ERR_INVALID, "normed and logits must be 16-byte aligned");
     if (((uintptr_t)d_norm_weight) & 3) return fail(QS_ERR_INVALID, "norm_weight must be 4-byte aligned");
     const size_t need = qs_lm_head_w4_workspace(batch, weight->hidden_dim, weight->group);
-    if (!d_workspace || workspace_bytes < need || (((uintptr_t)d_workspace) & 15))
+    if (need > 0 && (!d_workspace || workspace_bytes < need || (((uintptr_t)d_workspace) & 15)))
         return fail(QS_ERR_INVALID, "workspace is NULL, unaligned or below %zu bytes", need);
     int dev = 0, sms = 148;
     CK(cudaGetDevice(&dev));

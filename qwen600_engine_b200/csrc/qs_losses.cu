@@ -264,9 +264,13 @@ struct ScoreArgs {
 // shared memory.
 //
 // Bound: memory, as long as enough rows are under way: from its copy to its
-// last store a CTA of 38 KB (a bf16 row of 151,936 over 8) takes about 8 us, so
-// an SM needs some 200 KB in flight.  Shared memory holds five such CTAs; in
-// registers (80 a thread of 256) it were three, 293 us for REPLACE.
+// last store a CTA of 38 KB (a bf16 row of 151,936 over 8) takes about 10 us
+// with its neighbours, so an SM needs some 200 KB in flight.  Shared memory
+// holds five such CTAs, 226 us for 2048 bf16 rows of 151,936 a quarter of which
+// is left out (1089 MB, 4.8 TB/s); with the shares in registers (80 a thread of
+// 256) it were three, 293 us.  Without the exchange it would take 207 us,
+// without the exponentials 216.  Shares of 76 KB on 4 CTAs: 224 us; of 19 KB on
+// 16: 282.
 template <typename T, bool kPolicy>
 __global__ void __launch_bounds__(kScoreThreads)
 score_kernel(const __grid_constant__ ScoreArgs<T> a) {
@@ -335,8 +339,8 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
     const float xe = edge >= 0 ? elem(x, edge) : -INFINITY;
     const float xt = elem(x, tok);
     __syncthreads();
-    const bool whole = mbar_wait(&loaded, 0, &gave_up, kLoadWaitNs);
-    if (!whole) mbar_wait(&loaded, 0, &gave_up, kLoadWaitNs, false);  // the copy lands before the CTA leaves
+    if (!mbar_wait(&loaded, 0, &gave_up, kLoadWaitNs))
+        mbar_wait(&loaded, 0, &gave_up, kLoadWaitNs, false);  // the copy lands before the CTA leaves
 
     // the maximum of this CTA's part
     float own_max = xe;
@@ -411,7 +415,7 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
     __syncthreads();
     if (C > 1) cluster_wait();  // every CTA of the cluster runs
     if (t < C) {
-        Part p{m, 0, whole ? 0.0 : (double)NAN};
+        Part p{m, 0, *(volatile int*)&gave_up ? (double)NAN : 0.0};
         for (int w = 0; w < thr / 32; w++) {
             p.others += (double)red_sum[w];
             p.at_max += red_n[w];
@@ -514,9 +518,10 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
 // is a stream: rows are cut into units of 256 vectors (4 KB), every warp of a
 // persistent grid takes units in turn through its own ring of bulk copies and
 // leaves each unit's maximum and sum of exponentials, and a second kernel joins
-// a row's units.  Warps never wait for one another, so the copies keep running
-// while others compute (the cluster kernel spends a third of its time
-// waiting: 68.7 us against REPLACE for 1024 bf16 rows of 151,936).
+// a row's units.  Warps never wait for one another, so copies keep running
+// while others compute.  1024 bf16 rows of 151,936: 62.5 us (50 of them this
+// kernel, 6.2 TB/s, its exponentials at 75% of the unit's rate), 78 with a
+// cluster per row.  24 warps with rings of 2 units; 16 with 3 were 16 us slower.
 constexpr int kUnitVecs = 256;
 constexpr int kStreamWarps = 24;
 constexpr int kStreamStages = 2;
@@ -787,14 +792,12 @@ join_kernel(const __grid_constant__ StreamArgs<T> a) {
 // grad = coef * ([j = t] - p_j) / T.  Rows are cut into pieces of kGradThreads
 // x kGradVpt vectors, one CTA each.  Rows are taken from the last to the
 // first: the scoring before read them in the other order, so the ones it read
-// last come from L2.  A gradient larger than L2 is stored past it (241 to 231 us
-// for 1900 rows of 151,936 bf16); a smaller one is left there for whoever reads
-// it next (and 15.4 against 16.2 us for 509 rows of 50,021).
+// last come from L2; the gradient is stored past it (241 to 228 us for 1900
+// rows of 151,936 bf16, 20.5 to 18.8 us for 509 of 50,021).
 constexpr int kGradThreads = 256;
-constexpr int kGradVpt = 4;
-constexpr size_t kL2Bytes = (size_t)126 << 20;
+constexpr int kGradVpt = 6;
 
-template <typename T, bool kPast>
+template <typename T>
 __global__ void __launch_bounds__(kGradThreads)
 grad_kernel(const T* logits, int rows, int V, long long ld, const int* __restrict__ tokens, const float* stats,
             int stat_words, const float* coefs, float scale, double inv_t, T* grad, long long gld, int pieces) {
@@ -813,8 +816,7 @@ grad_kernel(const T* logits, int rows, int V, long long ld, const int* __restric
     if (coef == 0.0f) {
         const RowShape<T> gs(g, V);
         for (int k = piece * kGradThreads + t; k < gs.vecs; k += pieces * kGradThreads)
-            if (kPast) store16_past(g + gs.head + (size_t)k * kN, make_uint4(0u, 0u, 0u, 0u));
-            else store16(g + gs.head + (size_t)k * kN, make_uint4(0u, 0u, 0u, 0u));
+            store16_past(g + gs.head + (size_t)k * kN, make_uint4(0u, 0u, 0u, 0u));
         const int e = piece == 0 ? gs.edge(t, V) : -1;
         if (e >= 0) put(g, e, 0.0f);
         return;
@@ -847,8 +849,7 @@ grad_kernel(const T* logits, int rows, int V, long long ld, const int* __restric
         for (int j = 0; j < kN; j++) o[j] = f * exp2_fast((o[j] - M) * scale);
         if (k < end) {
             if (aligned) {
-                if (kPast) store16_past(gbody + (size_t)k * kN, Pack<T>::narrow(o));
-                else store16(gbody + (size_t)k * kN, Pack<T>::narrow(o));
+                store16_past(gbody + (size_t)k * kN, Pack<T>::narrow(o));
             } else {
 #pragma unroll
                 for (int j = 0; j < kN; j++) put(gbody, (long long)k * kN + j, o[j]);
@@ -962,8 +963,8 @@ static int check_rows(const Rows& r, double temperature) {
     if (r.rows > 1 << 27) return fail(QS_ERR_UNSUPPORTED, "rows %d above 2^27", r.rows);
     if (r.vocab < 1 || r.vocab > kMaxVocab)
         return fail(QS_ERR_UNSUPPORTED, "vocab %d outside [1, %d]", r.vocab, kMaxVocab);
-    if (!(temperature >= 1e-6) || isinf(temperature))
-        return fail(QS_ERR_INVALID, "temperature %g is not a finite number of at least 1e-6", temperature);
+    if (!(temperature >= 1e-6 && temperature <= 1e6))
+        return fail(QS_ERR_INVALID, "temperature %g outside [1e-6, 1e6]", temperature);
     if (r.rows == 0) return QS_OK;
     if (!r.logits || !r.tokens) return fail(QS_ERR_INVALID, "NULL device pointer");
     if (((uintptr_t)r.logits | (uintptr_t)r.grad) % r.esz())
@@ -1000,6 +1001,7 @@ struct DeviceOnce {
 template <typename... P, typename... A>
 static int launch(const char* name, void (*kernel)(P...), long long grid, int threads, int cluster, size_t smem,
                   bool after, cudaStream_t st, A... args) {
+    if (grid > 0x7FFFFFFFll) return fail(QS_ERR_UNSUPPORTED, "%s: %lld CTAs", name, grid);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(threads);
@@ -1114,9 +1116,8 @@ template <typename T>
 static int grad(const Rows& r, const float* stats, int stat_words, const float* coefs, bool after, cudaStream_t st) {
     const int vecs = r.vocab / Pack<T>::kN;
     const int pieces = max(1, (vecs + kGradThreads * kGradVpt - 1) / (kGradThreads * kGradVpt));
-    const bool past = (size_t)r.rows * r.vocab * sizeof(T) > kL2Bytes;
-    return launch("grad_kernel", past ? grad_kernel<T, true> : grad_kernel<T, false>, (long long)r.rows * pieces,
-                  kGradThreads, 1, 0, after, st, (const T*)r.logits, r.rows, r.vocab, r.ld, r.tokens, stats, stat_words, coefs,
+    return launch("grad_kernel", grad_kernel<T>, (long long)r.rows * pieces, kGradThreads, 1, 0, after, st,
+                  (const T*)r.logits, r.rows, r.vocab, r.ld, r.tokens, stats, stat_words, coefs,
                   (float)(r.inv_t * 1.4426950408889634), r.inv_t, (T*)r.grad, r.gld, pieces);
 }
 

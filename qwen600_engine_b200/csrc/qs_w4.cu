@@ -8,8 +8,8 @@
 // tokens, tokens on the narrow side.  A code needs no conversion: as the low
 // bits of an fp16 number, q is the number q 2^-24 and 16 q is 16 q 2^-24, so a
 // word of 8 codes becomes four operand registers with one shift and four
-// ands.  (Made into bf16 pairs, shift, and / or, subtract, it took 11
-// instructions, and 21.4 us instead of REPLACE for one token.)  The tokens are
+// ands.  (Made into bf16 pairs, by shift, and / or, subtract, it took 11
+// instructions.)  The tokens are
 // scaled by a power of two to fp16 (exact for values within 2^-28 of a row's
 // largest), the columns that meet 16 q by another 1 / 16, and the zero point is
 // taken out of a group's sum: sum (q - z) x = sum q x - z sum x, with the

@@ -90,10 +90,10 @@ def _matrix(name: str, t):
 
 
 def _vector(name: str, t, dtype, n: int, device) -> int:
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.device != device:
-        raise _invalid(f"{name} must be a contiguous {dtype} tensor [{n}] on {device}, got {t.dtype} "
-                       f"{tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+    if t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous() and t.device == device:
+        return t.data_ptr()
+    raise _invalid(f"{name} must be a contiguous {dtype} tensor [{n}] on {device}, got {t.dtype} {tuple(t.shape)} "
+                   f"on {t.device}")
 
 
 def _grad_stride(out, logits) -> int:

@@ -57,8 +57,6 @@ class W4Weight:
         L = _lib.lib
 
         def run(st):
-            if vocab < 1 or vocab > L.qs_max_vocab() or hidden < 64:
-                raise _invalid(f"vocab {vocab} or hidden_dim {hidden} outside the library's limits")
             pc = torch.empty(L.qs_w4_codes_bytes(vocab, hidden), dtype=torch.uint8, device=dev)
             ps = torch.empty(L.qs_w4_scales_bytes(vocab, hidden, group), dtype=torch.uint8, device=dev)
             pz = None if zeros is None else torch.empty(L.qs_w4_zeros_bytes(vocab, hidden, group), dtype=torch.uint8,
@@ -68,6 +66,8 @@ class W4Weight:
                                st))
             return pc, ps, pz
 
+        if not L.qs_w4_codes_bytes(vocab, hidden):
+            raise _invalid(f"vocab {vocab} or hidden_dim {hidden} outside the library's limits")
         if group not in (32, 64, 128):
             raise _invalid(f"scales make a group of {group} columns (want 32, 64 or 128)")
         pc, ps, pz = _on_stream(dev, stream, (codes, scales, zeros), run)
@@ -89,6 +89,8 @@ def quantize_w4(weight, group: int = 128, *, stream=None):
     vocab, hidden = int(weight.shape[0]), int(weight.shape[1])
     if group not in (32, 64, 128) or hidden % group:
         raise _invalid(f"group {group} must be 32, 64 or 128 and divide hidden_dim {hidden}")
+    if not _lib.lib.qs_w4_codes_bytes(vocab, hidden):
+        raise _invalid(f"vocab {vocab} or hidden_dim {hidden} outside the library's limits")
     dev = weight.device
 
     def run(st):

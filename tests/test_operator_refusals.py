@@ -41,7 +41,7 @@ NAN, INF = float("nan"), float("inf")
 ROWS = [dict(dtype=QS_F16), dict(dtype=7), dict(rows=-1), dict(logits=None), dict(tokens=None), dict(ld=999),
         dict(logits=P + 1), dict(dtype=QS_F32, logits=P + 2)]
 LIMITS = [dict(rows=(1 << 27) + 1), dict(vocab=0), dict(vocab=-5), dict(vocab=1 << 20, ld=1 << 20)]
-TEMPS = [dict(T=0.0), dict(T=1e-7), dict(T=-1.0), dict(T=NAN), dict(T=INF)]
+TEMPS = [dict(T=0.0), dict(T=1e-7), dict(T=-1.0), dict(T=NAN), dict(T=INF), dict(T=1e7)]
 GRADS = [dict(grad=P + 2), dict(grad=P + 2000), dict(grad=P, gld=1008), dict(grad=P - 16), dict(gld=999), dict(grad=FAR + 1)]
 
 
@@ -92,6 +92,18 @@ def test_w4_weight_refused(bad, code):
     w = weight(**bad)
     assert L.qs_lm_head_w4(P, None, C.byref(w), 1, P, P, P, 1 << 20, None) == code
     assert L.qs_last_error()
+
+
+def test_sizes_outside_the_limits_are_0_bytes():
+    for vocab, hidden, group in ((0, 1024, 128), (-1, 1024, 128), (1000, 0, 64), (1 << 30, 1024, 64), (1000, 1 << 20, 32)):
+        assert L.qs_w4_codes_bytes(vocab, hidden) == 0
+        assert L.qs_w4_scales_bytes(vocab, hidden, group) == 0 and L.qs_w4_zeros_bytes(vocab, hidden, group) == 0
+    for group in (0, -32, 48, 1 << 30):
+        assert L.qs_w4_scales_bytes(1000, 1024, group) == 0 and L.qs_w4_zeros_bytes(1000, 1024, group) == 0
+        assert L.qs_lm_head_w4_workspace(4, 1024, group) == 0
+    assert L.qs_lm_head_w4_workspace(-1, 1024, 64) == 0
+    assert L.qs_policy_loss_workspace(-5) > 0 and L.qs_preference_loss_workspace(QS_F32, -5, 1000) == 0
+    assert L.qs_token_logprobs_workspace(9, 10, 1000) == 0 and L.qs_token_logprobs_workspace(QS_F32, 10, -1) == 0
 
 
 def test_w4_calls_refused():
