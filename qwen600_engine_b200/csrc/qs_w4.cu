@@ -332,6 +332,8 @@ struct W4Out {
     int segk_stride;
 };
 
+constexpr int kStageRow = 40;  // a token's 32 values in a warp's staging rows, 80 bytes apart: the lanes' stores meet no bank twice
+
 // Stores a finished tile: 32 vocabulary rows of up to 8 kNt tokens, through the
 // warp's staging rows so that a lane stores 16 bytes of one token.
 template <int kNt>
@@ -347,26 +349,27 @@ __device__ __forceinline__ void w4_store(const float (&acc)[2][kNt][4], const fl
             const float2 f = unscale[token];
 #pragma unroll
             for (int b = 0; b < 4; b++)  // row g + 8 b
-                stage[token * 32 + g + b * 8] = __float2bfloat16_rn(acc[b >> 1][n][(b & 1) * 2 + j] * f.x * f.y);
+                stage[token * kStageRow + g + b * 8] = __float2bfloat16_rn(acc[b >> 1][n][(b & 1) * 2 + j] * f.x * f.y);
         }
     }
     __syncwarp();
+    const bool whole = (V & 7) == 0;  // every row of logits starts on 16 bytes
+    if (whole || o.segk) {
 #pragma unroll
-    for (int i = 0; i < kNt; i++) {
-        const int p = i * 32 + lane, token = p >> 2, col = tile * 32 + (p & 3) * 8;
-        const uint4 v = *reinterpret_cast<const uint4*>(stage + p * 8);
-        if (token >= o.tokens || col >= V) continue;
-        __nv_bfloat16* d = o.logits + (size_t)token * V + col;
-        if (col + 8 <= V && (V & 7) == 0) {
-            *reinterpret_cast<uint4*>(d) = v;
-        } else {
-            const __nv_bfloat16* e = stage + p * 8;
-            for (int j = 0; j < 8 && col + j < V; j++) d[j] = e[j];
+        for (int i = 0; i < kNt; i++) {
+            const int p = i * 32 + lane, token = p >> 2, col = tile * 32 + (p & 3) * 8;
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + token * kStageRow + (p & 3) * 8);
+            if (token >= o.tokens || col >= V) continue;
+            if (whole) *reinterpret_cast<uint4*>(o.logits + (size_t)token * V + col) = v;
+            // whole blocks of 16 columns, as the bf16 epilogue folds them: they never straddle a 256-column segment,
+            // and the sampler takes the maxima of whole segments
+            if (o.segk && (col & ~15) + 16 <= V)
+                atomicMax(o.segk + (size_t)token * o.segk_stride + (col >> 8), fkey(vec_max<__nv_bfloat16>(v)));
         }
-        // whole blocks of 16 columns, as the bf16 epilogue folds them: they never straddle a 256-column segment, and the
-        // sampler takes the maxima of whole segments
-        if (o.segk && (col & ~15) + 16 <= V)
-            atomicMax(o.segk + (size_t)token * o.segk_stride + (col >> 8), fkey(vec_max<__nv_bfloat16>(v)));
+    }
+    if (!whole && tile * 32 + lane < V) {  // a column a lane
+        for (int token = 0; token < o.tokens; token++)
+            o.logits[(size_t)token * V + tile * 32 + lane] = stage[token * kStageRow + lane];
     }
 }
 
@@ -387,10 +390,10 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
     unsigned char* xs = smem;                                           // fp16 rows
     float4* slots = reinterpret_cast<float4*>(smem + kNt * 8 * pitch);  // [warp][continued, begun][2][kNt][lane]
     __nv_bfloat16* stage = reinterpret_cast<__nv_bfloat16*>(slots + kWarps * 2 * 2 * kNt * 32);
-    float2* unscale = reinterpret_cast<float2*>(stage + kWarps * kNt * 256);  // [token] two factors
+    float2* unscale = reinterpret_cast<float2*>(stage + kWarps * kNt * 8 * kStageRow);  // [token] two factors
     float* sums = reinterpret_cast<float*>(unscale + kNt * 8);                // [group][token] sum of its columns
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-    stage += warp * kNt * 256;
+    stage += warp * kNt * 8 * kStageRow;
     const int t0 = (int)((long long)blockIdx.x * tiles / gridDim.x), t1 = (int)((long long)(blockIdx.x + 1) * tiles / gridDim.x);
     const int u0 = t0 * chunks, un = (t1 - t0) * chunks;
     const auto share = [&](int wi) { return u0 + (int)((long long)un * wi / kWarps); };
@@ -544,7 +547,7 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
 }
 
 static size_t w4_smem(int nt, int K, int group) {
-    return (size_t)nt * 8 * (w4_chunks(K) * 256 + 64) + (size_t)(nt <= 2 ? 16 : 8) * nt * (2 * 2 * 512 + 512) +
+    return (size_t)nt * 8 * (w4_chunks(K) * 256 + 64) + (size_t)(nt <= 2 ? 16 : 8) * nt * (2 * 2 * 512 + 16 * kStageRow) +
            (size_t)nt * 8 * (sizeof(float2) + w4_chunks(K) * (128 / group) * sizeof(float));
 }
 
