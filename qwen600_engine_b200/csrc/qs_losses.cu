@@ -141,6 +141,7 @@ struct Pack<float> {
         o[0] = __uint_as_float(v.x); o[1] = __uint_as_float(v.y);
         o[2] = __uint_as_float(v.z); o[3] = __uint_as_float(v.w);
     }
+    __device__ __forceinline__ static void widen_word(uint32_t w, float* o) { o[0] = __uint_as_float(w); }
     __device__ __forceinline__ static uint4 narrow(const float* o) {
         return make_uint4(__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3]));
     }
@@ -154,13 +155,15 @@ struct Pack<__nv_bfloat16> {
     __device__ __forceinline__ static uint4 lowest() {
         return make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u);
     }
+    __device__ __forceinline__ static void widen_word(uint32_t w, float* o) {
+        o[0] = __uint_as_float(w << 16);
+        o[1] = __uint_as_float(w & 0xFFFF0000u);
+    }
     __device__ __forceinline__ static void widen(const uint4& v, float* o) {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            o[2 * i] = __uint_as_float(w[i] << 16);
-            o[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
+        widen_word(v.x, o);
+        widen_word(v.y, o + 2);
+        widen_word(v.z, o + 4);
+        widen_word(v.w, o + 6);
     }
     __device__ __forceinline__ static uint4 narrow(const float* o) {
         uint32_t w[4];
@@ -517,10 +520,13 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
 // Without a gradient a row need not stay on the chip, and a call of many rows
 // is a stream: rows are cut into units of 256 vectors (4 KB), every warp of a
 // persistent grid takes units in turn through its own ring of bulk copies and
-// leaves each unit's maximum and sum of exponentials, and a second kernel joins
-// a row's units.  Warps never wait for one another, so copies keep running
-// while others compute.  1024 bf16 rows of 151,936: 62.5 us (50 of them this
-// kernel, 6.2 TB/s, its exponentials at 75% of the unit's rate), 78 with a
+// leaves each unit's maximum and sums, and a second kernel joins a row's units.
+// The maximum's own term is left out of the fp32 sum as in score_kernel: where
+// one lane holds the maximum, the warp takes that lane's 128 bytes once more,
+// two elements a lane.  (Where several do, the row's sum is at least 2, and the
+// 1 costs it less than the exponentials do.)  Warps never wait for one another, so copies keep running
+// while others compute.  1024 bf16 rows of 151,936: 61 us (52 of them this
+// kernel, 6.0 TB/s, its exponentials at 75% of the unit's rate), 78 with a
 // cluster per row.  24 warps with rings of 2 units; 16 with 3 were 16 us slower.
 constexpr int kUnitVecs = 256;
 constexpr int kStreamWarps = 24;
@@ -535,7 +541,7 @@ struct StreamArgs {
     float scale;
     double inv_t;
     int units;     // per row
-    float2* parts; // [rows][units]: maximum, sum of exponentials against it
+    float4* parts; // [rows][units]: maximum, sum of exponentials against it, how many 1s were left out of it
     RowScore* out;
     float* coefs;  // with out: set to 0
     float* logprobs;
@@ -631,18 +637,36 @@ stream_kernel(const __grid_constant__ StreamArgs<T> a) {
                 u.z = Pack<T>::max2(u.z, v[i].z);
                 u.w = Pack<T>::max2(u.w, v[i].w);
             }
+            float o[kN];
+            Pack<T>::widen(u, o);
+            float own = xe;
+#pragma unroll
+            for (int j = 0; j < kN; j++) own = fmaxf(own, o[j]);
+            const float m = warp_max(own);
+            const uint32_t holders = __ballot_sync(0xffffffffu, own == m);
+            const bool one = (holders & (holders - 1)) == 0;
+            const int holder = __ffs(holders) - 1;
+            float again = 0.0f;  // this lane's share of the holder's elements
+            int at_max = 0;
+            if (one) {
+                const int k = (lane >> 2) * 32 + holder;
+                const uint32_t word = k < cnt ? reinterpret_cast<const uint32_t*>(mine + stage * kUnitVecs + k)[lane & 3]
+                                              : Pack<T>::lowest().x;
+                float e[kN / 4];
+                Pack<T>::widen_word(word, e);
+#pragma unroll
+                for (int j = 0; j < kN / 4; j++) {
+                    const float d = e[j] - m;
+                    at_max += __popc(__ballot_sync(0xffffffffu, d == 0.0f));
+                    again += d == 0.0f ? 0.0f : exp2_fast(d * a.scale);
+                }
+            }
             __syncwarp();  // every lane has read the stage
             live &= ~(1u << stage);
             if (next && !dead) {
                 request(ahead, stage);
                 live |= 1u << stage;
             }
-            float o[kN];
-            Pack<T>::widen(u, o);
-            float m = xe;
-#pragma unroll
-            for (int j = 0; j < kN; j++) m = fmaxf(m, o[j]);
-            m = warp_max(m);
             const float ref = m == -INFINITY ? 0.0f : m;
             // 2^(x scale - bias), each 2^-slip too large for the rounding of bias
             const float bias = ref * a.scale;
@@ -670,10 +694,17 @@ stream_kernel(const __grid_constant__ StreamArgs<T> a) {
                     for (int j = 0; j < kN; j++) s += exp2_fast((o[j] - ref) * a.scale);
                 }
             }
+            if (one) {
+                const float held = __shfl_sync(0xffffffffu, xe, holder) - m;  // the holder's element outside the vectors
+                at_max += held == 0.0f;
+                if (lane == holder) s = held == 0.0f ? 0.0f : exp2_fast(held * a.scale);
+                s += again;
+            }
             s = warp_sum(s);
-            if (lane == 0) a.parts[(size_t)now.row * a.units + now.unit] = make_float2(m, dead ? NAN : s);
+            if (lane == 0)
+                a.parts[(size_t)now.row * a.units + now.unit] = make_float4(m, dead ? NAN : s, (float)at_max, 0.0f);
         } else {
-            if (lane == 0 && dead) a.parts[(size_t)now.row * a.units + now.unit] = make_float2(0.0f, NAN);
+            if (lane == 0 && dead) a.parts[(size_t)now.row * a.units + now.unit] = make_float4(0.0f, NAN, 0.0f, 0.0f);
             if (next && !dead) {
                 request(ahead, stage);
                 live |= 1u << stage;
@@ -685,10 +716,7 @@ stream_kernel(const __grid_constant__ StreamArgs<T> a) {
     }
 }
 
-// Joins a row's units, one warp a row.  The maximum's own term is exactly 1;
-// where the others together are less than that, the unit that holds it is read
-// again to sum the others apart from it (beyond, the 1 in a fp32 sum costs less
-// than the exponentials do).
+// Joins a row's units, one warp a row.
 constexpr int kJoinRows = 4;                                    // a CTA: small enough to start beside the stream
 constexpr int kMaxUnits = kMaxVocab / 4 / kUnitVecs;            // of a row
 static_assert(kMaxUnits % 32 == 0, "units of a lane");
@@ -696,7 +724,6 @@ static_assert(kMaxUnits % 32 == 0, "units of a lane");
 template <typename T>
 __global__ void __launch_bounds__(kJoinRows * 32)
 join_kernel(const __grid_constant__ StreamArgs<T> a) {
-    constexpr int kN = Pack<T>::kN;
     constexpr int kMine = kMaxUnits / 32;
     const int row = blockIdx.x * kJoinRows + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     dependents_may_start();
@@ -708,68 +735,30 @@ join_kernel(const __grid_constant__ StreamArgs<T> a) {
     if (row >= a.rows) return;
     RowScore r{0.0, 0.0f, 0.0f, 0, 0};
     if (scored) {
-        const float2* all = a.parts + (size_t)row * a.units;
-        float2 p[kMine];
+        const float4* all = a.parts + (size_t)row * a.units;
+        float4 p[kMine];
         float M = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kMine; i++) {
-            p[i] = i * 32 + lane < a.units ? all[i * 32 + lane] : make_float2(-INFINITY, 0.0f);
+            p[i] = i * 32 + lane < a.units ? all[i * 32 + lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
             M = fmaxf(M, p[i].x);
         }
         M = warp_max(M);
-        double rest = 0.0, held = 0.0;  // units below the maximum, units that hold it
-        uint32_t hold = 0;              // this lane's units that hold it
+        double others = 0.0;
+        int at_max = 0;
 #pragma unroll
         for (int i = 0; i < kMine; i++) {
-            const bool in = i * 32 + lane < a.units, top = in && p[i].x == M;
-            if (top) held += (double)p[i].y;
-            else if (in) rest += (double)(exp2_fast((p[i].x - M) * a.scale) * p[i].y);
-            hold |= (uint32_t)top << i;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            rest += __shfl_xor_sync(0xffffffffu, rest, o);
-            held += __shfl_xor_sync(0xffffffffu, held, o);
-        }
-        double excess = rest + held - 1.0;
-        if (excess < 1.0) {
-            const RowShape<T> sh(x, a.V);
-            double sum = 0.0;
-            int n = 0;
-#pragma unroll 1
-            for (int i = 0; i < kMine; i++) {
-                uint32_t lanes = __ballot_sync(0xffffffffu, hold >> i & 1);
-                for (; lanes; lanes &= lanes - 1) {
-                    const int unit = i * 32 + __ffs(lanes) - 1, first = unit * kUnitVecs;
-                    const int cnt = max(0, min(kUnitVecs, sh.vecs - first));
-                    const int edge = unit == 0 ? sh.edge(lane, a.V) : -1;
-                    float s = 0.0f;
-                    const auto add = [&](float v) {
-                        const float d = v - M;
-                        n += d == 0.0f;
-                        s += d == 0.0f ? 0.0f : exp2_fast(d * a.scale);
-                    };
-                    if (edge >= 0) add(elem(x, edge));
-                    uint4 v[kUnitVecs / 32];
-#pragma unroll
-                    for (int k = 0; k < kUnitVecs / 32; k++)
-                        v[k] = k * 32 + lane < cnt ? load16(x + sh.head + (size_t)(first + k * 32 + lane) * kN)
-                                                   : Pack<T>::lowest();
-#pragma unroll
-                    for (int k = 0; k < kUnitVecs / 32; k++) {
-                        float o[kN];
-                        Pack<T>::widen(v[k], o);
-#pragma unroll
-                        for (int j = 0; j < kN; j++) add(o[j]);
-                    }
-                    sum += (double)s;
-                }
+            if (i * 32 + lane >= a.units) break;
+            if (p[i].x == M) {
+                others += (double)p[i].y;
+                at_max += (int)p[i].z;
+            } else {
+                others += (double)(exp2_fast((p[i].x - M) * a.scale) * (p[i].y + p[i].z));
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            n = warp_sum_int(n);
-            excess = rest + sum + (double)(n - 1);
         }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) others += __shfl_xor_sync(0xffffffffu, others, o);
+        double excess = others + (double)(warp_sum_int(at_max) - 1);
         if (isinf(M)) excess = NAN;
         r.scored = 1;
         r.max = M;
@@ -1058,24 +1047,24 @@ static ScoreArgs<T> score_args(const Rows& r) {
     return a;
 }
 
-// Calls of at least this many bytes of logits stream; below, a cluster per row
-// ends sooner, in one launch: 13.7 us against 16.6 for 39 MB, 78 against 62.5
-// for 311 MB, even near 74 MB.
-constexpr size_t kStreamBytes = (size_t)72 << 20;
-
 static int row_units(int dtype, int vocab) {
     const int vecs = vocab / (dtype == QS_F32 ? 4 : 8);
     return vecs > kUnitVecs ? (vecs + kUnitVecs - 1) / kUnitVecs : 1;
 }
+// Large calls stream; smaller ones take a cluster per row, in one launch.  Long
+// bf16 rows from 72 MB (22.0 us against 22.4 at 72 MB, 30.4 against 33.2 at
+// 120), fp32 rows and rows of less than a CTA's 40 KB from 40 MB (fp32 of
+// 151,936: 14.6 against 17.3 us at 48 MB; bf16 of 4,099: 18.5 against 24.0).
 static bool streams(int dtype, int rows, int vocab) {
-    return (size_t)rows * vocab * (dtype == QS_F32 ? 4 : 2) >= kStreamBytes;
+    const size_t row = (size_t)vocab * (dtype == QS_F32 ? 4 : 2);
+    return rows * row >= (size_t)(dtype == QS_BF16 && row >= 40 * 1024 ? 72 : 40) << 20;
 }
 static size_t score_workspace(int dtype, int rows, int vocab) {
-    return streams(dtype, rows, vocab) ? round256((size_t)rows * row_units(dtype, vocab) * sizeof(float2)) : 0;
+    return streams(dtype, rows, vocab) ? round256((size_t)rows * row_units(dtype, vocab) * sizeof(float4)) : 0;
 }
 
 template <typename T>
-static int score(const Rows& r, RowScore* out, float* coefs, float* logprobs, float* stats, float2* parts,
+static int score(const Rows& r, RowScore* out, float* coefs, float* logprobs, float* stats, float4* parts,
                  cudaStream_t st) {
     if (!streams(r.dtype, r.rows, r.vocab)) {
         ScoreArgs<T> a = score_args<T>(r);
@@ -1143,8 +1132,8 @@ int qs_token_logprobs(const void* d_logits, int dtype, int rows, int vocab, long
     rc = check_workspace(d_workspace, workspace_bytes, score_workspace(dtype, rows, vocab));
     if (rc) return rc;
     const cudaStream_t st = (cudaStream_t)stream;
-    return dtype == QS_F32 ? score<float>(r, nullptr, nullptr, d_logprobs, d_stats, (float2*)d_workspace, st)
-                           : score<__nv_bfloat16>(r, nullptr, nullptr, d_logprobs, d_stats, (float2*)d_workspace, st);
+    return dtype == QS_F32 ? score<float>(r, nullptr, nullptr, d_logprobs, d_stats, (float4*)d_workspace, st)
+                           : score<__nv_bfloat16>(r, nullptr, nullptr, d_logprobs, d_stats, (float4*)d_workspace, st);
 }
 
 int qs_token_logprobs_backward(const void* d_logits, int dtype, int rows, int vocab, long long row_stride,
@@ -1231,7 +1220,7 @@ int qs_preference_loss(const void* d_logits, int dtype, int rows, int vocab, lon
     const cudaStream_t st = (cudaStream_t)stream;
     RowScore* sc = (RowScore*)d_workspace;
     float* coefs = (float*)((char*)d_workspace + round256((size_t)rows * sizeof(RowScore)));
-    float2* parts = (float2*)((char*)coefs + round256((size_t)rows * sizeof(float)));
+    float4* parts = (float4*)((char*)coefs + round256((size_t)rows * sizeof(float)));
     if (rows > 0) {
         const int e = dtype == QS_F32 ? score<float>(r, sc, coefs, nullptr, nullptr, parts, st)
                                       : score<__nv_bfloat16>(r, sc, coefs, nullptr, nullptr, parts, st);
