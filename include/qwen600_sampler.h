@@ -361,14 +361,15 @@ QS_API int qs_w4_pack(const void* d_plain_codes, const void* d_plain_scales, con
 /* qs_lm_head with such a weight:
  *   normed[b] as qs_lm_head's, logits[b] = bf16(normed[b] . w^T)
  * A normed row is taken at the fp16 precision of its values scaled to its
- * largest one, which is exact for those within 2^-28 of it; products with codes
- * are then exact.  Sums are fp32 per group, less the zero point times the
- * group's sum, then scaled and added in fp32.  d_hidden and d_normed bf16
+ * largest one, which is exact for those of at least 2^-31 of it (smaller ones
+ * lose what lies 2^-39 below it); products with codes less their zero points
+ * are then exact.  Sums are fp32 per group, then scaled and added in
+ * fp32.  d_hidden and d_normed bf16
  * [batch, hidden_dim], d_logits bf16 [batch, vocab], all 16-byte aligned, as
  * d_workspace is (qs_lm_head_w4_workspace bytes; calls that overlap on the GPU
  * need workspaces of their own).  The weight is streamed once per block of 8 to
  * 32 rows (the most that fit in shared memory).  Allocates nothing. */
-QS_API size_t qs_lm_head_w4_workspace(int batch, int hidden_dim, int group);
+QS_API size_t qs_lm_head_w4_workspace(int batch, int hidden_dim);
 QS_API int qs_lm_head_w4(const void* d_hidden, const void* d_norm_weight, const qs_w4_weight* weight,
                          int batch, void* d_normed, void* d_logits, void* d_workspace,
                          size_t workspace_bytes, void* stream);

@@ -135,7 +135,7 @@ def _load() -> C.CDLL:
     lib.qs_w4_zeros_bytes.argtypes = [i32, i32, i32]
     lib.qs_w4_quantize.argtypes = [vp, i32, i32, i32, vp, vp, vp, vp]
     lib.qs_w4_pack.argtypes = [vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp]
-    lib.qs_lm_head_w4_workspace.argtypes = [i32, i32, i32]
+    lib.qs_lm_head_w4_workspace.argtypes = [i32, i32]
     lib.qs_lm_head_w4.argtypes = [vp, vp, P(W4Desc), i32, vp, vp, vp, sz, vp]
     lib.qs_lm_head_w4_sample.argtypes = [vp, vp, vp, P(W4Desc), i32, vp, vp, u32]
     lib.qs_token_logprobs_workspace.argtypes = [i32, i32, i32]

@@ -1107,8 +1107,8 @@ int qs_w4_pack(const void* d_plain_codes, const void* d_plain_scales, const void
     return QS_OK;
 }
 
-size_t qs_lm_head_w4_workspace(int batch, int hidden_dim, int group) {
-    return batch >= 1 && w4_sizes(1, hidden_dim, group) ? w4_workspace(batch, hidden_dim, group) : 0;
+size_t qs_lm_head_w4_workspace(int batch, int hidden_dim) {
+    return batch >= 1 && w4_sizes(1, hidden_dim, 128) ? w4_workspace(batch, hidden_dim) : 0;
 }
 
 int qs_lm_head_w4(const void* d_hidden, const void* d_norm_weight, const qs_w4_weight* weight, int batch,
@@ -1122,7 +1122,7 @@ int qs_lm_head_w4(const void* d_hidden, const void* d_norm_weight, const qs_w4_w
     if ((((uintptr_t)d_normed) | ((uintptr_t)d_logits)) & 15)
         return fail(QS_ERR_INVALID, "normed and logits must be 16-byte aligned");
     if (((uintptr_t)d_norm_weight) & 3) return fail(QS_ERR_INVALID, "norm_weight must be 4-byte aligned");
-    const size_t need = qs_lm_head_w4_workspace(batch, weight->hidden_dim, weight->group);
+    const size_t need = qs_lm_head_w4_workspace(batch, weight->hidden_dim);
     if (need > 0 && (!d_workspace || workspace_bytes < need || (((uintptr_t)d_workspace) & 15)))
         return fail(QS_ERR_INVALID, "workspace is NULL, unaligned or below %zu bytes", need);
     int dev = 0, sms = 148;
@@ -1147,7 +1147,7 @@ int qs_lm_head_w4_sample(qs_sampler* s, const void* d_hidden, const void* d_norm
     DeviceGuard dg(s->device);
     rc = tail_workspace(s, weight->hidden_dim);
     if (rc) return rc;
-    const size_t need = qs_lm_head_w4_workspace(s->max_batch, weight->hidden_dim, weight->group);
+    const size_t need = qs_lm_head_w4_workspace(s->max_batch, weight->hidden_dim);
     if (s->lh_w4_bytes < need) {
         if (s->lh_w4) cudaFree(s->lh_w4);
         s->lh_w4 = nullptr; s->lh_w4_bytes = 0;

@@ -5,17 +5,16 @@
 // the measured 6549 GB/s, so all else has to fit beside 23 bytes a clock and
 // SM.  What counts is the instructions a code costs.  Codes go from memory to
 // registers and meet the tokens on mma.sync m16n8k16, 16 vocabulary rows x 8
-// tokens, tokens on the narrow side.  A code needs no conversion: as the low
-// bits of an fp16 number, q is the number q 2^-24 and 16 q is 16 q 2^-24, so a
-// word of 8 codes becomes four operand registers with one shift and four
-// ands.  (Made into bf16 pairs, by shift, and / or, subtract, it took 11
-// instructions.)  The tokens are
-// scaled by a power of two to fp16 (exact for values within 2^-28 of a row's
-// largest), the columns that meet 16 q by another 1 / 16, and the zero point is
-// taken out of a group's sum: sum (q - z) x = sum q x - z sum x, with the
-// group's sum x made once per launch.  (tcgen05 takes its wider operand
-// from shared or tensor memory; 4-bit weights would have to be written there
-// as 16-bit numbers, four times the bytes of their stream.)
+// tokens, tokens on the narrow side.  A word of 8 codes becomes four registers of fp16
+// pairs q - z with 9 instructions: one shift, four and / ors into 1024 + q or
+// 1024 + 16 q, four fp16 subtractions or multiply-adds, all exact.  (As fp16
+// denormals, q 2^-24, codes need only the shift and four ands, but the tensor
+// cores align products by nominal exponents and lose 6 bits of a sum; as bf16
+// pairs they take 11.)  The tokens are scaled by a power of two to fp16, exactly
+// for values of at least 2^-31 of a row's largest (smaller ones lose what lies
+// 2^-39 below it).  (tcgen05 takes its wider operand from shared or tensor
+// memory; 4-bit weights would have to be written there as 16-bit numbers, four
+// times the bytes of their stream.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -125,31 +124,24 @@ cudaError_t launch_w4_pack(const unsigned char* codes, const void* scales, const
 
 // -------------------------------------------------------------------- rows
 // RMSNorm of one token's row per CTA, and the row as the products take it, in
-// the workspace: fp16 columns scaled by 2^s so that the largest finite value
-// lies in [2^14, 2^15) (columns 2, 3, 6 and 7 of each 8 meet 16 q and get
-// 2^(s - 4)), the sums of its groups' columns times -2^(s - 24) (the products'
-// scale) and, where every zero point is 8, times that; and 2^(24 - s) as two
-// factors.
-__host__ __device__ static inline size_t w4_row_bytes(int chunks, int groups) {
-    return (size_t)chunks * 256 + 16 + (((size_t)chunks * groups * 4 + 15) & ~(size_t)15);
-}
+// the workspace: fp16 columns (zeros behind the last) scaled by 2^s so that the
+// largest finite value lies in [2^14, 2^15), then 2^-s.
+__host__ __device__ static inline size_t w4_row_bytes(int chunks) { return (size_t)chunks * 256 + 16; }
 
 // kPairs: column pairs of a thread, the row's whole share, requested with its
 // norm weights before anything waits.
 template <int kPairs>
 __global__ void __launch_bounds__(kNormThreads)
 w4_rows_kernel(const __nv_bfloat16* __restrict__ X, const __nv_bfloat16* __restrict__ w, __nv_bfloat16* __restrict__ Y,
-               int K, int chunks, int groups, bool zeros, unsigned char* __restrict__ ws, float inv_d, float eps) {
+               int K, int chunks, unsigned char* __restrict__ ws, float inv_d, float eps) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the projection may request its first codes
-    __shared__ float red_max[kNormThreads / 32], red_sum[kPairs][kNormThreads / 32];
+    __shared__ float red_max[kNormThreads / 32];
     const int t = threadIdx.x, warp = t >> 5, half = K / 2;
     const __nv_bfloat162* in = reinterpret_cast<const __nv_bfloat162*>(X + (size_t)blockIdx.x * K);
     const __nv_bfloat162* wt = reinterpret_cast<const __nv_bfloat162*>(w);
     __nv_bfloat162* out = reinterpret_cast<__nv_bfloat162*>(Y + (size_t)blockIdx.x * K);
-    ws += blockIdx.x * w4_row_bytes(chunks, groups);
+    ws += blockIdx.x * w4_row_bytes(chunks);
     uint32_t* xs = reinterpret_cast<uint32_t*>(ws);
-    float2* unscale = reinterpret_cast<float2*>(ws + (size_t)chunks * 256);
-    float* sums = reinterpret_cast<float*>(ws + (size_t)chunks * 256 + 16);
     __nv_bfloat162 xv[kPairs], wv[kPairs];
 #pragma unroll
     for (int j = 0; j < kPairs; j++) {
@@ -184,39 +176,14 @@ w4_rows_kernel(const __nv_bfloat16* __restrict__ X, const __nv_bfloat16* __restr
     for (int k = 0; k < kNormThreads / 32; k++) m = fmaxf(m, red_max[k]);
     const int e = (int)(__float_as_uint(m) >> 23) - 127;
     const int s = m == 0.0f ? 0 : min(14 - e, 120);
-    const float up = __uint_as_float((uint32_t)(s + 127) << 23), f = t & 1 ? 0.0625f : 1.0f;
-    if (t == 0) {
-        const int h = (24 - s) >> 1, r = 24 - s - h;
-        *unscale = make_float2(__uint_as_float((uint32_t)(h + 127) << 23), __uint_as_float((uint32_t)(r + 127) << 23));
-    }
-    const int per = 64 / groups;  // pairs of a group: 16, 32 or 64
-    const float by = zeros ? -0x1p-24f : -0x1p-21f;
+    const float up = __uint_as_float((uint32_t)(s + 127) << 23);
+    if (t == 0) *reinterpret_cast<float*>(ws + (size_t)chunks * 256) = __uint_as_float((uint32_t)(127 - s) << 23);
 #pragma unroll
     for (int j = 0; j < kPairs; j++) {
         const int i = j * kNormThreads + t;
-        if (j * kNormThreads + warp * 32 >= chunks * 64) break;  // alike for the warp: 64 pairs a chunk
-        const float a = y[j].x * up, b = y[j].y * up;
-        const __half2 h = __floats2half2_rn(a * f, b * f);
-        xs[i] = *reinterpret_cast<const uint32_t*>(&h);
-        float sum = (a + b) * by;
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (per == 16) {
-            if ((t & 15) == 0) sums[i / 16] = sum;
-        } else {
-            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-            if (per == 32) {
-                if ((t & 31) == 0) sums[i / 32] = sum;
-            } else if ((t & 31) == 0) {
-                red_sum[j][warp] = sum;
-            }
-        }
-    }
-    if (per == 64) {
-        __syncthreads();
-        for (int i = t; i < chunks; i += kNormThreads) {
-            const int j = i / 4, k = (i & 3) * 2;
-            sums[i] = red_sum[j][k] + red_sum[j][k + 1];
+        if (i < chunks * 64) {  // 64 pairs a chunk
+            const __half2 h = __floats2half2_rn(y[j].x * up, y[j].y * up);
+            xs[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
     }
 }
@@ -240,18 +207,8 @@ __device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigne
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
-__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
-    unsigned long long r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
-    unsigned long long r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 
-// d = a * b + d, or + c, on 16 x 8 x 16.
+// d = a * b + d, or a * b alone, on 16 x 8 x 16.
 __device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
     asm volatile(
@@ -260,13 +217,33 @@ __device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_first(float* d, float c0, float c1, float c2, float c3, uint32_t a0, uint32_t a1,
-                                          uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_first(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%10, %11, %12, %13};"
+        "{%10, %10, %10, %10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// (v & mask) | 1024 in each half.
+__device__ __forceinline__ __half2 code_bits(uint32_t v, uint32_t mask) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(0x64006400u));
+    return *reinterpret_cast<const __half2*>(&r);
+}
+__device__ __forceinline__ uint32_t bits_of(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ __half2 half2_of(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
+
+// The eight codes of a word minus their zero point: columns 0 and 1, 2 and 3, 4
+// and 5, 6 and 7.  z1024: 1024 + z twice; z64: -(64 + z) twice.
+__device__ __forceinline__ void code_pairs(uint32_t v, __half2 z1024, __half2 z64, uint32_t* r) {
+    const uint32_t v8 = v >> 8;
+    const __half2 sixteenth = half2_of(0x2C002C00u);
+    r[0] = bits_of(__hsub2(code_bits(v, 0x000F000Fu), z1024));
+    r[1] = bits_of(__hfma2(code_bits(v, 0x00F000F0u), sixteenth, z64));
+    r[2] = bits_of(__hsub2(code_bits(v8, 0x000F000Fu), z1024));
+    r[3] = bits_of(__hfma2(code_bits(v8, 0x00F000F0u), sixteenth, z64));
 }
 
 // The scales of rows g (low half) and g + 8.
@@ -337,7 +314,7 @@ constexpr int kStageRow = 40;  // a token's 32 values in a warp's staging rows, 
 // Stores a finished tile: 32 vocabulary rows of up to 8 kNt tokens, through the
 // warp's staging rows so that a lane stores 16 bytes of one token.
 template <int kNt>
-__device__ __forceinline__ void w4_store(const float (&acc)[2][kNt][4], const float2* unscale, __nv_bfloat16* stage,
+__device__ __forceinline__ void w4_store(const float (&acc)[2][kNt][4], const float* unscale, __nv_bfloat16* stage,
                                          const W4Out& o, int V, int tile, int lane) {
     const int g = lane >> 2, q = lane & 3;
     __syncwarp();
@@ -346,10 +323,10 @@ __device__ __forceinline__ void w4_store(const float (&acc)[2][kNt][4], const fl
 #pragma unroll
         for (int j = 0; j < 2; j++) {  // token 2 q or 2 q + 1
             const int token = n * 8 + 2 * q + j;
-            const float2 f = unscale[token];
+            const float f = unscale[token];
 #pragma unroll
             for (int b = 0; b < 4; b++)  // row g + 8 b
-                stage[token * kStageRow + g + b * 8] = __float2bfloat16_rn(acc[b >> 1][n][(b & 1) * 2 + j] * f.x * f.y);
+                stage[token * kStageRow + g + b * 8] = __float2bfloat16_rn(acc[b >> 1][n][(b & 1) * 2 + j] * f);
         }
     }
     __syncwarp();
@@ -390,8 +367,7 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
     unsigned char* xs = smem;                                           // fp16 rows
     float4* slots = reinterpret_cast<float4*>(smem + kNt * 8 * pitch);  // [warp][continued, begun][2][kNt][lane]
     __nv_bfloat16* stage = reinterpret_cast<__nv_bfloat16*>(slots + kWarps * 2 * 2 * kNt * 32);
-    float2* unscale = reinterpret_cast<float2*>(stage + kWarps * kNt * 8 * kStageRow);  // [token] two factors
-    float* sums = reinterpret_cast<float*>(unscale + kNt * 8);                // [group][token] sum of its columns
+    float* unscale = reinterpret_cast<float*>(stage + kWarps * kNt * 8 * kStageRow);  // [token]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     stage += warp * kNt * 8 * kStageRow;
     const int t0 = (int)((long long)blockIdx.x * tiles / gridDim.x), t1 = (int)((long long)(blockIdx.x + 1) * tiles / gridDim.x);
@@ -407,19 +383,21 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
 #pragma unroll
     for (int d = 0; d < kW4Depth; d++)
         if (a + d < b) w4_load<kGroups, kZeros>(buf[d], at, d);
+    // two more units on their way to L2 while the RMSNorm runs (one token 18.2 to 17.7 us, 5 tokens of 32,003 x 4,096
+    // 19.3 to 18.3; 4 or 8 units gain less)
+    for (int i = lane; i < min(2, b - a - kW4Depth) * (kUnitCodes / 128); i += 32)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(w.codes + (size_t)(a + kW4Depth) * kUnitCodes + i * 128));
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the RMSNorm's rows
-    const size_t row_bytes = w4_row_bytes(chunks, kGroups);
+    const size_t row_bytes = w4_row_bytes(chunks);
     for (int i = threadIdx.x; i < kNt * 8 * chunks * 16; i += kWarps * 32) {
         const int row = i / (chunks * 16), c = i - row * (chunks * 16);
         *reinterpret_cast<uint4*>(xs + row * pitch + c * 16) =
             row < o.tokens ? *reinterpret_cast<const uint4*>(rows + row * row_bytes + c * 16) : make_uint4(0u, 0u, 0u, 0u);
     }
-    for (int i = threadIdx.x; i < kNt * 8 * (chunks * kGroups + 1); i += kWarps * 32) {
-        const int row = i % (kNt * 8), j = i / (kNt * 8);
-        const unsigned char* p = rows + row * row_bytes + chunks * 256;
-        if (j == 0) unscale[row] = row < o.tokens ? *reinterpret_cast<const float2*>(p) : make_float2(0.0f, 0.0f);
-        else sums[i - kNt * 8] = row < o.tokens ? reinterpret_cast<const float*>(p + 16)[j - 1] : 0.0f;
-    }
+    if (threadIdx.x < kNt * 8)
+        unscale[threadIdx.x] = threadIdx.x < o.tokens
+                                   ? *reinterpret_cast<const float*>(rows + threadIdx.x * row_bytes + chunks * 256)
+                                   : 0.0f;
     __syncthreads();
 
     float acc[2][kNt][4];
@@ -436,8 +414,6 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
     bool begun = c == 0;
     const unsigned char* xl = xs + g * pitch + q * 16;
     const unsigned char* xc = xl + c * 256;
-    const float* sl0 = sums + 2 * q;
-    const float* sc = sl0 + c * kGroups * kNt * 8;
     for (int left = b - a; left > 0; left -= kW4Depth) {
         at.codes += kW4Depth * kUnitCodes;
         at.scales += kW4Depth * 64 * kGroups;
@@ -447,39 +423,33 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
             if (d >= left) break;
 #pragma unroll
             for (int j = 0; j < kGroups; j++) {
+                __half2 z1024[4], z64[4];
+#pragma unroll
+                for (int b4 = 0; b4 < 4; b4++) {
+                    if (kZeros) {  // bytes z, 0x64, z, 0x64
+                        z1024[b4] = half2_of(__byte_perm(buf[d].zeros[j], 0x64646464u, 0x4040u + 0x0101u * b4));
+                        z64[b4] = __hsub2(half2_of(0x63806380u), z1024[b4]);  // 960 - (1024 + z)
+                    } else {
+                        z1024[b4] = half2_of(0x64086408u);
+                        z64[b4] = half2_of(0xD480D480u);
+                    }
+                }
                 float part[2][kNt][4];
 #pragma unroll
                 for (int k = 0; k < 4 / kGroups; k++) {
                     const int word = j * (4 / kGroups) + k;
-                    uint32_t r[4][4];  // codes of rows g + 8 b: q, 16 q, q, 16 q
+                    uint32_t r[4][4];  // rows g + 8 b
 #pragma unroll
-                    for (int b4 = 0; b4 < 4; b4++) {
-                        const uint32_t v = reinterpret_cast<const uint32_t*>(&buf[d].codes[b4])[word], v8 = v >> 8;
-                        r[b4][0] = v & 0x000F000Fu;
-                        r[b4][1] = v & 0x00F000F0u;
-                        r[b4][2] = v8 & 0x000F000Fu;
-                        r[b4][3] = v8 & 0x00F000F0u;
-                    }
+                    for (int b4 = 0; b4 < 4; b4++)
+                        code_pairs(reinterpret_cast<const uint32_t*>(&buf[d].codes[b4])[word], z1024[b4], z64[b4], r[b4]);
 #pragma unroll
                     for (int n = 0; n < kNt; n++) {
                         const uint4 xv = *reinterpret_cast<const uint4*>(xc + n * 8 * pitch + word * 64);
-                        float2 sx;
-                        if (k == 0) sx = *reinterpret_cast<const float2*>(sc + j * kNt * 8 + n * 8);
 #pragma unroll
                         for (int m = 0; m < 2; m++) {
                             const uint32_t *lo = r[2 * m], *hi = r[2 * m + 1];
-                            // a group's sum begins at minus its zero point times the group's sum of x
-                            if (k == 0 && kZeros) {
-                                const uint32_t z = buf[d].zeros[j] >> (16 * m);
-                                const float zl = (float)(z & 0xFFu), zh = (float)((z >> 8) & 0xFFu);
-                                const unsigned long long sx2 = pair2(sx.x, sx.y);
-                                const float2 cl = unpair2(mul2(pair2(zl, zl), sx2)), ch = unpair2(mul2(pair2(zh, zh), sx2));
-                                mma_first(part[m][n], cl.x, cl.y, ch.x, ch.y, lo[0], hi[0], lo[1], hi[1], xv.x, xv.y);
-                            } else if (k == 0) {
-                                mma_first(part[m][n], sx.x, sx.y, sx.x, sx.y, lo[0], hi[0], lo[1], hi[1], xv.x, xv.y);
-                            } else {
-                                mma(part[m][n], lo[0], hi[0], lo[1], hi[1], xv.x, xv.y);
-                            }
+                            if (k == 0) mma_first(part[m][n], lo[0], hi[0], lo[1], hi[1], xv.x, xv.y);
+                            else mma(part[m][n], lo[0], hi[0], lo[1], hi[1], xv.x, xv.y);
                             mma(part[m][n], lo[2], hi[2], lo[3], hi[3], xv.z, xv.w);
                         }
                     }
@@ -502,7 +472,6 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
             if (d + kW4Depth < left) w4_load<kGroups, kZeros>(buf[d], at, d);
             const bool ends = ++c == chunks;
             xc += 256;
-            sc += kGroups * kNt * 8;
             if (ends || d + 1 == left) {
                 if (ends && begun) {
                     w4_store<kNt>(acc, unscale, stage, o, w.vocab, tile, lane);
@@ -518,7 +487,6 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
                 if (ends) {
                     c = 0;
                     xc = xl;
-                    sc = sl0;
                     tile++;
                     begun = true;
                 }
@@ -546,14 +514,14 @@ lm_head_w4_kernel(const unsigned char* rows, const __grid_constant__ W4View w, c
     }
 }
 
-static size_t w4_smem(int nt, int K, int group) {
+static size_t w4_smem(int nt, int K) {
     return (size_t)nt * 8 * (w4_chunks(K) * 256 + 64) + (size_t)(nt <= 2 ? 16 : 8) * nt * (2 * 2 * 512 + 16 * kStageRow) +
-           (size_t)nt * 8 * (sizeof(float2) + w4_chunks(K) * (128 / group) * sizeof(float));
+           (size_t)nt * 8 * sizeof(float);
 }
 
 template <int kNt, int kGroups, bool kZeros, bool kF16>
 static cudaError_t w4_go(const unsigned char* rows, const W4View& w, const W4Out& o, int grid, cudaStream_t st) {
-    const size_t smem = w4_smem(kNt, w.hidden, w.group);
+    const size_t smem = w4_smem(kNt, w.hidden);
     static std::atomic<unsigned long long> raised{0};  // devices on which the kernel may use all shared memory
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -593,26 +561,25 @@ static cudaError_t w4_group(const unsigned char* rows, const W4View& w, const W4
                           : w4_types<kNt, 4>(rows, w, o, grid, st);
 }
 
-size_t w4_workspace(int batch, int K, int group) { return (size_t)batch * w4_row_bytes(w4_chunks(K), 128 / group); }
+size_t w4_workspace(int batch, int K) { return (size_t)batch * w4_row_bytes(w4_chunks(K)); }
 
 cudaError_t launch_lm_head_w4(const __nv_bfloat16* hidden, const __nv_bfloat16* norm_weight, const W4View& w, int batch,
                               __nv_bfloat16* normed, __nv_bfloat16* logits, unsigned char* ws, int num_sms,
                               uint32_t* segk, int segk_stride, cudaStream_t st) {
-    const int chunks = w4_chunks(w.hidden), groups = 128 / w.group;
+    const int chunks = w4_chunks(w.hidden);
     const auto rows_kernel = w.hidden <= 1024 ? w4_rows_kernel<2> : w.hidden <= 4096 ? w4_rows_kernel<8> : w4_rows_kernel<16>;
-    rows_kernel<<<batch, kNormThreads, 0, st>>>(hidden, norm_weight, normed, w.hidden, chunks, groups,
-                                               w.zeros != nullptr, ws,
+    rows_kernel<<<batch, kNormThreads, 0, st>>>(hidden, norm_weight, normed, w.hidden, chunks, ws,
                                                1.0f / (float)w.hidden, kNormEps);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     const int tiles = w4_tiles(w.vocab), grid = tiles < num_sms ? tiles : num_sms;
     int most = 4;  // blocks of 8 tokens whose rows fit in shared memory
-    while (w4_smem(most, w.hidden, w.group) > 227 * 1024) most--;
+    while (w4_smem(most, w.hidden) > 227 * 1024) most--;
     for (int b = 0; b < batch;) {
         const int left = (batch - b + 7) / 8, nt = left < most ? left : most;
         const int n = batch - b < nt * 8 ? batch - b : nt * 8;
         const W4Out o{logits + (size_t)b * w.vocab, n, segk ? segk + (size_t)b * segk_stride : nullptr, segk_stride};
-        const unsigned char* rows = ws + b * w4_row_bytes(chunks, groups);
+        const unsigned char* rows = ws + b * w4_row_bytes(chunks);
         e = nt == 1 ? w4_group<1>(rows, w, o, grid, st)
           : nt == 2 ? w4_group<2>(rows, w, o, grid, st)
           : nt == 3 ? w4_group<3>(rows, w, o, grid, st)

@@ -27,7 +27,7 @@ cudaError_t launch_w4_pack(const unsigned char* codes, const void* scales, const
 // RMSNorm of the hidden rows into normed, and logits[batch, vocab] of them;
 // with segk the epilogue also folds the rows' maxima of 256-column segments
 // into it, as launch_lm_head does.  ws: w4_workspace bytes.
-size_t w4_workspace(int batch, int K, int group);
+size_t w4_workspace(int batch, int K);
 cudaError_t launch_lm_head_w4(const __nv_bfloat16* hidden, const __nv_bfloat16* norm_weight, const W4View& w, int batch,
                               __nv_bfloat16* normed, __nv_bfloat16* logits, unsigned char* ws, int num_sms,
                               uint32_t* segk, int segk_stride, cudaStream_t st);

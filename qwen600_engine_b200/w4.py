@@ -32,7 +32,7 @@ class W4Weight:
         self._w4_desc = _lib.W4Desc(codes.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(),
                                     vocab, hidden_dim, group, scale_dtype)
         self._w4_ref = C.byref(self._w4_desc)
-        self._row_bytes = _lib.lib.qs_lm_head_w4_workspace(1, hidden_dim, group)
+        self._row_bytes = _lib.lib.qs_lm_head_w4_workspace(1, hidden_dim)
 
     @classmethod
     def pack(cls, codes, scales, zeros=None, *, stream=None) -> "W4Weight":

@@ -107,6 +107,27 @@ def test_one_row_does_not_depend_on_the_batch():
     assert torch.isnan(b[[4, 7]]).all()
 
 
+def test_rows_of_any_magnitude():
+    """Rows whose values differ by up to 2^24, tiny and huge rows, a row of zeros."""
+    from qwen600_engine_b200.w4 import W4Weight, lm_head_w4
+    K, V = 512, 1000
+    for group, zeros in ((32, True), (128, False)):
+        codes, scales, z, g = plain_weight(V, K, group, zeros, torch.bfloat16, seed=group)
+        w = W4Weight.pack(codes, scales, z)
+        h, nw = inputs(g, 10, K)
+        h[1] = (h[1].float() * torch.exp2(torch.randint(-12, 13, (K,), generator=g, device="cuda").float())).to(torch.bfloat16)
+        h[2] = 0.0
+        h[3] *= 2.0 ** -80
+        h[4, 5] = 3.0e4
+        h[5, 1:] = 0.0
+        big = (nw.float() * 2.0 ** 90).to(torch.bfloat16)
+        small = (nw.float() * 2.0 ** -100).to(torch.bfloat16)
+        for weight in (nw, big, small):
+            normed, logits = lm_head_w4(h, w, weight)
+            assert torch.isfinite(logits).all() and (logits[2] == 0).all()
+            check_logits(normed, dense(codes, scales, z), logits)
+
+
 def test_quantize():
     from qwen600_engine_b200.w4 import W4Weight, lm_head_w4, quantize_w4
     g = torch.Generator(device="cuda")

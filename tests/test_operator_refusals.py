@@ -100,8 +100,7 @@ def test_sizes_outside_the_limits_are_0_bytes():
         assert L.qs_w4_scales_bytes(vocab, hidden, group) == 0 and L.qs_w4_zeros_bytes(vocab, hidden, group) == 0
     for group in (0, -32, 48, 1 << 30):
         assert L.qs_w4_scales_bytes(1000, 1024, group) == 0 and L.qs_w4_zeros_bytes(1000, 1024, group) == 0
-        assert L.qs_lm_head_w4_workspace(4, 1024, group) == 0
-    assert L.qs_lm_head_w4_workspace(-1, 1024, 64) == 0
+    assert L.qs_lm_head_w4_workspace(-1, 1024) == 0 and L.qs_lm_head_w4_workspace(4, 1 << 20) == 0
     assert L.qs_policy_loss_workspace(-5) > 0 and L.qs_preference_loss_workspace(QS_F32, -5, 1000) == 0
     assert L.qs_token_logprobs_workspace(9, 10, 1000) == 0 and L.qs_token_logprobs_workspace(QS_F32, 10, -1) == 0
 
