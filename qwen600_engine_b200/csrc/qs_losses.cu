@@ -30,8 +30,6 @@ struct RowScore {
     double logprob;  // 0 for a row that scores nothing
     float max;
     float excess;
-    int scored;
-    int pad;
 };
 
 template <typename T>
@@ -296,7 +294,7 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
     if (!scored) {  // alike for the whole cluster
         if (rank == 0 && t == 0) {
             if (a.out) {
-                a.out[row] = RowScore{0.0, 0.0f, 0.0f, 0, 0};
+                a.out[row] = RowScore{0.0, 0.0f, 0.0f};
                 a.coefs[row] = 0.0f;
             }
             if (a.logprobs) a.logprobs[row] = 0.0f;
@@ -449,7 +447,7 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
             const double lp = ((double)xt - (double)M) * a.inv_t - log1p(excess);
             if (rank == 0) {
                 if (a.out) {
-                    a.out[row] = RowScore{lp, M, (float)excess, 1, 0};
+                    a.out[row] = RowScore{lp, M, (float)excess};
                     a.coefs[row] = 0.0f;
                 }
                 if (a.logprobs) a.logprobs[row] = (float)lp;
@@ -733,7 +731,7 @@ join_kernel(const __grid_constant__ StreamArgs<T> a) {
     const float xt = scored ? elem(x, tok) : 0.0f;
     wait_for_previous();
     if (row >= a.rows) return;
-    RowScore r{0.0, 0.0f, 0.0f, 0, 0};
+    RowScore r{0.0, 0.0f, 0.0f};
     if (scored) {
         const float4* all = a.parts + (size_t)row * a.units;
         float4 p[kMine];
@@ -760,7 +758,6 @@ join_kernel(const __grid_constant__ StreamArgs<T> a) {
         for (int o = 16; o > 0; o >>= 1) others += __shfl_xor_sync(0xffffffffu, others, o);
         double excess = others + (double)(warp_sum_int(at_max) - 1);
         if (isinf(M)) excess = NAN;
-        r.scored = 1;
         r.max = M;
         r.excess = (float)excess;
         if (lane == 0) r.logprob = ((double)xt - (double)M) * a.inv_t - log1p(excess);
