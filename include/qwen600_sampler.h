@@ -376,7 +376,7 @@ QS_API int qs_lm_head_w4(const void* d_hidden, const void* d_norm_weight, const 
 
 /* qs_lm_head_sample with such a weight (weight->vocab must be the handle's):
  * qs_lm_head_w4 into the handle's workspace (a first call, and one with a new
- * hidden_dim or group, may allocate it), then qs_sample on its logits. */
+ * hidden_dim, allocates it), then qs_sample on its logits. */
 QS_API int qs_lm_head_w4_sample(qs_sampler* s, const void* d_hidden, const void* d_norm_weight,
                                 const qs_w4_weight* weight, int batch, int* d_tokens, void* stream,
                                 unsigned flags);
