@@ -615,6 +615,37 @@ def test_captured_graphs():
         g.reset()
 
 
+def test_large_calls_captured_and_on_streams():
+    """The streaming kernels in a graph, replayed on changed logits while another stream runs the same calls."""
+    c = policy_case(300, 151936, torch.bfloat16, seed=91)
+    pair = pairs_case(3, 151936, torch.bfloat16, seed=92, lengths=[60, 50, 30, 70, 20, 50], tail=1)
+    gl = torch.ones((300,), device="cuda")
+
+    def calls():
+        t = L().token_logprobs(c[0], c[1])
+        return (t.logprobs, t.stats, L().token_logprobs_backward(c[0], c[1], t.stats, gl),
+                *L().policy_loss(c[0], c[1], c[2], c[4], weights=c[5]), *L().preference_loss(*pair[:4]))
+
+    calls()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = calls()
+    c[0].copy_(rows_of(300, 151936, torch.bfloat16, seed=93)[0])
+    pair[0].mul_(0.5)
+    want = calls()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        g.replay()
+        with torch.cuda.stream(side):
+            other = calls()
+        torch.cuda.synchronize()
+        for a, b, d in zip(outs, want, other):
+            assert torch.equal(a, b) and torch.equal(d, b)
+    g.reset()
+
+
 def test_refused_on_the_gpu():
     from qwen600_engine_b200._lib import SamplerError
     x, tok, old, ref, adv, w = policy_case(4, 100, torch.float32, seed=81)

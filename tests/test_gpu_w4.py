@@ -186,6 +186,32 @@ def test_sample_from_4_bit_weights(B, V, params):
     apart.free()
 
 
+def test_sample_on_a_stream_into_the_callers_buffer():
+    from qwen600_engine_b200._lib import SamplerError
+    from qwen600_engine_b200.sampler import Sampler
+    from qwen600_engine_b200.w4 import W4Weight
+    codes, scales, z, g = plain_weight(2003, 256, 32, True, torch.float16, seed=12)
+    w = W4Weight.pack(codes, scales, z)
+    a, b = (Sampler(0.8, 0.9, 0.0, 10, 1.1, 0.0, 0.0, 16, 3, max_batch=5, vocab=2003) for _ in range(2))
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        h, nw = inputs(g, 5, 256)
+        want = a.lm_head_sample(h, w, nw)
+        out = torch.full((7,), -5, dtype=torch.int32, device="cuda")
+        side.wait_stream(torch.cuda.current_stream())
+        got = b.lm_head_sample(h, w, nw, out=out, stream=side)
+        del h, nw  # kept until the stream is done with them
+        torch.cuda.synchronize()
+        assert got is out and torch.equal(out[:5], want) and (out[5:] == -5).all()
+    h, nw = inputs(g, 1, 256)
+    assert b.lm_head_sample(h[0], w, nw).shape == (1,)  # one row without a batch dimension
+    for bad in (out[:3], out.long(), out.cpu()):
+        with pytest.raises(SamplerError, match="out must be"):
+            b.lm_head_sample(torch.zeros((5, 256), dtype=torch.bfloat16, device="cuda"), w, out=bad)
+    a.free()
+    b.free()
+
+
 def test_streams_and_graphs():
     from qwen600_engine_b200.w4 import W4Weight, lm_head_w4
     codes, scales, z, g = plain_weight(50021, 1024, 128, False, torch.bfloat16, seed=3)
