@@ -1,7 +1,8 @@
 """Builds the sampler's CUDA library in-tree for sm_100a.
 
 Produces qwen600_engine_b200/libqwen600_sampler.so from csrc/*.cu with nvcc
-(no GPU needed: nvcc cross-compiles).  --fmad=false keeps every fp32
+(no GPU needed: nvcc cross-compiles), and _torch.so, the torch binding of the
+scoring, loss and 4-bit lm_head calls, from csrc/qs_torch.cpp.  --fmad=false keeps every fp32
 multiply and add separately rounded, as the reference host sampler computes
 them; -lineinfo keeps profiler source correlation.
 """
@@ -98,8 +99,40 @@ def build(verbose: bool = False, ptxas_info: bool = False, force: bool = False) 
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stderr}")
+    build_binding(verbose, force)
     build_integration(verbose, force)
     return LIB
+
+
+BINDING = os.path.join(HERE, "_torch.so")
+
+
+def build_binding(verbose: bool = False, force: bool = False) -> str:
+    """_torch.so: the scoring, loss and 4-bit lm_head calls for torch tensors
+    (csrc/qs_torch.cpp), linked to the sampler library and torch's own."""
+    src = os.path.join(CSRC, "qs_torch.cpp")
+    deps = [src, os.path.join(ROOT, "include", "qwen600_sampler.h"), __file__]
+    if not force and not _stale(BINDING, deps):
+        return BINDING
+    import sysconfig
+
+    import torch
+    top = os.path.dirname(torch.__file__)
+    inc = [os.path.join(ROOT, "include"), os.path.join(top, "include"),
+           os.path.join(top, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"],
+           os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")]
+    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for d in inc:
+        cmd += ["-isystem" if d.startswith(top) else "-I", d]
+    cmd += [src, "-o", BINDING, "-L", HERE, "-lqwen600_sampler", "-Wl,-rpath,$ORIGIN", "-L", os.path.join(top, "lib"),
+            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd))
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"building the torch binding failed:\n{r.stderr}")
+    return BINDING
 
 
 INTEG = os.path.join(ROOT, "integration")

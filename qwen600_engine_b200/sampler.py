@@ -254,8 +254,7 @@ class Sampler:
 
     def _lm_head_w4_sample(self, hidden, weight, norm_weight, out, flags: int, stream):
         torch = _torch()
-        from .losses import _on_stream
-        from .w4 import _check_rows
+        from .w4 import _check_rows, _on_stream
         h = _check_rows(hidden, weight, norm_weight)
         B = int(h.shape[0])
         if out is not None and (out.dtype != torch.int32 or not out.is_contiguous() or out.numel() < B
@@ -266,7 +265,7 @@ class Sampler:
 
         def run(st):
             tokens = torch.empty(B, dtype=torch.int32, device=h.device) if out is None else out
-            check(_lib.lib.qs_lm_head_w4_sample(self._h, _ptr(h), _ptr(norm_weight), weight._w4_ref, B, _ptr(tokens), st,
+            check(_lib.lib.qs_lm_head_w4_sample(self._h, _ptr(h), _ptr(norm_weight), C.byref(weight._w4_desc), B, _ptr(tokens), st,
                                                 int(flags)))
             return tokens
 

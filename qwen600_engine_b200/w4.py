@@ -15,10 +15,34 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._lib import QS_BF16, QS_F16, check
-from .losses import _invalid, _on_stream
+from . import _torch
+from ._lib import QS_BF16, QS_ERR_INVALID, QS_F16, SamplerError, check
+from .losses import _on
 
 _SCALES = {torch.bfloat16: QS_BF16, torch.float16: QS_F16}
+
+
+def _invalid(msg: str) -> SamplerError:
+    return SamplerError(QS_ERR_INVALID, msg)
+
+
+def _on_stream(device, stream, inputs, run):
+    """run(stream handle) on the device and stream of one call.  Buffers made
+    by run belong to the stream that uses them, and inputs used on another
+    stream than the current one are kept until it is done with them."""
+    if device.type != "cuda":
+        raise _invalid("the tensors must be on a GPU")
+    with torch.cuda.device(device):
+        if stream is None:
+            return run(torch.cuda.current_stream().cuda_stream)
+        if stream.device != device:
+            raise _invalid(f"stream of {stream.device} for tensors on {device}")
+        if stream != torch.cuda.current_stream():
+            for t in inputs:
+                if t is not None:
+                    t.record_stream(stream)
+        with torch.cuda.stream(stream):
+            return run(stream.cuda_stream)
 
 
 class W4Weight:
@@ -31,8 +55,7 @@ class W4Weight:
         self.device = codes.device
         self._w4_desc = _lib.W4Desc(codes.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(),
                                     vocab, hidden_dim, group, scale_dtype)
-        self._w4_ref = C.byref(self._w4_desc)
-        self._row_bytes = _lib.lib.qs_lm_head_w4_workspace(1, hidden_dim)
+        self._parts = (codes, scales, zeros, vocab, hidden_dim, group, scale_dtype)
 
     @classmethod
     def pack(cls, codes, scales, zeros=None, *, stream=None) -> "W4Weight":
@@ -121,19 +144,7 @@ def lm_head_w4(hidden, weight: W4Weight, norm_weight=None, *, stream=None):
     [B, hidden_dim]; returns (normed [B, hidden_dim], logits [B, vocab]) bf16,
     as ``sampler.lm_head`` does."""
     h = _check_rows(hidden, weight, norm_weight)
-    B, dev = h.shape[0], weight.device
-
-    def run(st):
-        normed = torch.empty_like(h)
-        logits = h.new_empty((B, weight.vocab))
-        if B:
-            work = torch.empty(B * weight._row_bytes, dtype=torch.uint8, device=dev)
-            check(_lib.lib.qs_lm_head_w4(h.data_ptr(), None if norm_weight is None else norm_weight.data_ptr(),
-                                         weight._w4_ref, B, normed.data_ptr(), logits.data_ptr(), work.data_ptr(),
-                                         B * weight._row_bytes, st))
-        return normed, logits
-
-    return _on_stream(dev, stream, (h, norm_weight, weight.codes, weight.scales, weight.zeros), run)
+    return _on(stream, _torch.lm_head_w4, h, norm_weight, *weight._parts)
 
 
 __all__ = ["W4Weight", "quantize_w4", "lm_head_w4"]
