@@ -75,16 +75,17 @@ __device__ __forceinline__ f32x2 exp2_pair(f32x2 v) {
     return pair2(exp2_fast(t.x), exp2_fast(t.y));
 }
 
-// Block-wide sum of one double per thread, in a fixed order.
+// Block-wide sum of one double per thread, in a fixed order; in warp 0.
 __device__ __forceinline__ double block_sum(double v, double* red) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
-    double s = 0.0;
-    for (int w = 0; w < (int)(blockDim.x >> 5); w++) s += red[w];
-    return s;
+    if (threadIdx.x >= 32) return 0.0;
+    v = threadIdx.x < blockDim.x >> 5 ? red[threadIdx.x] : 0.0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
 }
 
 // Vectors of 16 bytes of a row, at any alignment of its first element: up to
@@ -869,7 +870,7 @@ preference_pairs_kernel(const RowScore* score, int rows, const int* __restrict__
     dependents_may_start();
     wait_for_previous();
     double sum = 0.0;
-    for (int q = warp; q < pairs; q += 32) {
+    for (int q = warp; q < pairs; q += blockDim.x >> 5) {
         const int a[2] = {offsets[q], offsets[pairs + q]}, b[2] = {offsets[q + 1], offsets[pairs + q + 1]};
         const bool fine = a[0] >= 0 && a[0] <= b[0] && b[0] <= rows && a[1] >= 0 && a[1] <= b[1] && b[1] <= rows;
         double s[2] = {NAN, NAN};
@@ -1050,11 +1051,12 @@ static int row_units(int dtype, int vocab) {
 }
 // Large calls stream; smaller ones take a cluster per row, in one launch.  Long
 // bf16 rows from 72 MB (22.0 us against 22.4 at 72 MB, 30.4 against 33.2 at
-// 120), fp32 rows and rows of less than a CTA's 40 KB from 40 MB (fp32 of
-// 151,936: 14.6 against 17.3 us at 48 MB; bf16 of 4,099: 18.5 against 24.0).
+// 120), fp32 rows and rows of less than a CTA's 40 KB from 24 MB (at 32 MB fp32
+// of 151,936: 9.7 against 12.3 us, bf16 of 4,099: 13.3 against 16.9; at 16 MB
+// 7.2 against 7.0 and 9.5 against 9.9).
 static bool streams(int dtype, int rows, int vocab) {
     const size_t row = (size_t)vocab * (dtype == QS_F32 ? 4 : 2);
-    return rows * row >= (size_t)(dtype == QS_BF16 && row >= 40 * 1024 ? 72 : 40) << 20;
+    return rows * row >= (size_t)(dtype == QS_BF16 && row >= 40 * 1024 ? 72 : 24) << 20;
 }
 static size_t score_workspace(int dtype, int rows, int vocab) {
     return streams(dtype, rows, vocab) ? round256((size_t)rows * row_units(dtype, vocab) * sizeof(float4)) : 0;
@@ -1186,7 +1188,7 @@ int qs_policy_loss(const void* d_logits, int dtype, int rows, int vocab, long lo
         const int e = dtype == QS_F32 ? go(score_args<float>(r)) : go(score_args<__nv_bfloat16>(r));
         if (e) return e;
     }
-    return launch("sum_rows_kernel", sum_rows_kernel, 1, 1024, 1, 0, rows > 0, st, row_loss, rows, d_loss);
+    return launch("sum_rows_kernel", sum_rows_kernel, 1, rows > 512 ? 1024 : 128, 1, 0, rows > 0, st, row_loss, rows, d_loss);
 }
 
 size_t qs_preference_loss_workspace(int dtype, int rows, int vocab) {
@@ -1223,7 +1225,7 @@ int qs_preference_loss(const void* d_logits, int dtype, int rows, int vocab, lon
                                       : score<__nv_bfloat16>(r, sc, coefs, nullptr, nullptr, parts, st);
         if (e) return e;
     }
-    const int e = launch("preference_pairs_kernel", preference_pairs_kernel, 1, 1024, 1, 0, rows > 0, st, sc, rows,
+    const int e = launch("preference_pairs_kernel", preference_pairs_kernel, 1, pairs > 4 ? 1024 : 128, 1, 0, rows > 0, st, sc, rows,
                          d_seq_offsets, pairs, d_ref_logprobs, d_weights, p, coefs, d_seq_logprobs, d_loss);
     if (e || rows == 0 || !d_grad) return e;
     return dtype == QS_F32 ? grad<float>(r, &sc->max, sizeof(RowScore) / 4, coefs, true, st)

@@ -202,7 +202,7 @@ def test_masked_and_special_logits(dtype):
     check(out, ref, (rel_sum(V) + 100 * U + half_step(dtype)) * ref.abs().nan_to_num(0) + 4 * U * rel_sum(V) + 1e-30, "gradient")
 
 
-# Large calls (from 40 or 72 MB of logits) take the kernels that stream many rows.
+# Large calls (from 24 or 72 MB of logits) take the kernels that stream many rows.
 MANY = [(torch.bfloat16, 250, 151936, 0, 0), (torch.bfloat16, 800, 50021, 3, 1), (torch.float32, 128, 151936, 0, 0),
         (torch.float32, 500, 37999, 1, 2), (torch.bfloat16, 38000, 1003, 0, 0), (torch.float32, 19000, 1024, 8, 0),
         (torch.bfloat16, 150, 262144, 0, 0)]
