@@ -523,10 +523,11 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
 // The maximum's own term is left out of the fp32 sum as in score_kernel: where
 // one lane holds the maximum, the warp takes that lane's 128 bytes once more,
 // two elements a lane.  (Where several do, the row's sum is at least 2, and the
-// 1 costs it less than the exponentials do.)  Warps never wait for one another, so copies keep running
-// while others compute.  1024 bf16 rows of 151,936: 61 us (52 of them this
-// kernel, 6.0 TB/s, its exponentials at 75% of the unit's rate), 78 with a
-// cluster per row.  24 warps with rings of 2 units; 16 with 3 were 16 us slower.
+// 1 costs it less than the exponentials do.)  Warps never wait for one another,
+// so copies keep running while others compute.  1024 bf16 rows of 151,936: 61 us
+// (52 of them this kernel, 6.0 TB/s, its exponentials at 75% of the unit's
+// rate), 78 with a cluster per row.  24 warps with rings of 2 units; 16 with 3
+// were 16 us slower.
 constexpr int kUnitVecs = 256;
 constexpr int kStreamWarps = 24;
 constexpr int kStreamStages = 2;
@@ -1008,7 +1009,9 @@ static int launch(const char* name, void (*kernel)(P...), long long grid, int th
     }
     cfg.attrs = attr;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
-    return e == cudaSuccess ? QS_OK : fail(QS_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+    if (e == cudaSuccess) return QS_OK;
+    cudaGetLastError();  // reported here, not by a later call
+    return fail(QS_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
 }
 
 // How a row is spread: CTAs per row (a power of two up to 8) such that a share
