@@ -299,9 +299,11 @@ QS_API int qs_ipc_free(void* d_ptr);
 /* qs_lm_head into the handle's workspace followed by qs_sample on the
  * resulting bf16 logits: the reference's forward() tail plus sample()
  * (main.cu:138-139) for a batch, without the fp32 widening and the host copy
- * of qwen_model.cuh:717-723.  The first call (and a call with a new
+ * of qwen_model.cuh:717-723.  The first call (and a call with a larger
  * hidden_dim) allocates the workspace: max_batch x (hidden_dim + vocab) bf16,
  * plus min(max_batch, 255) x ceil(vocab / 256) words for the segment maxima.
+ * Buffers that a larger hidden_dim replaces stay until the handle is destroyed,
+ * so graphs captured before remain valid.
  * For batches below 256 the lm_head epilogue folds each row's maxima of its
  * 256-column segments into that buffer, and the sampler then reads only the
  * segments that hold window tokens from the logits instead of streaming them
@@ -375,8 +377,8 @@ QS_API int qs_lm_head_w4(const void* d_hidden, const void* d_norm_weight, const 
                          size_t workspace_bytes, void* stream);
 
 /* qs_lm_head_sample with such a weight (weight->vocab must be the handle's):
- * qs_lm_head_w4 into the handle's workspace (a first call, and one with a new
- * hidden_dim, allocates it), then qs_sample on its logits. */
+ * qs_lm_head_w4 into the handle's workspace (a first call, and one with a
+ * larger hidden_dim, allocates it), then qs_sample on its logits. */
 QS_API int qs_lm_head_w4_sample(qs_sampler* s, const void* d_hidden, const void* d_norm_weight,
                                 const qs_w4_weight* weight, int batch, int* d_tokens, void* stream,
                                 unsigned flags);

@@ -148,14 +148,15 @@ struct qs_sampler {
     uint32_t* exp_bloom = nullptr;
     // lm_head tail (allocated by the first qs_lm_head_sample call)
     int num_sms = 148;
-    int lh_dim = 0;
-    __nv_bfloat16* lh_normed = nullptr;  // [max_batch, lh_dim]
+    void* lh_normed = nullptr;           // bf16 [max_batch, largest hidden size so far]
+    size_t lh_normed_bytes = 0;
     __nv_bfloat16* lh_logits = nullptr;  // [max_batch, vocab]
     int* lh_err = nullptr;
     uint32_t* lh_segk = nullptr;  // [max_batch, lh_segs]: the epilogue's segment maxima (order keys)
     int lh_segs = 0;
     void* lh_w4 = nullptr;  // the rows of a 4-bit projection (allocated by the first qs_lm_head_w4_sample call)
     size_t lh_w4_bytes = 0;
+    std::vector<void*> lh_outgrown;  // replaced by larger ones; captured graphs may use them still
     ExpFix fix() const { return ExpFix{exp_off, exp_ent, exp_bloom, (uint32_t)QS_EXP_NB}; }
     // the row kernel's hand-over from a row's chunk scans to its finishing CTA
     float* rs_segm = nullptr;
@@ -243,6 +244,7 @@ static void release(qs_sampler* s) {
                     s->rs_gmax, s->rs_stash, s->rs_used, s->rs_chunk, s->rs_chunk_lb, s->rs_fb, s->st_hist, s->st_counts, s->st_count, s->st_rng, s->ph_row, s->ph_sel};
     for (void* p : ptrs)
         if (p) cudaFree(p);
+    for (void* p : s->lh_outgrown) cudaFree(p);
     for (auto& t : s->pending) { cudaEventDestroy(t.a); cudaEventDestroy(t.b); }
     for (auto e : s->event_pool) cudaEventDestroy(e);
     if (s->stream) cudaStreamDestroy(s->stream);
@@ -978,20 +980,33 @@ int qs_shard_handshake(void* const* d_bufs, int nranks, int rank, size_t flag_of
     return QS_OK;
 }
 
+// Makes one of the tail's buffers at least `need` bytes.  A smaller one is kept
+// until the handle is destroyed: a captured graph may use it still.
+static int tail_buffer(qs_sampler* s, void** p, size_t* bytes, size_t need) {
+    if (*bytes >= need) return QS_OK;
+    try {
+        s->lh_outgrown.reserve(s->lh_outgrown.size() + 1);
+    } catch (const std::bad_alloc&) {
+        return fail(QS_ERR_ALLOC, "out of host memory");
+    }
+    void* grown = nullptr;
+    CK(cudaMalloc(&grown, need));
+    if (*p) s->lh_outgrown.push_back(*p);
+    *p = grown;
+    *bytes = need;
+    return QS_OK;
+}
+
 // The decode tail's workspace in the handle, allocated on first use (and for a
-// new hidden size).
+// larger hidden size).
 static int tail_workspace(qs_sampler* s, int hidden_dim) {
-    if (s->lh_dim != hidden_dim) {
-        // first use (or a new hidden size): the tail's workspace
-        if (s->lh_normed) cudaFree(s->lh_normed);
-        if (s->lh_logits) cudaFree(s->lh_logits);
-        if (s->lh_err) cudaFree(s->lh_err);
-        s->lh_normed = nullptr; s->lh_logits = nullptr; s->lh_err = nullptr; s->lh_dim = 0;
-        CK(cudaMalloc(&s->lh_normed, sizeof(__nv_bfloat16) * (size_t)s->max_batch * hidden_dim));
-        CK(cudaMalloc(&s->lh_logits, sizeof(__nv_bfloat16) * (size_t)s->max_batch * s->vocab));
+    const int rc = tail_buffer(s, &s->lh_normed, &s->lh_normed_bytes,
+                               sizeof(__nv_bfloat16) * (size_t)s->max_batch * hidden_dim);
+    if (rc) return rc;
+    if (!s->lh_logits) CK(cudaMalloc(&s->lh_logits, sizeof(__nv_bfloat16) * (size_t)s->max_batch * s->vocab));
+    if (!s->lh_err) {
         CK(cudaMalloc(&s->lh_err, sizeof(int)));
         CK(cudaMemset(s->lh_err, 0, sizeof(int)));
-        s->lh_dim = hidden_dim;
     }
     if (!s->lh_segk) {
         s->lh_segs = (s->vocab + 255) / 256;
@@ -1016,7 +1031,7 @@ int qs_lm_head_sample(qs_sampler* s, const void* d_hidden, const void* d_norm_we
     // batches below kWideMinRows: the epilogue forms the segment maxima and
     // the sampler's scan reads only the window's segments from the logits
     uint32_t* segk = batch < kWideMinRows ? s->lh_segk : nullptr;
-    rc = lm_head_launch(d_hidden, d_norm_weight, d_weight, batch, hidden_dim, s->vocab, s->lh_normed,
+    rc = lm_head_launch(d_hidden, d_norm_weight, d_weight, batch, hidden_dim, s->vocab, (__nv_bfloat16*)s->lh_normed,
                         s->lh_logits, s->lh_err, s->num_sms, (cudaStream_t)stream, segk, s->lh_segs);
     if (rc) return rc;
     rc = sample_stateful(s, s->lh_logits, QS_BF16, batch, d_tokens, stream, flags, segk, s->lh_segs);
@@ -1147,16 +1162,11 @@ int qs_lm_head_w4_sample(qs_sampler* s, const void* d_hidden, const void* d_norm
     DeviceGuard dg(s->device);
     rc = tail_workspace(s, weight->hidden_dim);
     if (rc) return rc;
-    const size_t need = qs_lm_head_w4_workspace(s->max_batch, weight->hidden_dim);
-    if (s->lh_w4_bytes < need) {
-        if (s->lh_w4) cudaFree(s->lh_w4);
-        s->lh_w4 = nullptr; s->lh_w4_bytes = 0;
-        CK(cudaMalloc(&s->lh_w4, need));
-        s->lh_w4_bytes = need;
-    }
+    rc = tail_buffer(s, &s->lh_w4, &s->lh_w4_bytes, qs_lm_head_w4_workspace(s->max_batch, weight->hidden_dim));
+    if (rc) return rc;
     // the epilogue hands the sampler the segment maxima, as in qs_lm_head_sample
     uint32_t* segk = batch < kWideMinRows ? s->lh_segk : nullptr;
-    rc = w4_launch(d_hidden, d_norm_weight, weight, batch, s->lh_normed, s->lh_logits, s->lh_w4, s->num_sms,
+    rc = w4_launch(d_hidden, d_norm_weight, weight, batch, (__nv_bfloat16*)s->lh_normed, s->lh_logits, s->lh_w4, s->num_sms,
                    (cudaStream_t)stream, segk, s->lh_segs);
     if (rc) return rc;
     rc = sample_stateful(s, s->lh_logits, QS_BF16, batch, d_tokens, stream, flags, segk, s->lh_segs);

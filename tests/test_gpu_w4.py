@@ -322,3 +322,37 @@ def test_rollout_and_learning_step():
     sl = torch.log_softmax(y, 1).gather(1, tok.long()[:, None])[:, 0].view(B, steps).sum(1) - seq_ref.double()
     (-torch.nn.functional.logsigmoid(0.2 * (sl[:3] - sl[3:]))).mean().backward()
     assert ((p.grad.double() - y.grad).abs() <= 2.0 ** -8 * y.grad.abs() + 1e-6).all()
+
+
+def test_captured_sampling_outlives_a_larger_hidden_size():
+    # the handle's buffers grow in between; the graph keeps the ones it was captured with
+    from qwen600_engine_b200.sampler import Sampler
+    from qwen600_engine_b200.w4 import W4Weight
+    codes, scales, z, g = plain_weight(2003, 256, 64, True, torch.bfloat16, seed=21)
+    small = W4Weight.pack(codes, scales, z)
+    large = W4Weight.pack(*plain_weight(2003, 1024, 128, False, torch.float16, seed=22)[:3])
+    a, b = (Sampler(0.8, 0.9, 0.0, 10, 1.1, 0.0, 0.0, 16, 3, max_batch=3, vocab=2003) for _ in range(2))
+    h, nw = inputs(g, 3, 256)
+    hl, nl = inputs(g, 3, 1024)
+    want = [a.lm_head_sample(x, w, n) for x, w, n in
+            [(h, small, nw), (h, small, nw), (hl, large, nl), (h, small, nw), (hl, large, nl)]]
+    got = [b.lm_head_sample(h, small, nw)]
+    out = torch.empty(3, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.lm_head_sample(h, small, nw, out=out)
+    logits = b.lm_head_logits(3).data_ptr()
+    for x in (None, (hl, large, nl), None, (hl, large, nl)):
+        if x is None:
+            graph.replay()
+            got.append(out.clone())
+        else:
+            got.append(b.lm_head_sample(*x))
+    torch.cuda.synchronize()
+    assert b.lm_head_logits(3).data_ptr() == logits
+    for i, j in zip(got, want):
+        assert torch.equal(i, j)
+    graph.reset()
+    a.free()
+    b.free()
