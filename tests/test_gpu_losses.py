@@ -661,3 +661,72 @@ def test_refused_on_the_gpu():
         L().token_logprobs(x, tok.cpu())
     with pytest.raises(SamplerError, match="vocab"):
         L().token_logprobs(torch.zeros((1, 300000), device="cuda"), tok[:1])
+
+
+# Finite masks: numbers so low that a logit next to them has no weight, and rows that hold nothing else.  The tolerances
+# are those above: a row's terms are taken against its maximum, however far from zero that lies.
+MASKS = [-1e7, -2e7, -1e9, -1e10, -1e20, -1e30, None]  # None: the type's lowest value
+
+
+def masked_rows(N, V, dtype, seed):
+    """Ordinary rows with masked stretches, with few tokens left, with nothing but the mask, with the mask beside -inf or
+    beside the type's lowest value, with the mask added to the logits, and far above zero; and a token that is not below
+    the row's other values by more than ordinary logits are."""
+    x, tok, g = rows_of(N, V, dtype, seed)
+    low = torch.finfo(dtype).min
+    col = torch.arange(V, device="cuda")
+    for i in range(N):
+        mask = MASKS[i // 7 % len(MASKS)]
+        mask = low if mask is None else mask
+        t = int(tok[i])
+        ends = torch.full_like(x[i], mask)
+        if i % 7 == 0:    # the middle half
+            ends[: V // 4], ends[V - V // 4:] = x[i, : V // 4], x[i, V - V // 4:]
+        elif i % 7 == 1:  # a dozen tokens left
+            ends[torch.randint(0, V, (12,), generator=g, device="cuda")] = 1.5
+        elif i % 7 == 3:  # mask and -inf in turn, in stretches
+            ends[col // 300 % 2 == 1] = -math.inf
+        elif i % 7 == 4:  # mask and the type's lowest value, token by token
+            ends[1::2] = low
+        elif i % 7 == 5:  # added to the logits, as far as the type holds the sum
+            ends = (x[i].float() + max(mask, low / 2)).to(dtype)
+        elif i % 7 == 6:
+            ends = (x[i].float() - max(mask, low / 2)).to(dtype)
+        x[i] = ends
+        if i % 7 < 2:
+            x[i, t] = 2.0
+        else:
+            tok[i] = x[i].argmax()
+    return x, tok, g
+
+
+MASKED_T = [0.6, 0.7, 1.0, 1.5, 2.0]
+
+
+def check_logprobs(r, x, tok, T):
+    V = x.shape[1]
+    for a in range(0, x.shape[0], 256):
+        b = slice(a, a + 256)
+        lp, _, excess, m, tol = exact(x[b], tok[b], T)
+        check(r.logprobs[b], lp, tol, "logprobs")
+        assert torch.equal(r.stats[b, 0].double(), m)
+        check(r.stats[b, 1], excess, (rel_sum(V) + U) * excess + 1e-30, "excess")
+
+
+@pytest.mark.parametrize("T", MASKED_T)
+@pytest.mark.parametrize("dtype,N,V", [(torch.bfloat16, 250, 151936), (torch.float32, 130, 50021), (torch.bfloat16, 3200, 4099)])
+def test_finite_masks_in_many_rows(dtype, N, V, T):
+    x, tok, _ = masked_rows(N, V, dtype, seed=V)
+    check_logprobs(L().token_logprobs(x, tok, temperature=T), x, tok, T)
+
+
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 151936), (torch.float32, 50021)])
+def test_finite_masks_in_many_rows_of_pairs(dtype, V):
+    lengths = [60, 1, 82, 44, 34, 72, 0, 98]
+    x, tok, g = masked_rows(sum(lengths) + 2, V, dtype, seed=V + 1)
+    off = torch.tensor([0] + lengths, device="cuda").cumsum(0).to(torch.int32)
+    lp = exact(x, tok)[0]
+    seq = torch.stack([lp[a:b].sum() for a, b in zip(off.tolist(), off.tolist()[1:])])
+    ref = (seq + 4 * torch.randn((8,), generator=g, device="cuda")).float()
+    r = L().preference_loss(x, tok, off, ref, beta=0.2)
+    check_preference(r, x, tok, off, ref, None, 0.2, 0.0)
