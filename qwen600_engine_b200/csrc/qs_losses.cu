@@ -378,12 +378,10 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
 
     // The sum of exponentials against it.  The maximum's own terms (exactly 1
     // each) are counted apart, by the warps that hold one; they also subtract
-    // before they scale.  The others scale and subtract in one instruction,
-    // 2^(x scale - bias), where bias = ref scale rounded makes every term
-    // 2^-slip too large; their sum is set right below.  A maximum whose
-    // multiple is not finite leaves all warps to the first way.
+    // before they scale.  The others scale and subtract in one instruction
+    // where one_step allows it.
     const float bias = ref * a.scale;
-    const bool apart = __any_sync(0xffffffffu, own_max == ref) || !(fabsf(bias) < INFINITY);
+    const bool apart = __any_sync(0xffffffffu, own_max == ref) || !one_step(bias);
     float s = 0.0f;
     int n = 0;
     if (apart) {

@@ -730,3 +730,40 @@ def test_finite_masks_in_many_rows_of_pairs(dtype, V):
     ref = (seq + 4 * torch.randn((8,), generator=g, device="cuda")).float()
     r = L().preference_loss(x, tok, off, ref, beta=0.2)
     check_preference(r, x, tok, off, ref, None, 0.2, 0.0)
+
+
+def policy_around(x, tok, g, T):
+    """Inputs of the policy loss for given logits: ratios on both sides of the clip range, none at a border."""
+    N = x.shape[0]
+    lp = exact(x, tok, T)[0]
+    step = 0.3 * torch.randn((N,), generator=g, device="cuda", dtype=torch.float64)
+    near = ((step.exp() - 0.8).abs() < 1e-3) | ((step.exp() - 1.25).abs() < 1e-3)
+    old = (lp - torch.where(near, step + 0.01, step)).float()
+    ref = (lp + 0.3 * torch.randn((N,), generator=g, device="cuda")).float()
+    return x, tok, old, ref, torch.randn((N,), generator=g, device="cuda"), torch.rand((N,), generator=g, device="cuda") / N
+
+
+@pytest.mark.parametrize("T", MASKED_T)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,V", [(49, 257), (49, 5003), (49, 50021), (21, 151936)])
+def test_finite_masks_in_few_rows(dtype, N, V, T):
+    x, tok, g = masked_rows(N, V, dtype, seed=N + V)
+    r = L().token_logprobs(x, tok, temperature=T)
+    check_logprobs(r, x, tok, T)
+    gl = torch.randn((N,), generator=g, device="cuda")
+    check_grad(L().token_logprobs_backward(x, tok, r.stats, gl, temperature=T), *grad_of(x, tok, gl, T))
+    case = policy_around(x, tok, g, T)
+    alone = L().policy_loss(x, tok, case[2], case[4], ref_logprobs=case[3], weights=case[5], clip_low=0.2, clip_high=0.25,
+                            kl_coef=0.1, temperature=T, grad=False)
+    check_policy(alone, case, 0.2, 0.25, 0.1, T)
+
+
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 5003), (torch.float32, 257)])
+def test_finite_masks_in_few_rows_of_pairs(dtype, V):
+    lengths = [9, 1, 8, 7, 12, 7, 0, 4]
+    x, tok, g = masked_rows(sum(lengths) + 2, V, dtype, seed=V + 1)
+    off = torch.tensor([0] + lengths, device="cuda").cumsum(0).to(torch.int32)
+    lp = exact(x, tok)[0]
+    seq = torch.stack([lp[a:b].sum() for a, b in zip(off.tolist(), off.tolist()[1:])])
+    ref = (seq + 4 * torch.randn((8,), generator=g, device="cuda")).float()
+    check_preference(L().preference_loss(x, tok, off, ref, beta=0.2), x, tok, off, ref, None, 0.2, 0.0)
