@@ -480,7 +480,7 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
     __syncthreads();
     float f = factor_s;
     const float M = max_s, top = M * a.scale;
-    const bool plain = fabsf(top) < INFINITY;
+    const bool plain = one_step(top);
     if (plain) f *= exp2_fast(-__fmaf_rn(M, a.scale, -top));
     const auto grad_of = [&](float v) {
         return f == 0.0f ? 0.0f : f * exp2_fast(plain ? __fmaf_rn(v, a.scale, -top) : (v - M) * a.scale);

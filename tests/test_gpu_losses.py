@@ -767,3 +767,14 @@ def test_finite_masks_in_few_rows_of_pairs(dtype, V):
     seq = torch.stack([lp[a:b].sum() for a, b in zip(off.tolist(), off.tolist()[1:])])
     ref = (seq + 4 * torch.randn((8,), generator=g, device="cuda")).float()
     check_preference(L().preference_loss(x, tok, off, ref, beta=0.2), x, tok, off, ref, None, 0.2, 0.0)
+
+
+@pytest.mark.parametrize("T", MASKED_T)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,V", [(49, 257), (49, 5003), (49, 50021), (21, 151936)])
+def test_finite_masks_in_the_policy_gradient(dtype, N, V, T):
+    x, tok, g = masked_rows(N, V, dtype, seed=N + V + 1)
+    case = policy_around(x, tok, g, T)
+    r = L().policy_loss(x, tok, case[2], case[4], ref_logprobs=case[3], weights=case[5], clip_low=0.2, clip_high=0.25,
+                        kl_coef=0.1, temperature=T)
+    check_policy(r, case, 0.2, 0.25, 0.1, T)
