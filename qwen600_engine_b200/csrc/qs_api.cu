@@ -997,6 +997,22 @@ static int tail_buffer(qs_sampler* s, void** p, size_t* bytes, size_t need) {
     return QS_OK;
 }
 
+// Allocates one of the tail's buffers that start at zero.  The clear has run
+// when this returns: the caller's stream need not be ordered with any other (a
+// clear on the default stream could come after the call's own kernels).
+static int tail_zeroed(qs_sampler* s, void** p, size_t bytes) {
+    void* made = nullptr;
+    CK(cudaMalloc(&made, bytes));
+    cudaError_t e = cudaMemsetAsync(made, 0, bytes, s->stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s->stream);
+    if (e != cudaSuccess) {
+        cudaFree(made);
+        return fail(QS_ERR_CUDA, "clearing the tail's buffers: %s", cudaGetErrorString(e));
+    }
+    *p = made;
+    return QS_OK;
+}
+
 // The decode tail's workspace in the handle, allocated on first use (and for a
 // larger hidden size).
 static int tail_workspace(qs_sampler* s, int hidden_dim) {
@@ -1005,14 +1021,14 @@ static int tail_workspace(qs_sampler* s, int hidden_dim) {
     if (rc) return rc;
     if (!s->lh_logits) CK(cudaMalloc(&s->lh_logits, sizeof(__nv_bfloat16) * (size_t)s->max_batch * s->vocab));
     if (!s->lh_err) {
-        CK(cudaMalloc(&s->lh_err, sizeof(int)));
-        CK(cudaMemset(s->lh_err, 0, sizeof(int)));
+        const int bad = tail_zeroed(s, (void**)&s->lh_err, sizeof(int));
+        if (bad) return bad;
     }
     if (!s->lh_segk) {
         s->lh_segs = (s->vocab + 255) / 256;
         const size_t n = (size_t)(s->max_batch < kWideMinRows ? s->max_batch : kWideMinRows - 1) * s->lh_segs;
-        CK(cudaMalloc(&s->lh_segk, sizeof(uint32_t) * n));
-        CK(cudaMemset(s->lh_segk, 0, sizeof(uint32_t) * n));
+        const int bad = tail_zeroed(s, (void**)&s->lh_segk, sizeof(uint32_t) * n);
+        if (bad) return bad;
     }
     return QS_OK;
 }

@@ -356,3 +356,31 @@ def test_captured_sampling_outlives_a_larger_hidden_size():
     graph.reset()
     a.free()
     b.free()
+
+
+@pytest.mark.parametrize("four_bits", [True, False])
+def test_first_call_on_a_stream_beside_a_busy_default_stream(four_bits):
+    """A handle's first call makes and clears its buffers; work queued on another stream must not delay the clear."""
+    from qwen600_engine_b200.sampler import Sampler
+    from qwen600_engine_b200.w4 import W4Weight
+    V, K, B = 50021, 1024, 4
+    codes, scales, z, g = plain_weight(V, K, 64, True, torch.bfloat16, seed=41)
+    w = W4Weight.pack(codes, scales, z) if four_bits else (0.02 * torch.randn((V, K), generator=g, device="cuda")).to(torch.bfloat16)
+    h, nw = inputs(g, B, K)
+    a = torch.empty(1 << 30, dtype=torch.uint8, device="cuda")
+    b = torch.empty_like(a)
+    for trial in range(4):
+        first, second = (Sampler(0.8, 0.9, 0.0, 20, 1.1, 0.0, 0.0, 16, 3 + trial, max_batch=B, vocab=V) for _ in range(2))
+        want = [first.lm_head_sample(h, w, nw).clone() for _ in range(3)]
+        side = torch.cuda.Stream()
+        out = [torch.empty(B, dtype=torch.int32, device="cuda") for _ in range(3)]
+        torch.cuda.synchronize()
+        for _ in range(60):  # some 20 ms
+            b.copy_(a)
+        for o in out:
+            second.lm_head_sample(h, w, nw, out=o, stream=side)
+        torch.cuda.synchronize()
+        for i, (o, t) in enumerate(zip(out, want)):
+            assert torch.equal(o, t), f"trial {trial}, step {i}"
+        first.free()
+        second.free()
