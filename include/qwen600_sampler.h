@@ -456,8 +456,9 @@ QS_API int qs_policy_loss(const void* d_logits, int dtype, int rows, int vocab, 
  *   z = beta ((S[p] - ref[p]) - (S[pairs + p] - ref[pairs + p]))
  *   loss = sum_p w[p] (-(1 - label_smoothing) log sigmoid(z) - label_smoothing log sigmoid(-z))
  * w = d_weights[p] (NULL: 1 / pairs); a pair with w[p] = 0 adds nothing.  Rows
- * in no sequence have a zero gradient.  A pair whose offsets fall, or leave
- * [0, rows], has a NaN loss and touches no row.  d_loss fp32 [1], d_seq_logprobs fp32 [2 pairs] (S) or NULL, d_grad
+ * in no sequence have a zero gradient.  A pair with an offset outside [0, rows]
+ * has a NaN loss and touches no row; offsets that fall anywhere make every pair
+ * such a one.  d_loss fp32 [1], d_seq_logprobs fp32 [2 pairs] (S) or NULL, d_grad
  * NULL for the loss alone.  beta > 0, 0 <= label_smoothing < 0.5. */
 typedef struct {
     double beta;

@@ -866,7 +866,9 @@ sum_rows_kernel(const double* row_loss, int rows, float* __restrict__ loss) {
 }
 
 // One warp per pair in turn: the two sequences' sums, the pair's loss and the
-// coefficients of their rows' gradients (0 so far).
+// coefficients of their rows' gradients (0 so far).  Sequences share no row
+// unless an offset falls somewhere: then none counts, so that no two warps write
+// a row's coefficient.
 __global__ void __launch_bounds__(1024)
 preference_pairs_kernel(const RowScore* score, int rows, const int* __restrict__ offsets, int pairs,
                         const float* __restrict__ ref, const float* __restrict__ weights,
@@ -875,11 +877,14 @@ preference_pairs_kernel(const RowScore* score, int rows, const int* __restrict__
     __shared__ double red[32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     dependents_may_start();
+    int falls = 0;  // looked for while the rows are scored
+    for (int q = threadIdx.x; q < 2 * pairs; q += blockDim.x) falls |= offsets[q] > offsets[q + 1];
+    const bool ordered = !__syncthreads_or(falls);
     wait_for_previous();
     double sum = 0.0;
     for (int q = warp; q < pairs; q += blockDim.x >> 5) {
         const int a[2] = {offsets[q], offsets[pairs + q]}, b[2] = {offsets[q + 1], offsets[pairs + q + 1]};
-        const bool fine = a[0] >= 0 && a[0] <= b[0] && b[0] <= rows && a[1] >= 0 && a[1] <= b[1] && b[1] <= rows;
+        const bool fine = ordered && a[0] >= 0 && b[0] <= rows && a[1] >= 0 && b[1] <= rows;
         double s[2] = {NAN, NAN};
         if (fine) {
             s[0] = s[1] = 0.0;

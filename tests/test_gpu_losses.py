@@ -778,3 +778,20 @@ def test_finite_masks_in_the_policy_gradient(dtype, N, V, T):
     r = L().policy_loss(x, tok, case[2], case[4], ref_logprobs=case[3], weights=case[5], clip_low=0.2, clip_high=0.25,
                         kl_coef=0.1, temperature=T)
     check_policy(r, case, 0.2, 0.25, 0.1, T)
+
+
+@pytest.mark.parametrize("P,spoil", [(2, {1: 6, 2: 3}), (2, {4: 2}), (40, {80: 100}), (40, {41: 70})])
+def test_preference_offsets_that_fall_anywhere(P, spoil):
+    """Sequences could share rows then: every pair's sums are NaN and no row has a gradient, also where the pair beside the
+    fall has no weight."""
+    x, tok, off, ref, w = pairs_case(P, 301, torch.float32, seed=14, lengths=[3] * (2 * P))
+    r = L().preference_loss(x, tok, off, ref, weights=w)
+    assert math.isfinite(float(r.loss)) and (r.grad != 0).any()
+    for i, v in spoil.items():
+        off[i] = v
+    for q in range(2 * P):
+        if off[q] > off[q + 1]:
+            w[q % P] = 0.0
+    r = L().preference_loss(x, tok, off, ref, weights=w)
+    assert math.isnan(float(r.loss)) and torch.isnan(r.seq_logprobs).all()
+    assert (r.grad == 0).all()
