@@ -142,8 +142,11 @@ struct Gradient {
         ptr = made.data_ptr();
         ld = logits.size(1);
     }
-    PyObject* object() {  // a new reference
+    PyObject* object() {  // a new reference, after the call
         if (given) {
+            // autograd may hold the buffer (the logits themselves) for a backward: that has to fail now
+            const at::Tensor& t = THPVariable_Unpack(given);
+            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
             Py_INCREF(given);
             return given;
         }

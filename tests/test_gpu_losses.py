@@ -795,3 +795,28 @@ def test_preference_offsets_that_fall_anywhere(P, spoil):
     r = L().preference_loss(x, tok, off, ref, weights=w)
     assert math.isnan(float(r.loss)) and torch.isnan(r.seq_logprobs).all()
     assert (r.grad == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_gradient_in_place_is_seen_by_autograd(dtype):
+    """Logits that autograd keeps for its backward and that a gradient replaced are reported, not used."""
+    x, tok, old, _, adv, w = policy_case(5, 700, dtype, seed=95)
+    off = torch.tensor([0, 3, 5], dtype=torch.int32, device="cuda")
+    stats = L().token_logprobs(x, tok).stats
+    calls = [lambda y: L().policy_loss(y, tok, old, adv, weights=w, out=y),
+             lambda y: L().token_logprobs_backward(y, tok, stats, adv, out=y),
+             lambda y: L().preference_loss(y, tok, off, adv[:2], out=y)]
+    for call in calls:
+        leaf = x.clone().requires_grad_(True)
+        y = leaf * 1.0
+        kept = (y * y).sum()
+        call(y)
+        with pytest.raises(RuntimeError, match="inplace"):
+            kept.backward()
+        with torch.inference_mode():
+            z = x.clone()
+        call(z)  # tensors without a version
+        y = x.clone()
+        before = y._version
+        L().policy_loss(y, tok, old, adv, weights=w)
+        assert y._version == before  # only read
