@@ -77,23 +77,25 @@ using namespace qs;
 
 static thread_local std::string g_err;
 
+namespace qs {
+// Reports a failed call through qs_last_error, for this file and the others.
+// What the CUDA runtime keeps of the failure is dropped: the check behind the
+// next call's first launch would take it for its own.
+int set_error(int code, const char* msg) {
+    if (code == QS_ERR_CUDA || code == QS_ERR_ALLOC) cudaGetLastError();
+    g_err = msg;
+    return code;
+}
+}  // namespace qs
+
 static int fail(int code, const char* fmt, ...) {
     char buf[512];
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(buf, sizeof(buf), fmt, ap);
     va_end(ap);
-    g_err = buf;
-    return code;
+    return set_error(code, buf);
 }
-
-namespace qs {
-// Lets the other files' entry points report through qs_last_error.
-int set_error(int code, const char* msg) {
-    g_err = msg;
-    return code;
-}
-}  // namespace qs
 
 #define CK(call)                                                                        \
     do {                                                                                \

@@ -1021,7 +1021,6 @@ static int launch(const char* name, void (*kernel)(P...), long long grid, int th
     cfg.attrs = attr;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
     if (e == cudaSuccess) return QS_OK;
-    cudaGetLastError();  // reported here, not by a later call
     return fail(QS_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
 }
 

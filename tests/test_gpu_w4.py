@@ -384,3 +384,35 @@ def test_first_call_on_a_stream_beside_a_busy_default_stream(four_bits):
             assert torch.equal(o, t), f"trial {trial}, step {i}"
         first.free()
         second.free()
+
+
+def test_a_failed_call_leaves_no_error_for_the_next():
+    """Allocations that the device refuses (more than it has), then ordinary calls."""
+    import ctypes as C
+    from qwen600_engine_b200 import _lib
+    from qwen600_engine_b200._lib import SamplerError
+    from qwen600_engine_b200.sampler import Sampler, lm_head
+    from qwen600_engine_b200.w4 import W4Weight, lm_head_w4
+    codes, scales, z, g = plain_weight(1003, 256, 64, True, torch.bfloat16, seed=51)
+    w = W4Weight.pack(codes, scales, z)
+    h, nw = inputs(g, 2, 256)
+    want = lm_head_w4(h, w, nw)
+
+    def refused_bytes():
+        p, handle = C.c_void_p(), C.create_string_buffer(64)
+        assert _lib.lib.qs_ipc_alloc(1 << 45, C.byref(p), handle) < 0 and p.value is None
+
+    def refused_handle():
+        with pytest.raises(SamplerError):
+            Sampler(max_batch=1 << 30, vocab=151936)
+
+    s = Sampler(0.0, 1.0, 0.0, 0, 1.0, 0.0, 0.0, 0, 3, max_batch=2, vocab=1003)
+    for refused in (refused_bytes, refused_handle):
+        for call in (lambda: lm_head_w4(h, w, nw), lambda: W4Weight.pack(codes, scales, z),
+                     lambda: lm_head(h, torch.zeros((8, 256), dtype=torch.bfloat16, device="cuda"), nw),
+                     lambda: s.lm_head_sample(h, w, nw), lambda: s.sample(want[1])):
+            refused()
+            assert _lib.lib.qs_last_error()
+            call()
+    assert torch.equal(lm_head_w4(h, w, nw)[1], want[1])
+    s.free()
