@@ -47,9 +47,22 @@ def _on_stream(device, stream, inputs, run):
 
 class W4Weight:
     """A packed weight [vocab, hidden_dim] on one GPU: 4-bit codes, a scale and
-    a zero point for each ``group`` columns of a row."""
+    a zero point for each ``group`` columns of a row.  The constructor takes
+    buffers that ``pack`` laid out (another weight's ``codes``, ``scales`` and
+    ``zeros``)."""
 
     def __init__(self, codes, scales, zeros, vocab: int, hidden_dim: int, group: int, scale_dtype: int):
+        L = _lib.lib
+        if hidden_dim % 64 or group not in (32, 64, 128) or hidden_dim % group or scale_dtype not in _SCALES.values():
+            raise _invalid(f"hidden_dim {hidden_dim}, group {group} or scale dtype {scale_dtype} outside the library's limits")
+        for name, t, size in (("codes", codes, L.qs_w4_codes_bytes(vocab, hidden_dim)),
+                              ("scales", scales, L.qs_w4_scales_bytes(vocab, hidden_dim, group)),
+                              ("zeros", zeros, L.qs_w4_zeros_bytes(vocab, hidden_dim, group))):
+            if t is None and name == "zeros":
+                continue
+            if not size or t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() != size or t.device != codes.device:
+                raise _invalid(f"{name} must be {size} contiguous bytes on {codes.device} for [{vocab}, {hidden_dim}] in groups "
+                               f"of {group}, got {t.dtype} {tuple(t.shape)} on {t.device}")
         self.codes, self.scales, self.zeros = codes, scales, zeros
         self.vocab, self.hidden_dim, self.group = vocab, hidden_dim, group
         self.device = codes.device

@@ -178,3 +178,31 @@ def test_package_names():
     assert q.policy_loss is losses.policy_loss and q.preference_loss is losses.preference_loss
     assert q.token_logprobs is losses.token_logprobs and q.token_logprobs_backward is losses.token_logprobs_backward
     assert q.W4Weight is w4.W4Weight and q.lm_head_w4 is w4.lm_head_w4
+
+
+def w4_parts(vocab=100, hidden=256, group=64):
+    return (torch.zeros(L.qs_w4_codes_bytes(vocab, hidden), dtype=torch.uint8),
+            torch.zeros(L.qs_w4_scales_bytes(vocab, hidden, group), dtype=torch.uint8),
+            torch.zeros(L.qs_w4_zeros_bytes(vocab, hidden, group), dtype=torch.uint8))
+
+
+def test_w4_weight_of_packed_buffers():
+    codes, scales, zeros = w4_parts()
+    w = w4.W4Weight(codes, scales, zeros, 100, 256, 64, QS_F16)
+    assert (w.vocab, w.hidden_dim, w.group) == (100, 256, 64)
+    assert w4.W4Weight(codes, scales, None, 100, 256, 64, QS_BF16).zeros is None
+
+
+@pytest.mark.parametrize("bad", [
+    dict(codes=w4_parts()[0][1:]), dict(codes=w4_parts()[0][:-1]), dict(codes=w4_parts()[0].view(torch.int8)),
+    dict(codes=torch.zeros(2 * w4_parts()[0].numel(), dtype=torch.uint8)[::2]), dict(scales=w4_parts()[1][:-2]),
+    dict(scales=w4_parts()[1].view(torch.float16)), dict(zeros=w4_parts()[2][:-1]), dict(zeros=w4_parts()[1]),
+    dict(scales=w4_parts()[1].to("meta")), dict(vocab=101 + 32), dict(vocab=0), dict(vocab=-1), dict(vocab=1 << 20),
+    dict(hidden_dim=512), dict(hidden_dim=0), dict(hidden_dim=200), dict(group=32), dict(group=48), dict(group=0),
+    dict(scale_dtype=QS_F32), dict(scale_dtype=9)])
+def test_w4_weight_of_other_buffers_refused(bad):
+    """Sizes that do not fit the shape would be read out of range."""
+    codes, scales, zeros = w4_parts()
+    kw = dict(codes=codes, scales=scales, zeros=zeros, vocab=100, hidden_dim=256, group=64, scale_dtype=QS_F16) | bad
+    with pytest.raises(SamplerError):
+        w4.W4Weight(**kw)
