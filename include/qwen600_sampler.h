@@ -336,7 +336,8 @@ QS_API int qs_lm_head_set_wait_limit(unsigned long long ns);
  * zero points uint8 [vocab, hidden_dim / group], or none (all 8).
  * qs_w4_quantize makes one from a bf16 weight [vocab, hidden_dim]: per group
  * scale = bf16(range / 15) over the range that holds the group and zero,
- * codes rounded to nearest.  qs_w4_pack lays a plain weight out in the order
+ * codes rounded to nearest; a group with a NaN or an infinity gives NaN
+ * products.  qs_w4_pack lays a plain weight out in the order
  * the kernel reads, into buffers of qs_w4_codes_bytes, qs_w4_scales_bytes and
  * qs_w4_zeros_bytes bytes (16-byte aligned); the plain buffers are not needed
  * after it.  vocab <= qs_max_vocab(); hidden_dim a multiple of 64 up to 8192;

@@ -32,7 +32,8 @@
 namespace qs {
 
 // One thread per group of a row: the range that holds the group and zero, a
-// bf16 scale of a fifteenth of it, codes rounded to nearest.
+// bf16 scale of a fifteenth of it, codes rounded to nearest.  A NaN makes the
+// scale NaN, an infinity infinite: either way the group's products are NaN.
 __global__ void w4_quantize_kernel(const __nv_bfloat16* __restrict__ w, int V, int K, int group,
                                    unsigned char* __restrict__ codes, __nv_bfloat16* __restrict__ scales,
                                    unsigned char* __restrict__ zeros) {
@@ -41,12 +42,14 @@ __global__ void w4_quantize_kernel(const __nv_bfloat16* __restrict__ w, int V, i
     if (g >= (size_t)V * per) return;
     const __nv_bfloat16* x = w + g * group;
     float lo = 0.0f, hi = 0.0f;
+    bool number = true;
     for (int i = 0; i < group; i++) {
         const float v = __bfloat162float(x[i]);
-        lo = fminf(lo, v);
+        number &= v == v;
+        lo = fminf(lo, v);  // passes over a NaN
         hi = fmaxf(hi, v);
     }
-    const __nv_bfloat16 sb = __float2bfloat16_rn((hi - lo) / 15.0f);
+    const __nv_bfloat16 sb = __float2bfloat16_rn(number ? (hi - lo) / 15.0f : NAN);
     const float s = __bfloat162float(sb);
     const float d = s > 0.0f ? s : 1.0f;  // a group of zeros: scale 0, codes 0
     const float z = fminf(fmaxf(rintf(-lo / d), 0.0f), 15.0f);

@@ -416,3 +416,25 @@ def test_a_failed_call_leaves_no_error_for_the_next():
             call()
     assert torch.equal(lm_head_w4(h, w, nw)[1], want[1])
     s.free()
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_quantize_keeps_what_is_not_a_number(group):
+    """A NaN or an infinity in a weight shows in its own rows' logits, and in no others."""
+    from qwen600_engine_b200.w4 import W4Weight, lm_head_w4, quantize_w4
+    g = torch.Generator(device="cuda")
+    g.manual_seed(61)
+    V, K = 300, 256
+    wt = (0.02 * torch.randn((V, K), generator=g, device="cuda")).to(torch.bfloat16)
+    h, nw = inputs(g, 3, K)
+    want = lm_head_w4(h, W4Weight.quantize(wt, group), nw)[1]
+    spoiled = {3: float("nan"), 40: float("inf"), 77: -float("inf"), 299: float("nan")}
+    for r, v in spoiled.items():
+        wt[r, (37 * r) % K] = v
+    wt[120, :] = float("nan")
+    codes, scales, z = quantize_w4(wt, group)
+    assert int((~torch.isfinite(scales)).sum()) == 4 + K // group
+    got = lm_head_w4(h, W4Weight.pack(codes, scales, z), nw)[1]
+    bad = torch.zeros(V, dtype=torch.bool, device="cuda")
+    bad[list(spoiled) + [120]] = True
+    assert torch.isnan(got[:, bad]).all() and torch.equal(got[:, ~bad], want[:, ~bad])
