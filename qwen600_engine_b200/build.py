@@ -105,16 +105,25 @@ def build(verbose: bool = False, ptxas_info: bool = False, force: bool = False) 
 
 
 BINDING = os.path.join(HERE, "_torch.so")
+BINDING_MADE_FOR = os.path.join(OUT_DIR, "torch_binding_made_for")  # the torch and Python of the binding there is
 
 
 def build_binding(verbose: bool = False, force: bool = False) -> str:
     """_torch.so: the scoring, loss and 4-bit lm_head calls for torch tensors
-    (csrc/qs_torch.cpp), linked to the sampler library and torch's own."""
+    (csrc/qs_torch.cpp), linked to the sampler library and torch's own; made
+    anew for another torch or Python, whose ABI it would not fit."""
     src = os.path.join(CSRC, "qs_torch.cpp")
     deps = [src, os.path.join(ROOT, "include", "qwen600_sampler.h"), __file__]
-    if not force and not _stale(BINDING, deps):
-        return BINDING
+    import importlib.metadata
     import sysconfig
+    made_for = f"torch {importlib.metadata.version('torch')}, {sysconfig.get_config_var('SOABI')}"
+    try:
+        with open(BINDING_MADE_FOR) as f:
+            same = f.read() == made_for
+    except OSError:
+        same = False
+    if not force and same and not _stale(BINDING, deps):
+        return BINDING
 
     import torch
     top = os.path.dirname(torch.__file__)
@@ -132,6 +141,8 @@ def build_binding(verbose: bool = False, force: bool = False) -> str:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"building the torch binding failed:\n{r.stderr}")
+    with open(BINDING_MADE_FOR, "w") as f:
+        f.write(made_for)
     return BINDING
 
 

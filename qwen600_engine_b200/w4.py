@@ -15,9 +15,8 @@ import ctypes as C
 import torch
 
 from . import _lib
-from . import _torch
 from ._lib import QS_BF16, QS_ERR_INVALID, QS_F16, SamplerError, check
-from .losses import _on
+from .losses import _on, _torch  # the binding, with what to do where it does not load
 
 _SCALES = {torch.bfloat16: QS_BF16, torch.float16: QS_F16}
 
