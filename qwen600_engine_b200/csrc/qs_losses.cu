@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "qs_common.cuh"
+#include "qs_f32x2.cuh"
 #include "qs_pipe.cuh"
 #include "qwen600_sampler.h"
 
@@ -43,33 +44,6 @@ __device__ __forceinline__ float exp2_fast(float v) {
     return r;
 }
 
-// Two fp32 operations in one instruction.
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pair2(float x, float y) {
-    f32x2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ float2 unpair2(f32x2 v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 __device__ __forceinline__ f32x2 exp2_pair(f32x2 v) {
     const float2 t = unpair2(v);
     return pair2(exp2_fast(t.x), exp2_fast(t.y));

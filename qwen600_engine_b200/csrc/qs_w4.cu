@@ -26,6 +26,7 @@
 #include <atomic>
 
 #include "qs_common.cuh"
+#include "qs_f32x2.cuh"
 #include "qs_w4.h"
 #include "qs_rmsnorm.cuh"
 
@@ -197,23 +198,6 @@ w4_rows_kernel(const __nv_bfloat16* __restrict__ X, const __nv_bfloat16* __restr
 
 // -------------------------------------------------------------- projection
 constexpr int kW4Depth = 2;  // units a warp has in flight
-
-// Two fp32 operations in one instruction.
-__device__ __forceinline__ unsigned long long pair2(float x, float y) {
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ float2 unpair2(unsigned long long v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
-    unsigned long long r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
 
 // d = a * b + d, or a * b alone, on 16 x 8 x 16.
 __device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
