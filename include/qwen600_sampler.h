@@ -393,18 +393,20 @@ QS_API int qs_lm_head_w4_sample(qs_sampler* s, const void* d_hidden, const void*
  * token lies outside [0, vocab) scores nothing: its log-probability is 0, its
  * gradient zero, and its logits are not read.  With x = row i and t its token,
  *   logprob = (x[t] - max x) / T - log sum_j exp((x[j] - max x) / T)
- * for a temperature T in [1e-6, 1e6].  Entries of -inf (masked tokens) have probability 0; a row
- * with a NaN, with +inf or with nothing above -inf has a NaN log-probability
- * and gradient.  Gradients are d loss / d logits, [rows, vocab] in the logits'
+ * for a temperature T in [1e-6, 1e6].  Entries of -inf (masked tokens) have
+ * probability 0, as finite masks far below the row's maximum do (of any size, the
+ * type's lowest value among them); a row with a NaN, with +inf or with nothing
+ * above -inf has a NaN log-probability and gradient.  Gradients are d loss / d logits, [rows, vocab] in the logits'
  * type, rows grad_row_stride elements apart; d_grad may be d_logits itself
- * with the same stride (the gradient then replaces the logits), and may not
- * overlap it otherwise.  Exponentials and the first steps of a row's sum are
+ * with the same stride (the gradient then replaces the logits); otherwise the
+ * two buffers may not overlap, nor their rows lie between one another's.  Exponentials and the first steps of a row's sum are
  * fp32, what joins them, the losses and their slopes 64-bit, all in a fixed
  * order: the same inputs give the same bits.  vocab <= qs_max_vocab(), rows <= 2^27.  Nothing is
  * allocated and no state is kept.  A workspace of the *_workspace call's bytes
  * (where that is 0, it may be NULL) is 16-byte aligned, needs no
  * initialisation, and belongs to the call until it is done: calls that overlap
- * on the GPU need workspaces of their own. */
+ * on the GPU need workspaces of their own.  A copy into
+ * shared memory that has not landed after 2 s leaves NaN in the results. */
 
 /* d_logprobs fp32 [rows]; d_stats fp32 [rows, 2] (for the backward call): the
  * row's maximum, and sum_j exp((x[j] - max x) / T) - 1 (the maximum's own term

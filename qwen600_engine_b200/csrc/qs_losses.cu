@@ -213,7 +213,7 @@ __device__ __forceinline__ double beyond(float xt, float max, double excess, dou
 }
 
 constexpr int kScoreThreads = 256;                        // at most, in a CTA
-constexpr unsigned long long kLoadWaitNs = 2000000000ull;  // a copy that has not landed by then: NaN
+constexpr unsigned long long kLoadWaitNs = 2000000000ull;  // a copy that has not landed by then: NaN in the results
 
 template <typename T>
 struct ScoreArgs {
@@ -998,9 +998,12 @@ static int launch(const char* name, void (*kernel)(P...), long long grid, int th
     return fail(QS_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
 }
 
-// How a row is spread: CTAs per row (a power of two up to 8) such that a share
-// is at most 40 KB, and more of them while the rows alone would leave SMs idle
-// and a share keeps 4 KB.
+// How a row is spread: CTAs per row (a power of two up to 8), doubled while a
+// share is above 40 KB, and while the rows alone would leave some of the 148 SMs
+// idle and a share keeps 4 KB.  Rows above 320 KB keep 8 with larger shares, up
+// to 128 KB: fp32 rows of 151,936 (76 KB, two CTAs an SM) take 240 us for 1024
+// rows of the policy loss with its gradient (5.2 TB/s), those of 262,144 have
+// one CTA an SM.
 template <typename T, bool kPolicy>
 static int score_launch(ScoreArgs<T>& a, cudaStream_t st) {
     const int vecs = a.V / Pack<T>::kN;

@@ -10,7 +10,9 @@
 // 1024 + q or 1024 + 16 q, four fp16 subtractions or multiply-adds, all exact.
 // (As fp16 denormals, q 2^-24, codes need only the shift and four ands, but the
 // tensor cores align products by nominal exponents and lose 6 bits of a sum; as
-// bf16 pairs they take 11.)  The tokens are scaled by a power of two to fp16,
+// bf16 pairs they take 11.)  Turning codes into fp16 by the bits of 1024 is a
+// published method; layout, zero points and the sharing of units are this
+// file's.  The tokens are scaled by a power of two to fp16,
 // exactly for values of at least 2^-31 of a row's largest (smaller ones lose
 // what lies 2^-39 below it).  (tcgen05 takes its wider operand from shared or
 // tensor memory; 4-bit weights would have to be written there as 16-bit numbers,

@@ -6,8 +6,13 @@ csrc/qs_torch.cpp, checks the tensors and makes the buffers).
 returns beside a sampled token), ``token_logprobs_backward`` takes a gradient of
 those back to the logits.  ``policy_loss`` (clipped, with a KL term) and
 ``preference_loss`` (paired log ratios) return their loss and the gradient of
-the logits in one call; ``logits.backward(result.grad)`` hands it to autograd.
-The formulas stand in include/qwen600_sampler.h.
+the logits in one call.  The formulas stand in include/qwen600_sampler.h.
+
+Nothing these functions return has an autograd history, also where the logits
+require a gradient: ``loss.backward()`` raises, and in a sum with other losses
+this one's part would be missing without an error.  ``logits.backward(result.grad)``
+hands the gradient on; beside other losses over the same graph, use
+``torch.autograd.backward([logits, other], [result.grad, None])``.
 
 Tensors are on one GPU: logits [rows, vocab] fp32 or bf16 whose columns are
 contiguous (any row stride of at least vocab), tokens int32 [rows].  A token
@@ -99,7 +104,8 @@ def preference_loss(logits, tokens, seq_offsets, ref_logprobs, *, beta: float = 
     sequence p is chosen over sequence pairs + p.  ``ref_logprobs`` fp32
     [2 * pairs]: each sequence's log-probability under the reference model.
     ``weights`` fp32 [pairs] (default 1 / pairs).  ``out`` takes the gradient
-    and may be ``logits``."""
+    and may be ``logits``.  Offsets that fall anywhere make the loss and every
+    sum NaN, without a gradient."""
     return tuple.__new__(PreferenceLoss, _on(stream, _torch.preference_loss, logits, tokens, seq_offsets, ref_logprobs,
                                              weights, beta, label_smoothing, grad, out))
 

@@ -820,3 +820,19 @@ def test_a_gradient_in_place_is_seen_by_autograd(dtype):
         before = y._version
         L().policy_loss(y, tok, old, adv, weights=w)
         assert y._version == before  # only read
+
+
+def test_gradient_beside_another_loss():
+    """The documented way to take a loss of these together with one of autograd's; without a history of its own it
+    cannot be taken for one of them."""
+    x, tok, old, _, adv, w = policy_case(5, 300, torch.float32, seed=97)
+    leaf = x.clone().requires_grad_(True)
+    logits = leaf * 1.0
+    other = (logits * logits).sum()
+    r = L().policy_loss(logits, tok, old, adv, weights=w)
+    assert not r.loss.requires_grad and not r.logprobs.requires_grad and not r.grad.requires_grad
+    with pytest.raises(RuntimeError):
+        r.loss.backward()
+    torch.autograd.backward([logits, other], [r.grad, None])
+    want = r.grad.double() + 2 * x.double()
+    assert ((leaf.grad.double() - want).abs() <= 2 * U * (r.grad.double().abs() + 2 * x.double().abs())).all()
