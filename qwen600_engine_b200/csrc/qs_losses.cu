@@ -8,187 +8,12 @@
 //   d logprob / d x[j] = ([j = t] - exp((x[j] - m) / T) / (1 + excess)) / T
 // The maximum's own term is exactly 1; keeping it out of the fp32 sum lets a
 // peaked row (log-probability near 0) keep its relative precision.
-#include <cuda_bf16.h>
-#include <cuda_runtime.h>
-#include <math.h>
-#include <stdarg.h>
-#include <stdio.h>
-
-#include <atomic>
 #include <type_traits>
 
-#include "qs_common.cuh"
-#include "qs_f32x2.cuh"
-#include "qs_pipe.cuh"
-#include "qwen600_sampler.h"
+#include "qs_rows.cuh"
+#include "qs_stream.cuh"
 
 namespace qs {
-
-int set_error(int code, const char* msg);  // qs_api.cu
-
-// What a scored row leaves for the losses and the gradient.
-struct RowScore {
-    double logprob;  // 0 for a row that scores nothing
-    float max;
-    float excess;
-};
-
-template <typename T>
-__device__ __forceinline__ float elem(const T* p, long long i) { return Elem<T>::widen(p[i]); }
-__device__ __forceinline__ void put(float* p, long long i, float v) { p[i] = v; }
-__device__ __forceinline__ void put(__nv_bfloat16* p, long long i, float v) { p[i] = __float2bfloat16_rn(v); }
-
-__device__ __forceinline__ float exp2_fast(float v) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-    return r;
-}
-
-__device__ __forceinline__ f32x2 exp2_pair(f32x2 v) {
-    const float2 t = unpair2(v);
-    return pair2(exp2_fast(t.x), exp2_fast(t.y));
-}
-
-// A term 2^((x - ref) scale) in one multiply-add is 2^(x scale - bias), bias
-// the rounded ref * scale; every term is then 2^slip too large, slip being what
-// the rounding took, and 2^-slip sets a sum of them right.  Below 2^24 slip is
-// at most 1/2.  It grows with bias: from 2^31 on it can pass 128, and 2^slip
-// and 2^-slip are inf and 0, their product NaN (logits masked with -1e10 or
-// -1e30).  Larger values subtract before they scale.
-__device__ __forceinline__ bool one_step(float bias) { return fabsf(bias) < 16777216.0f; }
-
-// Block-wide sum of one double per thread, in a fixed order; in warp 0.
-__device__ __forceinline__ double block_sum(double v, double* red) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    if (threadIdx.x >= 32) return 0.0;
-    v = threadIdx.x < blockDim.x >> 5 ? red[threadIdx.x] : 0.0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
-// Vectors of 16 bytes of a row, at any alignment of its first element: up to
-// kN - 1 elements before the first aligned vector (head), whole vectors, up to
-// kN - 1 elements behind the last (tail).
-template <typename T>
-struct RowShape {
-    static constexpr int kN = 16 / (int)sizeof(T);
-    int head, vecs, tail;
-    __device__ __forceinline__ RowShape(const T* row, int V) {
-        head = min(V, (int)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T)));
-        vecs = (V - head) / kN;
-        tail = V - head - vecs * kN;
-    }
-    // The element outside the vectors that thread t of a row's first CTA takes, or -1.
-    __device__ __forceinline__ int edge(int t, int V) const {
-        return t < head ? t : t >= 8 && t < 8 + tail ? V - tail + t - 8 : -1;
-    }
-};
-
-// Plain (coherent) loads that do not stay in L1: the same kernel may write the
-// gradient over the logits, so the read-only path is not used.
-__device__ __forceinline__ uint4 load16(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p)
-                 : "memory");
-    return v;
-}
-__device__ __forceinline__ void store16(void* p, const uint4& v) {
-    asm volatile("st.global.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                 : "memory");
-}
-
-// The same for data that should not push others out of L2.
-__device__ __forceinline__ void store16_past(void* p, const uint4& v) {
-    asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                 : "memory");
-}
-
-// 16 bytes of logits as floats and back.
-template <typename T>
-struct Pack;
-template <>
-struct Pack<float> {
-    static constexpr int kN = 4;
-    __device__ __forceinline__ static uint4 lowest() {
-        return make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u);
-    }
-    __device__ __forceinline__ static void widen(const uint4& v, float* o) {
-        o[0] = __uint_as_float(v.x); o[1] = __uint_as_float(v.y);
-        o[2] = __uint_as_float(v.z); o[3] = __uint_as_float(v.w);
-    }
-    __device__ __forceinline__ static void widen_word(uint32_t w, float* o) { o[0] = __uint_as_float(w); }
-    __device__ __forceinline__ static uint4 narrow(const float* o) {
-        return make_uint4(__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3]));
-    }
-    __device__ __forceinline__ static uint32_t max2(uint32_t a, uint32_t b) {
-        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
-    }
-};
-template <>
-struct Pack<__nv_bfloat16> {
-    static constexpr int kN = 8;
-    __device__ __forceinline__ static uint4 lowest() {
-        return make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u);
-    }
-    __device__ __forceinline__ static void widen_word(uint32_t w, float* o) {
-        o[0] = __uint_as_float(w << 16);
-        o[1] = __uint_as_float(w & 0xFFFF0000u);
-    }
-    __device__ __forceinline__ static void widen(const uint4& v, float* o) {
-        widen_word(v.x, o);
-        widen_word(v.y, o + 2);
-        widen_word(v.z, o + 4);
-        widen_word(v.w, o + 6);
-    }
-    __device__ __forceinline__ static uint4 narrow(const float* o) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
-            w[i] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    __device__ __forceinline__ static uint32_t max2(uint32_t a, uint32_t b) {
-        const __nv_bfloat162 h = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a),
-                                         *reinterpret_cast<const __nv_bfloat162*>(&b));
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-};
-
-__device__ __forceinline__ void cluster_arrive_relaxed() {
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_arrive_release() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-// One CTA's part of a row: its maximum, how many elements equal it, and the
-// sum of the others' exponentials against it.
-struct __align__(16) Part {
-    float max;
-    int at_max;
-    double others;
-};
-
-// Writes p to *slot of the cluster's CTA `rank`.
-__device__ __forceinline__ void push_part(Part* slot, int rank, const Part& p) {
-    uint32_t addr;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-                 : "=r"(addr)
-                 : "r"((uint32_t)__cvta_generic_to_shared(slot)), "r"(rank));
-    const unsigned long long o = (unsigned long long)__double_as_longlong(p.others);
-    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(__float_as_uint(p.max)),
-                 "r"((uint32_t)p.at_max), "r"((uint32_t)o), "r"((uint32_t)(o >> 32))
-                 : "memory");
-}
 
 // Per-row term of the policy loss: returns l, and its slope dl / dlogprob.
 __device__ __forceinline__ double policy_term(double lp, double old_lp, double ref_lp, double adv, double lo,
@@ -212,8 +37,7 @@ __device__ __forceinline__ double beyond(float xt, float max, double excess, dou
     return xt == max ? excess / (1.0 + excess) : 1.0 - exp(((double)xt - (double)max) * inv_t) / (1.0 + excess);
 }
 
-constexpr int kScoreThreads = 256;                        // at most, in a CTA
-constexpr unsigned long long kLoadWaitNs = 2000000000ull;  // a copy that has not landed by then: NaN in the results
+constexpr int kScoreThreads = 256;  // at most, in a CTA
 
 template <typename T>
 struct ScoreArgs {
@@ -495,208 +319,7 @@ score_kernel(const __grid_constant__ ScoreArgs<T> a) {
     }
 }
 
-// ------------------------------------------------- scoring many rows
-// Without a gradient a row need not stay on the chip, and a call of many rows
-// is a stream: rows are cut into units of 256 vectors (4 KB), every warp of a
-// persistent grid takes units in turn through its own ring of bulk copies and
-// leaves each unit's maximum and sums, and a second kernel joins a row's units.
-// The maximum's own term is left out of the fp32 sum as in score_kernel: where
-// one lane holds the maximum, the warp takes that lane's 128 bytes once more,
-// two elements a lane.  (Where several do, the row's sum is at least 2, and the
-// 1 costs it less than the exponentials do.)  Warps never wait for one another,
-// so copies keep running while others compute.  1024 bf16 rows of 151,936: 61 us
-// (52 of them this kernel, 6.0 TB/s, its exponentials at 75% of the unit's
-// rate), 78 with a cluster per row.  24 warps with rings of 2 units; 16 with 3
-// were 16 us slower.
-constexpr int kUnitVecs = 256;
-constexpr int kStreamWarps = 24;
-constexpr int kStreamStages = 2;
-
-template <typename T>
-struct StreamArgs {
-    const T* logits;
-    int rows, V;
-    long long ld;
-    const int* tokens;
-    float scale;
-    double inv_t;
-    int units;     // per row
-    float4* parts; // [rows][units]: maximum, sum of exponentials against it, how many 1s were left out of it
-    RowScore* out;
-    float* coefs;  // with out: set to 0
-    float* logprobs;
-    float* stats;
-};
-
-// Where a warp is in its units: it takes every stride-th one.
-struct UnitAt {
-    int row, unit;
-    __device__ __forceinline__ void step(int rows, int units, int units_per_row) {
-        row += rows;
-        unit += units;
-        if (unit >= units_per_row) {
-            unit -= units_per_row;
-            row++;
-        }
-    }
-};
-
-template <typename T>
-__global__ void __launch_bounds__(kStreamWarps * 32, 1)
-stream_kernel(const __grid_constant__ StreamArgs<T> a) {
-    constexpr int kN = Pack<T>::kN;
-    extern __shared__ __align__(128) uint4 ring[];  // [warp][stage][kUnitVecs]
-    __shared__ unsigned long long full[kStreamWarps][kStreamStages];
-    __shared__ int gave_up;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint4* mine = ring + (size_t)warp * kStreamStages * kUnitVecs;
-    if (threadIdx.x == 0) gave_up = 0;
-    if (lane == 0) {
-        for (int i = 0; i < kStreamStages; i++) mbar_init(&full[warp][i], 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
-    __syncthreads();
-    dependents_may_start();
-
-    const long long stride = (long long)gridDim.x * kStreamWarps, begin = (long long)warp * gridDim.x + blockIdx.x;
-    const int dr = (int)(stride / a.units), du = (int)(stride % a.units);
-    UnitAt now{(int)(begin / a.units), (int)(begin % a.units)}, ahead = now;
-    const auto scored = [&](int row) {
-        if (row >= a.rows) return false;
-        const int tok = a.tokens[row];
-        return tok >= 0 && tok < a.V;
-    };
-    const auto request = [&](const UnitAt& u, int stage) {
-        if (lane == 0) {
-            const T* x = a.logits + (size_t)u.row * a.ld;
-            const RowShape<T> sh(x, a.V);
-            const int first = u.unit * kUnitVecs, cnt = max(0, min(kUnitVecs, sh.vecs - first));
-            mbar_expect_tx(&full[warp][stage], (uint32_t)cnt * 16u);
-            if (cnt > 0)
-                asm volatile(
-                    "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                        smem_u32(mine + stage * kUnitVecs)),
-                    "l"(x + sh.head + (size_t)first * kN), "r"((uint32_t)cnt * 16u), "r"(smem_u32(&full[warp][stage]))
-                    : "memory");
-        }
-    };
-    uint32_t live = 0;    // stages with a copy under way
-    uint32_t phases = 0;  // the parity each stage's next copy completes
-#pragma unroll
-    for (int i = 0; i < kStreamStages; i++) {
-        if (scored(ahead.row)) {
-            request(ahead, i);
-            live |= 1u << i;
-        }
-        ahead.step(dr, du, a.units);
-    }
-    bool next = scored(ahead.row);  // looked up one unit before it is asked for
-    bool dead = false;
-    for (int stage = 0; now.row < a.rows; stage = stage + 1 == kStreamStages ? 0 : stage + 1) {
-        if (live >> stage & 1) {
-            const bool landed = !dead && mbar_wait(&full[warp][stage], phases >> stage & 1, &gave_up, kLoadWaitNs);
-            if (!landed) {
-                mbar_wait(&full[warp][stage], phases >> stage & 1, &gave_up, kLoadWaitNs, false);
-                dead = true;
-            }
-            phases ^= 1u << stage;
-            const T* x = a.logits + (size_t)now.row * a.ld;
-            const RowShape<T> sh(x, a.V);
-            const int cnt = max(0, min(kUnitVecs, sh.vecs - now.unit * kUnitVecs));
-            const int edge = now.unit == 0 ? sh.edge(lane, a.V) : -1;
-            const float xe = edge >= 0 ? elem(x, edge) : -INFINITY;
-            uint4 v[kUnitVecs / 32];
-            uint4 u = Pack<T>::lowest();
-#pragma unroll
-            for (int i = 0; i < kUnitVecs / 32; i++) {
-                const int k = i * 32 + lane;
-                v[i] = k < cnt ? mine[stage * kUnitVecs + k] : Pack<T>::lowest();
-                u.x = Pack<T>::max2(u.x, v[i].x);
-                u.y = Pack<T>::max2(u.y, v[i].y);
-                u.z = Pack<T>::max2(u.z, v[i].z);
-                u.w = Pack<T>::max2(u.w, v[i].w);
-            }
-            float o[kN];
-            Pack<T>::widen(u, o);
-            float own = xe;
-#pragma unroll
-            for (int j = 0; j < kN; j++) own = fmaxf(own, o[j]);
-            const float m = warp_max(own);
-            const uint32_t holders = __ballot_sync(0xffffffffu, own == m);
-            const bool one = (holders & (holders - 1)) == 0;
-            const int holder = __ffs(holders) - 1;
-            float again = 0.0f;  // this lane's share of the holder's elements
-            int at_max = 0;
-            if (one) {
-                const int k = (lane >> 2) * 32 + holder;
-                const uint32_t word = k < cnt ? reinterpret_cast<const uint32_t*>(mine + stage * kUnitVecs + k)[lane & 3]
-                                              : Pack<T>::lowest().x;
-                float e[kN / 4];
-                Pack<T>::widen_word(word, e);
-#pragma unroll
-                for (int j = 0; j < kN / 4; j++) {
-                    const float d = e[j] - m;
-                    at_max += __popc(__ballot_sync(0xffffffffu, d == 0.0f));
-                    again += d == 0.0f ? 0.0f : exp2_fast(d * a.scale);
-                }
-            }
-            __syncwarp();  // every lane has read the stage
-            live &= ~(1u << stage);
-            if (next && !dead) {
-                request(ahead, stage);
-                live |= 1u << stage;
-            }
-            const float ref = m == -INFINITY ? 0.0f : m;
-            const float bias = ref * a.scale;
-            float s;
-            if (one_step(bias)) {
-                const f32x2 scale2 = pair2(a.scale, a.scale), bias2 = pair2(-bias, -bias);
-                f32x2 s2 = pair2(exp2_fast(__fmaf_rn(xe, a.scale, -bias)), 0.0f);
-#pragma unroll
-                for (int i = 0; i < kUnitVecs / 32; i++) {
-                    Pack<T>::widen(v[i], o);
-#pragma unroll
-                    for (int j = 0; j < kN; j += 2) s2 = add2(s2, exp2_pair(fma2(pair2(o[j], o[j + 1]), scale2, bias2)));
-                }
-                const float2 r = unpair2(s2);
-                s = (r.x + r.y) * exp2_fast(-__fmaf_rn(ref, a.scale, -bias));
-            } else {  // 1024 bf16 rows of 151,936, nearly all of -1e30: 86 us; shorter with packed operations, but
-                      // their code costs ordinary rows 1% and more
-                s = exp2_fast((xe - ref) * a.scale);
-#pragma unroll 1
-                for (int i = 0; i < kUnitVecs / 32; i++) {
-                    uint4 w = v[0];
-#pragma unroll
-                    for (int k = 1; k < kUnitVecs / 32; k++)
-                        if (k == i) w = v[k];
-                    Pack<T>::widen(w, o);
-                    for (int j = 0; j < kN; j++) s += exp2_fast((o[j] - ref) * a.scale);
-                }
-            }
-            if (one) {
-                const float held = __shfl_sync(0xffffffffu, xe, holder) - m;  // the holder's element outside the vectors
-                at_max += held == 0.0f;
-                if (lane == holder) s = held == 0.0f ? 0.0f : exp2_fast(held * a.scale);
-                s += again;
-            }
-            s = warp_sum(s);
-            if (lane == 0)
-                a.parts[(size_t)now.row * a.units + now.unit] = make_float4(m, dead ? NAN : s, (float)at_max, 0.0f);
-        } else {
-            if (lane == 0 && dead) a.parts[(size_t)now.row * a.units + now.unit] = make_float4(0.0f, NAN, 0.0f, 0.0f);
-            if (next && !dead) {
-                request(ahead, stage);
-                live |= 1u << stage;
-            }
-        }
-        now.step(dr, du, a.units);
-        ahead.step(dr, du, a.units);
-        next = scored(ahead.row);
-    }
-}
-
-// Joins a row's units, one warp a row.
+// Joins a row's units as the stream leaves them (qs_stream.cuh), one warp a row.
 constexpr int kJoinRows = 4;                                    // a CTA: small enough to start beside the stream
 constexpr int kMaxUnits = kMaxVocab / 4 / kUnitVecs;            // of a row
 static_assert(kMaxUnits % 32 == 0, "units of a lane");
@@ -828,17 +451,6 @@ grad_kernel(const T* logits, int rows, int V, long long ld, const int* __restric
     if (mine) put(g, tok, target);
 }
 
-// The policy loss: the rows' terms, added in a fixed order.
-__global__ void __launch_bounds__(1024)
-sum_rows_kernel(const double* row_loss, int rows, float* __restrict__ loss) {
-    __shared__ double red[32];
-    wait_for_previous();
-    double sum = 0.0;
-    for (int i = threadIdx.x; i < rows; i += blockDim.x) sum += row_loss[i];
-    sum = block_sum(sum, red);
-    if (threadIdx.x == 0) *loss = (float)sum;
-}
-
 // One warp per pair in turn: the two sequences' sums, the pair's loss and the
 // coefficients of their rows' gradients (0 so far).  Sequences share no row
 // unless an offset falls somewhere: then none counts, so that no two warps write
@@ -903,101 +515,6 @@ preference_pairs_kernel(const RowScore* score, int rows, const int* __restrict__
 }
 
 // --------------------------------------------------------------- host side
-static int fail(int code, const char* fmt, ...) {
-    char buf[512];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof(buf), fmt, ap);
-    va_end(ap);
-    return set_error(code, buf);
-}
-
-static size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
-
-struct Rows {
-    const void* logits;
-    int dtype, rows, vocab;
-    long long ld;
-    const int* tokens;
-    double inv_t;
-    void* grad;
-    long long gld;
-    size_t esz() const { return dtype == QS_F32 ? 4 : 2; }
-};
-
-static int check_workspace(const void* p, size_t bytes, size_t need) {
-    if (need == 0 || (p && bytes >= need && ((uintptr_t)p & 15) == 0)) return QS_OK;
-    return fail(QS_ERR_INVALID, "workspace is NULL, unaligned or below %zu bytes", need);
-}
-
-static int check_rows(const Rows& r, double temperature) {
-    if (r.dtype != QS_F32 && r.dtype != QS_BF16) return fail(QS_ERR_INVALID, "unknown dtype %d", r.dtype);
-    if (r.rows < 0) return fail(QS_ERR_INVALID, "rows %d < 0", r.rows);
-    if (r.rows > 1 << 27) return fail(QS_ERR_UNSUPPORTED, "rows %d above 2^27", r.rows);
-    if (r.vocab < 1 || r.vocab > kMaxVocab)
-        return fail(QS_ERR_UNSUPPORTED, "vocab %d outside [1, %d]", r.vocab, kMaxVocab);
-    if (!(temperature >= 1e-6 && temperature <= 1e6))
-        return fail(QS_ERR_INVALID, "temperature %g outside [1e-6, 1e6]", temperature);
-    if (r.rows == 0) return QS_OK;
-    if (!r.logits || !r.tokens) return fail(QS_ERR_INVALID, "NULL device pointer");
-    if (((uintptr_t)r.logits | (uintptr_t)r.grad) % r.esz())
-        return fail(QS_ERR_INVALID, "logits and gradient must be aligned to their element");
-    if (r.rows > 1 && r.ld < r.vocab) return fail(QS_ERR_INVALID, "row_stride %lld < vocab %d", r.ld, r.vocab);
-    if (r.grad) {
-        if (r.rows > 1 && r.gld < r.vocab)
-            return fail(QS_ERR_INVALID, "grad_row_stride %lld < vocab %d", r.gld, r.vocab);
-        const uintptr_t a = (uintptr_t)r.logits, g = (uintptr_t)r.grad;
-        const size_t an = ((size_t)(r.rows - 1) * r.ld + r.vocab) * r.esz();
-        const size_t gn = ((size_t)(r.rows - 1) * r.gld + r.vocab) * r.esz();
-        if (a < g + gn && g < a + an && !(a == g && (r.ld == r.gld || r.rows == 1)))
-            return fail(QS_ERR_INVALID, "the gradient overlaps the logits without being their own buffer");
-    }
-    return QS_OK;
-}
-
-// Lets a kernel use `bytes` of dynamic shared memory, once on each device.
-struct DeviceOnce {
-    std::atomic<unsigned long long> done{0};
-    int raise(const void* kernel, int bytes) {
-        int dev = 0;
-        cudaError_t e = cudaGetDevice(&dev);
-        if (e == cudaSuccess && (dev >= 64 || !(done.load() >> dev & 1))) {
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-            if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev);
-        }
-        return e == cudaSuccess ? QS_OK : fail(QS_ERR_CUDA, "shared memory: %s", cudaGetErrorString(e));
-    }
-};
-
-// Launches `kernel` in clusters of `cluster` CTAs; `after`: it may start while
-// the kernel before it ends (it waits for it before it reads its results).
-template <typename... P, typename... A>
-static int launch(const char* name, void (*kernel)(P...), long long grid, int threads, int cluster, size_t smem,
-                  bool after, cudaStream_t st, A... args) {
-    if (grid > 0x7FFFFFFFll) return fail(QS_ERR_UNSUPPORTED, "%s: %lld CTAs", name, grid);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2] = {};
-    if (cluster > 1) {
-        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        attr[cfg.numAttrs].val.clusterDim.x = cluster;
-        attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
-        cfg.numAttrs++;
-    }
-    if (after) {
-        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
-        cfg.numAttrs++;
-    }
-    cfg.attrs = attr;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
-    if (e == cudaSuccess) return QS_OK;
-    return fail(QS_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
-}
-
 // How a row is spread: CTAs per row (a power of two up to 8), doubled while a
 // share is above 40 KB, and while the rows alone would leave some of the 148 SMs
 // idle and a share keeps 4 KB.  Rows above 320 KB keep 8 with larger shares, up
@@ -1035,10 +552,6 @@ static ScoreArgs<T> score_args(const Rows& r) {
     return a;
 }
 
-static int row_units(int dtype, int vocab) {
-    const int vecs = vocab / (dtype == QS_F32 ? 4 : 8);
-    return vecs > kUnitVecs ? (vecs + kUnitVecs - 1) / kUnitVecs : 1;
-}
 // Large calls stream; smaller ones take a cluster per row, in one launch.  Long
 // bf16 rows from 72 MB (22.0 us against 22.4 at 72 MB, 30.4 against 33.2 at
 // 120), fp32 rows and rows of less than a CTA's 40 KB from 24 MB (at 32 MB fp32
@@ -1077,15 +590,7 @@ static int score(const Rows& r, RowScore* out, float* coefs, float* logprobs, fl
     a.coefs = coefs;
     a.logprobs = logprobs;
     a.stats = stats;
-    const size_t smem = (size_t)kStreamWarps * kStreamStages * kUnitVecs * 16;
-    static DeviceOnce once;
-    int rc = once.raise((const void*)stream_kernel<T>, (int)smem);
-    if (rc) return rc;
-    int dev = 0, sms = 148;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess) return fail(QS_ERR_CUDA, "device: %s", cudaGetErrorString(e));
-    rc = launch("stream_kernel", stream_kernel<T>, sms, kStreamWarps * 32, 1, smem, false, st, a);
+    const int rc = stream_rows<T, false>(a, st);
     if (rc) return rc;
     return launch("join_kernel", join_kernel<T>, (r.rows + kJoinRows - 1) / kJoinRows, kJoinRows * 32, 1, 0, true, st, a);
 }
