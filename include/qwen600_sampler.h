@@ -476,6 +476,123 @@ QS_API int qs_preference_loss(const void* d_logits, int dtype, int rows, int voc
                               void* d_grad, long long grad_row_stride, void* d_workspace,
                               size_t workspace_bytes, void* stream);
 
+/* Working with the best few tokens of a row: listing them, learning from a
+ * teacher's, and searching with them.  No counterpart in the reference (it
+ * draws one token of a row).
+ *
+ * Conventions as for the four calls above: d_logits [rows, vocab] fp32 or bf16,
+ * rows row_stride elements apart; temperature in [1e-6, 1e6]; vocab <=
+ * qs_max_vocab(), rows <= 2^27; nothing is allocated, no state is kept, the
+ * same inputs give the same bits; a workspace of the *_workspace call's bytes is
+ * 16-byte aligned, needs no initialisation and belongs to the call until it is
+ * done; a copy into shared memory that has not landed after 2 s leaves NaN. */
+
+#define QS_MAX_LISTED 256 /* tokens listed of a row, or chosen of a search's entry */
+#define QS_MAX_BEAMS 64   /* beams of a search's entry */
+
+/* The k tokens of each row with the largest logits, the larger first and equal
+ * ones by token, and their log-probabilities at the temperature (those of
+ * qs_token_logprobs): d_logprobs fp32 [rows, k], d_tokens int [rows, k].
+ * Entries of -inf (masked tokens) are not listed: where a row has fewer than k
+ * others, token -1 and log-probability -inf fill its list.  A row with a NaN or
+ * +inf has tokens -1 and log-probabilities NaN.  1 <= k <= QS_MAX_LISTED. */
+QS_API size_t qs_top_logprobs_workspace(int dtype, int rows, int vocab, int k);
+QS_API int qs_top_logprobs(const void* d_logits, int dtype, int rows, int vocab, long long row_stride, int k,
+                           double temperature, float* d_logprobs, int* d_tokens, void* d_workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* One step of beam search.  Row b * beams + i of d_logits [batch * beams, vocab]
+ * belongs to beam i of entry b, whose score so far is d_scores fp32 [batch,
+ * beams].  Its continuations are
+ *   (score + logprob(token), i, token)   for every token above -inf,
+ * or, where d_finished [batch, beams] (bytes, or NULL: none is) marks it,
+ *   (score, i, pad_token)                alone; its logits are not read.
+ * The n best of each entry, the larger score first and equal ones by beam, then
+ * by token: d_out_scores fp32 [batch, n], d_parents int [batch, n] (their beam),
+ * d_tokens int [batch, n], d_out_finished bytes [batch, n] or NULL: 1 where the
+ * parent is finished or the token is eos_token (-1: no such token).  A beam with
+ * score -inf has no continuations (a search that begins from one beam gives the
+ * others this score); where an entry has fewer than n, score -inf, parent -1,
+ * token -1 and finished 1 fill up.  An entry with a score of NaN or +inf, or a
+ * NaN or +inf among its logits read, has scores NaN, parents and tokens -1.
+ * Scores are compared as 64-bit numbers before they are rounded.
+ * keep_slots (n = beams): the chosen ones are the same, but each beam's best one
+ * stays in that beam's place and the others take the places left, the better
+ * first: then only places of beams that end change their state, each to that of
+ * a beam that stays where it is.  Beams 1 to QS_MAX_BEAMS, n 1 to QS_MAX_LISTED.
+ * The outputs may not overlap the inputs. */
+typedef struct {
+    double temperature;
+    int eos_token;
+    int pad_token;
+    int keep_slots;
+} qs_beam_params;
+
+QS_API size_t qs_beam_select_workspace(int dtype, int batch, int beams, int vocab, int n);
+QS_API int qs_beam_select(const void* d_logits, int dtype, int batch, int beams, int vocab, long long row_stride,
+                          const float* d_scores, const unsigned char* d_finished, int n,
+                          const qs_beam_params* params, float* d_out_scores, int* d_parents, int* d_tokens,
+                          unsigned char* d_out_finished, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* Moves per-row states (caches of keys and values, histories) to the beams that
+ * go on, in place: for every state, row b * beams + i becomes what row
+ * b * beams + d_parents[b, i] was.  A parent outside [0, beams) leaves its row as
+ * it is, as a row's own index does; rows that keep theirs are not written.
+ * A state's row is outer[0] x outer[1] x positions pieces of `unit` bytes, each
+ * level a stride in bytes apart (of any size where the count is 1).  d_lengths int
+ * [batch] or NULL: the first d_lengths[b] positions (bounded to 0 .. positions)
+ * of entry b's rows are moved, what lies behind them stays.  `states` is on the
+ * host.  Pieces may not overlap, nor states: two of them may lie between one
+ * another only with the same row stride and apart within it.
+ * batch * beams <= 2^27, beams <= 1024, at most 2^31 - 1 pieces of a row. */
+typedef struct {
+    void* d_base;
+    long long row_stride;
+    long long outer_stride[2];
+    long long position_stride;
+    long long unit;
+    int outer[2];
+    int positions;
+} qs_states;
+
+QS_API int qs_beam_reorder(const qs_states* states, int count, const int* d_parents, int batch, int beams,
+                           const int* d_lengths, void* stream);
+
+/* The same for rows [0, batch * beams) of a sampler's own history: the windows
+ * and cumulative counts that its penalties use.  RNG states stay with the rows. */
+QS_API int qs_reorder_history(qs_sampler* s, const int* d_parents, int batch, int beams, void* stream);
+
+/* Divergence from a teacher known by the best tokens of each row, and the
+ * gradient of the logits.  d_teacher_tokens int [rows, k], d_teacher_logprobs
+ * fp32 [rows, k]: a row's list, as qs_top_logprobs gives it for the teacher's
+ * logits at the same temperature T.  With p = softmax(x / T) and q = exp of the
+ * listed log-probabilities,
+ *   rest = 1:  l = sum q (log q - log p) + r (log r - log p_r)
+ *              r = max(0, 1 - sum q), p_r the sum of the unlisted p: what the
+ *              list leaves is one more outcome (of none where no unlisted token
+ *              is above -inf: r = 0 then)
+ *   rest = 0:  l = sum q (log q - log p), q divided by their sum first
+ *   loss = sum_i w[i] l
+ * w = d_weights[i] (NULL: 1 / rows).  A token outside the vocabulary is no entry;
+ * one listed again counts where it stands first.  A log-probability of -inf is
+ * q = 0, and 0 log 0 = 0.  A row with w[i] = 0, without entries, or with rest = 0
+ * whose q are all 0, adds nothing, has a zero gradient and is not read.  A
+ * teacher's token that the logits mask (-inf, with q > 0) makes the loss +inf.
+ * d_loss fp32 [1], d_row_losses fp32 [rows] (l, 0 for rows that add nothing) or
+ * NULL, d_grad as for the losses above (NULL: the loss alone).  1 <= k <=
+ * QS_MAX_LISTED. */
+typedef struct {
+    double temperature;
+    int rest;
+} qs_distill_params;
+
+QS_API size_t qs_distill_loss_workspace(int rows);
+QS_API int qs_distill_loss(const void* d_logits, int dtype, int rows, int vocab, long long row_stride,
+                           const int* d_teacher_tokens, const float* d_teacher_logprobs, int k,
+                           const float* d_weights, const qs_distill_params* params, float* d_loss,
+                           float* d_row_losses, void* d_grad, long long grad_row_stride, void* d_workspace,
+                           size_t workspace_bytes, void* stream);
+
 /* Message for the last error on the calling thread ("" if none). */
 QS_API const char* qs_last_error(void);
 

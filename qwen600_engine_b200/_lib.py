@@ -39,9 +39,11 @@ EXPORTS = (
     "qs_lm_head_w4_workspace", "qs_lm_head_w4", "qs_lm_head_w4_sample", "qs_token_logprobs_workspace", "qs_token_logprobs",
     "qs_token_logprobs_backward",
     "qs_policy_loss_workspace", "qs_policy_loss", "qs_preference_loss_workspace", "qs_preference_loss",
+    "qs_top_logprobs_workspace", "qs_top_logprobs", "qs_beam_select_workspace", "qs_beam_select", "qs_beam_reorder",
+    "qs_reorder_history", "qs_distill_loss_workspace", "qs_distill_loss",
 )
 _SIZES = ("qs_token_logprobs_workspace", "qs_lm_head_w4_workspace", "qs_w4_codes_bytes", "qs_w4_scales_bytes", "qs_w4_zeros_bytes", "qs_policy_loss_workspace",
-          "qs_preference_loss_workspace")
+          "qs_preference_loss_workspace", "qs_top_logprobs_workspace", "qs_beam_select_workspace", "qs_distill_loss_workspace")
 
 
 class Params(C.Structure):
@@ -77,6 +79,19 @@ class PolicyParams(C.Structure):
 
 class PreferenceParams(C.Structure):
     _fields_ = [("beta", C.c_double), ("label_smoothing", C.c_double)]
+
+
+class BeamParams(C.Structure):
+    _fields_ = [("temperature", C.c_double), ("eos_token", C.c_int), ("pad_token", C.c_int), ("keep_slots", C.c_int)]
+
+
+class States(C.Structure):
+    _fields_ = [("d_base", C.c_void_p), ("row_stride", C.c_longlong), ("outer_stride", C.c_longlong * 2),
+                ("position_stride", C.c_longlong), ("unit", C.c_longlong), ("outer", C.c_int * 2), ("positions", C.c_int)]
+
+
+class DistillParams(C.Structure):
+    _fields_ = [("temperature", C.c_double), ("rest", C.c_int)]
 
 
 ROW_DEBUG_FIELDS = [f for f, _ in RowDebug._fields_]
@@ -147,6 +162,14 @@ def _load() -> C.CDLL:
     lib.qs_preference_loss_workspace.argtypes = [i32, i32, i32]
     lib.qs_preference_loss.argtypes = [vp, i32, i32, i32, i64, vp, vp, i32, vp, vp, P(PreferenceParams),
                                        vp, vp, vp, i64, vp, sz, vp]
+    lib.qs_top_logprobs_workspace.argtypes = [i32, i32, i32, i32]
+    lib.qs_top_logprobs.argtypes = [vp, i32, i32, i32, i64, i32, f64, vp, vp, vp, sz, vp]
+    lib.qs_beam_select_workspace.argtypes = [i32, i32, i32, i32, i32]
+    lib.qs_beam_select.argtypes = [vp, i32, i32, i32, i32, i64, vp, vp, i32, P(BeamParams), vp, vp, vp, vp, vp, sz, vp]
+    lib.qs_beam_reorder.argtypes = [P(States), i32, vp, i32, i32, vp, vp]
+    lib.qs_reorder_history.argtypes = [vp, vp, i32, i32, vp]
+    lib.qs_distill_loss_workspace.argtypes = [i32]
+    lib.qs_distill_loss.argtypes = [vp, i32, i32, i32, i64, vp, vp, i32, vp, P(DistillParams), vp, vp, vp, i64, vp, sz, vp]
     lib.qs_last_error.restype = C.c_char_p
     lib.qs_last_error.argtypes = []
     lib.qs_max_vocab.argtypes = []

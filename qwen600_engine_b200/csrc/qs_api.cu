@@ -78,6 +78,9 @@ using namespace qs;
 static thread_local std::string g_err;
 
 namespace qs {
+int reorder_states(const qs_states* all, int count, const int* d_parents, int batch, int beams, const int* d_lengths,
+                   cudaStream_t st);  // qs_reorder.cu
+
 // Reports a failed call through qs_last_error, for this file and the others.
 // What the CUDA runtime keeps of the failure is dropped: the check behind the
 // next call's first launch would take it for its own.
@@ -454,6 +457,21 @@ int qs_get_rng_state(qs_sampler* s, unsigned long long* host_states, int n) {
     CK(cudaDeviceSynchronize());
     CK(cudaMemcpy(host_states, s->rng, sizeof(unsigned long long) * n, cudaMemcpyDeviceToHost));
     return QS_OK;
+}
+
+int qs_reorder_history(qs_sampler* s, const int* d_parents, int batch, int beams, void* stream) {
+    g_err.clear();
+    if (!s) return fail(QS_ERR_INVALID, "sampler is NULL");
+    if (batch < 0 || beams < 1 || batch > s->max_batch / beams)
+        return fail(QS_ERR_INVALID, "%d x %d rows outside [0, max_batch %d]", batch, beams, s->max_batch);
+    if (batch > 0 && !d_parents) return fail(QS_ERR_INVALID, "NULL pointer");
+    if (s->window == 0) return QS_OK;  // no history kept
+    DeviceGuard dg(s->device);
+    const auto rows_of = [](void* p, size_t bytes) { return qs_states{p, (long long)bytes, {0, 0}, 0, (long long)bytes, {1, 1}, 1}; };
+    const qs_states all[] = {rows_of(s->ring, sizeof(int) * s->window), rows_of(s->slot_counts, sizeof(float) * s->window),
+                             rows_of(s->hcount, sizeof(int)), rows_of(s->hpos, sizeof(int)),
+                             rows_of(s->token_counts, sizeof(float) * (size_t)s->vocab)};
+    return reorder_states(all, 5, d_parents, batch, beams, nullptr, (cudaStream_t)stream);
 }
 
 int qs_reset_sampler_history(qs_sampler* s) {

@@ -1,6 +1,6 @@
-// The scoring, loss and 4-bit lm_head calls for torch tensors: argument checks,
+// The scoring, loss, beam and 4-bit lm_head calls for torch tensors: argument checks,
 // output and workspace tensors, and the C ABI call on the current stream of the
-// tensors' device (qwen600_engine_b200/losses.py and w4.py hold the public
+// tensors' device (qwen600_engine_b200/losses.py, beams.py and w4.py hold the public
 // functions).  Small calls of these operators take a few microseconds on the
 // GPU; made from Python through ctypes, the checks and allocations took 10 to
 // 13 of a call's 20.
@@ -13,6 +13,7 @@
 
 #include <sstream>
 #include <string>
+#include <vector>
 
 #include "qwen600_sampler.h"
 
@@ -38,6 +39,7 @@ const char* name_of(at::ScalarType t) {
         case at::kBFloat16: return "torch.bfloat16";
         case at::kInt: return "torch.int32";
         case at::kLong: return "torch.int64";
+        case at::kBool: return "torch.bool";
         default: return c10::toString(t);
     }
 }
@@ -71,9 +73,28 @@ bool truth(PyObject* o) {
     return v != 0;
 }
 
+int64_t whole(PyObject* o) {
+    const long long v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) throw Refused{0, ""};
+    return v;
+}
+
 int count(const char* name, int64_t n) {
     if (n > INT32_MAX) throw Refused{QS_ERR_UNSUPPORTED, std::string(name) + ": " + std::to_string(n) + " above 2^31 - 1"};
     return (int)n;
+}
+
+// A length that outputs are made with: within the limit before they are.
+int listed(const char* name, int64_t n) {
+    if (n < 1 || n > QS_MAX_LISTED)
+        throw Refused{QS_ERR_UNSUPPORTED, std::string(name) + " " + std::to_string(n) + " outside [1, " + std::to_string(QS_MAX_LISTED) + "]"};
+    return (int)n;
+}
+
+int number_of_token(const char* name, PyObject* o) {
+    const int64_t v = whole(o);
+    if (v < INT32_MIN || v > INT32_MAX) invalid(std::string(name) + " " + std::to_string(v) + " is no 32-bit number");
+    return (int)v;
 }
 
 // A [rows, vocab] tensor whose columns are contiguous.
@@ -107,6 +128,17 @@ const T* vector(const char* name, PyObject* o, at::ScalarType type, int64_t n, c
 template <typename T>
 const T* vector_or_none(const char* name, PyObject* o, at::ScalarType type, int64_t n, const at::Tensor& with) {
     return o == Py_None ? nullptr : vector<T>(name, o, type, n, with);
+}
+
+// A contiguous [rows, columns] tensor.
+template <typename T>
+const T* table(const char* name, PyObject* o, at::ScalarType type, int64_t rows, int64_t columns, const at::Tensor& with) {
+    const at::Tensor& t = tensor(name, o);
+    if (t.scalar_type() != type || t.dim() != 2 || t.size(0) != rows || t.size(1) != columns || !t.is_contiguous() ||
+        t.device() != with.device())
+        invalid(std::string(name) + " must be a contiguous " + name_of(type) + " tensor [" + std::to_string(rows) + ", " +
+                std::to_string(columns) + "] on " + with.device().str() + ", got " + told(t));
+    return static_cast<const T*>(t.data_ptr());
 }
 
 // The device and current stream of a call.
@@ -294,6 +326,152 @@ PyObject* preference_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// (logits, k, temperature) -> (logprobs, tokens)
+PyObject* top_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return call(n, 3, [&] {
+        const at::Tensor& x = tensor("logits", a[0]);
+        const Matrix m("logits", x);
+        const int k = listed("k", whole(a[1]));
+        const double T = number(a[2]);
+        const On on(x);
+        at::Tensor lp = fresh({m.rows, k}, at::kFloat, x), tok = fresh({m.rows, k}, at::kInt, x);
+        const size_t size = qs_top_logprobs_workspace(m.dtype, m.rows, m.vocab, k);
+        at::Tensor work = workspace(size, x);
+        check(qs_top_logprobs(x.data_ptr(), m.dtype, m.rows, m.vocab, m.ld, k, T, (float*)lp.data_ptr(), (int*)tok.data_ptr(),
+                              pointer(work), size, on.stream));
+        return pack({THPVariable_Wrap(lp), THPVariable_Wrap(tok)});
+    });
+}
+
+// (logits, teacher_tokens, teacher_logprobs, weights, temperature, rest, grad, out) -> (loss, row_losses, gradient)
+PyObject* distill_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return call(n, 8, [&] {
+        const at::Tensor& x = tensor("logits", a[0]);
+        const Matrix m("logits", x);
+        const at::Tensor& teacher = tensor("teacher_tokens", a[1]);
+        if (teacher.dim() != 2) invalid("teacher_tokens must be [rows, k], got " + shape_of(teacher));
+        const int k = listed("k", teacher.size(1));
+        const int* tok = table<int>("teacher_tokens", a[1], at::kInt, m.rows, k, x);
+        const float* lps = table<float>("teacher_logprobs", a[2], at::kFloat, m.rows, k, x);
+        const float* w = vector_or_none<float>("weights", a[3], at::kFloat, m.rows, x);
+        const qs_distill_params p{number(a[4]), truth(a[5])};
+        const bool wanted = truth(a[6]);
+        Gradient grad(a[7], x, wanted);
+        const On on(x);
+        if (wanted) grad.make(x);
+        at::Tensor loss = fresh({}, at::kFloat, x), rows = fresh({m.rows}, at::kFloat, x);
+        const size_t size = qs_distill_loss_workspace(m.rows);
+        at::Tensor work = workspace(size, x);
+        check(qs_distill_loss(x.data_ptr(), m.dtype, m.rows, m.vocab, m.ld, tok, lps, k, w, &p, (float*)loss.data_ptr(),
+                              (float*)rows.data_ptr(), grad.ptr, grad.ld, pointer(work), size, on.stream));
+        return pack({THPVariable_Wrap(loss), THPVariable_Wrap(rows), grad.object()});
+    });
+}
+
+// (logits, scores, n, finished, eos_token, pad_token, temperature, keep_slots) -> (scores, parents, tokens, finished)
+PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return call(n, 8, [&] {
+        const at::Tensor& x = tensor("logits", a[0]);
+        const Matrix m("logits", x);
+        const at::Tensor& sc = tensor("scores", a[1]);
+        if (sc.dim() != 2) invalid("scores must be [batch, beams], got " + shape_of(sc));
+        const int batch = count("batch", sc.size(0)), beams = count("beams", sc.size(1));
+        const float* scores = table<float>("scores", a[1], at::kFloat, batch, beams, x);
+        if ((int64_t)batch * beams != m.rows)
+            invalid("logits must have a row for each of " + std::to_string(batch) + " x " + std::to_string(beams) + " beams, got " +
+                    shape_of(x));
+        const int chosen = listed("n", whole(a[2]));
+        const unsigned char* finished = a[3] == Py_None ? nullptr : table<unsigned char>("finished", a[3], at::kBool, batch, beams, x);
+        const qs_beam_params p{number(a[6]), number_of_token("eos_token", a[4]), number_of_token("pad_token", a[5]), truth(a[7])};
+        const On on(x);
+        at::Tensor out = fresh({batch, chosen}, at::kFloat, x), parents = fresh({batch, chosen}, at::kInt, x);
+        at::Tensor tok = fresh({batch, chosen}, at::kInt, x), done = fresh({batch, chosen}, at::kBool, x);
+        const size_t size = qs_beam_select_workspace(m.dtype, batch, beams, m.vocab, chosen);
+        at::Tensor work = workspace(size, x);
+        check(qs_beam_select(x.data_ptr(), m.dtype, batch, beams, m.vocab, m.ld, scores, finished, chosen, &p,
+                             (float*)out.data_ptr(), (int*)parents.data_ptr(), (int*)tok.data_ptr(),
+                             (unsigned char*)done.data_ptr(), pointer(work), size, on.stream));
+        return pack({THPVariable_Wrap(out), THPVariable_Wrap(parents), THPVariable_Wrap(tok), THPVariable_Wrap(done)});
+    });
+}
+
+// A state's layout as nested levels: contiguous bytes, positions, and up to two levels around them.
+qs_states layout(const at::Tensor& t, int64_t dim, int64_t length_dim) {
+    struct Level { int64_t stride, count; };
+    std::vector<Level> levels;
+    qs_states s = {};
+    s.d_base = t.data_ptr();
+    s.unit = (long long)t.element_size();
+    s.outer[0] = s.outer[1] = s.positions = 1;
+    s.row_stride = t.stride(dim) * (int64_t)t.element_size();
+    for (int64_t d = 0; d < t.dim(); d++) {
+        if (d == dim || t.size(d) == 1) continue;
+        const Level l{t.stride(d) * (int64_t)t.element_size(), t.size(d)};
+        if (d == length_dim) {
+            s.positions = count("positions", l.count);
+            s.position_stride = l.stride;
+            continue;
+        }
+        auto at = levels.end();
+        while (at != levels.begin() && (at - 1)->stride > l.stride) --at;
+        levels.insert(at, l);
+    }
+    std::vector<Level> outer;
+    for (const Level& l : levels) {
+        if (outer.empty() && l.stride == s.unit) s.unit *= l.count;
+        else if (!outer.empty() && l.stride == outer.back().stride * outer.back().count) outer.back().count *= l.count;
+        else outer.push_back(l);
+    }
+    size_t i = 0;
+    if (length_dim < 0 && outer.size() == 3) {
+        s.positions = count("positions", outer[0].count);
+        s.position_stride = outer[0].stride;
+        i = 1;
+    }
+    if (outer.size() - i > 2) invalid("a state's layout has too many levels: " + shape_of(t));
+    for (int k = 1; i < outer.size(); i++, k--) {
+        s.outer[k] = count("a state's level", outer[i].count);
+        s.outer_stride[k] = outer[i].stride;
+    }
+    return s;
+}
+
+// (parents, states, dim, lengths, length_dim) -> None
+PyObject* beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return call(n, 5, [&] {
+        const at::Tensor& pa = tensor("parents", a[0]);
+        if (pa.dim() != 2) invalid("parents must be [batch, beams], got " + shape_of(pa));
+        const int batch = count("batch", pa.size(0)), beams = count("beams", pa.size(1));
+        const int* parents = table<int>("parents", a[0], at::kInt, batch, beams, pa);
+        if (!PyTuple_Check(a[1])) invalid("states must be a tuple of tensors");
+        const int64_t dim = whole(a[2]), length_dim = whole(a[4]);
+        const int* lengths = vector_or_none<int>("lengths", a[3], at::kInt, batch, pa);
+        std::vector<qs_states> all;
+        std::vector<const at::Tensor*> moved;
+        for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(a[1]); i++) {
+            const at::Tensor& t = tensor("a state", PyTuple_GET_ITEM(a[1], i));
+            const int64_t d = dim < 0 ? dim + t.dim() : dim, l = length_dim < 0 ? length_dim + t.dim() : length_dim;
+            if (d < 0 || d >= t.dim() || t.size(d) != (int64_t)batch * beams)
+                invalid("a state must have " + std::to_string(batch) + " x " + std::to_string(beams) + " rows in dimension " +
+                        std::to_string(dim) + ", got " + shape_of(t));
+            if (lengths && (l < 0 || l >= t.dim() || l == d))
+                invalid("a state's positions must be a dimension of its own beside its rows, got " + std::to_string(length_dim) +
+                        " of " + shape_of(t));
+            if (t.device() != pa.device()) invalid("a state must be on " + pa.device().str() + ", got " + told(t));
+            if (t.layout() != at::kStrided) invalid("a state must be a dense tensor");
+            if (t.numel() == 0) continue;
+            all.push_back(layout(t, d, lengths ? l : -1));
+            moved.push_back(&t);
+        }
+        const On on(pa);
+        check(qs_beam_reorder(all.data(), count("states", (int64_t)all.size()), parents, batch, beams, lengths, on.stream));
+        for (const at::Tensor* t : moved)  // autograd may hold a state for a backward: that has to fail now
+            if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+        Py_INCREF(Py_None);
+        return Py_None;
+    });
+}
+
 // (hidden [B, hidden_dim], norm_weight, codes, scales, zeros, vocab, hidden_dim, group, scale dtype) -> (normed, logits)
 PyObject* lm_head_w4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return call(n, 9, [&] {
@@ -322,7 +500,8 @@ PyObject* lm_head_w4(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(token_logprobs), FAST(token_logprobs_backward), FAST(policy_loss), FAST(preference_loss),
-                         FAST(lm_head_w4), {nullptr, nullptr, 0, nullptr}};
+                         FAST(lm_head_w4), FAST(top_logprobs), FAST(distill_loss), FAST(beam_select), FAST(beam_reorder),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch", "torch tensors to the C ABI of libqwen600_sampler.so", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
 

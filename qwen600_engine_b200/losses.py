@@ -6,7 +6,8 @@ csrc/qs_torch.cpp, checks the tensors and makes the buffers).
 returns beside a sampled token), ``token_logprobs_backward`` takes a gradient of
 those back to the logits.  ``policy_loss`` (clipped, with a KL term) and
 ``preference_loss`` (paired log ratios) return their loss and the gradient of
-the logits in one call.  The formulas stand in include/qwen600_sampler.h.
+the logits in one call.  ``top_logprobs`` lists each row's best tokens with their
+log-probabilities, and ``distill_loss`` learns from a teacher's lists.  The formulas stand in include/qwen600_sampler.h.
 
 Nothing these functions return has an autograd history, also where the logits
 require a gradient: ``loss.backward()`` raises, and in a sum with other losses
@@ -54,6 +55,17 @@ class PreferenceLoss(NamedTuple):
     grad: Optional[torch.Tensor]  # [rows, vocab] in the logits' type
 
 
+class TopLogprobs(NamedTuple):
+    logprobs: torch.Tensor  # fp32 [rows, k], -inf: none
+    tokens: torch.Tensor    # int32 [rows, k], -1: none
+
+
+class DistillLoss(NamedTuple):
+    loss: torch.Tensor            # fp32 scalar
+    row_losses: torch.Tensor      # fp32 [rows]
+    grad: Optional[torch.Tensor]  # [rows, vocab] in the logits' type
+
+
 def _on(stream, call, *args):
     """call(*args) on the current stream of the tensors' device, or on `stream`:
     buffers made by the call belong to it, and tensors used on it from another
@@ -66,8 +78,9 @@ def _on(stream, call, *args):
             raise SamplerError(QS_ERR_INVALID, f"stream of {stream.device} for tensors on {device}")
         if stream != torch.cuda.current_stream(device):
             for t in args:
-                if isinstance(t, torch.Tensor) and t.is_cuda:
-                    t.record_stream(stream)
+                for u in t if isinstance(t, tuple) else (t,):
+                    if isinstance(u, torch.Tensor) and u.is_cuda:
+                        u.record_stream(stream)
     with torch.cuda.stream(stream):
         return call(*args)
 
@@ -110,5 +123,29 @@ def preference_loss(logits, tokens, seq_offsets, ref_logprobs, *, beta: float = 
                                              weights, beta, label_smoothing, grad, out))
 
 
-__all__ = ["TokenLogprobs", "PolicyLoss", "PreferenceLoss", "token_logprobs", "token_logprobs_backward", "policy_loss",
-           "preference_loss"]
+def top_logprobs(logits, k: int, *, temperature: float = 1.0, stream=None) -> TopLogprobs:
+    """The ``k`` (up to 256) largest logits' tokens of each row, the larger first
+    and equal ones by token, and their log-probabilities: alternatives beside a
+    sampled token, or what ``distill_loss`` takes of a teacher.  Masked tokens
+    (-inf) are not listed: token -1 and log-probability -inf fill up."""
+    return tuple.__new__(TopLogprobs, _on(stream, _torch.top_logprobs, logits, k, temperature))
+
+
+def distill_loss(logits, teacher_tokens, teacher_logprobs, *, weights=None, temperature: float = 1.0, rest: bool = True,
+                 grad: bool = True, out=None, stream=None) -> DistillLoss:
+    """Divergence of the logits' distributions from a teacher's, of which each
+    row's best tokens are known (int32 and fp32 [rows, k], as ``top_logprobs``
+    gives them for the teacher's logits at the same temperature; a token outside
+    the vocabulary is no entry), summed over the rows with ``weights`` (default
+    1 / rows; 0 leaves a row out), and the gradient of the logits (``grad=False``:
+    the loss alone).  ``rest``: what the list leaves of the teacher's probability
+    is one more outcome, held against the sum of all unlisted tokens; without it
+    the listed probabilities are divided by their sum first (so that the
+    teacher's logits divided by the temperature do as well).  ``out`` takes the
+    gradient and may be ``logits``."""
+    return tuple.__new__(DistillLoss, _on(stream, _torch.distill_loss, logits, teacher_tokens, teacher_logprobs, weights,
+                                          temperature, rest, grad, out))
+
+
+__all__ = ["TokenLogprobs", "PolicyLoss", "PreferenceLoss", "TopLogprobs", "DistillLoss", "token_logprobs",
+           "token_logprobs_backward", "policy_loss", "preference_loss", "top_logprobs", "distill_loss"]

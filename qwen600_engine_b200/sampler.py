@@ -306,6 +306,20 @@ class Sampler:
                                               out.ctypes.data_as(C.POINTER(C.c_longlong)), int(n)))
         return out
 
+    def reorder_history(self, parents, *, stream=None) -> None:
+        """Moves the rows' windows and token counts to the beams that go on:
+        row ``b * beams + i`` takes those of row ``b * beams + parents[b, i]``
+        (int32 [batch, beams] device tensor, as ``beams.beam_select`` gives it;
+        one outside [0, beams) leaves its row as it is).  RNG states stay."""
+        torch = _torch()
+        p = parents
+        if not p.is_cuda or p.dtype != torch.int32 or p.dim() != 2 or not p.is_contiguous() or p.device.index != self.device:
+            raise SamplerError(_lib.QS_ERR_INVALID, f"parents must be a contiguous int32 tensor [batch, beams] on cuda:{self.device}")
+        st = stream if stream is not None else torch.cuda.current_stream(p.device)
+        if stream is not None:
+            p.record_stream(stream)
+        check(_lib.lib.qs_reorder_history(self._h, _ptr(p), int(p.shape[0]), int(p.shape[1]), int(st.cuda_stream)))
+
     def reset_history(self) -> None:
         check(_lib.lib.qs_reset_sampler_history(self._h))
 
