@@ -39,13 +39,22 @@ struct StreamArgs {
     float scale;
     double inv_t;
     int units;     // per row
-    T* lanes;      // best tokens: [rows][units][32], the maximum of each lane's part of a unit
+    T* lanes;      // best tokens: [rows][units][32], the maximum of each lane's part of a unit: 8 vectors behind one
+                   // another (and of a row's first unit what lies outside the vectors)
     float4* parts; // [rows][units]: maximum, sum of exponentials against it, how many 1s were left out of it
     RowScore* out;
     float* coefs;  // with out: set to 0
     float* logprobs;
     float* stats;
 };
+
+// The vector of a unit that a lane takes i-th: for logprobs the lanes' vectors lie
+// between one another's, for the best tokens a lane has 128 bytes of its own, taken
+// from another one on in each lane, which keeps the banks apart.
+template <bool kBest>
+__device__ __forceinline__ int vec_of(int i, int lane) {
+    return kBest ? lane * (kUnitVecs / 32) + ((i + lane) & (kUnitVecs / 32 - 1)) : i * 32 + lane;
+}
 
 // Where a warp is in its units: it takes every stride-th one.
 struct UnitAt {
@@ -134,7 +143,7 @@ stream_kernel(const __grid_constant__ StreamArgs<T> a) {
             uint4 u = Pack<T>::lowest();
 #pragma unroll
             for (int i = 0; i < kUnitVecs / 32; i++) {
-                const int k = i * 32 + lane;
+                const int k = vec_of<kBest>(i, lane);
                 v[i] = k < cnt ? mine[stage * kUnitVecs + k] : Pack<T>::lowest();
                 u.x = Pack<T>::max2(u.x, v[i].x);
                 u.y = Pack<T>::max2(u.y, v[i].y);
@@ -154,7 +163,7 @@ stream_kernel(const __grid_constant__ StreamArgs<T> a) {
             float again = 0.0f;  // this lane's share of the holder's elements
             int at_max = 0;
             if (one) {
-                const int k = (lane >> 2) * 32 + holder;
+                const int k = vec_of<kBest>(lane >> 2, holder);
                 const uint32_t word = k < cnt ? reinterpret_cast<const uint32_t*>(mine + stage * kUnitVecs + k)[lane & 3]
                                               : Pack<T>::lowest().x;
                 float e[kN / 4];
