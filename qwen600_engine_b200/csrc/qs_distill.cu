@@ -16,6 +16,10 @@
 namespace qs {
 
 constexpr int kDistillThreads = 256;
+// Where the unlisted terms against the list's maximum come out below or above these,
+// they are summed again against their own.  A term's exponent is rounded to a 2^-24th of
+// itself; with sums from 2^-28 on it lies on the average below log2 V + 28.
+constexpr double kLeastRest = 0x1p-28, kMostRest = 0x1p20;
 static_assert(QS_MAX_LISTED <= kDistillThreads, "one entry a thread");
 
 template <typename T>
@@ -31,197 +35,197 @@ struct DistillArgs {
     double inv_t;
     int rest;
     int log_c;    // 1 << log_c CTAs per row, one cluster
-    int buckets;  // of the table of listed tokens: a power of two, at least 2 k
+    int share;    // vectors of a CTA
+    int slots;    // k, in whole warps
     double* row_loss;
     float* row_losses;
     T* grad;
     long long gld;
 };
 
-// The slot of `tok` in the table of entries, or the first free one.
-__device__ __forceinline__ int table_slot(const int* table, const int* listed, int mask, int tok) {
-    int h = (int)((uint32_t)tok * 2654435769u >> 16) & mask;
-    while (true) {
-        const int e = *(const volatile int*)&table[h];
-        if (e < 0 || listed[e] == tok) return h;
-        h = (h + 1) & mask;
-    }
+// Writes v to *slot of the cluster's CTA `rank`.
+__device__ __forceinline__ void push_double(double* slot, int rank, double v) {
+    uint32_t addr;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                 : "=r"(addr)
+                 : "r"((uint32_t)__cvta_generic_to_shared(slot)), "r"(rank));
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
 }
 
-// Sum of one double per thread over the CTA, in a fixed order, in every thread.
-__device__ __forceinline__ double all_sum(double v, double* red) {
+__device__ __forceinline__ double warp_sum_double(double v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.0;
-#pragma unroll
-    for (int w = 0; w < kDistillThreads / 32; w++) v += red[w];
-    __syncthreads();
-    return v;
-}
-__device__ __forceinline__ float all_max(float v, float* red) {
-    v = warp_max(v);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = red[0];
-#pragma unroll
-    for (int w = 1; w < kDistillThreads / 32; w++) v = fmaxf(v, red[w]);
-    __syncthreads();
     return v;
 }
 
-// One row per cluster of 1 to 8 CTAs, as the policy loss has it: each CTA brings
-// a contiguous share of the row's 16-byte vectors to shared memory with one bulk
-// copy, the row is read once and the gradient formed from the same copy.  The
-// listed entries are read apart and their places in the shares overwritten with
-// -inf, which takes them out of the maximum, the sum and the gradient's stream;
-// every CTA does the small work on the list itself while its copy is under way.
+// One row per cluster of 1 to 8 CTAs.  Each CTA holds a contiguous share of the row's
+// 16-byte vectors in shared memory, each of its warps a piece of that: a warp brings
+// its piece with one bulk copy, sums it, and once the cluster has exchanged its sums
+// forms the gradient from the same copy, so that the row is read from memory once.  The
+// listed entries are read apart and their places in the pieces overwritten with -inf,
+// which takes them out of the sum and of the gradient's stream; every CTA does the
+// small work on the list itself while the copies are under way.
 template <typename T>
-__global__ void __launch_bounds__(kDistillThreads)
-distill_kernel(const __grid_constant__ DistillArgs<T> a, int share_vecs) {
+__global__ void __launch_bounds__(kDistillThreads, 5)
+distill_kernel(const __grid_constant__ DistillArgs<T> a) {
     constexpr int kN = Pack<T>::kN;
     constexpr int kW = kDistillThreads / 32;
-    extern __shared__ __align__(16) uint4 vecs[];
-    int* listed = reinterpret_cast<int*>(vecs + share_vecs);  // [k] token, -1: no entry
-    int* table = listed + a.k;                                // [buckets] entry, -1: none
-    __shared__ Part parts[8];
-    __shared__ double redd[kW];
-    __shared__ float red_max[kW], red_sum[kW];
-    __shared__ float factor_s, max_s;
-    __shared__ double of_p_s, of_q_s, top_s;
-    __shared__ unsigned long long loaded;
+    extern __shared__ __align__(16) uint4 vecs[];  // [warp][piece], then the list's tokens, logits and log-probabilities
+    __shared__ double parts[3][8], redd[3][kW], pass_sum[kW], mass_s, sl_s;
+    __shared__ float red_lp[kW], red_x[kW], red_max[kW];
+    __shared__ unsigned long long full[kW];
     __shared__ int gave_up;
-    const int t = threadIdx.x, C = 1 << a.log_c;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, C = 1 << a.log_c;
     const int row = blockIdx.x >> a.log_c, rank = blockIdx.x & (C - 1);
     const T* x = a.logits + (size_t)row * a.ld;
-    T* g = a.grad ? a.grad + (size_t)row * a.gld : nullptr;
-    const float w_row = a.weights ? a.weights[row] : 1.0f;
-    dependents_may_start();
-    // what the row is when it adds nothing
-    const auto nothing = [&] {
-        if (rank == 0 && t == 0) {
-            a.row_loss[row] = 0.0;
-            if (a.row_losses) a.row_losses[row] = 0.0f;
-        }
-        if (g) {
-            const RowShape<T> gs(g, a.V);
-            for (int i = rank * kDistillThreads + t; i < gs.vecs; i += C * kDistillThreads)
-                store16(g + gs.head + (size_t)i * kN, make_uint4(0u, 0u, 0u, 0u));
-            const int e = rank == 0 ? gs.edge(t, a.V) : -1;
-            if (e >= 0) put(g, e, 0.0f);
-        }
-    };
-    if (w_row == 0.0f) {  // alike for the whole cluster
-        nothing();
-        return;
-    }
-
-    const RowShape<T> sh(x, a.V);
-    const int per = (sh.vecs + C - 1) >> a.log_c;
-    const int first = min(rank * per, sh.vecs), cnt = min(per, sh.vecs - first);
-    if (t == 0) {
-        gave_up = 0;
-        mbar_init(&loaded, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_expect_tx(&loaded, (uint32_t)cnt * 16u);
-        if (cnt > 0)
-            asm volatile(
-                "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                    smem_u32(vecs)),
-                "l"(x + sh.head + (size_t)first * kN), "r"((uint32_t)cnt * 16u), "r"(smem_u32(&loaded))
-                : "memory");
-    }
-    if (C > 1) cluster_arrive_relaxed();  // waited for before the first store into another CTA
-
-    // the list: one entry a thread, each token where it stands first
+    // this thread's entry, requested beside the row's weight
     int tok = -1;
     float lp = -INFINITY;
     if (t < a.k) {
         tok = a.tokens[(size_t)row * a.k + t];
         lp = a.lps[(size_t)row * a.k + t];
-        if (tok < 0 || tok >= a.V) tok = -1;
-        listed[t] = tok;
     }
-    for (int i = t; i < a.buckets; i += kDistillThreads) table[i] = -1;
-    const int edge = rank == 0 ? sh.edge(t, a.V) : -1;
-    float xe = edge >= 0 ? elem(x, edge) : -INFINITY;
+    const float w_row = a.weights ? a.weights[row] : 1.0f;
+    dependents_may_start();
+    const auto nothing = [&] {  // what a row is that adds nothing
+        if (rank == 0 && t == 0) {
+            a.row_loss[row] = 0.0;
+            if (a.row_losses) a.row_losses[row] = 0.0f;
+        }
+        if (!a.grad) return;
+        T* g = a.grad + (size_t)row * a.gld;
+        const RowShape<T> gs(g, a.V);
+        for (int i = rank * kDistillThreads + t; i < gs.vecs; i += C * kDistillThreads)
+            store16(g + gs.head + (size_t)i * kN, make_uint4(0u, 0u, 0u, 0u));
+        const int e = rank == 0 ? gs.edge(t, a.V) : -1;
+        if (e >= 0) put(g, e, 0.0f);
+    };
+    if (w_row == 0.0f) {  // alike for the whole cluster
+        nothing();
+        return;
+    }
+    const int piece = (a.share + kW - 1) / kW;
+    uint4* mine = vecs + warp * piece;
+    int* list_token = reinterpret_cast<int*>(vecs + kW * piece);  // -1: no entry
+    float* list_x = reinterpret_cast<float*>(list_token + a.slots);
+    float* list_lp = list_x + a.slots;
+    const RowShape<T> sh(x, a.V);
+    const int begin = rank * a.share + warp * piece;
+    const int cnt = max(0, min(min(piece, a.share - warp * piece), sh.vecs - begin)), from = sh.head + begin * kN;
+    if (lane == 0) {
+        mbar_init(&full[warp], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_expect_tx(&full[warp], (uint32_t)cnt * 16u);
+        if (cnt > 0)
+            asm volatile(
+                "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(mine)),
+                "l"(x + from), "r"((uint32_t)cnt * 16u), "r"(smem_u32(&full[warp]))
+                : "memory");
+    }
+    if (C > 1) cluster_arrive_relaxed();  // waited for before the first store into another CTA
+    if (t == 0) gave_up = 0;
+
+    // the list: each token where it stands first
+    if (tok < 0 || tok >= a.V) tok = -1;
     const float xk = tok >= 0 ? elem(x, tok) : -INFINITY;
+    if (t < a.slots) {
+        list_token[t] = tok;
+        list_x[t] = xk;
+        list_lp[t] = lp;
+    }
+    const int edge = rank == 0 && warp == 0 ? sh.edge(lane, a.V) : -1;
+    float xe = edge >= 0 ? elem(x, edge) : -INFINITY;
     __syncthreads();
-    if (tok >= 0) {
-        while (true) {
-            const int h = table_slot(table, listed, a.buckets - 1, tok);
-            const int e = atomicCAS(&table[h], -1, t);
-            if (e < 0) break;
-            if (listed[e] == tok) {
-                atomicMin(&table[h], t);
-                break;
-            }
+    bool entry = tok >= 0;
+    if (warp * 32 < a.k) {
+        const int4* all = reinterpret_cast<const int4*>(list_token);
+        uint32_t again = 0;
+#pragma unroll 4
+        for (int j = 0; j < warp * 8 + 8; j++) {  // up to this warp's own
+            const int4 o = all[j];
+            again |= (o.x == tok && j * 4 < t) | (o.y == tok && j * 4 + 1 < t) | (o.z == tok && j * 4 + 2 < t) | (o.w == tok && j * 4 + 3 < t);
+        }
+        entry &= !again;
+    }
+    // the teacher's numbers; without a rest they count up to a common factor
+    const float top_lp = warp_max(entry ? lp : -INFINITY), top_x = warp_max(entry ? xk : -INFINITY);
+    if (lane == 0) {
+        red_lp[warp] = top_lp;
+        red_x[warp] = top_x;
+    }
+    const bool some = __syncthreads_or(entry && (a.rest || !(lp == -INFINITY)));
+    if (t < a.slots && !entry) list_token[t] = -1;
+    float shift = -INFINITY, ml = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kW; w++) {
+        shift = fmaxf(shift, red_lp[w]);
+        ml = fmaxf(ml, red_x[w]);
+    }
+    if (a.rest) shift = 0.0f;
+    {
+        double m = 0.0, c = 0.0, s = 0.0;
+        if (warp * 32 < a.k) {
+            const double q = entry ? exp((double)lp - (double)shift) : 0.0;
+            const double d = ((double)xk - (double)(ml == -INFINITY ? 0.0f : ml)) * a.inv_t;
+            m = warp_sum_double(q);                                                       // sum q
+            c = warp_sum_double(q == 0.0 ? 0.0 : q * ((double)lp - (double)shift - d));  // sum q (log q - d)
+            s = warp_sum_double(entry ? exp(d) : 0.0);
+        }
+        if (lane == 0) {
+            redd[0][warp] = m;
+            redd[1][warp] = c;
+            redd[2][warp] = s;
         }
     }
-    __syncthreads();
-    const bool entry = tok >= 0 && table[table_slot(table, listed, a.buckets - 1, tok)] == t;
-    if (edge >= 0 && table[table_slot(table, listed, a.buckets - 1, edge)] >= 0) xe = -INFINITY;
-    // the teacher's numbers; without a rest they count up to a common factor
-    const float shift = a.rest ? 0.0f : all_max(entry ? lp : -INFINITY, red_max);
-    const bool some = __syncthreads_or(entry && (a.rest || !(lp == -INFINITY)));
-    const float ml = all_max(entry ? xk : -INFINITY, red_max);
-    const double q = entry ? exp((double)lp - (double)shift) : 0.0;
-    const double d = ((double)xk - (double)(ml == -INFINITY ? 0.0f : ml)) * a.inv_t;
-    const double mass = all_sum(q, redd);                                                             // sum q
-    const double cost = all_sum(q == 0.0 ? 0.0 : q * ((double)lp - (double)shift - d), redd);         // sum q (log q - d)
-    const double sl = all_sum(entry ? exp(d) : 0.0, redd);
-    if (!mbar_wait(&loaded, 0, &gave_up, kLoadWaitNs))
-        mbar_wait(&loaded, 0, &gave_up, kLoadWaitNs, false);  // the copy lands before the CTA leaves
+    __syncthreads();  // the list is complete
+    if (!mbar_wait(&full[warp], 0, &gave_up, kLoadWaitNs))
+        mbar_wait(&full[warp], 0, &gave_up, kLoadWaitNs, false);  // the copy lands before the CTA leaves
     if (!some) {
+        __syncthreads();  // every warp's
         if (C > 1) cluster_wait();
         nothing();
         return;
     }
-    const int at = tok - sh.head - first * kN;  // in this CTA's share
-    const bool held = entry && at >= 0 && at < cnt * kN;
-    if (held) put(reinterpret_cast<T*>(vecs), at, -INFINITY);
-    __syncthreads();
 
-    // the maximum of this CTA's part
-    float own_max = xe;
-    {
-        uint4 u = Pack<T>::lowest();
-#pragma unroll 4
-        for (int k = t; k < cnt; k += kDistillThreads) {
-            const uint4 v = vecs[k];
-            u.x = Pack<T>::max2(u.x, v.x);
-            u.y = Pack<T>::max2(u.y, v.y);
-            u.z = Pack<T>::max2(u.z, v.z);
-            u.w = Pack<T>::max2(u.w, v.w);
-        }
-        float o[kN];
-        Pack<T>::widen(u, o);
-#pragma unroll
-        for (int j = 0; j < kN; j++) own_max = fmaxf(own_max, o[j]);
+    // the listed entries of this warp's piece, and of what lies outside the vectors
+    for (int e = lane; e < a.k; e += 32) {
+        const int token = list_token[e], at = token - from;
+        if (token >= 0 && at >= 0 && at < cnt * kN) put(reinterpret_cast<T*>(mine), at, -INFINITY);
     }
-    const float m = all_max(own_max, red_max);
-    const float ref = m == -INFINITY ? 0.0f : m;
+    if (edge >= 0)
+        for (int e = 0; e < a.k; e++)
+            if (list_token[e] == edge) xe = -INFINITY;
+    __syncwarp();
 
-    // the sum of exponentials against it: subtract and scale in one instruction where one_step allows it
-    const float bias = ref * a.scale;
-    float s;
-    if (!one_step(bias)) {
-        s = exp2_fast((xe - ref) * a.scale);
-        for (int k = t; k < cnt; k += kDistillThreads) {
-            float o[kN];
-            Pack<T>::widen(vecs[k], o);
-#pragma unroll
-            for (int j = 0; j < kN; j++) s += exp2_fast((o[j] - ref) * a.scale);
+    // v of this CTA's threads 0 to C - 1 to every CTA's slots, then all may read them
+    const auto exchange = [&](double* slots, double v) {
+        if (C == 1) {
+            if (t == 0) slots[0] = v;
+            __syncthreads();
+            return;
         }
-    } else {
-        const f32x2 scale2 = pair2(a.scale, a.scale), bias2 = pair2(-bias, -bias);
+        if (t < C) push_double(&slots[rank], t, v);
+        if (t < 32) cluster_arrive_release();
+        else cluster_arrive_relaxed();
+        cluster_wait();
+    };
+    const auto sum_of = [&](const double* v, int n) {
+        double s = 0.0;
+        for (int i = 0; i < n; i++) s += v[i];
+        return s;
+    };
+
+    // the sum against the list's maximum: subtract and scale in one instruction where one_step allows it
+    const f32x2 scale2 = pair2(a.scale, a.scale);
+    float ref = ml, bias = ref * a.scale, s = INFINITY;
+    if (one_step(bias)) {
+        const f32x2 bias2 = pair2(-bias, -bias);
         f32x2 s2 = pair2(exp2_fast(__fmaf_rn(xe, a.scale, -bias)), 0.0f);
 #pragma unroll 2
-        for (int k = t; k < cnt; k += kDistillThreads) {
+        for (int k = lane; k < cnt; k += 32) {
             float o[kN];
-            Pack<T>::widen(vecs[k], o);
+            Pack<T>::widen(mine[k], o);
 #pragma unroll
             for (int j = 0; j < kN; j += 2) s2 = add2(s2, exp2_pair(fma2(pair2(o[j], o[j + 1]), scale2, bias2)));
         }
@@ -229,76 +233,93 @@ distill_kernel(const __grid_constant__ DistillArgs<T> a, int share_vecs) {
         s = (u.x + u.y) * exp2_fast(-__fmaf_rn(ref, a.scale, -bias));
     }
     s = warp_sum(s);
-    if ((t & 31) == 0) red_sum[t >> 5] = s;
+    if (lane == 0) pass_sum[warp] = *(volatile int*)&gave_up ? (double)NAN : (double)s;
     __syncthreads();
     if (C > 1) cluster_wait();  // every CTA of the cluster runs
-    if (t < C) {
-        Part p{m, 0, *(volatile int*)&gave_up ? (double)NAN : 0.0};
-        for (int w = 0; w < kW; w++) p.others += (double)red_sum[w];
-        if (C > 1) push_part(&parts[rank], t, p);
-        else parts[0] = p;
-    }
-    if (C > 1) {  // only the warp that stored into the others has stores to release
-        if (t < 32) cluster_arrive_release();
-        else cluster_arrive_relaxed();
-        cluster_wait();
-    }
-    if (t < 32) {
-        __syncwarp();
-        const Part p = t < C ? parts[t] : Part{-INFINITY, 0, 0.0};
-        const float mr = warp_max(p.max);
-        double sr = p.max == mr ? p.others : t < C ? exp(((double)p.max - (double)mr) * a.inv_t) * p.others : 0.0;
+    if (t == 64) mass_s = sum_of(redd[0], kW);
+    if (t == 96) sl_s = sum_of(redd[2], kW);
+    // the two are in order for this CTA's threads with the exchange: all of them arrive after their stores
+    if (C > 1 && (t == 64 || t == 96)) __threadfence_block();
+    exchange(parts[0], t < C ? sum_of(pass_sum, kW) : 0.0);
+    double sr = sum_of(parts[0], C);
+    double top = ref, dl = 0.0, dr = 0.0;  // the row's maximum, and the list's and the others' distances from it
+    const double least = a.rest ? kLeastRest : 0.0;
+    const bool far = !(sr >= least && sr <= kMostRest);
+    if (far) {
+        // the unlisted tokens against their own maximum
+        float m = xe;
+        for (int k = lane; k < cnt; k += 32) {
+            float o[kN];
+            Pack<T>::widen(mine[k], o);
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) sr += __shfl_xor_sync(0xffffffffu, sr, o);
-        if (t == 0) {
-            const double top = fmax((double)mr, (double)ml);
-            const double dr = mr == -INFINITY ? -(double)INFINITY : ((double)mr - top) * a.inv_t;
-            const double dl = ml == -INFINITY ? -(double)INFINITY : ((double)ml - top) * a.inv_t;
-            // an infinite maximum has no distribution; a NaN among the unlisted logits is in sr, one among the listed in sl
-            const double total = isinf(top) ? (double)NAN : sl * exp(dl) + sr * exp(dr);
-            const double log_total = log(total);
-            double left = 0.0, l;
-            if (a.rest) {
-                if (mass < 1.0 && !(mr == -INFINITY && sr == 0.0)) left = 1.0 - mass;
-                // the distance of d's reference from the row's, as log p has it: -inf - -inf where the logits mask the whole list
-                l = cost + (mass == 0.0 ? 0.0 : mass * (log_total - (ml == -INFINITY ? -top * a.inv_t : dl)));
-                if (left > 0.0) l += left * (log(left) - (dr + log(sr) - log_total));
-            } else {
-                l = cost / mass - log(mass) + log_total - (ml == -INFINITY ? -top * a.inv_t : dl);
-            }
-            const double w = a.weights ? (double)w_row : 1.0 / a.rows;
-            if (rank == 0) {
-                a.row_loss[row] = w * l;
-                if (a.row_losses) a.row_losses[row] = (float)l;
-            }
-            const double c = w * a.inv_t, norm = a.rest ? mass + left : mass / mass;  // NaN from the teacher reaches the row
-            of_p_s = c * norm / total;
-            of_q_s = a.rest ? c : c / mass;
-            top_s = top;
-            factor_s = (float)(c * (norm * exp(dr) / total - (left > 0.0 ? left / sr : 0.0)));
-            max_s = mr;
+            for (int j = 0; j < kN; j++) m = fmaxf(m, o[j]);
         }
+        m = warp_max(m);
+        if (lane == 0) red_max[warp] = m;
+        __syncthreads();
+        for (int w = 0; w < kW; w++) m = fmaxf(m, red_max[w]);
+        exchange(parts[1], (double)m);
+        ref = -INFINITY;
+        for (int c = 0; c < C; c++) ref = fmaxf(ref, (float)parts[1][c]);
+        const float zero = ref == -INFINITY ? 0.0f : ref;
+        s = exp2_fast((xe - zero) * a.scale);
+        for (int k = lane; k < cnt; k += 32) {
+            float o[kN];
+            Pack<T>::widen(mine[k], o);
+#pragma unroll
+            for (int j = 0; j < kN; j++) s += exp2_fast((o[j] - zero) * a.scale);
+        }
+        s = warp_sum(s);
+        if (lane == 0) pass_sum[warp] = *(volatile int*)&gave_up ? (double)NAN : (double)s;
+        __syncthreads();
+        exchange(parts[2], t < C ? sum_of(pass_sum, kW) : 0.0);
+        sr = sum_of(parts[2], C);
+        top = fmax((double)ref, (double)ml);
+        dr = ref == -INFINITY ? -(double)INFINITY : ((double)ref - top) * a.inv_t;
+        dl = ml == -INFINITY ? -(double)INFINITY : ((double)ml - top) * a.inv_t;
     }
-    if (!g) return;
-    __syncthreads();
-    float f = factor_s;
-    const float mr = max_s, top = mr * a.scale;
-    const bool plain = one_step(top);
-    if (plain) f *= exp2_fast(-__fmaf_rn(mr, a.scale, -top));
+    const double mass = mass_s, c = (a.weights ? (double)w_row : 1.0 / a.rows) * a.inv_t;
+    // an infinite maximum has no distribution; a NaN among the unlisted logits is in sr, one among the listed in sl
+    const double total = isinf(top) ? (double)NAN : far ? sl_s * exp(dl) + sr * exp(dr) : sl_s + sr;
+    const double left = a.rest && mass < 1.0 && !(ref == -INFINITY && sr == 0.0) ? 1.0 - mass : 0.0;
+    const double norm = a.rest ? mass + left : mass / mass;  // NaN from the teacher reaches the row
+    if (rank == 0 && t == kDistillThreads - 32) {
+        const double log_total = log(total), cost = sum_of(redd[1], kW);
+        // cost counts from the list's maximum (from 0 where all of it is masked), log p from the row's
+        const double away = log_total - (ml == -INFINITY ? -top * a.inv_t : dl);
+        double l;
+        if (a.rest) {
+            l = cost + (mass == 0.0 ? 0.0 : mass * away);
+            if (left > 0.0) l += left * (log(left) - (dr + log(sr) - log_total));
+        } else {
+            l = cost / mass - log(mass) + away;
+        }
+        a.row_loss[row] = l * (a.weights ? (double)w_row : 1.0 / a.rows);
+        if (a.row_losses) a.row_losses[row] = (float)l;
+    }
+    if (!a.grad) return;
+
+    // of every unlisted token; its two parts in fp32, which the sums' precision bears
+    float f = (float)(c * norm) / (float)total;
+    if (far) f *= (float)exp(dr);
+    if (left > 0.0) f -= (float)(c * left) / (float)sr;
+    bias = ref * a.scale;
+    const bool plain = one_step(bias);
+    if (plain) f *= exp2_fast(-__fmaf_rn(ref, a.scale, -bias));
     const auto grad_of = [&](float v) {
-        return f == 0.0f ? 0.0f : f * exp2_fast(plain ? __fmaf_rn(v, a.scale, -top) : (v - mr) * a.scale);
+        return f == 0.0f ? 0.0f : f * exp2_fast(plain ? __fmaf_rn(v, a.scale, -bias) : (v - ref) * a.scale);
     };
-    const f32x2 f2 = pair2(f, f), scale2 = pair2(a.scale, a.scale), top2 = pair2(-top, -top);
+    T* g = a.grad + (size_t)row * a.gld;
+    const f32x2 f2 = pair2(f, f), bias2 = pair2(-bias, -bias);
     const bool aligned = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
-    T* gbody = g + sh.head + (size_t)first * kN;
 #pragma unroll 2
-    for (int k = t; k < cnt; k += kDistillThreads) {
+    for (int k = lane; k < cnt; k += 32) {
         float o[kN];
-        Pack<T>::widen(vecs[k], o);
+        Pack<T>::widen(mine[k], o);
         if (plain && f != 0.0f) {
 #pragma unroll
             for (int j = 0; j < kN; j += 2) {
-                const float2 r = unpair2(mul2(f2, exp2_pair(fma2(pair2(o[j], o[j + 1]), scale2, top2))));
+                const float2 r = unpair2(mul2(f2, exp2_pair(fma2(pair2(o[j], o[j + 1]), scale2, bias2))));
                 o[j] = r.x;
                 o[j + 1] = r.y;
             }
@@ -307,22 +328,28 @@ distill_kernel(const __grid_constant__ DistillArgs<T> a, int share_vecs) {
             for (int j = 0; j < kN; j++) o[j] = grad_of(o[j]);
         }
         if (aligned) {
-            store16(gbody + (size_t)k * kN, Pack<T>::narrow(o));
+            store16(g + from + (size_t)k * kN, Pack<T>::narrow(o));
         } else {
 #pragma unroll
-            for (int j = 0; j < kN; j++) put(gbody, (long long)k * kN + j, o[j]);
+            for (int j = 0; j < kN; j++) put(g + from, (long long)k * kN + j, o[j]);
         }
     }
     if (edge >= 0) put(g, edge, grad_of(xe));
-    __syncthreads();  // the listed ones over what the stream left in their places
-    const bool outside = rank == 0 && (tok < sh.head || tok >= sh.head + sh.vecs * kN);
-    if (entry && (held || outside))
-        put(g, tok, (float)(of_p_s * exp(xk == -INFINITY ? -(double)INFINITY : ((double)xk - top_s) * a.inv_t) - of_q_s * q));
+    __syncwarp();  // then the listed ones, over what the stream left in their places
+    for (int e = lane; e < a.k; e += 32) {
+        const int token = list_token[e], at = token - from;
+        const bool outside = rank == 0 && warp == 0 && (token < sh.head || token >= sh.head + sh.vecs * kN);
+        if (token < 0 || !(outside || (at >= 0 && at < cnt * kN))) continue;
+        const float v = list_x[e];
+        const double q = exp((double)list_lp[e] - (double)shift);
+        const double p = norm / total * exp(v == -INFINITY ? -(double)INFINITY : ((double)v - top) * a.inv_t);
+        put(g, token, (float)(c * (p - (a.rest ? q : q / mass))));
+    }
 }
 
-// How a row is spread: as the policy loss's rows (qs_losses.cu), CTAs per row
-// doubled while a share is above 40 KB, and while the rows alone would leave some
-// of the 148 SMs idle and a share keeps 4 KB.
+// How rows are spread: as the policy loss's (qs_losses.cu), CTAs per row doubled
+// while a share is above 40 KB, and while the rows alone would leave some of the 148
+// SMs idle and a share keeps 4 KB.
 template <typename T>
 static int distill_launch(DistillArgs<T>& a, cudaStream_t st) {
     const int vecs = a.V / Pack<T>::kN;
@@ -330,14 +357,13 @@ static int distill_launch(DistillArgs<T>& a, cudaStream_t st) {
     const auto share = [&] { return (vecs + (1 << log_c) - 1) >> log_c; };
     while (log_c < 3 && (share() > 2560 || ((long long)a.rows << log_c) < 148 && share() > 256)) log_c++;
     a.log_c = log_c;
-    a.buckets = 2;
-    while (a.buckets < 2 * a.k) a.buckets *= 2;
-    const size_t smem = (size_t)share() * 16 + (a.k + a.buckets) * sizeof(int);
+    a.share = share();
+    a.slots = (a.k + 31) & ~31;
+    const size_t smem = (size_t)((a.share + 7) / 8 * 8) * 16 + 3 * sizeof(int) * a.slots;
     static DeviceOnce once;
     const int rc = once.raise((const void*)distill_kernel<T>, 200 * 1024);
     if (rc) return rc;
-    return launch("distill_kernel", distill_kernel<T>, (long long)a.rows << log_c, kDistillThreads, 1 << log_c, smem, false, st, a,
-                  share());
+    return launch("distill_kernel", distill_kernel<T>, (long long)a.rows << log_c, kDistillThreads, 1 << log_c, smem, false, st, a);
 }
 
 }  // namespace qs
