@@ -586,7 +586,7 @@ typedef struct {
     int rest;
 } qs_distill_params;
 
-QS_API size_t qs_distill_loss_workspace(int rows);
+QS_API size_t qs_distill_loss_workspace(int rows, int k);
 QS_API int qs_distill_loss(const void* d_logits, int dtype, int rows, int vocab, long long row_stride,
                            const int* d_teacher_tokens, const float* d_teacher_logprobs, int k,
                            const float* d_weights, const qs_distill_params* params, float* d_loss,

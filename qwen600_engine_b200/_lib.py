@@ -168,7 +168,7 @@ def _load() -> C.CDLL:
     lib.qs_beam_select.argtypes = [vp, i32, i32, i32, i32, i64, vp, vp, i32, P(BeamParams), vp, vp, vp, vp, vp, sz, vp]
     lib.qs_beam_reorder.argtypes = [P(States), i32, vp, i32, i32, vp, vp]
     lib.qs_reorder_history.argtypes = [vp, vp, i32, i32, vp]
-    lib.qs_distill_loss_workspace.argtypes = [i32]
+    lib.qs_distill_loss_workspace.argtypes = [i32, i32]
     lib.qs_distill_loss.argtypes = [vp, i32, i32, i32, i64, vp, vp, i32, vp, P(DistillParams), vp, vp, vp, i64, vp, sz, vp]
     lib.qs_last_error.restype = C.c_char_p
     lib.qs_last_error.argtypes = []

@@ -22,6 +22,16 @@ constexpr int kDistillThreads = 256;
 constexpr double kLeastRest = 0x1p-28, kMostRest = 0x1p20;
 static_assert(QS_MAX_LISTED <= kDistillThreads, "one entry a thread");
 
+// A row's list as the list kernel leaves it.  Its entries follow: tokens (int), then
+// exp((x - m_l) / T) and q of each (double).
+struct __align__(16) RowList {
+    double mass;  // sum q
+    double cost;  // sum q (log q - (x - m_l) / T); where the logits mask all of it, of q (log q - x / T)
+    double sl;    // S_l
+    float ml;
+    int some;     // the row adds something
+};
+
 template <typename T>
 struct DistillArgs {
     const T* logits;
@@ -36,12 +46,101 @@ struct DistillArgs {
     int rest;
     int log_c;    // 1 << log_c CTAs per row, one cluster
     int share;    // vectors of a CTA
-    int slots;    // k, in whole warps
+    RowList* lists;
+    double* list_p;   // [rows][k] exp((x - m_l) / T)
+    double* list_q;   // [rows][k]
+    int* list_token;  // [rows][k] -1: no entry
     double* row_loss;
     float* row_losses;
     T* grad;
     long long gld;
 };
+
+__device__ __forceinline__ double warp_sum_double(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// The lists, a warp for a row: each token where it stands first, its logit, and what
+// the loss takes of both.  Once for a row, where the row's CTAs would all have to; a
+// launch of 3 us, which they begin beside.
+constexpr int kListWarps = 4;
+constexpr int kListMine = QS_MAX_LISTED / 32;
+
+template <typename T>
+__global__ void __launch_bounds__(kListWarps * 32)
+distill_list_kernel(const __grid_constant__ DistillArgs<T> a) {
+    __shared__ __align__(16) int tokens[kListWarps][QS_MAX_LISTED];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * kListWarps + warp;
+    dependents_may_start();
+    if (row >= a.rows || (a.weights && a.weights[row] == 0.0f)) return;
+    const T* x = a.logits + (size_t)row * a.ld;
+    const size_t at = (size_t)row * a.k;
+    int tok[kListMine];
+    float lp[kListMine], v[kListMine];
+#pragma unroll
+    for (int i = 0; i < kListMine; i++) {
+        const int e = i * 32 + lane;
+        tok[i] = e < a.k ? a.tokens[at + e] : -1;
+        lp[i] = e < a.k ? a.lps[at + e] : -INFINITY;
+        if (tok[i] < 0 || tok[i] >= a.V) tok[i] = -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kListMine; i++) {
+        v[i] = tok[i] >= 0 ? elem(x, tok[i]) : -INFINITY;
+        tokens[warp][i * 32 + lane] = tok[i];
+    }
+    __syncwarp();
+    // without a rest the teacher's numbers count up to a common factor
+    float ml = -INFINITY, shift = -INFINITY;
+    bool some = false;
+#pragma unroll
+    for (int i = 0; i < kListMine; i++) {
+        const int e = i * 32 + lane;
+        if (i * 32 >= a.k) break;
+        const int4* all = reinterpret_cast<const int4*>(tokens[warp]);
+        bool again = false;
+        for (int j = 0; j < i * 8 + 8; j++) {
+            const int4 o = all[j];
+            again |= (o.x == tok[i] && j * 4 < e) | (o.y == tok[i] && j * 4 + 1 < e) | (o.z == tok[i] && j * 4 + 2 < e) |
+                     (o.w == tok[i] && j * 4 + 3 < e);
+        }
+        if (again) tok[i] = -1;
+        if (tok[i] < 0) continue;
+        ml = fmaxf(ml, v[i]);
+        shift = fmaxf(shift, lp[i]);
+        some |= a.rest || !(lp[i] == -INFINITY);
+    }
+    ml = warp_max(ml);
+    shift = a.rest ? 0.0f : warp_max(shift);
+    some = __any_sync(0xffffffffu, some);
+    const double from = ml == -INFINITY ? 0.0 : (double)ml;
+    double mass = 0.0, cost = 0.0, sl = 0.0;
+#pragma unroll
+    for (int i = 0; i < kListMine; i++) {
+        const int e = i * 32 + lane;
+        if (i * 32 >= a.k) break;
+        double q = 0.0, p = 0.0;
+        if (tok[i] >= 0) {
+            const double l = (double)lp[i] - (double)shift, d = ((double)v[i] - from) * a.inv_t;
+            q = exp(l);
+            p = exp(d);
+            if (q != 0.0) cost += q * (l - d);
+        }
+        mass += q;
+        sl += p;
+        if (e < a.k) {
+            a.list_token[at + e] = tok[i];
+            a.list_p[at + e] = p;
+            a.list_q[at + e] = q;
+        }
+    }
+    mass = warp_sum_double(mass);
+    cost = warp_sum_double(cost);
+    sl = warp_sum_double(sl);
+    if (lane == 0) a.lists[row] = RowList{mass, cost, sl, ml, some};
+}
 
 // Writes v to *slot of the cluster's CTA `rank`.
 __device__ __forceinline__ void push_double(double* slot, int rank, double v) {
@@ -52,39 +151,25 @@ __device__ __forceinline__ void push_double(double* slot, int rank, double v) {
     asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
 }
 
-__device__ __forceinline__ double warp_sum_double(double v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
 // One row per cluster of 1 to 8 CTAs.  Each CTA holds a contiguous share of the row's
 // 16-byte vectors in shared memory, each of its warps a piece of that: a warp brings
 // its piece with one bulk copy, sums it, and once the cluster has exchanged its sums
-// forms the gradient from the same copy, so that the row is read from memory once.  The
-// listed entries are read apart and their places in the pieces overwritten with -inf,
-// which takes them out of the sum and of the gradient's stream; every CTA does the
-// small work on the list itself while the copies are under way.
+// forms the gradient from the same copy, so that the row is read from memory once and
+// a CTA's warps meet once.  The listed entries' places in the pieces are overwritten
+// with -inf, which takes them out of the sum and of the gradient's stream.
 template <typename T>
 __global__ void __launch_bounds__(kDistillThreads, 5)
 distill_kernel(const __grid_constant__ DistillArgs<T> a) {
     constexpr int kN = Pack<T>::kN;
     constexpr int kW = kDistillThreads / 32;
-    extern __shared__ __align__(16) uint4 vecs[];  // [warp][piece], then the list's tokens, logits and log-probabilities
-    __shared__ double parts[3][8], redd[3][kW], pass_sum[kW], mass_s, sl_s;
-    __shared__ float red_lp[kW], red_x[kW], red_max[kW];
+    extern __shared__ __align__(16) uint4 vecs[];  // [warp][piece]
+    __shared__ double parts[3][8], pass_sum[kW];
+    __shared__ float red_max[kW];
     __shared__ unsigned long long full[kW];
     __shared__ int gave_up;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, C = 1 << a.log_c;
     const int row = blockIdx.x >> a.log_c, rank = blockIdx.x & (C - 1);
     const T* x = a.logits + (size_t)row * a.ld;
-    // this thread's entry, requested beside the row's weight
-    int tok = -1;
-    float lp = -INFINITY;
-    if (t < a.k) {
-        tok = a.tokens[(size_t)row * a.k + t];
-        lp = a.lps[(size_t)row * a.k + t];
-    }
     const float w_row = a.weights ? a.weights[row] : 1.0f;
     dependents_may_start();
     const auto nothing = [&] {  // what a row is that adds nothing
@@ -106,9 +191,6 @@ distill_kernel(const __grid_constant__ DistillArgs<T> a) {
     }
     const int piece = (a.share + kW - 1) / kW;
     uint4* mine = vecs + warp * piece;
-    int* list_token = reinterpret_cast<int*>(vecs + kW * piece);  // -1: no entry
-    float* list_x = reinterpret_cast<float*>(list_token + a.slots);
-    float* list_lp = list_x + a.slots;
     const RowShape<T> sh(x, a.V);
     const int begin = rank * a.share + warp * piece;
     const int cnt = max(0, min(min(piece, a.share - warp * piece), sh.vecs - begin)), from = sh.head + begin * kN;
@@ -125,63 +207,28 @@ distill_kernel(const __grid_constant__ DistillArgs<T> a) {
     }
     if (C > 1) cluster_arrive_relaxed();  // waited for before the first store into another CTA
     if (t == 0) gave_up = 0;
-
-    // the list: each token where it stands first
-    if (tok < 0 || tok >= a.V) tok = -1;
-    const float xk = tok >= 0 ? elem(x, tok) : -INFINITY;
-    if (t < a.slots) {
-        list_token[t] = tok;
-        list_x[t] = xk;
-        list_lp[t] = lp;
-    }
     const int edge = rank == 0 && warp == 0 ? sh.edge(lane, a.V) : -1;
     float xe = edge >= 0 ? elem(x, edge) : -INFINITY;
-    __syncthreads();
-    bool entry = tok >= 0;
-    if (warp * 32 < a.k) {
-        const int4* all = reinterpret_cast<const int4*>(list_token);
-        uint32_t again = 0;
-#pragma unroll 4
-        for (int j = 0; j < warp * 8 + 8; j++) {  // up to this warp's own
-            const int4 o = all[j];
-            again |= (o.x == tok && j * 4 < t) | (o.y == tok && j * 4 + 1 < t) | (o.z == tok && j * 4 + 2 < t) | (o.w == tok && j * 4 + 3 < t);
-        }
-        entry &= !again;
-    }
-    // the teacher's numbers; without a rest they count up to a common factor
-    const float top_lp = warp_max(entry ? lp : -INFINITY), top_x = warp_max(entry ? xk : -INFINITY);
-    if (lane == 0) {
-        red_lp[warp] = top_lp;
-        red_x[warp] = top_x;
-    }
-    const bool some = __syncthreads_or(entry && (a.rest || !(lp == -INFINITY)));
-    if (t < a.slots && !entry) list_token[t] = -1;
-    float shift = -INFINITY, ml = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kW; w++) {
-        shift = fmaxf(shift, red_lp[w]);
-        ml = fmaxf(ml, red_x[w]);
-    }
-    if (a.rest) shift = 0.0f;
-    {
-        double m = 0.0, c = 0.0, s = 0.0;
-        if (warp * 32 < a.k) {
-            const double q = entry ? exp((double)lp - (double)shift) : 0.0;
-            const double d = ((double)xk - (double)(ml == -INFINITY ? 0.0f : ml)) * a.inv_t;
-            m = warp_sum_double(q);                                                       // sum q
-            c = warp_sum_double(q == 0.0 ? 0.0 : q * ((double)lp - (double)shift - d));  // sum q (log q - d)
-            s = warp_sum_double(entry ? exp(d) : 0.0);
-        }
-        if (lane == 0) {
-            redd[0][warp] = m;
-            redd[1][warp] = c;
-            redd[2][warp] = s;
+    wait_for_previous();
+    const RowList list = a.lists[row];
+    const int* list_token = a.list_token + (size_t)row * a.k;
+    const float ml = list.ml;
+    // this lane's entries that lie in the warp's piece, or outside the vectors; requested again at the end
+    uint32_t own = 0;
+    const bool outside = rank == 0 && warp == 0;
+    for (int i = 0; i * 32 < a.k; i++) {
+        const int e = i * 32 + lane, token = e < a.k ? list_token[e] : -1, at = token - from;
+        if (token < 0) continue;
+        if ((at >= 0 && at < cnt * kN) || (outside && (token < sh.head || token >= sh.head + sh.vecs * kN))) {
+            own |= 1u << i;
+            asm volatile("prefetch.global.L1 [%0];" ::"l"(a.list_p + (size_t)row * a.k + e));
+            asm volatile("prefetch.global.L1 [%0];" ::"l"(a.list_q + (size_t)row * a.k + e));
         }
     }
-    __syncthreads();  // the list is complete
+    __syncthreads();  // gave_up, and each warp's barrier for all of its lanes
     if (!mbar_wait(&full[warp], 0, &gave_up, kLoadWaitNs))
         mbar_wait(&full[warp], 0, &gave_up, kLoadWaitNs, false);  // the copy lands before the CTA leaves
-    if (!some) {
+    if (!list.some) {
         __syncthreads();  // every warp's
         if (C > 1) cluster_wait();
         nothing();
@@ -189,9 +236,9 @@ distill_kernel(const __grid_constant__ DistillArgs<T> a) {
     }
 
     // the listed entries of this warp's piece, and of what lies outside the vectors
-    for (int e = lane; e < a.k; e += 32) {
-        const int token = list_token[e], at = token - from;
-        if (token >= 0 && at >= 0 && at < cnt * kN) put(reinterpret_cast<T*>(mine), at, -INFINITY);
+    for (uint32_t m = own; m; m &= m - 1) {
+        const int at = list_token[(__ffs(m) - 1) * 32 + lane] - from;
+        if (at >= 0 && at < cnt * kN) put(reinterpret_cast<T*>(mine), at, -INFINITY);
     }
     if (edge >= 0)
         for (int e = 0; e < a.k; e++)
@@ -206,7 +253,7 @@ distill_kernel(const __grid_constant__ DistillArgs<T> a) {
             return;
         }
         if (t < C) push_double(&slots[rank], t, v);
-        if (t < 32) cluster_arrive_release();
+        if (t < 32) cluster_arrive_release();  // only this warp has stores to release
         else cluster_arrive_relaxed();
         cluster_wait();
     };
@@ -236,10 +283,6 @@ distill_kernel(const __grid_constant__ DistillArgs<T> a) {
     if (lane == 0) pass_sum[warp] = *(volatile int*)&gave_up ? (double)NAN : (double)s;
     __syncthreads();
     if (C > 1) cluster_wait();  // every CTA of the cluster runs
-    if (t == 64) mass_s = sum_of(redd[0], kW);
-    if (t == 96) sl_s = sum_of(redd[2], kW);
-    // the two are in order for this CTA's threads with the exchange: all of them arrive after their stores
-    if (C > 1 && (t == 64 || t == 96)) __threadfence_block();
     exchange(parts[0], t < C ? sum_of(pass_sum, kW) : 0.0);
     double sr = sum_of(parts[0], C);
     double top = ref, dl = 0.0, dr = 0.0;  // the row's maximum, and the list's and the others' distances from it
@@ -278,23 +321,23 @@ distill_kernel(const __grid_constant__ DistillArgs<T> a) {
         dr = ref == -INFINITY ? -(double)INFINITY : ((double)ref - top) * a.inv_t;
         dl = ml == -INFINITY ? -(double)INFINITY : ((double)ml - top) * a.inv_t;
     }
-    const double mass = mass_s, c = (a.weights ? (double)w_row : 1.0 / a.rows) * a.inv_t;
+    const double w = a.weights ? (double)w_row : 1.0 / a.rows, c = w * a.inv_t;
     // an infinite maximum has no distribution; a NaN among the unlisted logits is in sr, one among the listed in sl
-    const double total = isinf(top) ? (double)NAN : far ? sl_s * exp(dl) + sr * exp(dr) : sl_s + sr;
-    const double left = a.rest && mass < 1.0 && !(ref == -INFINITY && sr == 0.0) ? 1.0 - mass : 0.0;
-    const double norm = a.rest ? mass + left : mass / mass;  // NaN from the teacher reaches the row
+    const double total = isinf(top) ? (double)NAN : far ? list.sl * exp(dl) + sr * exp(dr) : list.sl + sr;
+    const double left = a.rest && list.mass < 1.0 && !(ref == -INFINITY && sr == 0.0) ? 1.0 - list.mass : 0.0;
+    const double norm = a.rest ? list.mass + left : list.mass / list.mass;  // NaN from the teacher reaches the row
     if (rank == 0 && t == kDistillThreads - 32) {
-        const double log_total = log(total), cost = sum_of(redd[1], kW);
+        const double log_total = log(total);
         // cost counts from the list's maximum (from 0 where all of it is masked), log p from the row's
         const double away = log_total - (ml == -INFINITY ? -top * a.inv_t : dl);
         double l;
         if (a.rest) {
-            l = cost + (mass == 0.0 ? 0.0 : mass * away);
+            l = list.cost + (list.mass == 0.0 ? 0.0 : list.mass * away);
             if (left > 0.0) l += left * (log(left) - (dr + log(sr) - log_total));
         } else {
-            l = cost / mass - log(mass) + away;
+            l = list.cost / list.mass - log(list.mass) + away;
         }
-        a.row_loss[row] = l * (a.weights ? (double)w_row : 1.0 / a.rows);
+        a.row_loss[row] = w * l;
         if (a.row_losses) a.row_losses[row] = (float)l;
     }
     if (!a.grad) return;
@@ -336,14 +379,10 @@ distill_kernel(const __grid_constant__ DistillArgs<T> a) {
     }
     if (edge >= 0) put(g, edge, grad_of(xe));
     __syncwarp();  // then the listed ones, over what the stream left in their places
-    for (int e = lane; e < a.k; e += 32) {
-        const int token = list_token[e], at = token - from;
-        const bool outside = rank == 0 && warp == 0 && (token < sh.head || token >= sh.head + sh.vecs * kN);
-        if (token < 0 || !(outside || (at >= 0 && at < cnt * kN))) continue;
-        const float v = list_x[e];
-        const double q = exp((double)list_lp[e] - (double)shift);
-        const double p = norm / total * exp(v == -INFINITY ? -(double)INFINITY : ((double)v - top) * a.inv_t);
-        put(g, token, (float)(c * (p - (a.rest ? q : q / mass))));
+    for (uint32_t m = own; m; m &= m - 1) {
+        const int e = (__ffs(m) - 1) * 32 + lane, token = list_token[e];
+        const double p = a.list_p[(size_t)row * a.k + e], q = a.list_q[(size_t)row * a.k + e];
+        put(g, token, (float)(c * (norm / total * (far ? p * exp(dl) : p) - (a.rest ? q : q / list.mass))));
     }
 }
 
@@ -358,12 +397,19 @@ static int distill_launch(DistillArgs<T>& a, cudaStream_t st) {
     while (log_c < 3 && (share() > 2560 || ((long long)a.rows << log_c) < 148 && share() > 256)) log_c++;
     a.log_c = log_c;
     a.share = share();
-    a.slots = (a.k + 31) & ~31;
-    const size_t smem = (size_t)((a.share + 7) / 8 * 8) * 16 + 3 * sizeof(int) * a.slots;
+    const size_t smem = (size_t)((a.share + 7) / 8 * 8) * 16;
     static DeviceOnce once;
-    const int rc = once.raise((const void*)distill_kernel<T>, 200 * 1024);
+    int rc = once.raise((const void*)distill_kernel<T>, 200 * 1024);
     if (rc) return rc;
-    return launch("distill_kernel", distill_kernel<T>, (long long)a.rows << log_c, kDistillThreads, 1 << log_c, smem, false, st, a);
+    rc = launch("distill_list_kernel", distill_list_kernel<T>, (a.rows + kListWarps - 1) / kListWarps, kListWarps * 32, 1, 0, false, st, a);
+    if (rc) return rc;
+    return launch("distill_kernel", distill_kernel<T>, (long long)a.rows << log_c, kDistillThreads, 1 << log_c, smem, true, st, a);
+}
+
+// Workspace: the rows' losses, their lists, and the entries.
+static size_t distill_bytes(int rows, int k) {
+    const size_t n = rows > 0 ? (size_t)rows : 1, e = n * k;
+    return round256(n * sizeof(double)) + round256(n * sizeof(RowList)) + 2 * round256(e * sizeof(double)) + round256(e * sizeof(int));
 }
 
 }  // namespace qs
@@ -372,7 +418,7 @@ using namespace qs;
 
 extern "C" {
 
-size_t qs_distill_loss_workspace(int rows) { return round256((rows > 0 ? (size_t)rows : 1) * sizeof(double)); }
+size_t qs_distill_loss_workspace(int rows, int k) { return k < 1 || k > QS_MAX_LISTED ? 0 : distill_bytes(rows, k); }
 
 int qs_distill_loss(const void* d_logits, int dtype, int rows, int vocab, long long row_stride,
                     const int* d_teacher_tokens, const float* d_teacher_logprobs, int k, const float* d_weights,
@@ -390,7 +436,7 @@ int qs_distill_loss(const void* d_logits, int dtype, int rows, int vocab, long l
     double* row_loss = (double*)d_workspace;
     if (rows > 0) {
         if (!d_teacher_logprobs) return fail(QS_ERR_INVALID, "NULL device pointer");
-        const int bad = check_workspace(d_workspace, workspace_bytes, qs_distill_loss_workspace(rows));
+        const int bad = check_workspace(d_workspace, workspace_bytes, distill_bytes(rows, k));
         if (bad) return bad;
         const auto go = [&](auto a) {
             a.rows = rows;
@@ -403,7 +449,12 @@ int qs_distill_loss(const void* d_logits, int dtype, int rows, int vocab, long l
             a.scale = (float)(r.inv_t * 1.4426950408889634);
             a.inv_t = r.inv_t;
             a.rest = p.rest != 0;
+            const size_t e = round256((size_t)rows * k * sizeof(double));
             a.row_loss = row_loss;
+            a.lists = (RowList*)((char*)d_workspace + round256((size_t)rows * sizeof(double)));
+            a.list_p = (double*)((char*)a.lists + round256((size_t)rows * sizeof(RowList)));
+            a.list_q = (double*)((char*)a.list_p + e);
+            a.list_token = (int*)((char*)a.list_q + e);
             a.row_losses = d_row_losses;
             a.logits = (decltype(a.logits))d_logits;
             a.grad = (decltype(a.grad))d_grad;

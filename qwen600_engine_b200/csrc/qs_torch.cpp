@@ -360,7 +360,7 @@ PyObject* distill_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const On on(x);
         if (wanted) grad.make(x);
         at::Tensor loss = fresh({}, at::kFloat, x), rows = fresh({m.rows}, at::kFloat, x);
-        const size_t size = qs_distill_loss_workspace(m.rows);
+        const size_t size = qs_distill_loss_workspace(m.rows, k);
         at::Tensor work = workspace(size, x);
         check(qs_distill_loss(x.data_ptr(), m.dtype, m.rows, m.vocab, m.ld, tok, lps, k, w, &p, (float*)loss.data_ptr(),
                               (float*)rows.data_ptr(), grad.ptr, grad.ld, pointer(work), size, on.stream));

@@ -73,7 +73,7 @@ def test_sizes_outside_the_limits_are_0_bytes():
     for bad in ((QS_F32, 2, 65, 1000, 5), (QS_F32, 0, 4, 1000, 5), (QS_F32, 1 << 30, 4, 1000, 5), (QS_F32, 2, -1, 1000, 5)):
         assert L.qs_beam_select_workspace(*bad) == 0
     assert L.qs_top_logprobs_workspace(QS_BF16, 4, 151936, 20) > 0 and L.qs_beam_select_workspace(QS_F32, 2, 4, 151936, 8) > 0
-    assert L.qs_distill_loss_workspace(-3) > 0
+    assert L.qs_distill_loss_workspace(-3, 5) > 0 and L.qs_distill_loss_workspace(4, 0) == 0 and L.qs_distill_loss_workspace(4, 257) == 0
 
 
 def state(base=FAR, row=1000, outer=(1, 1), outer_stride=(0, 0), positions=1, stride=0, unit=1000):
