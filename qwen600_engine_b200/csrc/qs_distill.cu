@@ -30,6 +30,9 @@ struct __align__(16) RowList {
     double sl;    // S_l
     float ml;
     int some;     // the row adds something
+    double sr;    // S_r, against ref
+    float ref;    // m_l, or where the list lies far from them the unlisted tokens' maximum
+    int unused;
 };
 
 template <typename T>
@@ -50,8 +53,6 @@ struct DistillArgs {
     double* list_p;   // [rows][k] exp((x - m_l) / T)
     double* list_q;   // [rows][k]
     int* list_token;  // [rows][k] -1: no entry
-    double* row_loss;
-    float* row_losses;
     T* grad;
     long long gld;
 };
@@ -139,7 +140,7 @@ distill_list_kernel(const __grid_constant__ DistillArgs<T> a) {
     mass = warp_sum_double(mass);
     cost = warp_sum_double(cost);
     sl = warp_sum_double(sl);
-    if (lane == 0) a.lists[row] = RowList{mass, cost, sl, ml, some};
+    if (lane == 0) a.lists[row] = RowList{mass, cost, sl, ml, some, 0.0, 0.0f, 0};
 }
 
 // Writes v to *slot of the cluster's CTA `rank`.
@@ -173,10 +174,6 @@ distill_kernel(const __grid_constant__ DistillArgs<T> a) {
     const float w_row = a.weights ? a.weights[row] : 1.0f;
     dependents_may_start();
     const auto nothing = [&] {  // what a row is that adds nothing
-        if (rank == 0 && t == 0) {
-            a.row_loss[row] = 0.0;
-            if (a.row_losses) a.row_losses[row] = 0.0f;
-        }
         if (!a.grad) return;
         T* g = a.grad + (size_t)row * a.gld;
         const RowShape<T> gs(g, a.V);
@@ -326,19 +323,9 @@ distill_kernel(const __grid_constant__ DistillArgs<T> a) {
     const double total = isinf(top) ? (double)NAN : far ? list.sl * exp(dl) + sr * exp(dr) : list.sl + sr;
     const double left = a.rest && list.mass < 1.0 && !(ref == -INFINITY && sr == 0.0) ? 1.0 - list.mass : 0.0;
     const double norm = a.rest ? list.mass + left : list.mass / list.mass;  // NaN from the teacher reaches the row
-    if (rank == 0 && t == kDistillThreads - 32) {
-        const double log_total = log(total);
-        // cost counts from the list's maximum (from 0 where all of it is masked), log p from the row's
-        const double away = log_total - (ml == -INFINITY ? -top * a.inv_t : dl);
-        double l;
-        if (a.rest) {
-            l = list.cost + (list.mass == 0.0 ? 0.0 : list.mass * away);
-            if (left > 0.0) l += left * (log(left) - (dr + log(sr) - log_total));
-        } else {
-            l = list.cost / list.mass - log(list.mass) + away;
-        }
-        a.row_loss[row] = w * l;
-        if (a.row_losses) a.row_losses[row] = (float)l;
+    if (rank == 0 && t == 0) {  // for the loss
+        a.lists[row].sr = sr;
+        a.lists[row].ref = ref;
     }
     if (!a.grad) return;
 
@@ -386,6 +373,41 @@ distill_kernel(const __grid_constant__ DistillArgs<T> a) {
     }
 }
 
+// The rows' losses from their sums, and their sum in a fixed order.
+__global__ void __launch_bounds__(1024)
+distill_loss_kernel(const RowList* lists, int rows, const float* __restrict__ weights, double inv_t, int rest, float* row_losses,
+                    float* __restrict__ loss) {
+    __shared__ double red[32];
+    wait_for_previous();
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < rows; i += blockDim.x) {
+        const double w = weights ? (double)weights[i] : 1.0 / rows;
+        double l = 0.0;
+        if (w != 0.0 && lists[i].some) {
+            const RowList r = lists[i];
+            // distances of the list's and the others' maximum from the row's
+            const double top = fmax((double)r.ref, (double)r.ml);
+            const double dr = r.ref == -INFINITY ? -(double)INFINITY : ((double)r.ref - top) * inv_t;
+            const double dl = r.ml == -INFINITY ? -(double)INFINITY : ((double)r.ml - top) * inv_t;
+            const double total = isinf(top) ? (double)NAN : r.sl * (dl == 0.0 ? 1.0 : exp(dl)) + r.sr * (dr == 0.0 ? 1.0 : exp(dr));
+            const double log_total = log(total);
+            // cost counts from the list's maximum (from 0 where all of it is masked), log p from the row's
+            const double away = log_total - (r.ml == -INFINITY ? -top * inv_t : dl);
+            if (rest) {
+                const double left = r.mass < 1.0 && !(r.ref == -INFINITY && r.sr == 0.0) ? 1.0 - r.mass : 0.0;
+                l = r.cost + (r.mass == 0.0 ? 0.0 : r.mass * away);
+                if (left > 0.0) l += left * (log(left) - (dr + log(r.sr) - log_total));
+            } else {
+                l = r.cost / r.mass - log(r.mass) + away;
+            }
+            sum += w * l;
+        }
+        if (row_losses) row_losses[i] = (float)l;
+    }
+    sum = block_sum(sum, red);
+    if (threadIdx.x == 0) *loss = (float)sum;
+}
+
 // How rows are spread: as the policy loss's (qs_losses.cu), CTAs per row doubled
 // while a share is above 40 KB, and while the rows alone would leave some of the 148
 // SMs idle and a share keeps 4 KB.
@@ -406,10 +428,10 @@ static int distill_launch(DistillArgs<T>& a, cudaStream_t st) {
     return launch("distill_kernel", distill_kernel<T>, (long long)a.rows << log_c, kDistillThreads, 1 << log_c, smem, true, st, a);
 }
 
-// Workspace: the rows' losses, their lists, and the entries.
+// Workspace: the rows' lists, and their entries.
 static size_t distill_bytes(int rows, int k) {
     const size_t n = rows > 0 ? (size_t)rows : 1, e = n * k;
-    return round256(n * sizeof(double)) + round256(n * sizeof(RowList)) + 2 * round256(e * sizeof(double)) + round256(e * sizeof(int));
+    return round256(n * sizeof(RowList)) + 2 * round256(e * sizeof(double)) + round256(e * sizeof(int));
 }
 
 }  // namespace qs
@@ -433,7 +455,6 @@ int qs_distill_loss(const void* d_logits, int dtype, int rows, int vocab, long l
     if (k < 1 || k > QS_MAX_LISTED) return fail(QS_ERR_UNSUPPORTED, "k %d outside [1, %d]", k, QS_MAX_LISTED);
     if (!d_loss) return fail(QS_ERR_INVALID, "NULL output buffer");
     const cudaStream_t st = (cudaStream_t)stream;
-    double* row_loss = (double*)d_workspace;
     if (rows > 0) {
         if (!d_teacher_logprobs) return fail(QS_ERR_INVALID, "NULL device pointer");
         const int bad = check_workspace(d_workspace, workspace_bytes, distill_bytes(rows, k));
@@ -450,12 +471,10 @@ int qs_distill_loss(const void* d_logits, int dtype, int rows, int vocab, long l
             a.inv_t = r.inv_t;
             a.rest = p.rest != 0;
             const size_t e = round256((size_t)rows * k * sizeof(double));
-            a.row_loss = row_loss;
-            a.lists = (RowList*)((char*)d_workspace + round256((size_t)rows * sizeof(double)));
+            a.lists = (RowList*)d_workspace;
             a.list_p = (double*)((char*)a.lists + round256((size_t)rows * sizeof(RowList)));
             a.list_q = (double*)((char*)a.list_p + e);
             a.list_token = (int*)((char*)a.list_q + e);
-            a.row_losses = d_row_losses;
             a.logits = (decltype(a.logits))d_logits;
             a.grad = (decltype(a.grad))d_grad;
             a.gld = grad_row_stride;
@@ -464,7 +483,8 @@ int qs_distill_loss(const void* d_logits, int dtype, int rows, int vocab, long l
         const int e = dtype == QS_F32 ? go(DistillArgs<float>{}) : go(DistillArgs<__nv_bfloat16>{});
         if (e) return e;
     }
-    return launch("sum_rows_kernel", sum_rows_kernel, 1, rows > 512 ? 1024 : 128, 1, 0, rows > 0, st, row_loss, rows, d_loss);
+    return launch("distill_loss_kernel", distill_loss_kernel, 1, rows > 128 ? 1024 : 128, 1, 0, rows > 0, st, (const RowList*)d_workspace, rows,
+                  d_weights, r.inv_t, p.rest != 0, d_row_losses, d_loss);
 }
 
 }  // extern "C"
