@@ -75,7 +75,8 @@ distill_list_kernel(const __grid_constant__ DistillArgs<T> a) {
     __shared__ __align__(16) int tokens[kListWarps][QS_MAX_LISTED];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * kListWarps + warp;
     dependents_may_start();
-    if (row >= a.rows || (a.weights && a.weights[row] == 0.0f)) return;
+    if (row >= a.rows) return;
+    const float w = a.weights ? a.weights[row] : 1.0f;
     const T* x = a.logits + (size_t)row * a.ld;
     const size_t at = (size_t)row * a.k;
     int tok[kListMine];
@@ -87,6 +88,7 @@ distill_list_kernel(const __grid_constant__ DistillArgs<T> a) {
         lp[i] = e < a.k ? a.lps[at + e] : -INFINITY;
         if (tok[i] < 0 || tok[i] >= a.V) tok[i] = -1;
     }
+    if (w == 0.0f) return;
 #pragma unroll
     for (int i = 0; i < kListMine; i++) {
         v[i] = tok[i] >= 0 ? elem(x, tok[i]) : -INFINITY;
