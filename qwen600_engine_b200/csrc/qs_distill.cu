@@ -20,7 +20,6 @@ constexpr int kDistillThreads = 256;
 // they are summed again against their own.  A term's exponent is rounded to a 2^-24th of
 // itself; with sums from 2^-28 on it lies on the average below log2 V + 28.
 constexpr double kLeastRest = 0x1p-28, kMostRest = 0x1p20;
-static_assert(QS_MAX_LISTED <= kDistillThreads, "one entry a thread");
 
 // A row's list as the list kernel leaves it.  Its entries follow: tokens (int), then
 // exp((x - m_l) / T) and q of each (double).
@@ -161,7 +160,7 @@ __device__ __forceinline__ void push_double(double* slot, int rank, double v) {
 // a CTA's warps meet once.  The listed entries' places in the pieces are overwritten
 // with -inf, which takes them out of the sum and of the gradient's stream.
 template <typename T>
-__global__ void __launch_bounds__(kDistillThreads, 5)
+__global__ void __launch_bounds__(kDistillThreads, 2)
 distill_kernel(const __grid_constant__ DistillArgs<T> a) {
     constexpr int kN = Pack<T>::kN;
     constexpr int kW = kDistillThreads / 32;
@@ -410,15 +409,18 @@ distill_loss_kernel(const RowList* lists, int rows, const float* __restrict__ we
     if (threadIdx.x == 0) *loss = (float)sum;
 }
 
-// How rows are spread: as the policy loss's (qs_losses.cu), CTAs per row doubled
-// while a share is above 40 KB, and while the rows alone would leave some of the 148
-// SMs idle and a share keeps 4 KB.
+// How rows are spread: CTAs per row (a power of two up to 8), doubled while a share is
+// above 80 KB, two of which fit on an SM, and while the rows alone would leave some of
+// the 148 SMs idle and a share keeps 4 KB.  2048 bf16 rows of 151,936, a quarter of them
+// left out: 218 us with 4 CTAs a row (76 KB shares), 241 with 8 (38 KB, five an SM), 312
+// with 2; 300 fp32 rows of 37,999 29 us with 2, 31 with 4.  CTAs of 224 threads 232 us, of
+// 384 259.
 template <typename T>
 static int distill_launch(DistillArgs<T>& a, cudaStream_t st) {
     const int vecs = a.V / Pack<T>::kN;
     int log_c = 0;
     const auto share = [&] { return (vecs + (1 << log_c) - 1) >> log_c; };
-    while (log_c < 3 && (share() > 2560 || ((long long)a.rows << log_c) < 148 && share() > 256)) log_c++;
+    while (log_c < 3 && (share() > 5120 || ((long long)a.rows << log_c) < 148 && share() > 256)) log_c++;
     a.log_c = log_c;
     a.share = share();
     const size_t smem = (size_t)((a.share + 7) / 8 * 8) * 16;
