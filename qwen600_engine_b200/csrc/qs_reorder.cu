@@ -14,6 +14,7 @@ namespace qs {
 
 constexpr int kMoveThreads = 256;
 constexpr int kMoveVecs = 4;      // of a thread at a time
+constexpr int kMaxChunks = 8;     // of a CTA
 constexpr int kMaxMoveBeams = 1024;
 constexpr int kMoveStates = 40;   // of a launch: they travel in its parameters
 
@@ -25,7 +26,6 @@ struct MoveState {
     uint32_t outers;    // outer[0] * outer[1]
     int positions;
     int joined;         // positions behind one another: a run holds all that are moved
-    int log_width;      // of a vector, in bytes
     int ctas;           // per entry
 };
 
@@ -46,7 +46,8 @@ template <> struct MoveWord<8> { using T = uint2; };
 template <> struct MoveWord<16> { using T = uint4; };
 
 // The list of moves for `parents`, by one thread: list[i] = {place written, place
-// read}; place written -1: into the registers' copy, place read -1: from it.
+// read}; place written -1: into the registers' copy, place read -1: from it.  Returns
+// its length, and 2^16 more where it has cycles.
 __device__ int list_moves(const int* parents, int beams, short* readers, short* ready, short2* list) {
     int n = 0, todo = 0, front = 0, back = 0;
     for (int i = 0; i < beams; i++) readers[i] = 0;
@@ -66,6 +67,7 @@ __device__ int list_moves(const int* parents, int beams, short* readers, short* 
         todo--;
         if (--readers[p] == 0 && parents[p] >= 0) ready[back++] = (short)p;
     }
+    const int cycles = todo > 0;
     for (int i = 0; todo > 0 && i < beams; i++) {
         if (parents[i] < 0 || readers[i] < 0) continue;
         // every place left is read by exactly one other: a cycle through i
@@ -81,11 +83,17 @@ __device__ int list_moves(const int* parents, int beams, short* readers, short* 
         readers[d] = -1;
         todo--;
     }
-    return n;
+    return n | cycles << 16;
 }
 
-template <int kBytes>
-__device__ void move_bytes(const MoveState& s, int entry, int beams, int length, int cta, const short2* list, int n) {
+// Loads that do not stay in L1: most places are read once.
+template <typename W> __device__ __forceinline__ W take(const char* p) { return *reinterpret_cast<const W*>(p); }
+template <> __device__ __forceinline__ uint4 take<uint4>(const char* p) { return load16(p); }
+
+// The list for this thread's bytes of an entry's rows, kMoveVecs vectors at a time.
+// kCycles: some moves go through the registers' copy.
+template <int kBytes, bool kCycles>
+__device__ __forceinline__ void move_bytes(const MoveState& s, int entry, int beams, int length, int cta, const short2* list, int n) {
     using W = typename MoveWord<kBytes>::T;
     const uint32_t run = s.joined ? s.run_vecs * (uint32_t)length : s.run_vecs;
     const uint32_t per_outer = s.joined ? run : run * (uint32_t)length;
@@ -97,38 +105,37 @@ __device__ void move_bytes(const MoveState& s, int entry, int beams, int length,
 #pragma unroll
         for (int j = 0; j < kMoveVecs; j++) {
             const uint32_t i = i0 + j * kMoveThreads;
-            const uint32_t o = i / per_outer, in = i - o * per_outer;
+            const uint32_t o = s.outers == 1 ? 0 : i / per_outer, in = i - o * per_outer;
             const uint32_t position = s.joined ? 0 : in / run, v = in - position * run;
-            const uint32_t o0 = o / s.outer1, o1 = o - o0 * s.outer1;
+            const uint32_t o0 = s.outer1 == 1 ? o : o / s.outer1, o1 = o - o0 * s.outer1;
             at[j] = i < total ? rows + (long long)o0 * s.outer_stride[0] + (long long)o1 * s.outer_stride[1] +
                                     (long long)position * s.position_stride + (size_t)v * kBytes
                               : nullptr;
         }
-        W kept[kMoveVecs], v[kMoveVecs];
+        W kept[kMoveVecs] = {};
         for (int k = 0; k < n; k++) {
             const short2 m = list[k];
-            if (m.y >= 0) {
+            W v[kMoveVecs];
 #pragma unroll
-                for (int j = 0; j < kMoveVecs; j++)
-                    if (at[j]) v[j] = *reinterpret_cast<const W*>(at[j] + m.y * s.row_stride);
-            } else {
-#pragma unroll
-                for (int j = 0; j < kMoveVecs; j++) v[j] = kept[j];
+            for (int j = 0; j < kMoveVecs; j++) {
+                if (kCycles && m.y < 0) v[j] = kept[j];
+                else if (at[j]) v[j] = take<W>(at[j] + m.y * s.row_stride);
+                if (kCycles && m.x < 0) kept[j] = v[j];
             }
-            if (m.x >= 0) {
+            if (kCycles && m.x < 0) continue;
 #pragma unroll
-                for (int j = 0; j < kMoveVecs; j++)
-                    if (at[j]) *reinterpret_cast<W*>(at[j] + m.x * s.row_stride) = v[j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < kMoveVecs; j++) kept[j] = v[j];
-            }
+            for (int j = 0; j < kMoveVecs; j++)
+                if (at[j]) *reinterpret_cast<W*>(at[j] + m.x * s.row_stride) = v[j];
         }
     }
 }
 
-// Bound: memory.
-__global__ void __launch_bounds__(kMoveThreads)
+// Bound: memory; 64 KB of loads under way on an SM.  56 caches of 8 entries x 4 beams of
+// up to 1000 positions of 2 KB, half of the places written: 443 us for 2.87 GB, 6.5 TB/s (a
+// copy's rate).  Several moves' loads at once 618 us, 8 vectors a thread 636, two or five
+// CTAs an SM 553 and 506; lists without cycles have code without the registers' copy (465).
+template <int kBytes>
+__global__ void __launch_bounds__(kMoveThreads, 4)
 reorder_kernel(const __grid_constant__ MoveArgs a) {
     extern __shared__ int smem[];
     int* parents = smem;                                            // [beams] -1: keeps its own
@@ -142,6 +149,7 @@ reorder_kernel(const __grid_constant__ MoveArgs a) {
     const int at = blockIdx.x - a.first_cta[i], entry = at / s.ctas, cta = at - entry * s.ctas;
     int length = s.positions;
     if (a.lengths) length = max(0, min(length, a.lengths[entry]));
+    if (threadIdx.x == 0) moves_s = 0;
     bool some = false;
     for (int j = threadIdx.x; j < a.beams; j += kMoveThreads) {
         int p = a.parents[(size_t)entry * a.beams + j];
@@ -150,16 +158,20 @@ reorder_kernel(const __grid_constant__ MoveArgs a) {
         some |= p >= 0;
     }
     if (!__syncthreads_or(some) || length == 0) return;
-    if (threadIdx.x == 0) moves_s = list_moves(parents, a.beams, readers, ready, list);
-    __syncthreads();
-    const int n = moves_s;
-    switch (s.log_width) {
-        case 4: return move_bytes<16>(s, entry, a.beams, length, cta, list, n);
-        case 3: return move_bytes<8>(s, entry, a.beams, length, cta, list, n);
-        case 2: return move_bytes<4>(s, entry, a.beams, length, cta, list, n);
-        case 1: return move_bytes<2>(s, entry, a.beams, length, cta, list, n);
-        default: return move_bytes<1>(s, entry, a.beams, length, cta, list, n);
+    // where no place that is read is written (each beam's best child stayed in its place), any order will do
+    bool meets = false;
+    for (int j = threadIdx.x; j < a.beams; j += kMoveThreads) meets |= parents[j] >= 0 && parents[parents[j]] >= 0;
+    if (__syncthreads_or(meets)) {
+        if (threadIdx.x == 0) moves_s = list_moves(parents, a.beams, readers, ready, list);
+    } else {
+        for (int j = threadIdx.x; j < a.beams; j += kMoveThreads)
+            if (parents[j] >= 0) list[atomicAdd(&moves_s, 1)] = make_short2((short)j, (short)parents[j]);
     }
+    __syncthreads();
+    const int n = moves_s & 0xFFFF;
+    const bool cycles = moves_s >> 16;
+    if (cycles) move_bytes<kBytes, true>(s, entry, a.beams, length, cta, list, n);
+    else move_bytes<kBytes, false>(s, entry, a.beams, length, cta, list, n);
 }
 
 // --------------------------------------------------------------- host side
@@ -211,6 +223,18 @@ static bool apart_within(const qs_states& a, const Level* la, int na, const qs_s
     return false;
 }
 
+// The largest vectors that a state's addresses allow: 2^width bytes.
+static int width_of(const qs_states& s, int rows) {
+    unsigned long long bits = (unsigned long long)(uintptr_t)s.d_base | (unsigned long long)s.unit;
+    Level l[4];
+    const int n = levels_of(s, rows, l);
+    for (int i = 0; i < n; i++) bits |= (unsigned long long)l[i].stride;
+    int width = 0;
+    while (width < 4 && !(bits >> width & 1)) width++;
+    return width;
+}
+static long long vecs_of(const qs_states& s, int width) { return (s.unit >> width) * s.positions * s.outer[0] * s.outer[1]; }
+
 static int check_states(const qs_states* all, int count, int rows) {
     for (int i = 0; i < count; i++) {
         const qs_states& s = all[i];
@@ -221,6 +245,8 @@ static int check_states(const qs_states* all, int count, int rows) {
         const int n = levels_of(s, rows, l);
         if (s.unit > 1ll << 44 || span_of(s.unit, l, n, kAllLevels) < 0)
             return fail(QS_ERR_INVALID, "state %d: its pieces overlap, or its strides are not those of nested blocks", i);
+        if ((double)s.unit * s.positions * s.outer[0] * s.outer[1] > 2147483647.0 * (1 << width_of(s, rows)))
+            return fail(QS_ERR_UNSUPPORTED, "state %d: above 2^31 - 1 vectors of %d bytes in a row", i, 1 << width_of(s, rows));
         for (int j = 0; j < i; j++) {
             Level k[4];
             const int m = levels_of(all[j], rows, k);
@@ -233,8 +259,8 @@ static int check_states(const qs_states* all, int count, int rows) {
 }
 
 // Moves a call's states, as many at a time as a launch's parameters hold.  A CTA
-// takes up to 8 chunks of 1024 vectors of a row, fewer where that would leave the
-// call with less than two CTAs per SM.
+// takes up to kMaxChunks chunks of 1024 vectors of a row (one more parents' list for each
+// CTA otherwise), fewer where that would leave the call with less than two CTAs per SM.
 int reorder_states(const qs_states* all, int count, const int* d_parents, int batch, int beams, const int* d_lengths,
                    cudaStream_t st) {
     if (batch < 0) return fail(QS_ERR_INVALID, "batch %d < 0", batch);
@@ -245,49 +271,53 @@ int reorder_states(const qs_states* all, int count, const int* d_parents, int ba
     if (!all || !d_parents) return fail(QS_ERR_INVALID, "NULL pointer");
     const int bad = check_states(all, count, batch * beams);
     if (bad) return bad;
-    for (int begin = 0; begin < count; begin += kMoveStates) {
-        MoveArgs a = {};
-        a.count = count - begin < kMoveStates ? count - begin : kMoveStates;
-        a.parents = d_parents;
-        a.beams = beams;
-        a.lengths = d_lengths;
-        long long chunks = 0;
-        for (int i = 0; i < a.count; i++) {
-            const qs_states& s = all[begin + i];
-            MoveState& m = a.s[i];
-            m.base = (char*)s.d_base;
-            m.row_stride = s.row_stride;
-            m.outer_stride[0] = s.outer_stride[0];
-            m.outer_stride[1] = s.outer_stride[1];
-            m.position_stride = s.position_stride;
-            m.positions = s.positions;
-            m.outer1 = s.outer[1];
-            m.joined = s.positions == 1 || s.position_stride == s.unit;
-            unsigned long long bits = (unsigned long long)(uintptr_t)s.d_base | (unsigned long long)s.unit;
-            if (batch * beams > 1) bits |= (unsigned long long)s.row_stride;
-            if (s.outer[0] > 1) bits |= (unsigned long long)s.outer_stride[0];
-            if (s.outer[1] > 1) bits |= (unsigned long long)s.outer_stride[1];
-            if (s.positions > 1) bits |= (unsigned long long)s.position_stride;
-            while (m.log_width < 4 && !(bits >> m.log_width & 1)) m.log_width++;
-            const double total = (double)(s.unit >> m.log_width) * s.positions * s.outer[0] * s.outer[1];
-            if (total > 2147483647.0) return fail(QS_ERR_UNSUPPORTED, "state %d: %g pieces of a row", begin + i, total);
-            m.run_vecs = (uint32_t)(s.unit >> m.log_width);
-            m.outers = (uint32_t)s.outer[0] * s.outer[1];
-            m.ctas = (int)(((long long)total + kMoveThreads * kMoveVecs - 1) / (kMoveThreads * kMoveVecs));
-            chunks += (long long)m.ctas * batch;
+    const int rows = batch * beams;
+    // states whose vectors have the same width go together
+    for (int width = 0; width <= 4; width++) {
+        int begin = 0;
+        while (begin < count) {
+            MoveArgs a = {};
+            a.parents = d_parents;
+            a.beams = beams;
+            a.lengths = d_lengths;
+            long long chunks = 0;
+            for (; begin < count && a.count < kMoveStates; begin++) {
+                const qs_states& s = all[begin];
+                if (width_of(s, rows) != width) continue;
+                MoveState& m = a.s[a.count++];
+                m.base = (char*)s.d_base;
+                m.row_stride = s.row_stride;
+                m.outer_stride[0] = s.outer_stride[0];
+                m.outer_stride[1] = s.outer_stride[1];
+                m.position_stride = s.position_stride;
+                m.positions = s.positions;
+                m.outer1 = s.outer[1];
+                m.joined = s.positions == 1 || s.position_stride == s.unit;
+                m.run_vecs = (uint32_t)(s.unit >> width);
+                m.outers = (uint32_t)s.outer[0] * s.outer[1];
+                m.ctas = (int)((vecs_of(s, width) + kMoveThreads * kMoveVecs - 1) / (kMoveThreads * kMoveVecs));
+                chunks += (long long)m.ctas * batch;
+            }
+            if (a.count == 0) break;
+            const long long each = chunks / (148 * 2) < 1 ? 1 : chunks / (148 * 2) > kMaxChunks ? kMaxChunks : chunks / (148 * 2);
+            long long grid = 0;
+            for (int i = 0; i < a.count; i++) {
+                a.s[i].ctas = (int)((a.s[i].ctas + each - 1) / each);
+                a.first_cta[i] = (int)grid;
+                grid += (long long)a.s[i].ctas * batch;
+                if (grid > 0x7FFFFFFFll) return fail(QS_ERR_UNSUPPORTED, "reorder_kernel: %lld CTAs", grid);
+            }
+            a.first_cta[a.count] = (int)grid;
+            const auto go = [&](auto kernel) {
+                return launch("reorder_kernel", kernel, grid, kMoveThreads, 1, (size_t)beams * 16, false, st, a);
+            };
+            const int rc = width == 4   ? go(reorder_kernel<16>)
+                           : width == 3 ? go(reorder_kernel<8>)
+                           : width == 2 ? go(reorder_kernel<4>)
+                           : width == 1 ? go(reorder_kernel<2>)
+                                        : go(reorder_kernel<1>);
+            if (rc) return rc;
         }
-        const long long each = chunks / (148 * 2) < 1 ? 1 : chunks / (148 * 2) > 8 ? 8 : chunks / (148 * 2);
-        long long grid = 0;
-        for (int i = 0; i < a.count; i++) {
-            MoveState& m = a.s[i];
-            m.ctas = (int)((m.ctas + each - 1) / each);
-            a.first_cta[i] = (int)grid;
-            grid += (long long)m.ctas * batch;
-            if (grid > 0x7FFFFFFFll) return fail(QS_ERR_UNSUPPORTED, "reorder_kernel: %lld CTAs", grid);
-        }
-        a.first_cta[a.count] = (int)grid;
-        const int rc = launch("reorder_kernel", reorder_kernel, grid, kMoveThreads, 1, (size_t)beams * 16, false, st, a);
-        if (rc) return rc;
     }
     return QS_OK;
 }
