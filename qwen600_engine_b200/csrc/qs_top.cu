@@ -199,6 +199,78 @@ __device__ __forceinline__ Bound<S> narrow(Bound<S> within, int n, int slack, S 
     return Bound<S>{v, (uint32_t)enough};
 }
 
+// The usual way to a first bound: the items counted by their distance below the best,
+// in 256 steps of a quarter.  The steps are made smaller within one that holds too many,
+// and larger behind the last where fewer than n items came; where that does not end
+// soon (many equal scores, or masks of finite numbers near which n lies) narrow() does.
+// The CTA's threads find the same: an item is within if it is less than `from` below the
+// best, or its step behind that is at most `step`.
+constexpr int kSteps = 256;
+struct Within {
+    float best, from, per;  // steps a unit
+    int step;               // -1: all; -2: not found
+    __device__ __forceinline__ bool has(float s) const {
+        const float d = best - s;
+        return s > -INFINITY && (step == -1 || d < from || (int)fminf((d - from) * per, 1e6f) <= step);
+    }
+};
+
+template <int kThreads>
+__device__ __forceinline__ Within find_within(const float* score, int items, int n, int slack, float best, int* steps, int2* found) {
+    const int t = threadIdx.x;
+    Within w{best, 0.0f, 4.0f, -2};
+    int before = 0;
+    for (int pass = 0; pass < 4; pass++) {  // as long as every step's border is a number of 24 bits, so that none counts twice
+        for (int i = t; i <= kSteps; i += kThreads) steps[i] = 0;
+        __syncthreads();
+        for (int i = t; i < items; i += kThreads) {
+            const float s = score[i], d = best - s;
+            if (s > -INFINITY && d >= w.from) atomicAdd(&steps[(int)fminf((d - w.from) * w.per, (float)kSteps)], 1);
+        }
+        __syncthreads();
+        if (t < 32) {  // eight steps a lane: where the count reaches n
+            int own[kSteps / 32], sum = 0;
+#pragma unroll
+            for (int i = 0; i < kSteps / 32; i++) {
+                own[i] = steps[t * (kSteps / 32) + i];
+                sum += own[i];
+            }
+            int upto = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (t >= o) upto += v;
+            }
+            const int total = __shfl_sync(0xffffffffu, upto, 31), all = before + total + steps[kSteps];
+            if (t == 0) *found = make_int2(all <= n + slack ? -1 : -2, before + total);
+            __syncwarp();
+            int c = before + upto - sum;
+            if (all > n + slack && c < n && c + sum >= n) {
+#pragma unroll
+                for (int i = 0; i < kSteps / 32; i++) {
+                    if (c < n && c + own[i] >= n) *found = make_int2(t * (kSteps / 32) + i, c + own[i] <= n + slack ? -1 : c);
+                    c += own[i];
+                }
+            }
+        }
+        __syncthreads();
+        const int2 f = *found;
+        if (f.x == -1 || (f.x >= 0 && f.y < 0)) {
+            w.step = f.x;
+            return w;
+        }
+        before = f.y;
+        if (f.x >= 0) {
+            w.from += (float)f.x / w.per;
+            w.per *= (float)kSteps;
+        } else {
+            w.from += (float)kSteps / w.per;
+            w.per /= (float)kSteps;
+        }
+    }
+    return w;
+}
+
 // A group as the pick sees it.
 template <typename T, bool kRows>
 struct Group {
@@ -207,15 +279,28 @@ struct Group {
     static constexpr int kPartVecs = kUnitVecs / 32;
     const T* logits;  // its first row
     const T* lanes;
-    const float* max;   // of beams
-    const double* add;  // and what their logits' distances from it are added to
-    const int* item_list;
-    const int* part_list;
+    const float4* unit_parts;
+    const unsigned char* state;  // of beams, 0: offers its tokens
+    const float* max;            // of beams
+    const double* add;           // and what their logits' distances from it are added to
+    int* item_list;
+    int* part_list;
     long long ld;
     double inv_t;
     float per_unit;  // 1 / units
-    int V, units, lg;
+    int V, units, lg;  // 2^lg lanes an item
 
+    // An item's largest logit; of a beam that offers nothing -inf.
+    __device__ __forceinline__ float item(int i) const {
+        if (!kRows && state[beam_of(i >> (5 - lg))] != 0) return -INFINITY;
+        if (lg == 5) return unit_parts[i].x;
+        if (lg == 0) return elem(lanes, i);
+        float o[kN];
+        Pack<T>::widen(*reinterpret_cast<const uint4*>(lanes + (size_t)i * kN), o);
+#pragma unroll
+        for (int j = 1; j < kN; j++) o[0] = fmaxf(o[0], o[j]);
+        return o[0];
+    }
     __device__ __forceinline__ double logprob(float x, int beam) const { return ((double)x - (double)max[beam]) * inv_t + add[beam]; }
     __device__ __forceinline__ S score(float x, int beam) const {
         if constexpr (kRows) return x;
@@ -248,16 +333,24 @@ struct Group {
     }
 };
 
-// Narrows by the listed items' lanes, or by the listed parts' elements: for what
-// few calls reach, out of line so that the usual way's values stay in registers.
+// Narrows by the items, by the listed items' lanes, or by the listed parts' elements: for
+// what few calls reach, out of line so that the usual way's values stay in registers.
+enum { kByItems, kByLanes, kByElements };
+
 template <typename T, bool kRows, int kThreads>
-__device__ __noinline__ Bound<typename Group<T, kRows>::S> narrow_by(Group<T, kRows> g, bool elements, int count,
+__device__ __noinline__ Bound<typename Group<T, kRows>::S> narrow_by(Group<T, kRows> g, int by, int count,
                                                                      Bound<typename Group<T, kRows>::S> within, int n, int slack,
-                                                                     typename Group<T, kRows>::S best, Counter<kThreads> counter) {
+                                                                     typename Group<T, kRows>::S best, uint2 (*red)[kThreads / 32]) {
     using S = typename Group<T, kRows>::S;
     __syncthreads();
+    Counter<kThreads> counter{red, 0};
     const Bound<S> b = narrow(within, n, slack, best, counter, [&](auto f) {
-        if (!elements) {
+        if (by == kByItems) {
+            for (int i = threadIdx.x; i < count; i += kThreads)
+                f(g.score(g.item(i), g.beam_of(i >> (5 - g.lg))), [&] { return g.last_place(i << g.lg, 1 << g.lg); });
+            return;
+        }
+        if (by == kByLanes) {
             for (int i = threadIdx.x; i < count << g.lg; i += kThreads) {
                 const int id = (g.item_list[i >> g.lg] << g.lg) + (i & ((1 << g.lg) - 1));
                 f(g.score(elem(g.lanes, id), g.beam_of(id >> 5)), [&] { return g.last_place(id, 1); });
@@ -274,6 +367,21 @@ __device__ __noinline__ Bound<typename Group<T, kRows>::S> narrow_by(Group<T, kR
         }
     });
     __syncthreads();
+    return b;
+}
+
+// By the items, and lists them.
+template <typename T, bool kRows, int kThreads>
+__device__ __noinline__ Bound<typename Group<T, kRows>::S> list_items(Group<T, kRows> g, int items, int n, int cap,
+                                                                      typename Group<T, kRows>::S best, uint2 (*red)[kThreads / 32],
+                                                                      int* listed) {
+    using S = typename Group<T, kRows>::S;
+    const Bound<S> b = narrow_by<T, kRows, kThreads>(g, kByItems, items, Bound<S>{kLowest<S>, 0xFFFFFFFFu}, n, cap - kExtra - n, best, red);
+    for (int i = threadIdx.x; i < items; i += kThreads)
+        if (b.has(g.score(g.item(i), g.beam_of(i >> (5 - g.lg))), [&] { return g.first_place(i << g.lg); })) {
+            const int at = atomicAdd(listed, 1);
+            if (at < cap) g.item_list[at] = i;
+        }
     return b;
 }
 
@@ -300,7 +408,7 @@ pick_kernel(const __grid_constant__ PickArgs<T> a) {
     constexpr int kWarps = kThreads / 32;
     constexpr int kRoom = kMaxCands + (kRows ? 0 : QS_MAX_BEAMS);
     extern __shared__ __align__(16) unsigned char pool[];
-    S* item_score = reinterpret_cast<S*>(pool);
+    float* item_score = reinterpret_cast<float*>(pool);  // of sums, rounded
     __shared__ double add_s[kRows ? 1 : QS_MAX_BEAMS];
     __shared__ float max_s[kRows ? 1 : QS_MAX_BEAMS], floor_s[kRows ? 1 : QS_MAX_BEAMS];
     __shared__ unsigned char state_s[kRows ? 1 : QS_MAX_BEAMS];  // 0: offers its tokens, 1: ended, 2: nothing, 3: NaN
@@ -309,23 +417,27 @@ pick_kernel(const __grid_constant__ PickArgs<T> a) {
     __shared__ uint2 red[2][kWarps];
     __shared__ double sum_s[kWarps];
     __shared__ float top_s[kWarps];
-    __shared__ int items_s, parts_s, cands_s;
+    __shared__ int items_s, parts_s, cands_s, steps[kSteps + 1];
+    __shared__ int2 found_s;
+    __shared__ uint32_t least_s;
     __shared__ unsigned char slot_of[QS_MAX_BEAMS], parent_of[QS_MAX_BEAMS];
     __shared__ unsigned owns_s[2], stays_s[2];
     Cand<S>* cand = reinterpret_cast<Cand<S>*>(cand_raw);
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, group = blockIdx.x;
     const int beams = kRows ? 1 : a.beams;
     const int lg = a.log_lanes, all_items = beams * a.units << (5 - lg);
-    int* item_list = reinterpret_cast<int*>(item_score + ((all_items + 1) & ~1));  // [item_cap]
-    int* part_list = item_list + a.item_cap;                                       // [part_cap]
-    Counter<kThreads> counter{red, 0};
-    if (t == 0) items_s = parts_s = cands_s = 0;
+    int* item_list = reinterpret_cast<int*>(item_score + all_items);  // [item_cap]
+    int* part_list = item_list + a.item_cap;                          // [part_cap]
+    if (t == 0) {
+        items_s = parts_s = cands_s = 0;
+        least_s = 0xFFFFFFFFu;
+    }
     dependents_may_start();
     wait_for_previous();
     const float4* unit_parts = a.parts + (size_t)group * beams * a.units;
     const T* all_lanes = a.lanes + (size_t)group * beams * a.units * 32;
     T* stage = reinterpret_cast<T*>((reinterpret_cast<uintptr_t>(part_list + a.part_cap) + 15) & ~(uintptr_t)15);
-    const G g{a.logits + (size_t)group * beams * a.ld, a.staged ? stage : all_lanes, max_s, add_s, item_list,
+    const G g{a.logits + (size_t)group * beams * a.ld, a.staged ? stage : all_lanes, unit_parts, state_s, max_s, add_s, item_list,
               part_list, a.ld, a.inv_t, 1.0f / (float)a.units, a.V, a.units, lg};
     const auto no_part = [] { return make_float4(-INFINITY, 0.0f, 0.0f, 0.0f); };
     // a unit's sum against the row's maximum
@@ -384,7 +496,7 @@ pick_kernel(const __grid_constant__ PickArgs<T> a) {
     const auto put_item = [&](int i, float x, int beam) {
         const bool offered = kRows || state_s[beam] == 0;
         if (offered) top = fmaxf(top, x);
-        item_score[i] = offered ? g.score(x, beam) : -(S)INFINITY;
+        item_score[i] = offered && x > -INFINITY ? fmaxf((float)g.score(x, beam), kLowest<float>) : -INFINITY;
     };
     if (a.staged || lg == kLog) {
         const int vecs = beams * a.units * (32 / kN);
@@ -448,15 +560,29 @@ pick_kernel(const __grid_constant__ PickArgs<T> a) {
     }
     const size_t out = (size_t)group * a.n;
     if (!bad) {
-        Bound<S> bound = narrow(Bound<S>{kLowest<S>, 0xFFFFFFFFu}, a.n, a.item_cap - kExtra - a.n, best, counter, [&](auto f) {
-#pragma unroll 4
-            for (int i = t; i < all_items; i += kThreads) f(item_score[i], [&] { return g.last_place(i << lg, 1 << lg); });
-        });
-        for (int i = t; i < all_items; i += kThreads)
-            if (bound.has(item_score[i], [&] { return g.first_place(i << lg); })) {
-                const int at = atomicAdd(&items_s, 1);
-                if (at < a.item_cap) item_list[at] = i;
+        const Within within =
+            find_within<kThreads>(item_score, all_items, a.n, a.item_cap - kExtra - a.n, (float)best, steps, &found_s);
+        Bound<S> bound{kLowest<S>, 0xFFFFFFFFu};
+        if (within.step > -2) {
+            uint32_t least = 0xFFFFFFFFu;
+            for (int i = t; i < all_items; i += kThreads)
+                if (within.has(item_score[i])) {
+                    least = min(least, key_of(item_score[i]));
+                    const int at = atomicAdd(&items_s, 1);
+                    if (at < a.item_cap) item_list[at] = i;
+                }
+            if (within.step >= 0) {  // the least of them is the bound
+                least = __reduce_min_sync(0xffffffffu, least);
+                if (lane == 0) atomicMin(&least_s, least);
+                __syncthreads();
+                bound.v = score_at(least_s);
+                // of rounded sums: below all that round to it
+                if constexpr (!kRows)
+                    bound.v = score_at(least_s) > kLowest<float> ? (double)nextafterf(score_at(least_s), -INFINITY) : kLowest<double>;
             }
+        } else {
+            bound = list_items<T, kRows, kThreads>(g, all_items, a.n, a.item_cap, best, red, &items_s);
+        }
         __syncthreads();
         if (kRows && t == kThreads - 1) {  // needed when the list is written
             double sum = 0.0;
@@ -502,7 +628,7 @@ pick_kernel(const __grid_constant__ PickArgs<T> a) {
             }
             __syncthreads();
             if (parts_s <= a.part_cap) break;
-            bound = narrow_by<T, kRows, kThreads>(g, false, items, bound, a.n, a.part_cap - kExtra - a.n, best, counter);
+            bound = narrow_by<T, kRows, kThreads>(g, kByLanes, items, bound, a.n, a.part_cap - kExtra - a.n, best, red);
             if (t == 0) parts_s = 0;
             __syncthreads();
         }
@@ -558,7 +684,7 @@ pick_kernel(const __grid_constant__ PickArgs<T> a) {
             }
             __syncthreads();
             if (cands_s <= kMaxCands) break;  // else few parts hold them, or few parts there are
-            bound = narrow_by<T, kRows, kThreads>(g, true, parts, bound, a.n, kMaxCands - a.n, best, counter);
+            bound = narrow_by<T, kRows, kThreads>(g, kByElements, parts, bound, a.n, kMaxCands - a.n, best, red);
             if (t == 0) cands_s = 0;
             if constexpr (!kRows) {
                 for (int i = t; i < beams; i += kThreads) floor_s[i] = -INFINITY;  // the score decides
@@ -677,18 +803,19 @@ static int best(const Rows& r, PickArgs<T> p, void* workspace, cudaStream_t st) 
     p.log_lanes = units >= 3 * p.n ? 5 : units << (5 - log_n) >= 3 * p.n ? log_n : 0;
     p.item_cap = p.n + p.n / 4 + 16 + kExtra;
     p.part_cap = 3 * p.n + 2 * kExtra < kMaxParts ? 3 * p.n + 2 * kExtra : kMaxParts;
-    // lanes that a CTA brings to shared memory: 40 KB leave room for several groups an SM
-    const size_t lanes = (size_t)units * 32 * sizeof(T), items = ((size_t)units << (5 - p.log_lanes)) + 1;
-    p.staged = lanes <= 40 * 1024;
-    const auto go = [&](auto kernel, int threads, size_t score, DeviceOnce& once) {
+    // The lanes' maxima go to shared memory where all of them are looked at (40 KB leave room for several groups an SM);
+    // where units are narrowed down first, few are, and are read when their units are known.
+    const size_t lanes = (size_t)units * 32 * sizeof(T), items = (size_t)units << (5 - p.log_lanes);
+    p.staged = p.log_lanes != 5 && lanes <= 40 * 1024;
+    const auto go = [&](auto kernel, int threads, DeviceOnce& once) {
         const int e = once.raise((const void*)kernel, 160 * 1024);
         if (e) return e;
-        const size_t smem = items * score + ((size_t)p.item_cap + p.part_cap) * sizeof(int) + (p.staged ? lanes + 16 : 0);
+        const size_t smem = items * sizeof(float) + ((size_t)p.item_cap + p.part_cap) * sizeof(int) + (p.staged ? lanes + 16 : 0);
         return launch("pick_kernel", kernel, r.rows / p.beams, threads, 1, smem, true, st, p);
     };
     static DeviceOnce once[4];
-    if (!p.parents) return p.n > 64 ? go(pick_kernel<T, true, 512>, 512, 4, once[0]) : go(pick_kernel<T, true, 128>, 128, 4, once[1]);
-    return p.n > 64 || p.beams > 4 ? go(pick_kernel<T, false, 256>, 256, 8, once[2]) : go(pick_kernel<T, false, 128>, 128, 8, once[3]);
+    if (!p.parents) return p.n > 64 ? go(pick_kernel<T, true, 512>, 512, once[0]) : go(pick_kernel<T, true, 128>, 128, once[1]);
+    return p.n > 64 || p.beams > 4 ? go(pick_kernel<T, false, 256>, 256, once[2]) : go(pick_kernel<T, false, 128>, 128, once[3]);
 }
 
 }  // namespace qs
