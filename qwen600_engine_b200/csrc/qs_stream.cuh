@@ -69,10 +69,6 @@ struct UnitAt {
     }
 };
 
-__device__ __forceinline__ bool takes_part(const float* scores, const unsigned char* finished, int row) {
-    return !(finished && finished[row]) && !(scores && !isfinite(scores[row]));
-}
-
 template <typename T, bool kBest>
 __global__ void __launch_bounds__(kStreamWarps * 32, 1)
 stream_kernel(const __grid_constant__ StreamArgs<T> a) {
@@ -94,12 +90,23 @@ stream_kernel(const __grid_constant__ StreamArgs<T> a) {
     const long long stride = (long long)gridDim.x * kStreamWarps, begin = (long long)warp * gridDim.x + blockIdx.x;
     const int dr = (int)(stride / a.units), du = (int)(stride % a.units);
     UnitAt now{(int)(begin / a.units), (int)(begin % a.units)}, ahead = now;
-    const auto scored = [&](int row) {
-        if (row >= a.rows) return false;
-        if (kBest) return takes_part(a.scores, a.finished, row);
-        const int tok = a.tokens[row];
-        return tok >= 0 && tok < a.V;
+    // what says whether a row takes part, as it is loaded: looked at when it is needed, one unit later
+    struct Look {
+        int mark;
+        float score;
     };
+    const auto look = [&](int row) {
+        Look l{-1, 0.0f};
+        if (row >= a.rows) return l;
+        if (kBest) {
+            l.mark = a.finished ? -(int)a.finished[row] : 0;
+            if (a.scores) l.score = a.scores[row];
+        } else {
+            l.mark = a.tokens[row];
+        }
+        return l;
+    };
+    const auto scored = [&](const Look& l) { return l.mark >= 0 && (kBest ? isfinite(l.score) : l.mark < a.V); };
     const auto request = [&](const UnitAt& u, int stage) {
         if (lane == 0) {
             const T* x = a.logits + (size_t)u.row * a.ld;
@@ -118,13 +125,13 @@ stream_kernel(const __grid_constant__ StreamArgs<T> a) {
     uint32_t phases = 0;  // the parity each stage's next copy completes
 #pragma unroll
     for (int i = 0; i < kStreamStages; i++) {
-        if (scored(ahead.row)) {
+        if (scored(look(ahead.row))) {
             request(ahead, i);
             live |= 1u << i;
         }
         ahead.step(dr, du, a.units);
     }
-    bool next = scored(ahead.row);  // looked up one unit before it is asked for
+    Look next = look(ahead.row);
     bool dead = false;
     for (int stage = 0; now.row < a.rows; stage = stage + 1 == kStreamStages ? 0 : stage + 1) {
         if (live >> stage & 1) {
@@ -177,7 +184,7 @@ stream_kernel(const __grid_constant__ StreamArgs<T> a) {
             }
             __syncwarp();  // every lane has read the stage
             live &= ~(1u << stage);
-            if (next && !dead) {
+            if (scored(next) && !dead) {
                 request(ahead, stage);
                 live |= 1u << stage;
             }
@@ -219,14 +226,14 @@ stream_kernel(const __grid_constant__ StreamArgs<T> a) {
                 a.parts[(size_t)now.row * a.units + now.unit] = make_float4(m, dead ? NAN : s, (float)at_max, 0.0f);
         } else {
             if (lane == 0 && dead) a.parts[(size_t)now.row * a.units + now.unit] = make_float4(0.0f, NAN, 0.0f, 0.0f);
-            if (next && !dead) {
+            if (scored(next) && !dead) {
                 request(ahead, stage);
                 live |= 1u << stage;
             }
         }
         now.step(dr, du, a.units);
         ahead.step(dr, du, a.units);
-        next = scored(ahead.row);
+        next = look(ahead.row);
     }
 }
 
