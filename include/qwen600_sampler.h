@@ -520,7 +520,7 @@ QS_API int qs_top_logprobs(const void* d_logits, int dtype, int rows, int vocab,
  * stays in that beam's place and the others take the places left, the better
  * first: then only places of beams that end change their state, each to that of
  * a beam that stays where it is.  Beams 1 to QS_MAX_BEAMS, n 1 to QS_MAX_LISTED.
- * The outputs may not overlap the inputs. */
+ * The outputs may not overlap the scores and marks that are read. */
 typedef struct {
     double temperature;
     int eos_token;
@@ -575,8 +575,8 @@ QS_API int qs_reorder_history(qs_sampler* s, const int* d_parents, int batch, in
  *   loss = sum_i w[i] l
  * w = d_weights[i] (NULL: 1 / rows).  A token outside the vocabulary is no entry;
  * one listed again counts where it stands first.  A log-probability of -inf is
- * q = 0, and 0 log 0 = 0.  A row with w[i] = 0, without entries, or with rest = 0
- * whose q are all 0, adds nothing, has a zero gradient and is not read.  A
+ * q = 0, and 0 log 0 = 0.  A row with w[i] = 0 (which is not read), without entries,
+ * or with rest = 0 whose q are all 0, adds nothing and has a zero gradient.  A
  * teacher's token that the logits mask (-inf, with q > 0) makes the loss +inf.
  * d_loss fp32 [1], d_row_losses fp32 [rows] (l, 0 for rows that add nothing) or
  * NULL, d_grad as for the losses above (NULL: the loss alone).  1 <= k <=

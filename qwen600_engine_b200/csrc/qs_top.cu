@@ -561,7 +561,7 @@ pick_kernel(const __grid_constant__ PickArgs<T> a) {
     const size_t out = (size_t)group * a.n;
     if (!bad) {
         const Within within =
-            find_within<kThreads>(item_score, all_items, a.n, a.item_cap - kExtra - a.n, (float)best, steps, &found_s);
+            find_within<kThreads>(item_score, all_items, a.n, a.item_cap - kExtra - a.n, fmaxf((float)best, kLowest<float>), steps, &found_s);
         Bound<S> bound{kLowest<S>, 0xFFFFFFFFu};
         if (within.step > -2) {
             uint32_t least = 0xFFFFFFFFu;
@@ -598,7 +598,8 @@ pick_kernel(const __grid_constant__ PickArgs<T> a) {
         while (true) {
             if constexpr (!kRows) {
                 for (int i = t; i < beams; i += kThreads) {
-                    const double x = (double)max_s[i] + (bound.v - add_s[i]) / a.inv_t;
+                    // the sum's rounding, 2^-53 of its parts, hides what is smaller
+                    const double x = (double)max_s[i] + (bound.v - add_s[i] - 1e-15 * (fabs(bound.v) + fabs(add_s[i]))) / a.inv_t;
                     floor_s[i] = __double2float_rd(x - 1e-6 * (fabs(x) + fabs((double)max_s[i])));
                 }
                 __syncthreads();
@@ -873,6 +874,13 @@ int qs_beam_select(const void* d_logits, int dtype, int batch, int beams, int vo
     if (batch == 0) return QS_OK;
     if (!d_scores) return fail(QS_ERR_INVALID, "NULL device pointer");
     if (!d_out_scores || !d_parents || !d_tokens) return fail(QS_ERR_INVALID, "NULL output buffer");
+    const size_t in = (size_t)batch * beams, out = (size_t)batch * n;
+    const struct { const void* p; size_t bytes; } reads[] = {{d_scores, in * sizeof(float)}, {d_finished, in}},
+        writes[] = {{d_out_scores, out * sizeof(float)}, {d_parents, out * sizeof(int)}, {d_tokens, out * sizeof(int)}, {d_out_finished, out}};
+    for (const auto& r : reads)
+        for (const auto& w : writes)
+            if (r.p && w.p && (uintptr_t)r.p < (uintptr_t)w.p + w.bytes && (uintptr_t)w.p < (uintptr_t)r.p + r.bytes)
+                return fail(QS_ERR_INVALID, "an output overlaps the scores or marks");
     rc = check_workspace(d_workspace, workspace_bytes, best_workspace(dtype, batch * beams, vocab, n));
     if (rc) return rc;
     const auto go = [&](auto p) {

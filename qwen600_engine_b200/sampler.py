@@ -317,6 +317,8 @@ class Sampler:
             raise SamplerError(_lib.QS_ERR_INVALID, f"parents must be a contiguous int32 tensor [batch, beams] on cuda:{self.device}")
         st = stream if stream is not None else torch.cuda.current_stream(p.device)
         if stream is not None:
+            if stream.device != p.device:
+                raise SamplerError(_lib.QS_ERR_INVALID, f"stream of {stream.device} for parents on {p.device}")
             p.record_stream(stream)
         check(_lib.lib.qs_reorder_history(self._h, _ptr(p), int(p.shape[0]), int(p.shape[1]), int(st.cuda_stream)))
 

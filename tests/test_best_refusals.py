@@ -20,7 +20,7 @@ def top(logits=P, dtype=QS_BF16, rows=4, vocab=1000, ld=1000, k=5, T=1.0, lp=P, 
 
 
 def select(logits=P, dtype=QS_BF16, batch=2, width=2, vocab=1000, ld=1000, scores=P, finished=None, n=2, T=1.0, eos=-1, pad=-1, keep=0,
-           out=P, parents=P, tok=P, done=P, ws=P, size=1 << 30, params=True):
+           out=FAR, parents=FAR + 64, tok=FAR + 128, done=FAR + 192, ws=P, size=1 << 30, params=True):
     p = _lib.BeamParams(T, eos, pad, keep)
     return L.qs_beam_select(logits, dtype, batch, width, vocab, ld, scores, finished, n, C.byref(p) if params else None, out, parents,
                             tok, done, ws, size, None)
@@ -42,7 +42,8 @@ WORK = [dict(ws=None), dict(ws=P + 4), dict(size=8)]
 @pytest.mark.parametrize("call,bad", [(top, b) for b in ROWS + TEMPS + WORK + [dict(rows=-1), dict(lp=None), dict(tok=None)]]
                          + [(select, b) for b in ROWS + TEMPS + WORK + [
                              dict(batch=-1), dict(scores=None), dict(out=None), dict(parents=None), dict(tok=None), dict(params=False),
-                             dict(eos=1000), dict(eos=-2), dict(keep=1, n=3), dict(keep=1, n=1)]]
+                             dict(eos=1000), dict(eos=-2), dict(keep=1, n=3), dict(keep=1, n=1),
+                             dict(out=P), dict(parents=P + 12), dict(tok=P - 12), dict(done=P + 3), dict(finished=FAR + 128), dict(finished=FAR - 3)]]
                          + [(distill, b) for b in ROWS + TEMPS + GRADS + WORK + [
                              dict(rows=-1), dict(tokens=None), dict(lps=None), dict(loss=None), dict(params=False)]])
 def test_c_abi_refuses(call, bad):

@@ -258,6 +258,31 @@ def test_beams(dtype, batch, beams, V, n):
     check_beams(rows_of(batch * beams, V, dtype, seed=batch + V), scores_of(batch, beams, n), n, T=0.9)
 
 
+@pytest.mark.parametrize("T", [1e-3, 0.05, 40.0])
+@pytest.mark.parametrize("keep", [False, True])
+def test_beams_at_any_temperature(T, keep):
+    """Sums of up to 2^24 and more: the 64-bit sums' spacing is far below an fp32 logit's."""
+    x = rows_of(15, 5003, torch.float32, seed=16)
+    r = select(x, scores_of(3, 5, 8), n=5, temperature=T, keep_slots=keep)
+    for b, ref in enumerate(exact_beams(x, scores_of(3, 5, 8), 5, None, -1, -1, T, keep)):
+        got = sorted(zip(r.scores[b].tolist(), r.parents[b].tolist(), r.tokens[b].tolist()), key=lambda g: (-g[0], g[1], g[2]))
+        for g, e in zip(got, ref):
+            total = max(1.0, 5003 ** 0.5 / T)
+            assert abs(g[0] - e[0]) <= rel_sum(5003) * total + 2 * U * abs(e[0])
+        assert {g[1:] for g in got} == {e[1:] for e in ref[:5]}
+
+
+@pytest.mark.parametrize("kind", ["few values", "equal", "masked", "lowest", "block", "rising"])
+@pytest.mark.parametrize("beams,n", [(1, 200), (6, 12), (16, 256)])
+def test_beams_where_order_is_hard(kind, beams, n):
+    """Rows alike but for their scores, so that equal sums are equal bits."""
+    x = rows_of(1, 8192, torch.bfloat16, seed=17, kind=kind).repeat(3 * beams, 1)
+    scores = -torch.arange(3 * beams, device="cuda").view(3, beams).float() % 7
+    check_beams(x, scores, n)
+    check_beams(x, torch.zeros_like(scores), n)
+    check_beams(x, scores - 2.0 ** 22, n)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("keep", [False, True])
 @pytest.mark.parametrize("share", [0.0, 0.4, 1.0])
@@ -322,6 +347,20 @@ def test_entries_with_nan(bad):
             assert all(torch.equal(p[b], q[b]) for p, q in zip(r, clean))
     finished[1, 1] = True  # a finished beam's logits are not read
     assert not select(x, scores, n=5, finished=finished).scores[1].isnan().any()
+
+
+@pytest.mark.parametrize("keep", [False, True])
+def test_beams_far_from_zero(keep):
+    """Scores so low that fp32 cannot tell candidates apart; the lowest of all."""
+    x = rows_of(12, 3001, torch.float32, seed=18)
+    scores = torch.full((3, 4), -3e6, device="cuda")
+    scores[1] = torch.finfo(torch.float32).min
+    scores[2] = torch.tensor([0.0, -1e30, 0.5, 1e30])
+    r = select(x, scores, n=4, keep_slots=keep)
+    ref = exact_beams(x, scores, 4, None, -1, -1, 1.0, keep)
+    assert {(p, t) for p, t in zip(r.parents[0].tolist(), r.tokens[0].tolist())} == {e[1:] for e in ref[0][:4]}
+    assert (r.scores[1] == torch.finfo(torch.float32).min).all() and (r.tokens[1] >= 0).all()
+    assert (r.parents[2] == 3).sum() == 4 and (r.scores[2] == 1e30).all()
 
 
 @pytest.mark.parametrize("keep", [False, True])
