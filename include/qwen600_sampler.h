@@ -543,7 +543,8 @@ QS_API int qs_beam_select(const void* d_logits, int dtype, int batch, int beams,
  * [batch] or NULL: the first d_lengths[b] positions (bounded to 0 .. positions)
  * of entry b's rows are moved, what lies behind them stays.  `states` is on the
  * host.  Pieces may not overlap, nor states: two of them may lie between one
- * another only with the same row stride and apart within it.
+ * another only if both repeat with the same stride and are apart within it; they may
+ * not overlap the parents and lengths.
  * batch * beams <= 2^27, beams <= 1024, at most 2^31 - 1 pieces of a row. */
 typedef struct {
     void* d_base;

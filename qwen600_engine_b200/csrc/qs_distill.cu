@@ -1,16 +1,18 @@
 // Divergence from a teacher known by the best tokens of each row, and the
 // gradient of the logits (include/qwen600_sampler.h gives the formula).
 //
-// With m_r the maximum of the unlisted logits and m_l that of the listed ones,
-//   S_r = sum over unlisted j of exp((x[j] - m_r) / T)     fp32, joined in 64 bits
+// With m_l the maximum of the listed logits,
 //   S_l = sum over listed e of exp((x[e] - m_l) / T)       64 bits
-// and S = S_l exp((m_l - m) / T) + S_r exp((m_r - m) / T), m the larger of the
-// two.  The unlisted sum is taken by itself, against its own maximum: as what is
-// left of 1 it would be nothing but rounding wherever the list holds nearly
-// all, and p_r stands in a logarithm and a denominator.  The gradient is
+//   S_r = sum over unlisted j of exp((x[j] - m_l) / T)     fp32, joined in 64 bits
+// and S their sum.  The unlisted sum is taken by itself: as what is left of 1 it
+// would be nothing but rounding wherever the list holds nearly all, and p_r stands
+// in a logarithm and a denominator.  The gradient is
 //   listed    w / T (Q p[e] - q[e])                        64 bits
-//   unlisted  f exp((x[j] - m_r) / T),  f = w / T (Q exp((m_r - m) / T) / S - r / S_r)
-// so that one coefficient serves every token but the listed.
+//   unlisted  f exp((x[j] - m_l) / T),  f = w / T (Q / S - r / S_r)
+// so that one coefficient, formed without a logarithm, serves every token but the
+// listed.  m_l is known before the row has arrived, which saves the pass that looks
+// for a maximum; where S_r shows that the list lies far from the unlisted tokens, they
+// are summed again against their own maximum.
 #include "qs_rows.cuh"
 
 namespace qs {
@@ -63,8 +65,9 @@ __device__ __forceinline__ double warp_sum_double(double v) {
 }
 
 // The lists, a warp for a row: each token where it stands first, its logit, and what
-// the loss takes of both.  Once for a row, where the row's CTAs would all have to; a
-// launch of 3 us, which they begin beside.
+// the loss takes of both.  Once for a row, where the row's CTAs would all have to
+// (2048 rows 279 us then, 247 with it).  Latency: 2.4 us for 8 rows with lists of 20, 8
+// for 300 with lists of 129; the rows' copies begin beside it.
 constexpr int kListWarps = 4;
 constexpr int kListMine = QS_MAX_LISTED / 32;
 
@@ -159,6 +162,10 @@ __device__ __forceinline__ void push_double(double* slot, int rank, double v) {
 // forms the gradient from the same copy, so that the row is read from memory once and
 // a CTA's warps meet once.  The listed entries' places in the pieces are overwritten
 // with -inf, which takes them out of the sum and of the gradient's stream.
+//
+// Bound: memory, and the waits between a row's phases, two CTAs an SM: 208 us for 2048 bf16
+// rows of 151,936 a quarter of which is left out (1089 MB, 5.2 TB/s), 26 for 300 fp32 rows
+// of 37,999.  Its exponentials alone, two a token, would take 104.
 template <typename T>
 __global__ void __launch_bounds__(kDistillThreads, 2)
 distill_kernel(const __grid_constant__ DistillArgs<T> a) {

@@ -451,6 +451,17 @@ grad_kernel(const T* logits, int rows, int V, long long ld, const int* __restric
     if (mine) put(g, tok, target);
 }
 
+// The policy loss: the rows' terms, added in a fixed order.
+__global__ void __launch_bounds__(1024)
+sum_rows_kernel(const double* row_loss, int rows, float* __restrict__ loss) {
+    __shared__ double red[32];
+    wait_for_previous();
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < rows; i += blockDim.x) sum += row_loss[i];
+    sum = block_sum(sum, red);
+    if (threadIdx.x == 0) *loss = (float)sum;
+}
+
 // One warp per pair in turn: the two sequences' sums, the pair's loss and the
 // coefficients of their rows' gradients (0 so far).  Sequences share no row
 // unless an offset falls somewhere: then none counts, so that no two warps write

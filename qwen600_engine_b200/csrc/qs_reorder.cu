@@ -269,9 +269,17 @@ int reorder_states(const qs_states* all, int count, const int* d_parents, int ba
     if (count < 0) return fail(QS_ERR_INVALID, "count %d < 0", count);
     if (batch == 0 || count == 0) return QS_OK;
     if (!all || !d_parents) return fail(QS_ERR_INVALID, "NULL pointer");
-    const int bad = check_states(all, count, batch * beams);
-    if (bad) return bad;
     const int rows = batch * beams;
+    const int bad = check_states(all, count, rows);
+    if (bad) return bad;
+    for (int i = 0; i < count; i++) {
+        Level l[4];
+        const int levels = levels_of(all[i], rows, l);
+        const uintptr_t from = (uintptr_t)all[i].d_base, to = from + span_of(all[i].unit, l, levels, kAllLevels);
+        const uintptr_t p = (uintptr_t)d_parents, n = (uintptr_t)d_lengths;
+        if ((p < to && from < p + rows * sizeof(int)) || (n && n < to && from < n + batch * sizeof(int)))
+            return fail(QS_ERR_INVALID, "state %d overlaps the parents or lengths", i);
+    }
     // states whose vectors have the same width go together
     for (int width = 0; width <= 4; width++) {
         int begin = 0;

@@ -178,17 +178,6 @@ __device__ __forceinline__ void push_part(Part* slot, int rank, const Part& p) {
                  : "memory");
 }
 
-// A loss: the rows' terms, added in a fixed order.
-static __global__ void __launch_bounds__(1024)
-sum_rows_kernel(const double* row_loss, int rows, float* __restrict__ loss) {
-    __shared__ double red[32];
-    wait_for_previous();
-    double sum = 0.0;
-    for (int i = threadIdx.x; i < rows; i += blockDim.x) sum += row_loss[i];
-    sum = block_sum(sum, red);
-    if (threadIdx.x == 0) *loss = (float)sum;
-}
-
 [[maybe_unused]] static int fail(int code, const char* fmt, ...) {
     char buf[512];
     va_list ap;

@@ -117,6 +117,10 @@ def test_reorder_calls_refused():
     assert reorder(state(), batch=1 << 30) == QS_ERR_UNSUPPORTED
     assert reorder(state(unit=1, positions=1 << 30, stride=3, outer=(1, 4), outer_stride=(0, 1 << 33), row=1 << 40)) == QS_ERR_UNSUPPORTED
     assert L.qs_reorder_history(None, P, 2, 3, None) == QS_ERR_INVALID
+    for at in (P, P + 20, P - 5999):  # a state that holds the parents, or the lengths
+        assert reorder(state(base=at)) == QS_ERR_INVALID
+        a = (_lib.States * 1)(state(base=at))
+        assert L.qs_beam_reorder(a, 1, FAR, 2, 3, P if at != P + 20 else P + 15, None) == QS_ERR_INVALID
 
 
 X = torch.zeros((4, 10))
