@@ -69,12 +69,12 @@ __device__ __forceinline__ double warp_sum_double(double v) {
 // (2048 rows 279 us then, 247 with it).  Latency: 2.4 us for 8 rows with lists of 20, 8
 // for 300 with lists of 129; the rows' copies begin beside it.
 constexpr int kListWarps = 4;
-constexpr int kListMine = QS_MAX_LISTED / 32;
 
-template <typename T>
+// kListMine: entries of a lane.
+template <typename T, int kListMine>
 __global__ void __launch_bounds__(kListWarps * 32)
 distill_list_kernel(const __grid_constant__ DistillArgs<T> a) {
-    __shared__ __align__(16) int tokens[kListWarps][QS_MAX_LISTED];
+    __shared__ __align__(16) int tokens[kListWarps][kListMine * 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * kListWarps + warp;
     dependents_may_start();
     if (row >= a.rows) return;
@@ -434,7 +434,13 @@ static int distill_launch(DistillArgs<T>& a, cudaStream_t st) {
     static DeviceOnce once;
     int rc = once.raise((const void*)distill_kernel<T>, 200 * 1024);
     if (rc) return rc;
-    rc = launch("distill_list_kernel", distill_list_kernel<T>, (a.rows + kListWarps - 1) / kListWarps, kListWarps * 32, 1, 0, false, st, a);
+    const auto lists = [&](auto kernel) {
+        return launch("distill_list_kernel", kernel, (a.rows + kListWarps - 1) / kListWarps, kListWarps * 32, 1, 0, false, st, a);
+    };
+    rc = a.k <= 32    ? lists(distill_list_kernel<T, 1>)
+         : a.k <= 64  ? lists(distill_list_kernel<T, 2>)
+         : a.k <= 128 ? lists(distill_list_kernel<T, 4>)
+                      : lists(distill_list_kernel<T, 8>);
     if (rc) return rc;
     return launch("distill_kernel", distill_kernel<T>, (long long)a.rows << log_c, kDistillThreads, 1 << log_c, smem, true, st, a);
 }
