@@ -17,7 +17,6 @@
 
 namespace qs {
 
-constexpr int kDistillThreads = 256;
 // Where the unlisted terms against the list's maximum come out below or above these,
 // they are summed again against their own.  A term's exponent is rounded to a 2^-24th of
 // itself; with sums from 2^-28 on it lies on the average below log2 V + 28.
@@ -166,11 +165,11 @@ __device__ __forceinline__ void push_double(double* slot, int rank, double v) {
 // Bound: memory, and the waits between a row's phases, two CTAs an SM: 208 us for 2048 bf16
 // rows of 151,936 a quarter of which is left out (1089 MB, 5.2 TB/s), 26 for 300 fp32 rows
 // of 37,999.  Its exponentials alone, two a token, would take 104.
-template <typename T>
-__global__ void __launch_bounds__(kDistillThreads, 2)
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, 512 / kThreads)
 distill_kernel(const __grid_constant__ DistillArgs<T> a) {
     constexpr int kN = Pack<T>::kN;
-    constexpr int kW = kDistillThreads / 32;
+    constexpr int kW = kThreads / 32;
     extern __shared__ __align__(16) uint4 vecs[];  // [warp][piece]
     __shared__ double parts[3][8], pass_sum[kW];
     __shared__ float red_max[kW];
@@ -185,7 +184,7 @@ distill_kernel(const __grid_constant__ DistillArgs<T> a) {
         if (!a.grad) return;
         T* g = a.grad + (size_t)row * a.gld;
         const RowShape<T> gs(g, a.V);
-        for (int i = rank * kDistillThreads + t; i < gs.vecs; i += C * kDistillThreads)
+        for (int i = rank * kThreads + t; i < gs.vecs; i += C * kThreads)
             store16(g + gs.head + (size_t)i * kN, make_uint4(0u, 0u, 0u, 0u));
         const int e = rank == 0 ? gs.edge(t, a.V) : -1;
         if (e >= 0) put(g, e, 0.0f);
@@ -421,7 +420,7 @@ distill_loss_kernel(const RowList* lists, int rows, const float* __restrict__ we
 // the 148 SMs idle and a share keeps 4 KB.  2048 bf16 rows of 151,936, a quarter of them
 // left out: 218 us with 4 CTAs a row (76 KB shares), 241 with 8 (38 KB, five an SM), 312
 // with 2; 300 fp32 rows of 37,999 29 us with 2, 31 with 4.  CTAs of 224 threads 232 us, of
-// 384 259.
+// 384 259.  CTAs that have an SM for themselves take 512 threads (8 rows 6.2 us, 7.0 with 256).
 template <typename T>
 static int distill_launch(DistillArgs<T>& a, cudaStream_t st) {
     const int vecs = a.V / Pack<T>::kN;
@@ -430,19 +429,22 @@ static int distill_launch(DistillArgs<T>& a, cudaStream_t st) {
     while (log_c < 3 && (share() > 5120 || ((long long)a.rows << log_c) < 148 && share() > 256)) log_c++;
     a.log_c = log_c;
     a.share = share();
-    const size_t smem = (size_t)((a.share + 7) / 8 * 8) * 16;
-    static DeviceOnce once;
-    int rc = once.raise((const void*)distill_kernel<T>, 200 * 1024);
-    if (rc) return rc;
     const auto lists = [&](auto kernel) {
         return launch("distill_list_kernel", kernel, (a.rows + kListWarps - 1) / kListWarps, kListWarps * 32, 1, 0, false, st, a);
     };
-    rc = a.k <= 32    ? lists(distill_list_kernel<T, 1>)
-         : a.k <= 64  ? lists(distill_list_kernel<T, 2>)
-         : a.k <= 128 ? lists(distill_list_kernel<T, 4>)
-                      : lists(distill_list_kernel<T, 8>);
+    int rc = a.k <= 32    ? lists(distill_list_kernel<T, 1>)
+             : a.k <= 64  ? lists(distill_list_kernel<T, 2>)
+             : a.k <= 128 ? lists(distill_list_kernel<T, 4>)
+                          : lists(distill_list_kernel<T, 8>);
     if (rc) return rc;
-    return launch("distill_kernel", distill_kernel<T>, (long long)a.rows << log_c, kDistillThreads, 1 << log_c, smem, true, st, a);
+    const auto rows = [&](auto kernel, int threads, DeviceOnce& once) {
+        const int warps = threads / 32, e = once.raise((const void*)kernel, 200 * 1024);
+        if (e) return e;
+        const size_t smem = (size_t)((a.share + warps - 1) / warps * warps) * 16;
+        return launch("distill_kernel", kernel, (long long)a.rows << log_c, threads, 1 << log_c, smem, true, st, a);
+    };
+    static DeviceOnce few, many;
+    return (long long)a.rows << log_c <= 148 ? rows(distill_kernel<T, 512>, 512, few) : rows(distill_kernel<T, 256>, 256, many);
 }
 
 // Workspace: the rows' lists, and their entries.

@@ -45,6 +45,7 @@ struct PickArgs {
     int log_lanes;  // lanes of an item of the first narrowing: 32 (a unit), a vector of maxima, or 1
     int item_cap, part_cap;
     int staged;  // the lanes' maxima are brought to shared memory
+    int coarse;  // few parts for what is wanted: their elements are narrowed down before any is listed
     const float* scores;            // of beams (NULL: 0)
     const unsigned char* finished;  // beams that go on with `pad` alone (NULL: none)
     int pad, eos, keep;
@@ -209,24 +210,33 @@ constexpr int kSteps = 256;
 struct Within {
     float best, from, per;  // steps a unit
     int step;               // -1: all; -2: not found
+    // Below all of them, whatever was rounded.
+    template <typename S>
+    __device__ __forceinline__ S below() const {
+        const S d = (S)(from + (float)(step + 1) / per);
+        return step < 0 ? kLowest<S> : (S)best - d - (S)1e-6f * ((S)fabsf(best) + d);
+    }
     __device__ __forceinline__ bool has(float s) const {
         const float d = best - s;
         return s > -INFINITY && (step == -1 || d < from || (int)fminf((d - from) * per, 1e6f) <= step);
     }
 };
 
-template <int kThreads>
-__device__ __forceinline__ Within find_within(const float* score, int items, int n, int slack, float best, int* steps, int2* found) {
+// each(f) calls f(score) for this thread's scores; `steps` is clear on entry.
+template <int kThreads, typename Each>
+__device__ __forceinline__ Within find_within(int n, int slack, float best, int* steps, int2* found, Each each) {
     const int t = threadIdx.x;
     Within w{best, 0.0f, 4.0f, -2};
     int before = 0;
     for (int pass = 0; pass < 4; pass++) {  // as long as every step's border is a number of 24 bits, so that none counts twice
-        for (int i = t; i <= kSteps; i += kThreads) steps[i] = 0;
-        __syncthreads();
-        for (int i = t; i < items; i += kThreads) {
-            const float s = score[i], d = best - s;
-            if (s > -INFINITY && d >= w.from) atomicAdd(&steps[(int)fminf((d - w.from) * w.per, (float)kSteps)], 1);
+        if (pass > 0) {
+            for (int i = t; i <= kSteps; i += kThreads) steps[i] = 0;
+            __syncthreads();
         }
+        each([&](float s) {
+            const float d = best - s;
+            if (s > -INFINITY && d >= w.from) atomicAdd(&steps[(int)fminf((d - w.from) * w.per, (float)kSteps)], 1);
+        });
         __syncthreads();
         if (t < 32) {  // eight steps a lane: where the count reaches n
             int own[kSteps / 32], sum = 0;
@@ -370,6 +380,40 @@ __device__ __noinline__ Bound<typename Group<T, kRows>::S> narrow_by(Group<T, kR
     return b;
 }
 
+// A score rounded to fp32 as the steps take it.
+__device__ __forceinline__ float rounded(float s) { return s; }
+__device__ __forceinline__ float rounded(double s) { return s > -(double)INFINITY ? fmaxf((float)s, kLowest<float>) : -INFINITY; }
+
+// By the listed parts' elements, counted in steps: where few parts there are (small
+// vocabularies and long lists) they hold thousands.  `steps` need not be clear.
+template <typename T, bool kRows, int kThreads>
+__device__ __noinline__ Bound<typename Group<T, kRows>::S> step_by_elements(Group<T, kRows> g, int count,
+                                                                            Bound<typename Group<T, kRows>::S> within, int n, int slack,
+                                                                            typename Group<T, kRows>::S best, uint2 (*red)[kThreads / 32],
+                                                                            int* steps, int2* found) {
+    using S = typename Group<T, kRows>::S;
+    __syncthreads();
+    for (int i = threadIdx.x; i <= kSteps; i += kThreads) steps[i] = 0;
+    __syncthreads();
+    const Within w = find_within<kThreads>(n, slack, rounded(best), steps, found, [&](auto f) {
+        for (int i = threadIdx.x; i < count * g.kPartVecs; i += kThreads) {
+            const auto at = g.at(i);
+            if (at.whole) {
+                float o[Group<T, kRows>::kN];
+                Pack<T>::widen(load16(at.row + at.token), o);
+#pragma unroll
+                for (int j = 0; j < g.kN; j++) f(rounded(g.score(o[j], at.beam)));
+            }
+            if (at.edge >= 0) f(rounded(g.score(elem(at.row, at.edge), at.beam)));
+        }
+    });
+    if (w.step == -1) return within;  // no more than that
+    if (w.step < 0 || !(w.template below<S>() > within.v))
+        return narrow_by<T, kRows, kThreads>(g, kByElements, count, within, n, slack, best, red);
+    __syncthreads();
+    return Bound<S>{w.template below<S>(), 0xFFFFFFFFu};
+}
+
 // By the items, and lists them.
 template <typename T, bool kRows, int kThreads>
 __device__ __noinline__ Bound<typename Group<T, kRows>::S> list_items(Group<T, kRows> g, int items, int n, int cap,
@@ -425,7 +469,6 @@ pick_kernel(const __grid_constant__ PickArgs<T> a) {
     __shared__ float top_s[kWarps];
     __shared__ int items_s, parts_s, cands_s, steps[kSteps + 1];
     __shared__ int2 found_s;
-    __shared__ uint32_t least_s;
     __shared__ unsigned char slot_of[QS_MAX_BEAMS], parent_of[QS_MAX_BEAMS];
     __shared__ unsigned owns_s[2], stays_s[2];
     Cand<S>* cand = reinterpret_cast<Cand<S>*>(cand_raw);
@@ -436,8 +479,8 @@ pick_kernel(const __grid_constant__ PickArgs<T> a) {
     int* part_list = item_list + a.item_cap;                          // [part_cap]
     if (t == 0) {
         items_s = parts_s = cands_s = 0;
-        least_s = 0xFFFFFFFFu;
     }
+    for (int i = t; i <= kSteps; i += kThreads) steps[i] = 0;
     dependents_may_start();
     wait_for_previous();
     const float4* unit_parts = a.parts + (size_t)group * beams * a.units;
@@ -567,25 +610,17 @@ pick_kernel(const __grid_constant__ PickArgs<T> a) {
     const size_t out = (size_t)group * a.n;
     if (!bad) {
         const Within within =
-            find_within<kThreads>(item_score, all_items, a.n, a.item_cap - kExtra - a.n, fmaxf((float)best, kLowest<float>), steps, &found_s);
+            find_within<kThreads>(a.n, a.item_cap - kExtra - a.n, fmaxf((float)best, kLowest<float>), steps, &found_s, [&](auto f) {
+                for (int i = t; i < all_items; i += kThreads) f(item_score[i]);
+            });
         Bound<S> bound{kLowest<S>, 0xFFFFFFFFu};
         if (within.step > -2) {
-            uint32_t least = 0xFFFFFFFFu;
             for (int i = t; i < all_items; i += kThreads)
                 if (within.has(item_score[i])) {
-                    least = min(least, key_of(item_score[i]));
                     const int at = atomicAdd(&items_s, 1);
                     if (at < a.item_cap) item_list[at] = i;
                 }
-            if (within.step >= 0) {  // the least of them is the bound
-                least = __reduce_min_sync(0xffffffffu, least);
-                if (lane == 0) atomicMin(&least_s, least);
-                __syncthreads();
-                bound.v = score_at(least_s);
-                // of rounded sums: below all that round to it
-                if constexpr (!kRows)
-                    bound.v = score_at(least_s) > kLowest<float> ? (double)nextafterf(score_at(least_s), -INFINITY) : kLowest<double>;
-            }
+            bound.v = within.below<S>();
         } else {
             bound = list_items<T, kRows, kThreads>(g, all_items, a.n, a.item_cap, best, red, &items_s);
         }
@@ -642,7 +677,14 @@ pick_kernel(const __grid_constant__ PickArgs<T> a) {
         const int parts = min(parts_s, a.part_cap);
 
         // Their elements, in the same way: kPartVecs vectors a part, and in a row's first unit what lies outside the vectors.
-        while (true) {
+        if (a.coarse) {
+            bound = step_by_elements<T, kRows, kThreads>(g, parts, bound, a.n, kMaxCands - 64 - a.n, best, red, steps, &found_s);
+            if constexpr (!kRows) {
+                for (int i = t; i < beams; i += kThreads) floor_s[i] = -INFINITY;  // the score decides
+                __syncthreads();
+            }
+        }
+        for (int again = a.coarse;; again++) {
             const int vecs = parts * kPartVecs;
             for (int i0 = t; i0 < vecs; i0 += 4 * kThreads) {
                 uint4 w[4];
@@ -691,7 +733,9 @@ pick_kernel(const __grid_constant__ PickArgs<T> a) {
             }
             __syncthreads();
             if (cands_s <= kMaxCands) break;  // else few parts hold them, or few parts there are
-            bound = narrow_by<T, kRows, kThreads>(g, kByElements, parts, bound, a.n, kMaxCands - a.n, best, red);
+            // by steps first, with room for what rounding lets through, then exactly
+            if (again == 0) bound = step_by_elements<T, kRows, kThreads>(g, parts, bound, a.n, kMaxCands - 64 - a.n, best, red, steps, &found_s);
+            else bound = narrow_by<T, kRows, kThreads>(g, kByElements, parts, bound, a.n, kMaxCands - a.n, best, red);
             if (t == 0) cands_s = 0;
             if constexpr (!kRows) {
                 for (int i = t; i < beams; i += kThreads) floor_s[i] = -INFINITY;  // the score decides
@@ -810,6 +854,7 @@ static int best(const Rows& r, PickArgs<T> p, void* workspace, cudaStream_t st) 
     p.log_lanes = units >= 3 * p.n ? 5 : units << (5 - log_n) >= 3 * p.n ? log_n : 0;
     p.item_cap = p.n + p.n / 4 + 16 + kExtra;
     p.part_cap = 3 * p.n + 2 * kExtra < kMaxParts ? 3 * p.n + 2 * kExtra : kMaxParts;
+    p.coarse = (long long)units * 32 < 2 * p.n;  // 700 bf16 rows of 15,000, 256 listed: 85 us without, 50 with it
     // The lanes' maxima go to shared memory where all of them are looked at (40 KB leave room for several groups an SM);
     // where units are narrowed down first, few are, and are read when their units are known.
     const size_t lanes = (size_t)units * 32 * sizeof(T), items = (size_t)units << (5 - p.log_lanes);
