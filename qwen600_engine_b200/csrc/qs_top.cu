@@ -743,6 +743,7 @@ pick_kernel(const __grid_constant__ PickArgs<T> a) {
             __syncthreads();
         }
         if constexpr (!kRows) {
+            __syncthreads();  // all have seen that there is room
             for (int i = t; i < beams; i += kThreads)
                 if (state_s[i] == 1) cand[atomicAdd(&cands_s, 1)] = Cand<S>(add_s[i], (uint32_t)i << kTokenBits);
             __syncthreads();
