@@ -258,6 +258,15 @@ def test_beams(dtype, batch, beams, V, n):
     check_beams(rows_of(batch * beams, V, dtype, seed=batch + V), scores_of(batch, beams, n), n, T=0.9)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["mixed", "few values", "masked", "block"])
+@pytest.mark.parametrize("beams,V,n", [(2, 1000, 200), (3, 3001, 256), (1, 6000, 129), (5, 600, 256)])
+def test_long_lists_of_few_parts(dtype, kind, beams, V, n):
+    x = rows_of(2 * beams, V, dtype, seed=V + n, kind=kind, pad=3)
+    check_beams(x, scores_of(2, beams, n), n)
+    check_top(x, n)
+
+
 @pytest.mark.parametrize("T", [1e-3, 0.05, 40.0])
 @pytest.mark.parametrize("keep", [False, True])
 def test_beams_at_any_temperature(T, keep):
