@@ -577,8 +577,10 @@ QS_API int qs_reorder_history(qs_sampler* s, const int* d_parents, int batch, in
  * w = d_weights[i] (NULL: 1 / rows).  A token outside the vocabulary is no entry;
  * one listed again counts where it stands first.  A log-probability of -inf is
  * q = 0, and 0 log 0 = 0.  A row with w[i] = 0 (which is not read), without entries,
- * or with rest = 0 whose q are all 0, adds nothing and has a zero gradient.  A
- * teacher's token that the logits mask (-inf, with q > 0) makes the loss +inf.
+ * or with rest = 0 whose q are all 0, adds nothing and has a zero gradient.  Any
+ * other row whose logits are no distribution (a NaN or +inf among them, or -inf
+ * alone) has a NaN loss and gradient.  A teacher's token that the logits mask
+ * (-inf, with q > 0) makes the loss +inf.
  * d_loss fp32 [1], d_row_losses fp32 [rows] (l, 0 for rows that add nothing) or
  * NULL, d_grad as for the losses above (NULL: the loss alone).  1 <= k <=
  * QS_MAX_LISTED. */

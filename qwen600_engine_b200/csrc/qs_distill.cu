@@ -407,6 +407,7 @@ distill_loss_kernel(const RowList* lists, int rows, const float* __restrict__ we
             } else {
                 l = r.cost / r.mass - log(r.mass) + away;
             }
+            if (isnan(total)) l = total;  // no distribution, also where nothing is summed: the gradient is NaN then
             sum += w * l;
         }
         if (row_losses) row_losses[i] = (float)l;
