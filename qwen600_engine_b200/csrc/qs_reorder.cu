@@ -194,14 +194,18 @@ static int levels_of(const qs_states& s, int rows, Level* out) {
     return n;
 }
 
+constexpr long long kMaxStride = 1ll << 44, kMaxSpan = 1ll << 46;  // bytes
+
 // Bytes from the first to behind the last of the levels whose stride is below
-// `under`; -1 where a level's pieces do not lie behind one another.
+// `under`; -1 where a level's pieces do not lie behind one another, or the last
+// lies farther than any memory reaches (a product of 75 bits at most: divided, not
+// multiplied).  `unit` is above 0.
 static long long span_of(long long unit, const Level* l, int n, long long under) {
     long long span = unit;
     for (int i = 0; i < n && l[i].stride < under; i++) {
-        if (l[i].stride < span || l[i].stride > 1ll << 44) return -1;
+        if (l[i].stride < span || l[i].stride > kMaxStride || l[i].count - 1 > kMaxSpan / l[i].stride) return -1;
         span += (l[i].count - 1) * l[i].stride;
-        if (span > 1ll << 46) return -1;
+        if (span > kMaxSpan) return -1;
     }
     return span;
 }
@@ -243,7 +247,7 @@ static int check_states(const qs_states* all, int count, int rows) {
             return fail(QS_ERR_INVALID, "state %d: a size below 1", i);
         Level l[4];
         const int n = levels_of(s, rows, l);
-        if (s.unit > 1ll << 44 || span_of(s.unit, l, n, kAllLevels) < 0)
+        if (s.unit > kMaxStride || span_of(s.unit, l, n, kAllLevels) < 0)
             return fail(QS_ERR_INVALID, "state %d: its pieces overlap, or its strides are not those of nested blocks", i);
         if ((double)s.unit * s.positions * s.outer[0] * s.outer[1] > 2147483647.0 * (1 << width_of(s, rows)))
             return fail(QS_ERR_UNSUPPORTED, "state %d: above 2^31 - 1 vectors of %d bytes in a row", i, 1 << width_of(s, rows));

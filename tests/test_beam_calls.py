@@ -1,0 +1,33 @@
+"""Refusals of the beam calls that need no GPU: layouts whose extent passes 64
+bits."""
+import ctypes as C
+
+import pytest
+
+from qwen600_engine_b200 import _lib
+from qwen600_engine_b200._lib import QS_ERR_INVALID
+
+L = _lib.lib
+BASE = 0x7F0000000000
+
+
+def state(row, outer=(1, 1), outer_stride=(0, 0), positions=1, stride=0, unit=16, base=BASE):
+    s = _lib.States()
+    s.d_base, s.row_stride, s.unit, s.positions, s.position_stride = base, row, unit, positions, stride
+    s.outer[0], s.outer[1] = outer
+    s.outer_stride[0], s.outer_stride[1] = outer_stride
+    return s
+
+
+# (count - 1) * stride of one level is 2^64 or near it: as a 64-bit number small or negative
+@pytest.mark.parametrize("wide", [
+    dict(row=1 << 40, positions=(1 << 29) + 1, stride=1 << 35), dict(row=16, positions=(1 << 30) + 1, stride=1 << 34),
+    dict(row=16, outer=(1, (1 << 29) + 1), outer_stride=(0, 1 << 35)), dict(row=16, outer=((1 << 30) + 1, 1), outer_stride=(1 << 34, 0)),
+    dict(row=16, positions=1 << 30, stride=1 << 34), dict(row=1 << 44, positions=(1 << 20) + 1, stride=1 << 43)])
+def test_states_wider_than_64_bits_refused(wide):
+    states = (_lib.States * 1)(state(**wide))
+    assert L.qs_beam_reorder(states, 1, 0x10000, 2, 3, None, None) == QS_ERR_INVALID
+    assert b"nested blocks" in L.qs_last_error()
+    both = (_lib.States * 2)(state(row=1000, unit=1000, base=BASE - (1 << 20)), state(**wide))
+    assert L.qs_beam_reorder(both, 2, 0x10000, 2, 3, None, None) == QS_ERR_INVALID
+    assert b"state 1" in L.qs_last_error()
