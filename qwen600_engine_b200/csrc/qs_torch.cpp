@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/Functions.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -459,6 +460,8 @@ PyObject* beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n) {
                         " of " + shape_of(t));
             if (t.device() != pa.device()) invalid("a state must be on " + pa.device().str() + ", got " + told(t));
             if (t.layout() != at::kStrided) invalid("a state must be a dense tensor");
+            if (t.requires_grad() && at::GradMode::is_enabled())  // autograd would not see the move
+                invalid("a state needs a gradient: move its detach(), or call under torch.no_grad()");
             if (t.numel() == 0) continue;
             all.push_back(layout(t, d, lengths ? l : -1));
             moved.push_back(&t);

@@ -1,11 +1,10 @@
 """Refusals of the beam calls that need no GPU: layouts whose extent passes 64
-bits."""
-import ctypes as C
-
+bits, and tensors that need a gradient."""
 import pytest
+import torch
 
-from qwen600_engine_b200 import _lib
-from qwen600_engine_b200._lib import QS_ERR_INVALID
+from qwen600_engine_b200 import _lib, beams
+from qwen600_engine_b200._lib import QS_ERR_INVALID, SamplerError
 
 L = _lib.lib
 BASE = 0x7F0000000000
@@ -31,3 +30,22 @@ def test_states_wider_than_64_bits_refused(wide):
     both = (_lib.States * 2)(state(row=1000, unit=1000, base=BASE - (1 << 20)), state(**wide))
     assert L.qs_beam_reorder(both, 2, 0x10000, 2, 3, None, None) == QS_ERR_INVALID
     assert b"state 1" in L.qs_last_error()
+
+
+PARENTS = torch.zeros((2, 2), dtype=torch.int32)
+
+
+@pytest.mark.parametrize("make", [lambda w: w, lambda w: w * 2, lambda w: (w * 2).view(4, 5, 2), lambda w: w[:, :4]])
+def test_states_that_need_a_gradient_refused(make):
+    """A leaf (a parameter given by mistake), a result of one, and views of both."""
+    w = torch.ones((4, 10), requires_grad=True)
+    for states in (make(w), [torch.zeros((4, 3)), make(w)]):
+        with pytest.raises(SamplerError, match="needs a gradient"):
+            beams.beam_reorder(states, PARENTS)
+    # what autograd does not record goes on to the next check
+    for t in (make(w).detach(), make(w.detach())):
+        with pytest.raises(SamplerError, match="on a GPU"):
+            beams.beam_reorder(t, PARENTS)
+    for mode in (torch.no_grad(), torch.inference_mode()):
+        with mode, pytest.raises(SamplerError, match="on a GPU"):
+            beams.beam_reorder(make(w), PARENTS)
