@@ -42,8 +42,6 @@ def beam_select(logits, scores, *, n: Optional[int] = None, finished=None, eos_t
     ``keep_slots``: each beam's best child stays in its parent's place, so that
     ``beam_reorder`` has only the places of beams that end to write; scores are
     then in no order."""
-    if n is None:
-        n = scores.shape[1]
     if pad_token is None:
         pad_token = eos_token
     return tuple.__new__(BeamStep, _on(stream, _torch.beam_select, logits, scores, n, finished, eos_token, pad_token, temperature,

@@ -369,7 +369,8 @@ PyObject* distill_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// (logits, scores, n, finished, eos_token, pad_token, temperature, keep_slots) -> (scores, parents, tokens, finished)
+// (logits, scores, n or None: as many as beams, finished, eos_token, pad_token, temperature, keep_slots)
+//   -> (scores, parents, tokens, finished)
 PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return call(n, 8, [&] {
         const at::Tensor& x = tensor("logits", a[0]);
@@ -381,7 +382,7 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if ((int64_t)batch * beams != m.rows)
             invalid("logits must have a row for each of " + std::to_string(batch) + " x " + std::to_string(beams) + " beams, got " +
                     shape_of(x));
-        const int chosen = listed("n", whole(a[2]));
+        const int chosen = listed("n", a[2] == Py_None ? beams : whole(a[2]));
         const unsigned char* finished = a[3] == Py_None ? nullptr : table<unsigned char>("finished", a[3], at::kBool, batch, beams, x);
         const qs_beam_params p{number(a[6]), number_of_token("eos_token", a[4]), number_of_token("pad_token", a[5]), truth(a[7])};
         const On on(x);

@@ -1,10 +1,10 @@
 """Refusals of the beam calls that need no GPU: layouts whose extent passes 64
-bits, and tensors that need a gradient."""
+bits, tensors that need a gradient, and scores of no shape to count beams by."""
 import pytest
 import torch
 
 from qwen600_engine_b200 import _lib, beams
-from qwen600_engine_b200._lib import QS_ERR_INVALID, SamplerError
+from qwen600_engine_b200._lib import QS_ERR_INVALID, QS_ERR_UNSUPPORTED, SamplerError
 
 L = _lib.lib
 BASE = 0x7F0000000000
@@ -49,3 +49,21 @@ def test_states_that_need_a_gradient_refused(make):
     for mode in (torch.no_grad(), torch.inference_mode()):
         with mode, pytest.raises(SamplerError, match="on a GPU"):
             beams.beam_reorder(make(w), PARENTS)
+
+
+@pytest.mark.parametrize("scores,match", [(torch.zeros(4), "scores must be"), (torch.tensor(0.0), "scores must be"), ([[0.0, 0.0]], "must be a tensor"),
+                                          (None, "must be a tensor"), (torch.zeros((4, 1, 1)), "scores must be")])
+def test_scores_that_give_no_number_of_beams_refused(scores, match):
+    """`n` is as many as beams where it is not given: what the scores are is looked at first."""
+    for n in ({}, {"n": 2}):
+        with pytest.raises(SamplerError, match=match) as e:
+            beams.beam_select(torch.zeros((4, 10)), scores, **n)
+        assert e.value.code == QS_ERR_INVALID
+
+
+def test_beams_above_the_list_refused():
+    with pytest.raises(SamplerError, match="300 outside \\[1, 256\\]") as e:
+        beams.beam_select(torch.zeros((300, 10)), torch.zeros((1, 300)))
+    assert e.value.code == QS_ERR_UNSUPPORTED
+    with pytest.raises(SamplerError, match="outside"):
+        beams.beam_select(torch.zeros((0, 10)), torch.zeros((2, 0)))
