@@ -27,7 +27,7 @@ from .losses import _on, _torch
 class BeamStep(NamedTuple):
     scores: torch.Tensor    # fp32 [batch, n]
     parents: torch.Tensor   # int32 [batch, n]: the beam that each one continues, -1: none
-    tokens: torch.Tensor    # int32 [batch, n], -1: none
+    tokens: torch.Tensor    # int32 [batch, n], -1: none (not a token to look up)
     finished: torch.Tensor  # bool [batch, n]
 
 

@@ -63,7 +63,7 @@ def search(prompt, masked):
     return [(s, toks) for s, toks, _ in held]
 
 
-@pytest.mark.parametrize("masked", [False])
+@pytest.mark.parametrize("masked", [False, True])
 def test_search_as_documented(masked):
     from qwen600_engine_b200.sampler import Sampler
     blocks = documented()
