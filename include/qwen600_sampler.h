@@ -515,7 +515,9 @@ QS_API int qs_top_logprobs(const void* d_logits, int dtype, int rows, int vocab,
  * others this score); where an entry has fewer than n, score -inf, parent -1,
  * token -1 and finished 1 fill up.  An entry with a score of NaN or +inf, or a
  * NaN or +inf among its logits read, has scores NaN, parents and tokens -1.
- * Scores are compared as 64-bit numbers before they are rounded.
+ * Scores are compared as 64-bit numbers before they are rounded.  A row's sum of
+ * exponentials is good to fp32, and its last bits depend on the row's alignment:
+ * rows alike give equal scores where their addresses are alike modulo 16 bytes.
  * keep_slots (n = beams): the chosen ones are the same, but each beam's best one
  * stays in that beam's place and the others take the places left, the better
  * first: then only places of beams that end change their state, each to that of
