@@ -547,7 +547,9 @@ QS_API int qs_beam_select(const void* d_logits, int dtype, int batch, int beams,
  * host.  Pieces may not overlap, nor states: two of them may lie between one
  * another only if both repeat with the same stride and are apart within it; they may
  * not overlap the parents and lengths.
- * batch * beams <= 2^27, beams <= 1024, at most 2^31 - 1 pieces of a row. */
+ * batch * beams <= 2^27, beams <= 1024.  A row is moved in vectors of 1, 2, 4, 8 or
+ * 16 bytes, the largest that divides the base, the unit and all strides: at most
+ * 2^31 - 1 of them a row.  Strides up to 2^44 bytes. */
 typedef struct {
     void* d_base;
     long long row_stride;
@@ -582,7 +584,9 @@ QS_API int qs_reorder_history(qs_sampler* s, const int* d_parents, int batch, in
  * or with rest = 0 whose q are all 0, adds nothing and has a zero gradient.  Any
  * other row whose logits are no distribution (a NaN or +inf among them, or -inf
  * alone) has a NaN loss and gradient.  A teacher's token that the logits mask
- * (-inf, with q > 0) makes the loss +inf.
+ * (-inf, with q > 0) makes the loss +inf.  Mask with -inf: unlisted tokens that a
+ * finite number hides are above -inf, and where they are all that the list leaves,
+ * what rounding makes of r (2^-24, say) is held against a p_r of 0.
  * d_loss fp32 [1], d_row_losses fp32 [rows] (l, 0 for rows that add nothing) or
  * NULL, d_grad as for the losses above (NULL: the loss alone).  1 <= k <=
  * QS_MAX_LISTED. */

@@ -239,6 +239,8 @@ static int width_of(const qs_states& s, int rows) {
 }
 static long long vecs_of(const qs_states& s, int width) { return (s.unit >> width) * s.positions * s.outer[0] * s.outer[1]; }
 
+// Each state for itself, and every pair of them: 29 us of host time for 56 states, where
+// one takes 1.5.
 static int check_states(const qs_states* all, int count, int rows) {
     for (int i = 0; i < count; i++) {
         const qs_states& s = all[i];

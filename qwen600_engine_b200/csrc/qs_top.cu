@@ -25,7 +25,10 @@ constexpr int kMaxCands = 2 * QS_MAX_LISTED;  // elements that are ranked, besid
 // also hold what lies behind the row's last vector), and as many that count from
 // the row's last place.
 constexpr int kExtra = 96;
-constexpr int kMaxParts = 1000;  // their elements are counted in 16 bits
+// Parts that are listed at most.  Their elements are counted in 16 bits: 64 bf16 a part,
+// and up to 14 of each beam's row outside its vectors.
+constexpr int kMaxParts = 3 * QS_MAX_LISTED + 2 * kExtra;
+static_assert(kMaxParts * 64 + QS_MAX_BEAMS * 14 < 1 << 16, "counts of elements");
 template <typename S> constexpr S kLowest = 0;  // the lowest finite number
 template <> constexpr float kLowest<float> = -3.402823466e38f;
 template <> constexpr double kLowest<double> = -1.7976931348623157e308;
@@ -343,8 +346,12 @@ struct Group {
     }
 };
 
-// Narrows by the items, by the listed items' lanes, or by the listed parts' elements: for
-// what few calls reach, out of line so that the usual way's values stay in registers.
+// Narrows by the items, by the listed items' lanes, or by the listed parts' elements: out
+// of line so that the usual way's values stay in registers.  Of full vocabularies few calls
+// reach it.  Short rows with short lists do by their size alone: where all items fit into the
+// first list the bound stays at the lowest number, and lanes or elements are narrowed down
+// instead.  One bf16 row's best token: 36 us of 10,000 columns, 20 of 4,000 (by elements), 7.5
+// of 40,000; a step of 4 beams of 2,000 54, of 151,936 10.2.
 enum { kByItems, kByLanes, kByElements };
 
 template <typename T, bool kRows, int kThreads>
@@ -444,7 +451,9 @@ __device__ __forceinline__ float element(const uint4& w, int j) {
 // elements, ranks) takes 10 to 20 thousand cycles, most of them round trips to memory and
 // barriers; 1024 rows' lists of 64 take 13 us behind a stream of 57, one row's of 20 8.1
 // with its stream, an entry of 4 beams 10.6.  More threads for long lists: 250 of 61 rows
-// 18 us with 512, 35 with 256; for several beams' sums a warp each.
+// 18 us with 512, 35 with 256; for several beams' sums a warp each.  64 registers for rows
+// (128 for beams) keep 1024 (512) threads on an SM; 68 to 84 bytes a thread of rows spill
+// then, 20 to 76 of beams.  Ranks compare all candidates with one another: up to 512 of them.
 //
 // One CTA per group.  kRows: a group is a row, and its logits are the scores that
 // are compared; else they are the beams' sums.
@@ -854,7 +863,7 @@ static int best(const Rows& r, PickArgs<T> p, void* workspace, cudaStream_t st) 
     const int units = p.beams * p.units, log_n = r.dtype == QS_F32 ? 2 : 3;
     p.log_lanes = units >= 3 * p.n ? 5 : units << (5 - log_n) >= 3 * p.n ? log_n : 0;
     p.item_cap = p.n + p.n / 4 + 16 + kExtra;
-    p.part_cap = 3 * p.n + 2 * kExtra < kMaxParts ? 3 * p.n + 2 * kExtra : kMaxParts;
+    p.part_cap = 3 * p.n + 2 * kExtra;
     p.coarse = (long long)units * 32 < 2 * p.n;  // 700 bf16 rows of 15,000, 256 listed: 85 us without, 50 with it
     // The lanes' maxima go to shared memory where all of them are looked at (40 KB leave room for several groups an SM);
     // where units are narrowed down first, few are, and are read when their units are known.
