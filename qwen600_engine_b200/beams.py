@@ -55,8 +55,8 @@ def beam_reorder(states, parents, *, dim: int = 0, lengths=None, length_dim: int
     once, or one tensor per layer); ``parents`` int32 [batch, beams], one outside
     [0, beams) leaves its row as it is.  ``lengths`` int32 [batch]: the positions
     in use of each entry, along ``length_dim``, with those that the step's model
-    call has written; what lies behind them is left as it is.  Tensors that need a gradient are refused while autograd records: the
-    move has no backward."""
+    call has written; what lies behind them is left as it is.  Tensors that need
+    a gradient are refused while autograd records: the move has no backward."""
     states = (states,) if isinstance(states, torch.Tensor) else tuple(states)
     _on(stream, _torch.beam_reorder, parents, states, dim, lengths, length_dim)
 

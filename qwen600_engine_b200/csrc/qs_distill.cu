@@ -193,6 +193,9 @@ distill_kernel(const __grid_constant__ DistillArgs<T> a) {
     };
     if (w_row == 0.0f) {  // alike for the whole cluster
         nothing();
+        // Where every row is left out, one CTA sees to it that this grid does not end before the list kernel has:
+        // what follows on the stream waits for this grid and the loss's, and may write what the lists are read from.
+        if (blockIdx.x == 0) wait_for_previous();
         return;
     }
     const int piece = (a.share + kW - 1) / kW;
@@ -420,10 +423,11 @@ distill_loss_kernel(const RowList* lists, int rows, const float* __restrict__ we
 
 // How rows are spread: CTAs per row (a power of two up to 8), doubled while a share is
 // above 80 KB, two of which fit on an SM, and while the rows alone would leave some of
-// the 148 SMs idle and a share is above 4 KB (halves of it are 2 KB and more).  2048 bf16 rows of 151,936, a quarter of them
-// left out: 218 us with 4 CTAs a row (76 KB shares), 241 with 8 (38 KB, five an SM), 312
-// with 2; 300 fp32 rows of 37,999 29 us with 2, 31 with 4.  CTAs of 224 threads 232 us, of
-// 384 259.  CTAs that have an SM for themselves take 512 threads (8 rows 6.2 us, 7.0 with 256).
+// the 148 SMs idle and a share is above 4 KB (halves of it are 2 KB and more).  2048 bf16
+// rows of 151,936, a quarter of them left out: 218 us with 4 CTAs a row (76 KB shares), 241
+// with 8 (38 KB, five an SM), 312 with 2; 300 fp32 rows of 37,999 29 us with 2, 31 with 4.
+// CTAs of 224 threads 232 us, of 384 259.  CTAs that have an SM for themselves take 512
+// threads (8 rows 6.2 us, 7.0 with 256).
 template <typename T>
 static int distill_launch(DistillArgs<T>& a, cudaStream_t st) {
     const int vecs = a.V / Pack<T>::kN;

@@ -1,5 +1,6 @@
 """Rows of the distillation whose logits are no distribution: loss and gradient
-agree that they are none, whatever the teacher gives the list."""
+agree that they are none, whatever the teacher gives the list.  And batches of
+nothing but rows that are left out, with their inputs written again at once."""
 import pytest
 import torch
 
@@ -49,3 +50,30 @@ def test_a_distribution_and_a_list_of_nothing(dtype):
     tok = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda")
     r = losses.distill_loss(x, tok, torch.full((1, 2), -INF, device="cuda"))
     assert float(r.loss) == 0 and not r.grad.any()
+
+
+@pytest.mark.parametrize("N,V,k", [(1, 5, 1), (8, 4003, 20), (3000, 40, 256), (300, 3001, 256)])
+def test_every_row_left_out_and_the_inputs_written_again(N, V, k):
+    """The next writes on the stream come behind all of the call's reads."""
+    from qwen600_engine_b200 import losses
+    g = torch.Generator(device="cuda")
+    g.manual_seed(N)
+    x = torch.randn((N, V), generator=g, device="cuda")
+    tok = torch.randint(0, V, (N, k), generator=g, device="cuda").int()
+    lps = torch.full((N, k), -6.0, device="cuda")
+    some = torch.rand((N,), generator=g, device="cuda") + 0.5
+    want = losses.distill_loss(x, tok, lps, weights=some)
+    w = torch.zeros((N,), device="cuda")
+    tokens = tok.clone()
+    for i in range(40):
+        out = torch.full_like(x, 3.0)
+        w.zero_()
+        r = losses.distill_loss(x, tokens, lps, weights=w, out=out)
+        w.copy_(some)
+        tokens.fill_(-1)
+        filler = torch.full((4 * N * k,), 7, dtype=torch.int32, device="cuda")  # where the call's workspace may have been
+        tokens.copy_(tok)
+        again = losses.distill_loss(x, tokens, lps, weights=w)
+        assert float(r.loss) == 0 and not r.row_losses.any() and not out.any()
+        assert torch.equal(again.grad, want.grad) and torch.equal(again.row_losses, want.row_losses)
+        assert (filler == 7).all()
